@@ -62,6 +62,26 @@ typedef struct {
     PkvDType dtype;     /* storage: F16 or BF16 (F32 pools serve only the decoder entry point) */
 } PkvPagedLayer;
 
+/* One layer of 8-bit pages: int8 values with one FP32 scale per block of
+ * tokens (page) and KV head, value = q * scale.  A lane is 128 columns of a
+ * token's row (one KV head of head_dim 128, or two of head_dim 64); there are
+ * lanes = ceil(kv_heads * head_dim / 128) of them, and the pools are
+ * [block_count][lanes][block_size][128] bytes: element c of lane j is column
+ * 128 j + c of the row, and one page of one lane is contiguous.  With an odd
+ * number of KV heads of head_dim 64 the second half of the last lane is
+ * unused (never read or written).  16, 32, 64 or 128 tokens a page. */
+typedef struct {
+    int8_t *key_pool;
+    int8_t *value_pool;
+    float *key_scales;   /* [block_count][kv_heads] */
+    float *value_scales; /* [block_count][kv_heads] */
+    size_t block_size;
+    size_t block_count;
+    size_t kv_heads;     /* 1..1024 */
+    size_t head_dim;     /* 64 or 128 */
+    PkvDType dtype;      /* F16 or BF16: rows, queries and 16-bit outputs */
+} PkvQ8Layer;
+
 /* The sequences of one batch, as the kernels see them (device pointers). */
 typedef struct {
     const uint32_t *block_tables; /* [batch][table_stride] page ids */
@@ -209,6 +229,39 @@ int pkv_paged_prefill(const PkvPagedLayer *layer, const PkvBatch *batch,
                       size_t max_query_len, float scale, int causal,
                       void *output, PkvDType output_dtype, PkvStream stream,
                       char *error, size_t error_capacity);
+
+/* Append, prefix import and gather for 8-bit pages; the arguments are those
+ * of pkv_kv_append, pkv_kv_import and pkv_kv_gather, rows in layer->dtype.
+ * Writing, per page and KV head, with a the largest |x| among the call's new
+ * rows of that page:
+ *     s = max(s_old, a / 127)   s_old = the page's scale if it holds earlier
+ *                               tokens of the sequence, else 0
+ *     q = rint(x * (1 / s))     (FP32, ties to even, within +-127)
+ * and where s > s_old the page's earlier tokens become
+ * rint(q * (s_old / s)): a page's scale only grows while the page fills, each
+ * growth rounding its earlier tokens once more (half a step of the new scale).
+ * s below 2^-126 is 0 and the block stores zeros.  A NaN is stored as 0 and
+ * an infinity as +-127, both outside a; fault code 5 is recorded.  Bytes of
+ * positions past the sequence's length are left as they are.  Gather writes
+ * q * s, rounded to layer->dtype. */
+int pkv_q8_append(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *row_offsets,
+                  const void *key_rows, const void *value_rows, size_t total_rows,
+                  PkvStream stream, char *error, size_t error_capacity);
+int pkv_q8_import(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *row_offsets,
+                  const void *key_rows, const void *value_rows, size_t total_rows,
+                  PkvStream stream, char *error, size_t error_capacity);
+int pkv_q8_gather(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *row_offsets,
+                  void *key_out, void *value_out, size_t total_rows, PkvStream stream, char *error,
+                  size_t error_capacity);
+
+/* pkv_paged_decode over 8-bit pages: q_heads 1 to 16 times kv_heads (any
+ * whole group), query in layer->dtype, output F32 or layer->dtype. */
+size_t pkv_q8_decode_workspace_bytes(size_t batch, size_t q_heads, size_t kv_heads,
+                                     size_t head_dim, size_t max_seq_len);
+int pkv_q8_decode(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads,
+                  const void *query, float scale, void *output, PkvDType output_dtype,
+                  size_t max_seq_len, void *workspace, size_t workspace_bytes, PkvStream stream,
+                  char *error, size_t error_capacity);
 
 /* Reads and clears the device fault word of `device` (synchronises it).
  * Kernels never trap: an out-of-range page id or position skips the access

@@ -43,6 +43,20 @@ class PkvPagedLayer(ctypes.Structure):
     ]
 
 
+class PkvQ8Layer(ctypes.Structure):
+    _fields_ = [
+        ("key_pool", _c_ptr),
+        ("value_pool", _c_ptr),
+        ("key_scales", _c_ptr),
+        ("value_scales", _c_ptr),
+        ("block_size", _c_size),
+        ("block_count", _c_size),
+        ("kv_heads", _c_size),
+        ("head_dim", _c_size),
+        ("dtype", _c_int),
+    ]
+
+
 class PkvBatch(ctypes.Structure):
     _fields_ = [
         ("block_tables", _c_ptr),
@@ -103,6 +117,7 @@ class TensorPagedKVDecodeRequest(ctypes.Structure):
 
 
 _LP = ctypes.POINTER(PkvPagedLayer)
+_QP = ctypes.POINTER(PkvQ8Layer)
 _BP = ctypes.POINTER(PkvBatch)
 _ERR = [_c_char_p, _c_size]
 
@@ -144,6 +159,12 @@ EXPORTS = {
                                                  _c_ptr, _c_int, _c_size, _c_ptr, *_ERR]),
     "pkv_paged_prefill": (_c_int, [_LP, _BP, _c_size, _c_ptr, _c_ptr, _c_size, _c_size,
                                    ctypes.c_float, _c_int, _c_ptr, _c_int, _c_ptr, *_ERR]),
+    "pkv_q8_append": (_c_int, [_QP, _BP, _c_ptr, _c_ptr, _c_ptr, _c_size, _c_ptr, *_ERR]),
+    "pkv_q8_import": (_c_int, [_QP, _BP, _c_ptr, _c_ptr, _c_ptr, _c_size, _c_ptr, *_ERR]),
+    "pkv_q8_gather": (_c_int, [_QP, _BP, _c_ptr, _c_ptr, _c_ptr, _c_size, _c_ptr, *_ERR]),
+    "pkv_q8_decode_workspace_bytes": (_c_size, [_c_size] * 5),
+    "pkv_q8_decode": (_c_int, [_QP, _BP, _c_size, _c_ptr, ctypes.c_float, _c_ptr, _c_int, _c_size,
+                               _c_ptr, _c_size, _c_ptr, *_ERR]),
     "pkv_device_fault": (_c_int, [_c_int, ctypes.POINTER(ctypes.c_uint32), *_ERR]),
     "pkv_selftest_wait_timeout": (_c_int, [ctypes.POINTER(ctypes.c_uint32), *_ERR]),
     "pkv_sdpa_workspace_bytes": (_c_size, [_c_size, _c_size, _c_size, _c_size, _c_size]),
@@ -400,6 +421,69 @@ def paged_prefill(layer: PkvPagedLayer, batch: PkvBatch, query, query_offsets, o
           _ptr(query_offsets), query.data_ptr(), query.shape[0], max_query_len,
           ctypes.c_float(scale), int(causal), output.data_ptr(), _dtype_code(output),
           _stream_ptr(stream))
+
+
+# ---------------------------------------------------------------------------
+# 8-bit pages: int8 values, one FP32 scale per page and KV head
+# ---------------------------------------------------------------------------
+
+def q8_lanes(kv_heads: int, head_dim: int) -> int:
+    """128-column lanes of a token's row: the second dimension of a pool."""
+    return -(-kv_heads * head_dim // 128)
+
+
+def make_q8_layer(key_pool, value_pool, key_scales, value_scales, kv_heads: int, head_dim: int,
+                  dtype) -> PkvQ8Layer:
+    """Layer view of two int8 [block_count, lanes, block_size, 128] pools and
+    their float32 [block_count, kv_heads] scales; dtype: torch.float16 or
+    torch.bfloat16, the type of rows and queries."""
+    import torch
+    n, lanes, block_size, width = key_pool.shape
+    assert key_pool.shape == value_pool.shape and key_pool.is_cuda
+    assert lanes == q8_lanes(kv_heads, head_dim) and width == 128
+    for pool in (key_pool, value_pool):
+        assert pool.dtype == torch.int8 and pool.is_contiguous()
+    for scales in (key_scales, value_scales):
+        assert scales.shape == (n, kv_heads) and scales.dtype == torch.float32
+        assert scales.is_contiguous()
+    code = {torch.float16: PKV_DTYPE_F16, torch.bfloat16: PKV_DTYPE_BF16}[dtype]
+    return PkvQ8Layer(key_pool.data_ptr(), value_pool.data_ptr(), key_scales.data_ptr(),
+                      value_scales.data_ptr(), block_size, n, kv_heads, head_dim, code)
+
+
+def q8_append(layer: PkvQ8Layer, batch: PkvBatch, key_rows, value_rows, row_offsets=None,
+              stream=None) -> None:
+    _call("pkv_q8_append", ctypes.byref(layer), ctypes.byref(batch), _ptr(row_offsets),
+          key_rows.data_ptr(), value_rows.data_ptr(), key_rows.shape[0], _stream_ptr(stream))
+
+
+def q8_import(layer: PkvQ8Layer, batch: PkvBatch, key_rows, value_rows, row_offsets,
+              stream=None) -> None:
+    _call("pkv_q8_import", ctypes.byref(layer), ctypes.byref(batch), _ptr(row_offsets),
+          key_rows.data_ptr(), value_rows.data_ptr(), key_rows.shape[0], _stream_ptr(stream))
+
+
+def q8_gather(layer: PkvQ8Layer, batch: PkvBatch, key_out, value_out, row_offsets,
+              stream=None) -> None:
+    _call("pkv_q8_gather", ctypes.byref(layer), ctypes.byref(batch), _ptr(row_offsets),
+          key_out.data_ptr(), value_out.data_ptr(), key_out.shape[0], _stream_ptr(stream))
+
+
+def q8_decode_workspace(batch: int, q_heads: int, kv_heads: int, head_dim: int, max_seq_len: int,
+                        device=None, stream=None):
+    """Zero-initialised scratch of q8_decode as a uint8 CUDA tensor."""
+    import torch
+    n = load().pkv_q8_decode_workspace_bytes(batch, q_heads, kv_heads, head_dim, max_seq_len)
+    ws = torch.empty(n, dtype=torch.uint8, device=device or "cuda")
+    _call("pkv_decode_workspace_init", ws.data_ptr(), n, _stream_ptr(stream))
+    return ws
+
+
+def q8_decode(layer: PkvQ8Layer, batch: PkvBatch, query, output, scale: float, max_seq_len: int,
+              workspace, stream=None) -> None:
+    _call("pkv_q8_decode", ctypes.byref(layer), ctypes.byref(batch), query.shape[-2],
+          query.data_ptr(), ctypes.c_float(scale), output.data_ptr(), _dtype_code(output),
+          max_seq_len, workspace.data_ptr(), workspace.numel(), _stream_ptr(stream))
 
 
 def device_fault(device: int = 0) -> int:

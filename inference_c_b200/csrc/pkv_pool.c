@@ -444,16 +444,24 @@ int pkv_device_fault(int device, uint32_t *code, char *error, size_t cap) {
     const int have_prev = cudaGetDevice(&prev) == cudaSuccess;
     cudaError_t st = cudaSetDevice(device);
     if (st == cudaSuccess) st = cudaDeviceSynchronize();
-    uint32_t a = 0, b = 0, c = 0, d = 0, e = 0;
-    int ok = st == cudaSuccess && pkv_internal_take_copy_fault(&a) &&
-             pkv_internal_take_decode_fault(&b) && pkv_internal_take_prefill_fault(&c) &&
-             pkv_internal_take_sequence_fault(&d) && pkv_internal_take_peer_fault(&e);
+    int (*const take[])(uint32_t *) = {
+        pkv_internal_take_copy_fault,     pkv_internal_take_decode_fault,
+        pkv_internal_take_prefill_fault,  pkv_internal_take_sequence_fault,
+        pkv_internal_take_peer_fault,     pkv_internal_take_q8_copy_fault,
+        pkv_internal_take_q8_decode_fault};
+    uint32_t first = 0;
+    int ok = st == cudaSuccess;
+    for (size_t i = 0; ok && i < sizeof take / sizeof take[0]; ++i) {
+        uint32_t word = 0;
+        ok = take[i](&word);
+        if (first == 0) first = word;
+    }
     if (have_prev) cudaSetDevice(prev);
     if (!ok) {
         pkv_internal_set_error(error, cap, "pkv_device_fault: %s",
                                cudaGetErrorString(st != cudaSuccess ? st : cudaGetLastError()));
         return 0;
     }
-    *code = a ? a : (b ? b : (c ? c : (d ? d : e)));
+    *code = first;
     return 1;
 }

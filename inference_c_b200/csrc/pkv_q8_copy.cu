@@ -1,0 +1,328 @@
+// pkv_q8_copy.cu -- rows into 8-bit pages (append, prefix import) and back
+// (gather).
+//
+// One unit is one (page of a sequence, lane, K or V); block_size / 16 warps
+// share it, each holding 16 rows x 128 columns in registers (thread: 8
+// columns of every second row), so every value crosses the bus once.  Append
+// and import: the largest |x| of the page's new rows of each head is reduced
+// over the warps, the scale follows, and the rows leave as 8-byte stores, two
+// whole 128-byte rows a warp instruction.  A page that holds earlier tokens
+// keeps its scale unless the new rows need a larger one; then its earlier
+// tokens are rescaled, q' = rint(q * (s_old / s)), by the threads that own
+// those rows.  Bound by HBM: 2 bytes read and 1 written a value (gather the
+// reverse).
+#include <stdio.h>
+
+#include "pkv_q8.cuh"
+#include "pkv_trace.h"
+
+namespace pkv {
+namespace {
+
+__device__ uint32_t g_q8_copy_fault;
+
+constexpr int kQ8Warps = 8;  // per CTA
+
+struct Q8RowArgs {
+    uint2 *pools[2];          // K, V: [pages][lanes][block][16] eight-byte groups
+    float *scales[2];         // [pages][kv_heads]
+    uint4 *rows[2];           // [total_rows][kv_width / 8]
+    const uint32_t *tables;
+    const int32_t *seq_lens;
+    const int32_t *offsets;   // null: one row per sequence
+    int32_t table_stride, batch, kv_heads, lanes, block_size;
+    uint32_t block_count;
+    int32_t units;            // upper bound of pages touched
+    int32_t row_vecs;         // uint4 per contiguous row
+    int32_t tail;             // rows are the sequence's last (append) or first positions
+};
+
+struct Q8Unit {
+    int b;
+    int32_t first, count, page0;  // first new position, new rows, first page touched
+};
+
+// Sequence b touches at most floor((n_b - 1) / block) + 2 pages, so giving it
+// the units from floor(offsets[b] / block) + 2 b on needs no scan: unit u
+// belongs to the last sequence whose first unit is <= u.
+__device__ __forceinline__ int32_t q8_first_unit(const Q8RowArgs &a, int b) {
+    return __ldg(a.offsets + b) / a.block_size + 2 * b;
+}
+
+// WRITE: rows -> pages.  Otherwise pages -> rows.
+template <typename T, int HD, bool WRITE>
+__global__ void __launch_bounds__(kQ8Warps * 32)
+q8_rows_kernel(const Q8RowArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    __shared__ float top[kQ8Warps][2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int per = a.block_size / 16;              // warps of one unit
+    const int u = blockIdx.x * (kQ8Warps / per) + warp / per;
+    const int part = warp % per;                    // this warp's 16 rows of the page
+    const int col_lane = blockIdx.y >> 1, kv = blockIdx.y & 1;
+    constexpr int kHeads = 128 / HD;                // heads of a lane
+    const int chunk = lane & 15;                    // this thread's 8 columns
+    const int hl = HD == 64 ? chunk >> 3 : 0;       // its head within the lane
+    const int head = col_lane * kHeads + hl;
+
+    // ---- which page ----
+    bool live = u < a.units && head < a.kv_heads;
+    const bool unit_live = u < a.units;
+    int b = 0;
+    int32_t first = 0, end = 0, row0 = 0, page = 0;
+    bool held = false;
+    uint32_t pid = 0;
+    if (unit_live) {
+        int32_t count = 1, slot = 0;
+        if (a.offsets == nullptr) {
+            b = u;
+            row0 = u;
+        } else {
+            int lo = 0, hi = a.batch - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (q8_first_unit(a, mid) <= u) lo = mid; else hi = mid - 1;
+            }
+            b = lo;
+            row0 = __ldg(a.offsets + b);
+            count = __ldg(a.offsets + b + 1) - row0;
+            slot = u - q8_first_unit(a, b);
+        }
+        const int32_t L = __ldg(a.seq_lens + b);
+        uint32_t fault = kFaultNone;
+        first = a.tail ? L - count : 0;
+        end = first + count;
+        page = first / a.block_size + slot;
+        if (count > L) fault = slot == 0 ? kFaultRowsMismatch : kFaultNone;
+        if (count > L || count <= 0 || (int64_t)page * a.block_size >= end) live = false;
+        if (live) {
+            if (page >= a.table_stride) fault = kFaultPositionOutOfRange;
+            else {
+                pid = __ldg(a.tables + (int64_t)b * a.table_stride + page);
+                if (pid >= a.block_count) fault = kFaultPageOutOfRange;
+            }
+        }
+        if (fault != kFaultNone) {
+            if (lane == 0) record_fault(&g_q8_copy_fault, fault);
+            live = false;
+        }
+        held = page * a.block_size < first;
+    }
+    // ---- the page's rows: i-th is row part*16 + 2 i + lane/16 ----
+    const int64_t base = (((int64_t)pid * a.lanes + col_lane) * a.block_size + part * 16 + (lane >> 4)) * 16 + chunk;
+    uint2 *cell = a.pools[kv] + base;
+    float *sp = a.scales[kv] + (int64_t)pid * a.kv_heads + head;
+    const int32_t pos0 = page * a.block_size + part * 16 + (lane >> 4);
+    uint4 *row = a.rows[kv] + ((int64_t)row0 + (pos0 - first)) * a.row_vecs + col_lane * 16 + chunk;
+
+    if constexpr (!WRITE) {
+        if (!live) return;
+        const float s = __ldg(sp);
+        uint2 q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            q[i] = pos0 + 2 * i < end ? __ldg(cell + i * 32) : make_uint2(0, 0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (pos0 + 2 * i >= end) continue;
+            float lo[4], hi[4];
+            q8_unpack4(q[i].x, lo);
+            q8_unpack4(q[i].y, hi);
+            T o[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                o[k] = from_f32<T>(lo[k] * s);
+                o[4 + k] = from_f32<T>(hi[k] * s);
+            }
+            row[(int64_t)i * 2 * a.row_vecs] = *reinterpret_cast<uint4 *>(o);
+        }
+        return;
+    }
+
+    uint4 x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int32_t p = pos0 + 2 * i;
+        x[i] = live && p >= first && p < end ? __ldg(row + (int64_t)i * 2 * a.row_vecs)
+                                             : make_uint4(0, 0, 0, 0);
+    }
+    float m = 0.f;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        float f[8];
+        unpack8<T>(x[i], f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float v = fabsf(f[k]);
+            if (v < INFINITY) m = fmaxf(m, v);
+            else odd = true;  // NaN or infinity
+        }
+    }
+    if (odd) record_fault(&g_q8_copy_fault, kFaultNotFinite);
+    // head_dim 64: lanes 0-7 and 16-23 hold one head, the others the second
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+    if (HD == 128) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    if (per > 1) {
+        if ((lane & 15) == (HD == 64 ? hl * 8 : 0) && lane < 16) top[warp][hl] = m;
+        __syncthreads();
+        const int w0 = warp - part;
+        for (int w = 0; w < per; ++w) m = fmaxf(m, top[w0 + w][hl]);
+    }
+    // every thread of the unit reads the old scale before one of them stores
+    // the new one
+    const float s_old = live && held ? *sp : 0.f;
+    __syncthreads();
+    if (!live) return;
+    float s = fmaxf(s_old, __fdiv_rn(m, 127.f));
+    if (s < kQ8MinScale) s = 0.f;
+    const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+    if (part == 0 && lane < 16 && (lane & (HD == 64 ? 7 : 15)) == 0) *sp = s;
+    const bool rescale = held && s > s_old;
+    const float ratio = s > 0.f ? __fdiv_rn(s_old, s) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int32_t p = pos0 + 2 * i;
+        int lo[4], hi[4];
+        if (p >= first) {
+            if (p >= end) continue;
+            float f[8];
+            unpack8<T>(x[i], f);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                // an infinity times a zero inverse (all others zero) is not a number
+                lo[k] = q8_round(fabsf(f[k]) == INFINITY ? copysignf(127.f, f[k]) : f[k] * inv);
+                hi[k] = q8_round(fabsf(f[4 + k]) == INFINITY ? copysignf(127.f, f[4 + k])
+                                                             : f[4 + k] * inv);
+            }
+        } else {
+            if (!rescale) continue;
+            const uint2 q = cell[i * 32];
+            float g[4], h[4];
+            q8_unpack4(q.x, g);
+            q8_unpack4(q.y, h);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                lo[k] = q8_round(g[k] * ratio);
+                hi[k] = q8_round(h[k] * ratio);
+            }
+        }
+        cell[i * 32] = make_uint2(q8_pack4(lo), q8_pack4(hi));
+    }
+}
+
+template <typename T, int HD, bool WRITE>
+cudaError_t launch_q8(const Q8RowArgs &a, cudaStream_t s) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    const int per_cta = kQ8Warps / (a.block_size / 16);
+    cfg.gridDim = dim3((unsigned)((a.units + per_cta - 1) / per_cta), (unsigned)(a.lanes * 2));
+    cfg.blockDim = dim3(kQ8Warps * 32);
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, q8_rows_kernel<T, HD, WRITE>, a);
+}
+
+template <bool WRITE>
+int q8_rows(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *offsets,
+            const void *krows, const void *vrows, size_t total_rows, bool tail, PkvStream stream,
+            char *error, size_t cap, const char *what) {
+    if (!q8_check(layer, batch, error, cap, what)) return 0;
+    if (krows == nullptr || vrows == nullptr) {
+        pkv_internal_set_error(error, cap, "%s: null rows", what);
+        return 0;
+    }
+    if (((uintptr_t)krows | (uintptr_t)vrows) % 16 != 0) {
+        pkv_internal_set_error(error, cap, "%s: rows must be 16-byte aligned", what);
+        return 0;
+    }
+    if (offsets == nullptr && total_rows != batch->batch) {
+        pkv_internal_set_error(error, cap, "%s: one row per sequence needs total_rows == batch",
+                               what);
+        return 0;
+    }
+    if (total_rows > INT32_MAX / 4) {
+        pkv_internal_set_error(error, cap, "%s: too many rows", what);
+        return 0;
+    }
+    if (total_rows == 0) return 1;
+    Q8RowArgs a;
+    a.pools[0] = static_cast<uint2 *>(static_cast<void *>(layer->key_pool));
+    a.pools[1] = static_cast<uint2 *>(static_cast<void *>(layer->value_pool));
+    a.scales[0] = layer->key_scales;
+    a.scales[1] = layer->value_scales;
+    a.rows[0] = static_cast<uint4 *>(const_cast<void *>(krows));
+    a.rows[1] = static_cast<uint4 *>(const_cast<void *>(vrows));
+    a.tables = batch->block_tables;
+    a.seq_lens = batch->seq_lens;
+    a.offsets = offsets;
+    a.table_stride = (int32_t)batch->table_stride;
+    a.batch = (int32_t)batch->batch;
+    a.kv_heads = (int32_t)layer->kv_heads;
+    a.lanes = (int32_t)q8_lanes(layer->kv_heads, layer->head_dim);
+    a.block_size = (int32_t)layer->block_size;
+    a.block_count = (uint32_t)layer->block_count;
+    a.units = offsets == nullptr
+                  ? (int32_t)batch->batch
+                  : (int32_t)(total_rows / layer->block_size + 2 * batch->batch);
+    a.row_vecs = (int32_t)(layer->kv_heads * layer->head_dim / 8);
+    a.tail = tail ? 1 : 0;
+    const cudaStream_t s = (cudaStream_t)stream;
+    cudaError_t st;
+    if (layer->dtype == PKV_DTYPE_F16)
+        st = layer->head_dim == 128 ? launch_q8<__half, 128, WRITE>(a, s)
+                                    : launch_q8<__half, 64, WRITE>(a, s);
+    else
+        st = layer->head_dim == 128 ? launch_q8<__nv_bfloat16, 128, WRITE>(a, s)
+                                    : launch_q8<__nv_bfloat16, 64, WRITE>(a, s);
+    if (st == cudaSuccess) st = cudaGetLastError();
+    if (st != cudaSuccess) {
+        pkv_internal_set_error(error, cap, "%s: launch failed: %s", what, cudaGetErrorString(st));
+        return 0;
+    }
+    return 1;
+}
+
+}  // namespace
+}  // namespace pkv
+
+extern "C" {
+
+int pkv_q8_append(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *row_offsets,
+                  const void *key_rows, const void *value_rows, size_t total_rows,
+                  PkvStream stream, char *error, size_t error_capacity) {
+    PKV_RANGE("pkv_q8_append");
+    return pkv::q8_rows<true>(layer, batch, row_offsets, key_rows, value_rows, total_rows, true,
+                              stream, error, error_capacity, "pkv_q8_append");
+}
+
+int pkv_q8_import(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *row_offsets,
+                  const void *key_rows, const void *value_rows, size_t total_rows,
+                  PkvStream stream, char *error, size_t error_capacity) {
+    PKV_RANGE("pkv_q8_import");
+    return pkv::q8_rows<true>(layer, batch, row_offsets, key_rows, value_rows, total_rows, false,
+                              stream, error, error_capacity, "pkv_q8_import");
+}
+
+int pkv_q8_gather(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *row_offsets,
+                  void *key_out, void *value_out, size_t total_rows, PkvStream stream, char *error,
+                  size_t error_capacity) {
+    PKV_RANGE("pkv_q8_gather");
+    return pkv::q8_rows<false>(layer, batch, row_offsets, key_out, value_out, total_rows, false,
+                               stream, error, error_capacity, "pkv_q8_gather");
+}
+
+int pkv_internal_take_q8_copy_fault(uint32_t *code) {
+    uint32_t zero = 0;
+    if (cudaMemcpyFromSymbol(code, pkv::g_q8_copy_fault, sizeof(uint32_t)) != cudaSuccess) return 0;
+    return cudaMemcpyToSymbol(pkv::g_q8_copy_fault, &zero, sizeof(uint32_t)) == cudaSuccess;
+}
+
+}  // extern "C"

@@ -1,0 +1,179 @@
+"""8-bit pages on the GPU: rows written, rescaled and read back bit for bit
+against the header's rule, and decode attention against 64 bits, over head
+layouts, page sizes, types and lengths from none to several pages."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import inference_c_b200 as P
+from inference_c_b200 import workloads as W
+from tests.gpu_cases import to_device_bits, to_host_bits, torch_dtype
+from tests.q8_cases import Q8Case, attend64, attend_tol, widen
+
+pytestmark = pytest.mark.gpu
+
+SHAPES = [  # kv_heads, head_dim, block_size, dtype
+    (8, 128, 16, "f16"), (8, 128, 16, "bf16"), (2, 128, 32, "bf16"), (1, 128, 64, "f16"),
+    (3, 128, 128, "f16"), (8, 64, 16, "f16"), (3, 64, 16, "bf16"), (1, 64, 128, "f16"),
+    (4, 64, 32, "bf16"), (5, 64, 64, "f16"),
+]
+
+
+def _rows(seed, n, kv_heads, hd, dtype, stream, amp=None):
+    x = W.normal(seed, n * kv_heads * hd, stream=stream).reshape(n, kv_heads * hd)
+    if amp is not None:
+        x = x * amp[:, None].astype(np.float32)
+    return W.storage_bits(x, dtype)
+
+
+def _append(case, new, seed, device, dtype, one_row=False, amp=None):
+    """Appends new[b] rows behind every sequence's current length minus
+    new[b] (the lengths already count them), on both sides."""
+    import torch
+    offs = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    kb, vb = (_rows(seed, int(offs[-1]), case.kv_heads, case.hd, dtype, s, amp) for s in (61, 62))
+    P.q8_append(case.layer(), case.batch(), to_device_bits(kb, dtype, device),
+                to_device_bits(vb, dtype, device),
+                None if one_row else torch.from_numpy(offs).to(device))
+    for pool, bits in ((case.k, kb), (case.v, vb)):
+        x = widen(bits, dtype).reshape(-1, case.kv_heads, case.hd)
+        for b, L in enumerate(case.lengths):
+            pool.write(case.tables[b], int(L) - int(new[b]), x[offs[b]:offs[b + 1]])
+
+
+@pytest.mark.parametrize("kv_heads,hd,bs,dtype", SHAPES)
+def test_append_rescale_import_gather(lib, cuda, kv_heads, hd, bs, dtype):
+    import torch
+    lengths = np.array([0, 1, 2, bs - 1, bs, bs + 1, 3 * bs + 5, 150])
+    case = Q8Case(lengths, kv_heads, kv_heads, hd, bs, dtype, seed=7, device=cuda)
+    # the last rows again: none, one, some of a page, over a page's end, all
+    new = np.minimum(lengths, np.array([0, 1, 1, 3, bs, bs + 1, bs + 2, 99]))
+    amp = 1.0 + 3.0 * W.uniform(9, int(new.sum()))
+    _append(case, new, 11, cuda, dtype, amp=amp)
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 0
+    case.same_pages()
+    # one row for every sequence that has room for it
+    some = lengths > 0
+    case.lengths, case.tables = lengths[some], case.tables[some]
+    case.d_tables = torch.from_numpy(np.ascontiguousarray(case.tables).view(np.int32)).to(cuda)
+    case.d_lens = torch.from_numpy(case.lengths.astype(np.int32)).to(cuda)
+    n = len(case.lengths)
+    _append(case, np.ones(n, np.int64), 13, cuda, dtype, one_row=True, amp=np.full(n, 9.0))
+    torch.cuda.synchronize()
+    case.same_pages()
+    # gather: q * s rounded to the row type
+    offs = np.concatenate([[0], np.cumsum(case.lengths)]).astype(np.int32)
+    kvw = kv_heads * hd
+    outs = [torch.full((int(offs[-1]), kvw), float("nan"), dtype=torch_dtype(dtype), device=cuda)
+            for _ in range(2)]
+    P.q8_gather(case.layer(), case.batch(), *outs, torch.from_numpy(offs).to(cuda))
+    torch.cuda.synchronize()
+    for pool, out in ((case.k, outs[0]), (case.v, outs[1])):
+        want = np.concatenate([pool.read(case.tables[b], int(L)).reshape(-1, kvw)
+                               for b, L in enumerate(case.lengths)])
+        assert np.array_equal(to_host_bits(out), W.storage_bits(want, dtype))
+    case.same_pages()
+    assert P.device_fault(0) == 0
+
+
+@pytest.mark.parametrize("kv_heads,hd,bs,dtype", SHAPES[::3])
+def test_import_equals_write_at_zero(lib, cuda, kv_heads, hd, bs, dtype):
+    import torch
+    lengths = np.array([bs, 0, 1, 5 * bs + 3, 40])
+    case = Q8Case(lengths, kv_heads, kv_heads, hd, bs, dtype, seed=21, device=cuda)
+    offs = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32)
+    kb, vb = (_rows(23, int(offs[-1]), kv_heads, hd, dtype, s) for s in (4, 5))
+    P.q8_import(case.layer(), case.batch(), to_device_bits(kb, dtype, cuda),
+                to_device_bits(vb, dtype, cuda), torch.from_numpy(offs).to(cuda))
+    torch.cuda.synchronize()
+    for pool, bits in ((case.k, kb), (case.v, vb)):
+        x = widen(bits, dtype).reshape(-1, kv_heads, hd)
+        for b in range(len(lengths)):
+            pool.write(case.tables[b], 0, x[offs[b]:offs[b + 1]])
+    case.same_pages()
+    assert P.device_fault(0) == 0
+
+
+def test_extreme_values(lib, cuda):
+    """Zeros, the smallest and largest numbers, infinities and NaN."""
+    import torch
+    for dtype, tiny, huge in (("bf16", 1e-39, 3e38), ("f16", 6e-8, 65504.0)):
+        case = Q8Case([16, 16, 16, 16, 16], 1, 1, 128, 16, dtype, seed=5, device=cuda)
+        x = np.zeros((80, 128), np.float32)
+        x[16:32] = tiny                       # bf16: a subnormal, its scale underflows
+        x[32:48] = huge
+        x[48:64] = W.normal(3, 16 * 128).reshape(16, 128)
+        x[50, 3], x[51, 4], x[52, 5] = np.inf, -np.inf, np.nan
+        x[64, :2] = np.inf, np.nan            # nothing finite but zeros
+        bits = W.storage_bits(x, dtype)
+        d = to_device_bits(bits, dtype, cuda)
+        offs = torch.arange(0, 81, 16, dtype=torch.int32, device=cuda)
+        P.q8_import(case.layer(), case.batch(), d, d, offs)
+        torch.cuda.synchronize()
+        assert P.device_fault(0) == 5 and P.device_fault(0) == 0
+        y = widen(bits, dtype).reshape(80, 1, 128)
+        for pool in (case.k, case.v):
+            for b in range(5):
+                pool.write(case.tables[b], 0, y[16 * b:16 * b + 16])
+        case.same_pages()
+
+
+def test_bad_pages_and_lengths_are_reported(lib, cuda):
+    import torch
+    case = Q8Case([20, 20], 2, 2, 64, 16, "f16", seed=3, device=cuda)
+    before = case.d_kq.clone()
+    bad = case.d_tables.clone()
+    bad[:, 1] = case.d_kq.shape[0] + 5
+    rows = torch.zeros(2, 128, dtype=torch.float16, device=cuda)
+    P.q8_append(case.layer(), P.make_batch(bad, case.d_lens), rows, rows)
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 1
+    lens = torch.zeros(2, dtype=torch.int32, device=cuda)  # no room for a row
+    P.q8_append(case.layer(), P.make_batch(case.d_tables, lens), rows, rows)
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 3
+    lens += 40  # past the table
+    P.q8_append(case.layer(), P.make_batch(case.d_tables, lens), rows, rows)
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 2
+    assert torch.equal(case.d_kq, before)
+
+
+def check_decode(case, got, out_eps, what=""):
+    q = widen(case.qbits, case.dtype).astype(np.float64)
+    for b, L in enumerate(case.lengths):
+        L = int(L)
+        k, v = case.k.read64(case.tables[b], L), case.v.read64(case.tables[b], L)
+        want, _, worst = attend64(q[b:b + 1], k, v, case.scale)
+        vmax = float(np.abs(v).max()) if L else 0.0
+        tol = attend_tol(worst, case.hd, vmax, want, out_eps)
+        diff = np.abs(got[b] - want[0])
+        assert np.all(diff <= tol[0]), (what, b, L, float(diff.max()), float(tol.min()))
+
+
+DECODE = [  # q_heads, kv_heads, head_dim, block_size, dtype, out
+    (32, 8, 128, 16, "f16", "f32"), (32, 8, 128, 16, "bf16", "bf16"),
+    (8, 8, 64, 16, "f16", "f32"), (8, 8, 64, 16, "f16", "f16"),
+    (16, 1, 128, 64, "bf16", "f32"), (7, 1, 128, 32, "f16", "f32"),
+    (15, 3, 64, 16, "bf16", "f32"), (14, 2, 64, 128, "f16", "f32"),
+    (48, 3, 64, 32, "f16", "f32"), (6, 2, 128, 128, "bf16", "f32"), (1, 1, 64, 16, "bf16", "f32"),
+    (24, 8, 128, 16, "f16", "f32"), (16, 2, 128, 16, "bf16", "f32"), (33, 3, 128, 16, "f16", "f32"),
+]
+LENGTHS = [0, 1, 2, 15, 16, 17, 127, 128, 129, 255, 257, 700, 1031]
+
+
+@pytest.mark.parametrize("q_heads,kv_heads,hd,bs,dtype,out", DECODE)
+def test_decode(lib, cuda, q_heads, kv_heads, hd, bs, dtype, out):
+    import torch
+    case = Q8Case(LENGTHS, q_heads, kv_heads, hd, bs, dtype, seed=31, device=cuda)
+    od = torch.float32 if out == "f32" else torch_dtype(out)
+    ws = P.q8_decode_workspace(len(LENGTHS), q_heads, kv_heads, hd, max(LENGTHS))
+    for _ in range(2):  # the scratch serves the next call as it was left
+        got = torch.full((len(LENGTHS), q_heads, hd), float("nan"), dtype=od, device=cuda)
+        P.q8_decode(case.layer(), case.batch(), case.d_q, got, case.scale, max(LENGTHS), ws)
+        torch.cuda.synchronize()
+        assert P.device_fault(0) == 0
+        check_decode(case, got.double().cpu().numpy(), 0 if out == "f32" else torch.finfo(od).eps)
+    case.same_pages()

@@ -1,0 +1,85 @@
+"""Refusals of the 8-bit page entry points: a 0 result and a message before
+any device work (no GPU needed)."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+import inference_c_b200 as P
+
+
+def _layer(**kw):
+    a = dict(key_pool=256, value_pool=256, key_scales=256, value_scales=256, block_size=16,
+             block_count=4, kv_heads=2, head_dim=128, dtype=P.PKV_DTYPE_F16)
+    a.update(kw)
+    return P.PkvQ8Layer(*[a[n] for n, _ in P.PkvQ8Layer._fields_])
+
+
+def _batch(**kw):
+    a = dict(block_tables=256, table_stride=4, seq_lens=256, batch=2)
+    a.update(kw)
+    return P.PkvBatch(*[a[n] for n, _ in P.PkvBatch._fields_])
+
+
+BAD = [
+    (dict(key_pool=None), {}, "null"), (dict(value_scales=None), {}, "null"),
+    ({}, dict(block_tables=None), "null"), ({}, dict(seq_lens=None), "null"),
+    (dict(dtype=P.PKV_DTYPE_F32), {}, "dtype"), (dict(dtype=9), {}, "dtype"),
+    (dict(block_size=8), {}, "16, 32, 64 or 128"), (dict(block_size=24), {}, "16, 32, 64 or 128"),
+    (dict(head_dim=96), {}, "head_dim 64 or 128"), (dict(kv_heads=0), {}, "KV heads"),
+    (dict(kv_heads=1025), {}, "KV heads"), (dict(block_count=0), {}, "block count"),
+    ({}, dict(batch=0), "batch"), ({}, dict(table_stride=0), "stride"),
+    ({}, dict(table_stride=1 << 31), "stride"), (dict(key_pool=264), {}, "16-byte aligned"),
+    (dict(key_scales=258), {}, "4-byte aligned"),
+]
+
+
+def _err():
+    return ctypes.create_string_buffer(256)
+
+
+@pytest.mark.parametrize("layer,batch,text", BAD)
+def test_layer_and_batch_are_checked(lib, layer, batch, text):
+    L, B = _layer(**layer), _batch(**batch)
+    for name in ("pkv_q8_append", "pkv_q8_import", "pkv_q8_gather"):
+        e = _err()
+        assert getattr(lib, name)(ctypes.byref(L), ctypes.byref(B), 256, 256, 256, 2, None, e,
+                                  len(e)) == 0
+        assert text in e.value.decode() and name in e.value.decode()
+    e = _err()
+    assert lib.pkv_q8_decode(ctypes.byref(L), ctypes.byref(B), 4, 256, ctypes.c_float(1), 256,
+                             P.PKV_DTYPE_F32, 64, 256, 1 << 30, None, e, len(e)) == 0
+    assert text in e.value.decode() and "pkv_q8_decode" in e.value.decode()
+
+
+def test_rows_are_checked(lib):
+    L, B = _layer(), _batch()
+    for args, text in (((256, None, 256, 2), "null"), ((256, 256, 264, 2), "aligned"),
+                       ((None, 256, 256, 3), "total_rows"), ((256, 256, 256, 1 << 30), "rows")):
+        e = _err()
+        assert lib.pkv_q8_append(ctypes.byref(L), ctypes.byref(B), *args, None, e, len(e)) == 0
+        assert text in e.value.decode()
+    e = _err()
+    assert lib.pkv_q8_append(None, ctypes.byref(B), 256, 256, 256, 2, None, e, len(e)) == 0
+    assert lib.pkv_q8_append(ctypes.byref(L), None, 256, 256, 256, 2, None, e, len(e)) == 0
+    # no rows: nothing to do, no device touched
+    assert lib.pkv_q8_append(ctypes.byref(L), ctypes.byref(B), 256, 256, 256, 0, None, e, len(e)) == 1
+
+
+def _decode(lib, L, B, q_heads=4, query=256, scale=1.0, out=256, dtype=P.PKV_DTYPE_F32, max_len=64,
+            ws=256, ws_bytes=1 << 30):
+    e = _err()
+    ok = lib.pkv_q8_decode(ctypes.byref(L), ctypes.byref(B), q_heads, query, ctypes.c_float(scale),
+                           out, dtype, max_len, ws, ws_bytes, None, e, len(e))
+    return ok, e.value.decode()
+
+
+def test_decode_arguments_are_checked(lib):
+    L, B = _layer(), _batch()
+    for kw, text in ((dict(query=None), "null"), (dict(out=None), "null"),
+                     (dict(dtype=P.PKV_DTYPE_BF16), "output dtype"), (dict(dtype=0), "output dtype"),
+                     (dict(q_heads=3), "times kv_heads"), (dict(q_heads=0), "times kv_heads"),
+                     (dict(q_heads=34), "times kv_heads")):
+        ok, text_got = _decode(lib, L, B, **kw)
+        assert ok == 0 and text in text_got, (kw, text_got)
