@@ -32,6 +32,18 @@ __device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t *bar, uint32_t by
                  "r"(bytes)
                  : "memory");
 }
+// Arrives on `bar` when this thread's earlier cp.async copies have landed; the
+// arrival is one of the barrier's expected count.
+__device__ __forceinline__ void cp_async_mbar_arrive(uint64_t *bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+// 4-byte asynchronous copy to shared memory; zero without reading when !read.
+__device__ __forceinline__ void cp_async4_or_zero(void *smem, const void *gmem, bool read) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(smem_u32(smem)),
+                 "l"(gmem), "r"(read ? 4u : 0u)
+                 : "memory");
+}
 __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
@@ -176,6 +188,16 @@ __device__ __forceinline__ void mma_f16_ts_at(uint32_t d_tmem, uint32_t a_tmem, 
         "r"(a_tmem), "l"(b_base), "r"(idesc), "r"(accumulate), "n"(ACOL), "n"(BOFF)
         : "memory");
 }
+// D[tmem] (+)= A[smem] * B[smem], kind::i8 (8-bit integers, exact 32-bit sums).
+__device__ __forceinline__ void mma_i8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                          uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
 // Arrive on `bar` once every tcgen05 operation issued so far by this thread
 // has completed.
 __device__ __forceinline__ void mma_commit(uint64_t *bar) {
@@ -305,6 +327,13 @@ __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool bf16, bool a
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) |
            ((a_mn_major ? 1u : 0u) << 15) | ((b_mn_major ? 1u : 0u) << 16) |
            ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+// Instruction descriptor of tcgen05.mma kind::i8: signed A and B, S32 sums.
+__host__ __device__ constexpr uint32_t idesc_s8(int m, int n, bool a_mn_major, bool b_mn_major) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((a_mn_major ? 1u : 0u) << 15) |
+           ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+           ((uint32_t)(m >> 4) << 24);
 }
 
 // Byte offset of element (row, col) in a K-major 128B-swizzled tile whose
