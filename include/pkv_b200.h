@@ -263,6 +263,21 @@ int pkv_q8_decode(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads
                   size_t max_seq_len, void *workspace, size_t workspace_bytes, PkvStream stream,
                   char *error, size_t error_capacity);
 
+/* pkv_paged_prefill over 8-bit pages; max_seq_len bounds seq_lens (fault
+ * code 2 and no keys for a longer sequence).  The pages are widened to
+ * layer->dtype (q * s, one rounding) in the workspace first, so scores and
+ * outputs are those of a 16-bit cache of the gathered rows.  The byte count is
+ * for the whole batch; a smaller workspace that holds at least one sequence
+ * (the count for batch 1) also works and runs the batch in parts. */
+size_t pkv_q8_prefill_workspace_bytes(size_t batch, size_t kv_heads, size_t head_dim,
+                                      size_t max_seq_len);
+int pkv_q8_prefill(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads,
+                   const int32_t *query_offsets, const void *query, size_t total_query_rows,
+                   size_t max_query_len, float scale, int causal, void *output,
+                   PkvDType output_dtype, size_t max_seq_len, void *workspace,
+                   size_t workspace_bytes, PkvStream stream, char *error,
+                   size_t error_capacity);
+
 /* Reads and clears the device fault word of `device` (synchronises it).
  * Kernels never trap: an out-of-range page id or position skips the access
  * and records a code here.  *code == 0 means no fault was recorded. */

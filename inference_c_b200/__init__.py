@@ -165,6 +165,10 @@ EXPORTS = {
     "pkv_q8_decode_workspace_bytes": (_c_size, [_c_size] * 5),
     "pkv_q8_decode": (_c_int, [_QP, _BP, _c_size, _c_ptr, ctypes.c_float, _c_ptr, _c_int, _c_size,
                                _c_ptr, _c_size, _c_ptr, *_ERR]),
+    "pkv_q8_prefill_workspace_bytes": (_c_size, [_c_size] * 4),
+    "pkv_q8_prefill": (_c_int, [_QP, _BP, _c_size, _c_ptr, _c_ptr, _c_size, _c_size,
+                                ctypes.c_float, _c_int, _c_ptr, _c_int, _c_size, _c_ptr, _c_size,
+                                _c_ptr, *_ERR]),
     "pkv_device_fault": (_c_int, [_c_int, ctypes.POINTER(ctypes.c_uint32), *_ERR]),
     "pkv_selftest_wait_timeout": (_c_int, [ctypes.POINTER(ctypes.c_uint32), *_ERR]),
     "pkv_sdpa_workspace_bytes": (_c_size, [_c_size, _c_size, _c_size, _c_size, _c_size]),
@@ -484,6 +488,22 @@ def q8_decode(layer: PkvQ8Layer, batch: PkvBatch, query, output, scale: float, m
     _call("pkv_q8_decode", ctypes.byref(layer), ctypes.byref(batch), query.shape[-2],
           query.data_ptr(), ctypes.c_float(scale), output.data_ptr(), _dtype_code(output),
           max_seq_len, workspace.data_ptr(), workspace.numel(), _stream_ptr(stream))
+
+
+def q8_prefill_workspace(layer: PkvQ8Layer, batch: int, max_seq_len: int, device=None):
+    """Scratch of q8_prefill (needs no clearing) as a uint8 CUDA tensor."""
+    import torch
+    n = load().pkv_q8_prefill_workspace_bytes(batch, layer.kv_heads, layer.head_dim, max_seq_len)
+    return torch.empty(n, dtype=torch.uint8, device=device or "cuda")
+
+
+def q8_prefill(layer: PkvQ8Layer, batch: PkvBatch, query, query_offsets, output, scale: float,
+               max_query_len: int, max_seq_len: int, workspace, causal: bool = True,
+               stream=None) -> None:
+    _call("pkv_q8_prefill", ctypes.byref(layer), ctypes.byref(batch), query.shape[-2],
+          _ptr(query_offsets), query.data_ptr(), query.shape[0], max_query_len,
+          ctypes.c_float(scale), int(causal), output.data_ptr(), _dtype_code(output), max_seq_len,
+          workspace.data_ptr(), workspace.numel(), _stream_ptr(stream))
 
 
 def device_fault(device: int = 0) -> int:

@@ -11,7 +11,14 @@
 // tokens are rescaled, q' = rint(q * (s_old / s)), by the threads that own
 // those rows.  Bound by HBM: 2 bytes read and 1 written a value (gather the
 // reverse).
-#include <stdio.h>
+//
+// Prefill expands the batch's pages to 16-bit rows in its workspace, once, and
+// runs the paged prefill kernel on them: a chunk's pages are read by every
+// 128-row query tile and head pair, so widening them inside the attention
+// kernel would repeat each conversion that many times, while the expansion is
+// one pass of 3 bytes a value.  K and V are rounded to the row type there, as
+// a 16-bit cache holds them.
+#include <math.h>
 
 #include "pkv_q8.cuh"
 #include "pkv_trace.h"
@@ -35,6 +42,10 @@ struct Q8RowArgs {
     int32_t units;            // upper bound of pages touched
     int32_t row_vecs;         // uint4 per contiguous row
     int32_t tail;             // rows are the sequence's last (append) or first positions
+    // > 0: every sequence's first seq_lens[b] rows go to rows b * pad_rows on,
+    // and table_out gets the identity table of those rows in pages of 128
+    int32_t pad_rows;
+    uint32_t *table_out;
 };
 
 struct Q8Unit {
@@ -75,7 +86,21 @@ q8_rows_kernel(const Q8RowArgs a) {
     uint32_t pid = 0;
     if (unit_live) {
         int32_t count = 1, slot = 0;
-        if (a.offsets == nullptr) {
+        if (!WRITE && a.pad_rows > 0) {
+            const int per_seq = a.pad_rows / a.block_size;
+            b = u / per_seq;
+            slot = u - b * per_seq;
+            row0 = b * a.pad_rows;
+            count = max(0, __ldg(a.seq_lens + b));
+            if (blockIdx.y == 0 && part == 0 && lane == 0 && slot * a.block_size % 128 == 0) {
+                const int at = (row0 + slot * a.block_size) / 128;
+                a.table_out[at] = (uint32_t)at;
+            }
+            if (count > a.pad_rows) {  // longer than the caller's bound
+                if (lane == 0) record_fault(&g_q8_copy_fault, kFaultPositionOutOfRange);
+                count = 0;
+            }
+        } else if (a.offsets == nullptr) {
             b = u;
             row0 = u;
         } else {
@@ -89,7 +114,7 @@ q8_rows_kernel(const Q8RowArgs a) {
             count = __ldg(a.offsets + b + 1) - row0;
             slot = u - q8_first_unit(a, b);
         }
-        const int32_t L = __ldg(a.seq_lens + b);
+        const int32_t L = !WRITE && a.pad_rows > 0 ? count : __ldg(a.seq_lens + b);
         uint32_t fault = kFaultNone;
         first = a.tail ? L - count : 0;
         end = first + count;
@@ -232,8 +257,8 @@ cudaError_t launch_q8(const Q8RowArgs &a, cudaStream_t s) {
 
 template <bool WRITE>
 int q8_rows(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *offsets,
-            const void *krows, const void *vrows, size_t total_rows, bool tail, PkvStream stream,
-            char *error, size_t cap, const char *what) {
+            const void *krows, const void *vrows, size_t total_rows, bool tail, size_t pad_rows,
+            uint32_t *table_out, PkvStream stream, char *error, size_t cap, const char *what) {
     if (!q8_check(layer, batch, error, cap, what)) return 0;
     if (krows == nullptr || vrows == nullptr) {
         pkv_internal_set_error(error, cap, "%s: null rows", what);
@@ -243,7 +268,7 @@ int q8_rows(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *offse
         pkv_internal_set_error(error, cap, "%s: rows must be 16-byte aligned", what);
         return 0;
     }
-    if (offsets == nullptr && total_rows != batch->batch) {
+    if (offsets == nullptr && pad_rows == 0 && total_rows != batch->batch) {
         pkv_internal_set_error(error, cap, "%s: one row per sequence needs total_rows == batch",
                                what);
         return 0;
@@ -274,6 +299,9 @@ int q8_rows(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *offse
                   : (int32_t)(total_rows / layer->block_size + 2 * batch->batch);
     a.row_vecs = (int32_t)(layer->kv_heads * layer->head_dim / 8);
     a.tail = tail ? 1 : 0;
+    a.pad_rows = (int32_t)pad_rows;
+    a.table_out = table_out;
+    if (pad_rows > 0) a.units = (int32_t)(total_rows / layer->block_size);
     const cudaStream_t s = (cudaStream_t)stream;
     cudaError_t st;
     if (layer->dtype == PKV_DTYPE_F16)
@@ -290,6 +318,23 @@ int q8_rows(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *offse
     return 1;
 }
 
+// Scratch of the prefill: 16-bit rows of every sequence, padded to whole pages
+// of 128, and their identity table.
+struct PrefillSpace {
+    size_t pad, k, v, table, total;
+};
+
+PrefillSpace prefill_space(size_t batch, size_t kv_heads, size_t head_dim, size_t max_seq_len) {
+    PrefillSpace w;
+    w.pad = (max_seq_len + 127) / 128 * 128;
+    const size_t bytes = batch * w.pad * kv_heads * head_dim * 2;  // a multiple of 256
+    w.k = 0;
+    w.v = bytes;
+    w.table = 2 * bytes;
+    w.total = w.table + (batch * (w.pad / 128) * 4 + 255) / 256 * 256;
+    return w;
+}
+
 }  // namespace
 }  // namespace pkv
 
@@ -300,7 +345,7 @@ int pkv_q8_append(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t 
                   PkvStream stream, char *error, size_t error_capacity) {
     PKV_RANGE("pkv_q8_append");
     return pkv::q8_rows<true>(layer, batch, row_offsets, key_rows, value_rows, total_rows, true,
-                              stream, error, error_capacity, "pkv_q8_append");
+                              0, nullptr, stream, error, error_capacity, "pkv_q8_append");
 }
 
 int pkv_q8_import(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *row_offsets,
@@ -308,7 +353,7 @@ int pkv_q8_import(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t 
                   PkvStream stream, char *error, size_t error_capacity) {
     PKV_RANGE("pkv_q8_import");
     return pkv::q8_rows<true>(layer, batch, row_offsets, key_rows, value_rows, total_rows, false,
-                              stream, error, error_capacity, "pkv_q8_import");
+                              0, nullptr, stream, error, error_capacity, "pkv_q8_import");
 }
 
 int pkv_q8_gather(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *row_offsets,
@@ -316,7 +361,91 @@ int pkv_q8_gather(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t 
                   size_t error_capacity) {
     PKV_RANGE("pkv_q8_gather");
     return pkv::q8_rows<false>(layer, batch, row_offsets, key_out, value_out, total_rows, false,
-                               stream, error, error_capacity, "pkv_q8_gather");
+                               0, nullptr, stream, error, error_capacity, "pkv_q8_gather");
+}
+
+size_t pkv_q8_prefill_workspace_bytes(size_t batch, size_t kv_heads, size_t head_dim,
+                                      size_t max_seq_len) {
+    return pkv::prefill_space(batch, kv_heads, head_dim, max_seq_len).total;
+}
+
+int pkv_q8_prefill(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads,
+                   const int32_t *query_offsets, const void *query, size_t total_query_rows,
+                   size_t max_query_len, float scale, int causal, void *output,
+                   PkvDType output_dtype, size_t max_seq_len, void *workspace,
+                   size_t workspace_bytes, PkvStream stream, char *error,
+                   size_t error_capacity) {
+    PKV_RANGE("pkv_q8_prefill");
+    const char *what = "pkv_q8_prefill";
+    if (!pkv::q8_check(layer, batch, error, error_capacity, what)) return 0;
+    if (query_offsets == nullptr || query == nullptr || output == nullptr) {
+        pkv_internal_set_error(error, error_capacity, "%s: null argument", what);
+        return 0;
+    }
+    // what the prefill kernel would refuse, before the pages are widened
+    const size_t kvh = layer->kv_heads, hd = layer->head_dim;
+    if (output_dtype != PKV_DTYPE_F32 && output_dtype != layer->dtype) {
+        pkv_internal_set_error(error, error_capacity,
+                               "%s: output dtype must be F32 or the row dtype", what);
+        return 0;
+    }
+    if (q_heads == 0 || q_heads % kvh != 0 || q_heads > 65535 || (uintptr_t)query % 16 != 0) {
+        pkv_internal_set_error(error, error_capacity,
+                               "%s: q_heads must be a multiple of kv_heads, query 16-byte aligned",
+                               what);
+        return 0;
+    }
+    if (max_seq_len == 0 || max_seq_len > INT32_MAX / 4 || max_query_len > INT32_MAX ||
+        total_query_rows >= (size_t(1) << 31) || !isfinite(scale) ||
+        (causal != 0 && causal != 1)) {
+        pkv_internal_set_error(error, error_capacity,
+                               "%s: invalid max_seq_len, sizes, scale or causal", what);
+        return 0;
+    }
+    if (total_query_rows == 0) return 1;
+    const pkv::PrefillSpace one = pkv::prefill_space(1, kvh, hd, max_seq_len);
+    // as many sequences at a time as the workspace holds (rows below 2^31)
+    size_t most = workspace_bytes / one.total;
+    if (most > batch->batch) most = batch->batch;
+    if (most > (size_t)INT32_MAX / 4 / one.pad) most = (size_t)INT32_MAX / 4 / one.pad;
+    if (workspace == nullptr || most == 0 || (uintptr_t)workspace % 256 != 0) {
+        pkv_internal_set_error(error, error_capacity,
+                               "%s: workspace needs %zu bytes a sequence, 256-byte aligned "
+                               "(got %zu)",
+                               what, one.total, workspace_bytes);
+        return 0;
+    }
+    for (size_t b0 = 0; b0 < batch->batch; b0 += most) {
+        const size_t n = batch->batch - b0 < most ? batch->batch - b0 : most;
+        const pkv::PrefillSpace w = pkv::prefill_space(n, kvh, hd, max_seq_len);
+        auto *base = static_cast<unsigned char *>(workspace);
+        PkvBatch part = *batch;
+        part.block_tables += b0 * batch->table_stride;
+        part.seq_lens += b0;
+        part.batch = n;
+        auto *table = reinterpret_cast<uint32_t *>(base + w.table);
+        PkvPagedLayer wide;
+        wide.key_pool = base + w.k;
+        wide.value_pool = base + w.v;
+        wide.block_size = 128;
+        wide.block_count = n * w.pad / 128;
+        wide.kv_heads = kvh;
+        wide.head_dim = hd;
+        wide.dtype = layer->dtype;
+        PkvBatch rows;
+        rows.block_tables = table;
+        rows.table_stride = w.pad / 128;
+        rows.seq_lens = part.seq_lens;
+        rows.batch = n;
+        if (!pkv::q8_rows<false>(layer, &part, nullptr, wide.key_pool, wide.value_pool, n * w.pad,
+                                 false, w.pad, table, stream, error, error_capacity, what) ||
+            !pkv_internal_paged_prefill_ex(&wide, &rows, q_heads, query_offsets + b0, query,
+                                           total_query_rows, max_query_len, scale, causal, output,
+                                           output_dtype, nullptr, 0, 0, 0, stream, error,
+                                           error_capacity, what))
+            return 0;
+    }
+    return 1;
 }
 
 int pkv_internal_take_q8_copy_fault(uint32_t *code) {

@@ -177,3 +177,58 @@ def test_decode(lib, cuda, q_heads, kv_heads, hd, bs, dtype, out):
         assert P.device_fault(0) == 0
         check_decode(case, got.double().cpu().numpy(), 0 if out == "f32" else torch.finfo(od).eps)
     case.same_pages()
+
+
+@pytest.mark.parametrize("q_heads,kv_heads,hd,bs,dtype,out,causal", [
+    (8, 2, 128, 16, "bf16", "bf16", True), (14, 2, 64, 32, "f16", "f16", True),
+    (5, 1, 128, 128, "f16", "f32", False), (9, 3, 64, 16, "bf16", "f32", True),
+    (4, 4, 128, 64, "f16", "f32", True),
+])
+@pytest.mark.parametrize("parts", [False, True])
+def test_prefill(lib, cuda, q_heads, kv_heads, hd, bs, dtype, out, causal, parts):
+    """Chunks of none, one and many rows; the attention is that over the
+    gathered 16-bit rows, so the reference rounds K and V once."""
+    import torch
+    lengths = np.array([1, 129, 0, 300, 131, 17])
+    rows = np.array([1, 129, 0, 40, 0, 5])
+    case = Q8Case(lengths, q_heads, kv_heads, hd, bs, dtype, seed=51, device=cuda)
+    offs = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+    qbits = W.normal_bits(53, (int(offs[-1]), q_heads, hd), dtype, stream=9)
+    od = torch.float32 if out == "f32" else torch_dtype(out)
+    got = torch.full((int(offs[-1]), q_heads, hd), float("nan"), dtype=od, device=cuda)
+    full = P.q8_prefill_workspace(case.layer(), 1 if parts else len(lengths), 300)
+    full.fill_(255)  # NaN wherever nothing is written
+    P.q8_prefill(case.layer(), case.batch(), to_device_bits(qbits, dtype, cuda),
+                 torch.from_numpy(offs).to(cuda), got, case.scale, int(rows.max()), 300, full,
+                 causal=causal)
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 0
+    q = widen(qbits, dtype).astype(np.float64)
+    got = got.double().cpu().numpy()
+    for b, L in enumerate(lengths):
+        L, n = int(L), int(rows[b])
+        if n == 0:
+            continue
+        k, v = (widen(W.storage_bits(p.read(case.tables[b], L), dtype), dtype).astype(np.float64)
+                for p in (case.k, case.v))
+        limits = L - n + 1 + np.arange(n) if causal else np.full(n, L)
+        want, _, worst = attend64(q[offs[b]:offs[b + 1]], k, v, case.scale, limits)
+        # the 16-bit prefill keeps weights as two 16-bit halves: bf16 2^-16,
+        # fp16 2^-22 of a weight, down to fp16's smallest step 2^-25
+        halves = 2.0 ** -16 if dtype == "bf16" else 2.0 ** -21
+        vmax = float(np.abs(v).max())
+        tol = attend_tol(worst, hd, vmax, want, 0 if out == "f32" else torch.finfo(od).eps)
+        diff = np.abs(got[offs[b]:offs[b + 1]] - want)
+        assert np.all(diff <= tol + halves * vmax), (b, float(diff.max()))
+
+
+def test_prefill_longer_than_bound_is_reported(lib, cuda):
+    import torch
+    case = Q8Case([200, 20], 4, 2, 128, 16, "f16", seed=3, device=cuda)
+    offs = torch.tensor([0, 1, 2], dtype=torch.int32, device=cuda)
+    ws = P.q8_prefill_workspace(case.layer(), 2, 100)
+    out = torch.empty(2, 4, 128, dtype=torch.float16, device=cuda)
+    P.q8_prefill(case.layer(), case.batch(), case.d_q, offs, out, case.scale, 1, 100, ws)
+    torch.cuda.synchronize()
+    assert P.device_fault(0) != 0
+    assert P.device_fault(0) == 0

@@ -83,3 +83,25 @@ def test_decode_arguments_are_checked(lib):
                      (dict(q_heads=34), "times kv_heads")):
         ok, text_got = _decode(lib, L, B, **kw)
         assert ok == 0 and text in text_got, (kw, text_got)
+
+
+def test_prefill_arguments_are_checked(lib):
+    L, B = _layer(), _batch()
+    f = ctypes.c_float
+    n = lib.pkv_q8_prefill_workspace_bytes(1, 2, 128, 200)
+    assert n >= 2 * 256 * 256 * 2 and n < lib.pkv_q8_prefill_workspace_bytes(2, 2, 128, 200)
+
+    def call(L=L, q_heads=4, offs=256, query=256, rows=2, scale=1.0, causal=1, out=256,
+             dtype=P.PKV_DTYPE_F16, max_len=200, ws=256, ws_bytes=1 << 30):
+        e = _err()
+        ok = lib.pkv_q8_prefill(ctypes.byref(L), ctypes.byref(B), q_heads, offs, query, rows, 1,
+                                f(scale), causal, out, dtype, max_len, ws, ws_bytes, None, e, len(e))
+        return ok, e.value.decode()
+    for kw, text in ((dict(L=_layer(block_size=8)), "16, 32, 64 or 128"), (dict(offs=None), "null"),
+                     (dict(query=None), "null"), (dict(out=None), "null"),
+                     (dict(max_len=0), "max_seq_len"), (dict(ws=None), "workspace"),
+                     (dict(ws_bytes=n - 1), "workspace"), (dict(ws=264), "workspace"),
+                     (dict(dtype=P.PKV_DTYPE_BF16), "output dtype"), (dict(q_heads=3), "multiple"),
+                     (dict(causal=2), "invalid"), (dict(scale=float("nan")), "invalid")):
+        ok, got = call(**kw)
+        assert ok == 0 and text in got and "pkv_q8_prefill" in got, (kw, got)
