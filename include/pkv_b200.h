@@ -263,6 +263,54 @@ int pkv_q8_decode(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads
                   size_t max_seq_len, void *workspace, size_t workspace_bytes, PkvStream stream,
                   char *error, size_t error_capacity);
 
+/* Decode that also adds up attention weights, for eviction:  mass is float32
+ * [block_count][kv_heads][block_size], laid out like the pages, and beside the
+ * output of pkv_paged_decode (pkv_q8_decode) every position t < seq_lens[b]
+ * and KV head g of the batch gets
+ *     mass[table[t / block_size]][g][t % block_size] += sum over the query
+ *     heads of g of their softmax weight of t.
+ * Cells of other positions are left as they are; a sequence's new positions
+ * start from what the cell holds, so clear a page's cells when it is taken.
+ * pkv_paged_decode_mass takes the shapes of the tensor-core decode (pages of
+ * 16 to 128 tokens; an even number of KV heads with head_dim 64).  Sequences
+ * of a batch share no page.  max_seq_len bounds seq_lens (a longer sequence
+ * records fault code 2 and adds nothing).  One workspace size serves both
+ * calls; it must start zeroed once (pkv_decode_workspace_init). */
+size_t pkv_decode_mass_workspace_bytes(size_t batch, size_t q_heads, size_t kv_heads,
+                                       size_t head_dim, size_t max_seq_len);
+int pkv_paged_decode_mass(const PkvPagedLayer *layer, const PkvBatch *batch, size_t q_heads,
+                          const void *query, float scale, void *output, PkvDType output_dtype,
+                          size_t max_seq_len, float *mass, void *workspace,
+                          size_t workspace_bytes, PkvStream stream, char *error,
+                          size_t error_capacity);
+int pkv_q8_decode_mass(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads,
+                       const void *query, float scale, void *output, PkvDType output_dtype,
+                       size_t max_seq_len, float *mass, void *workspace, size_t workspace_bytes,
+                       PkvStream stream, char *error, size_t error_capacity);
+
+/* Eviction by accumulated attention weight.  For each sequence b (length L =
+ * seq_lens[b]) and KV head g by itself, min(L, keep) positions stay: all when
+ * L <= keep, else the newest `recent` and, of the others, those with the
+ * largest mass, ties to the lower position (NaN counts as lowest).  Their
+ * ascending list goes to kept[b][g][0 ..] ([batch][kv_heads][keep], -1 behind
+ * it), and row i of the result -- K and V columns of the head, and its mass --
+ * is row kept[i] of the sequence.  Since every head keeps as many, the result
+ * is a sequence of length min(L, keep) (the caller sets it, e.g. with
+ * tensor_paged_kv_sequence_set_length, which frees the pages behind it).
+ * Keys keep the rotary position they were stored with.
+ * dst_tables ([batch][dst_stride]): pages of the result, none of them a
+ * source page of the batch; or NULL (or batch->block_tables): in place.
+ * Positions of the destination past the result, and the source when it is
+ * another place, are left as they are.  8-bit rows that meet in one block take
+ * the largest s of their scales, q' = rint(q * (s_row / s)).  max_seq_len
+ * should bound seq_lens (it only sizes the launch). */
+int pkv_kv_evict(const PkvPagedLayer *layer, const PkvBatch *batch, float *mass, size_t keep,
+                 size_t recent, const uint32_t *dst_tables, size_t dst_stride, int32_t *kept,
+                 size_t max_seq_len, PkvStream stream, char *error, size_t error_capacity);
+int pkv_q8_evict(const PkvQ8Layer *layer, const PkvBatch *batch, float *mass, size_t keep,
+                 size_t recent, const uint32_t *dst_tables, size_t dst_stride, int32_t *kept,
+                 size_t max_seq_len, PkvStream stream, char *error, size_t error_capacity);
+
 /* pkv_paged_prefill over 8-bit pages; max_seq_len bounds seq_lens (fault
  * code 2 and no keys for a longer sequence).  The pages are widened to
  * layer->dtype (q * s, one rounding) in the workspace first, so scores and

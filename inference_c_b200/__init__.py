@@ -165,6 +165,15 @@ EXPORTS = {
     "pkv_q8_decode_workspace_bytes": (_c_size, [_c_size] * 5),
     "pkv_q8_decode": (_c_int, [_QP, _BP, _c_size, _c_ptr, ctypes.c_float, _c_ptr, _c_int, _c_size,
                                _c_ptr, _c_size, _c_ptr, *_ERR]),
+    "pkv_decode_mass_workspace_bytes": (_c_size, [_c_size] * 5),
+    "pkv_paged_decode_mass": (_c_int, [_LP, _BP, _c_size, _c_ptr, ctypes.c_float, _c_ptr, _c_int,
+                                       _c_size, _c_ptr, _c_ptr, _c_size, _c_ptr, *_ERR]),
+    "pkv_q8_decode_mass": (_c_int, [_QP, _BP, _c_size, _c_ptr, ctypes.c_float, _c_ptr, _c_int,
+                                    _c_size, _c_ptr, _c_ptr, _c_size, _c_ptr, *_ERR]),
+    "pkv_kv_evict": (_c_int, [_LP, _BP, _c_ptr, _c_size, _c_size, _c_ptr, _c_size, _c_ptr,
+                              _c_size, _c_ptr, *_ERR]),
+    "pkv_q8_evict": (_c_int, [_QP, _BP, _c_ptr, _c_size, _c_size, _c_ptr, _c_size, _c_ptr,
+                              _c_size, _c_ptr, *_ERR]),
     "pkv_q8_prefill_workspace_bytes": (_c_size, [_c_size] * 4),
     "pkv_q8_prefill": (_c_int, [_QP, _BP, _c_size, _c_ptr, _c_ptr, _c_size, _c_size,
                                 ctypes.c_float, _c_int, _c_ptr, _c_int, _c_size, _c_ptr, _c_size,
@@ -488,6 +497,60 @@ def q8_decode(layer: PkvQ8Layer, batch: PkvBatch, query, output, scale: float, m
     _call("pkv_q8_decode", ctypes.byref(layer), ctypes.byref(batch), query.shape[-2],
           query.data_ptr(), ctypes.c_float(scale), output.data_ptr(), _dtype_code(output),
           max_seq_len, workspace.data_ptr(), workspace.numel(), _stream_ptr(stream))
+
+
+def decode_mass_workspace(batch: int, q_heads: int, kv_heads: int, head_dim: int,
+                          max_seq_len: int, device=None, stream=None):
+    """Zero-initialised scratch of paged_decode_mass and q8_decode_mass."""
+    import torch
+    n = load().pkv_decode_mass_workspace_bytes(batch, q_heads, kv_heads, head_dim, max_seq_len)
+    ws = torch.empty(n, dtype=torch.uint8, device=device or "cuda")
+    _call("pkv_decode_workspace_init", ws.data_ptr(), n, _stream_ptr(stream))
+    return ws
+
+
+def _decode_mass(name: str, layer, batch: PkvBatch, query, output, scale: float,
+                 max_seq_len: int, mass, workspace, stream) -> None:
+    if mass.shape != (layer.block_count, layer.kv_heads, layer.block_size) or \
+            not mass.is_contiguous():
+        raise ValueError("mass is a contiguous [block_count, kv_heads, block_size] tensor")
+    _call(name, ctypes.byref(layer), ctypes.byref(batch), query.shape[-2], query.data_ptr(),
+          ctypes.c_float(scale), output.data_ptr(), _dtype_code(output), max_seq_len,
+          mass.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream_ptr(stream))
+
+
+def paged_decode_mass(layer: PkvPagedLayer, batch: PkvBatch, query, output, scale: float,
+                      max_seq_len: int, mass, workspace, stream=None) -> None:
+    """paged_decode, and each position's softmax weights added to mass
+    (float32 [block_count, kv_heads, block_size])."""
+    _decode_mass("pkv_paged_decode_mass", layer, batch, query, output, scale, max_seq_len, mass,
+                 workspace, stream)
+
+
+def q8_decode_mass(layer: PkvQ8Layer, batch: PkvBatch, query, output, scale: float,
+                   max_seq_len: int, mass, workspace, stream=None) -> None:
+    _decode_mass("pkv_q8_decode_mass", layer, batch, query, output, scale, max_seq_len, mass,
+                 workspace, stream)
+
+
+def kv_evict(layer, batch: PkvBatch, mass, keep: int, recent: int, kept, max_seq_len: int,
+             dst_tables=None, stream=None) -> None:
+    """pkv_kv_evict, or pkv_q8_evict for a PkvQ8Layer: min(length, keep)
+    positions of every sequence and KV head stay, listed in kept (int32
+    [batch, kv_heads, keep]); dst_tables [batch, stride]: pages of the result
+    (None: in place)."""
+    if kept.shape != (batch.batch, layer.kv_heads, keep) or not kept.is_contiguous():
+        raise ValueError("kept is a contiguous [batch, kv_heads, keep] tensor")
+    if mass.shape != (layer.block_count, layer.kv_heads, layer.block_size) or \
+            not mass.is_contiguous():
+        raise ValueError("mass is a contiguous [block_count, kv_heads, block_size] tensor")
+    if dst_tables is not None and (dst_tables.shape[0] != batch.batch or
+                                   not dst_tables.is_contiguous()):
+        raise ValueError("dst_tables is a contiguous [batch, stride] tensor")
+    name = "pkv_q8_evict" if isinstance(layer, PkvQ8Layer) else "pkv_kv_evict"
+    _call(name, ctypes.byref(layer), ctypes.byref(batch), mass.data_ptr(), keep, recent,
+          _ptr(dst_tables), 0 if dst_tables is None else dst_tables.shape[1], kept.data_ptr(),
+          max_seq_len, _stream_ptr(stream))
 
 
 def q8_prefill_workspace(layer: PkvQ8Layer, batch: int, max_seq_len: int, device=None):

@@ -43,6 +43,7 @@
 
 #include "pkv_device.cuh"
 #include "pkv_internal.h"
+#include "pkv_mass.cuh"
 #include "pkv_trace.h"
 #include "pkv_sched.cuh"
 #include "pkv_sm100.cuh"
@@ -527,6 +528,10 @@ struct TcArgs {
     const uint4 *new_k, *new_v;
     uint4 *kpool, *vpool;
     int32_t row_vecs;  // uint4 per pool row (kv_heads * head_dim / 8)
+    // Mass (else null): every score by stream tile and head, and every query
+    // head's final maximum and sum (pkv_mass.cuh).
+    float *scores, *final_ml;
+    int64_t score_tiles;
 };
 
 // Tensor maps of one launch: K and V pools (one page x 64 columns per box)
@@ -567,12 +572,14 @@ struct IsBf16<__nv_bfloat16> { static constexpr bool value = true; };
 // is the weighted sum of the pieces' partial rows: `ps` threads share one
 // float4 (pieces c = lane-in-share mod ps, summed through `red`,
 // ps * nh * 32 float4s), each keeping up to 16 loads in flight.  `tid`/`nthr`
-// are the participating threads (whole warps); `sync` is their barrier.
+// are the participating threads (whole warps); `sync` is their barrier.  `fml`
+// non-null receives each head's final (m, l).
 template <typename OT, typename Sync>
 __device__ __forceinline__ void merge_segment(const TcArgs &a, int h0, int nh, int heads,
                                               int64_t seg, int nt, const Sched &sc, int tid,
                                               int nthr, int ps, float *wst, float *lst, int *slot,
-                                              float4 *red, int cap, OT *out, Sync sync) {
+                                              float4 *red, int cap, OT *out, float *fml,
+                                              Sync sync) {
     const int first = unit_of_tile(sc, seg);
     const int np = unit_of_tile(sc, seg + nt - 1) - first + 1;
     if (np > cap) {  // cannot happen with the host's choice of merge mode and unit sizes
@@ -605,6 +612,8 @@ __device__ __forceinline__ void merge_segment(const TcArgs &a, int h0, int nh, i
         lt = warp_sum(lt);
         const float inv = lt > 0.f ? 1.f / lt : 0.f;
         for (int c = lane; c < np; c += 32) wst[c * nh + hh] *= inv;
+        if (fml != nullptr && lane == 0)
+            reinterpret_cast<float2 *>(fml)[hh] = make_float2(mx, lt);
     }
     sync();
     const int nf = nh * 32;  // float4s of output
@@ -1117,6 +1126,8 @@ paged_decode_tc_kernel(const TcArgs a, const __grid_constant__ CUtensorMap kmap,
                 for (int h = 0; h < GV; ++h) {
                     const int col = PAIR && h >= G ? 8 + h - G : h;  // S^T column of head h
                     x[h] = live ? s[col] * a.scale_log2 : -INFINITY;
+                    if (a.scores != nullptr && P.seg + k < a.score_tiles)
+                        a.scores[((P.seg + k) * GV + h) * 128 + row] = x[h];
                     const float wm = warp_max(x[h]);
                     if (lane == 0) red[buf * 64 + q4 * 16 + h] = wm;
                 }
@@ -1168,6 +1179,9 @@ paged_decode_tc_kernel(const TcArgs a, const __grid_constant__ CUtensorMap kmap,
             for (int h = 0; h < GV; ++h) l[h] = lred[h] + lred[16 + h] + lred[32 + h] + lred[48 + h];
             group_sync();
             OT *out = static_cast<OT *>(a.out) + ((int64_t)P.b * q_heads + (int64_t)P.g * GV) * OD;
+            float *fml = a.final_ml == nullptr
+                             ? nullptr
+                             : a.final_ml + ((int64_t)P.b * q_heads + (int64_t)P.g * GV) * 2;
             if (P.k0 == 0 && P.k1 == P.nt) {  // the whole segment ran here
 #pragma unroll
                 for (int h = 0; h < GV; ++h) {
@@ -1177,6 +1191,8 @@ paged_decode_tc_kernel(const TcArgs a, const __grid_constant__ CUtensorMap kmap,
                     } else {
                         out[h * 128 + row] = from_f32<OT>(v);
                     }
+                    if (fml != nullptr && wt == h)
+                        reinterpret_cast<float2 *>(fml)[h] = make_float2(m_run[h], l[h]);
                 }
                 continue;
             }
@@ -1205,7 +1221,7 @@ paged_decode_tc_kernel(const TcArgs a, const __grid_constant__ CUtensorMap kmap,
             if (*ticket) {
                 __threadfence();
                 merge_segment<OT>(a, 0, GV, GV, P.seg, P.nt, sc, wt, 128, 1, mwst, mlst, mslot,
-                                  nullptr, kInKernelMergeMax, out, group_sync);
+                                  nullptr, kInKernelMergeMax, out, fml, group_sync);
                 if (wt == 0) a.counters[u0] = 0u;
             }
         }
@@ -1253,8 +1269,11 @@ pkv_tc_merge_kernel(const TcArgs a, int group, int grid) {
     OT *out = static_cast<OT *>(a.out) +
               ((int64_t)b * a.kv_heads * group + (int64_t)g * group + h) *
                   (a.pair_split != 0 ? 64 : 128);
+    float *fml = a.final_ml == nullptr
+                     ? nullptr
+                     : a.final_ml + ((int64_t)b * a.kv_heads * group + (int64_t)g * group + h) * 2;
     merge_segment<OT>(a, h, 1, group, seg, nt, sc, threadIdx.x, kMergeThreads, kMergeThreads / 32,
-                      wst, lst, slot, red, kTcMaxGrid, out, [] { __syncthreads(); });
+                      wst, lst, slot, red, kTcMaxGrid, out, fml, [] { __syncthreads(); });
 }
 
 int g_sm_count[64];
@@ -1494,11 +1513,12 @@ namespace {
 
 // pkv_paged_decode, and with key_rows/value_rows non-null
 // pkv_paged_decode_append: the tensor-core kernel stores the new rows itself
-// (TcArgs::new_k), the CUDA-core path launches the append kernel first.
+// (TcArgs::new_k), the CUDA-core path launches the append kernel first.  With
+// `mass` pkv_paged_decode_mass, whose scratch follows the decode's.
 int paged_decode_impl(const char *what, const PkvPagedLayer *layer, const PkvBatch *batch,
                       const void *key_rows, const void *value_rows, size_t q_heads,
                       const void *query, float scale, void *output, PkvDType output_dtype,
-                      size_t max_seq_len, size_t chunk_tokens, void *workspace,
+                      size_t max_seq_len, size_t chunk_tokens, float *mass, void *workspace,
                       size_t workspace_bytes, PkvStream stream, char *error,
                       size_t error_capacity) {
     if (layer == nullptr || batch == nullptr || query == nullptr || output == nullptr ||
@@ -1565,7 +1585,22 @@ int paged_decode_impl(const char *what, const PkvPagedLayer *layer, const PkvBat
     const pkv::TcWorkspace tws_dyn = pkv::tc_workspace(pkv::tc_units(ncta, true), gv);
     const bool dyn_fits = workspace_bytes >= tws_dyn.total;
     const pkv::TcWorkspace tws = dyn_fits ? tws_dyn : tws_static;
-    const size_t need = use_tc ? tws_static.total : ws.total;
+    if (mass != nullptr && !use_tc) {
+        pkv_internal_set_error(error, error_capacity,
+                               "%s: needs pages of 16, 32, 64 or 128 tokens, and an even number of "
+                               "KV heads with head_dim 64",
+                               what);
+        return 0;
+    }
+    // mass: the whole decode layout, then the scores
+    const size_t segs_all = hd == 64 ? kvh / 2 : kvh;
+    const size_t mass_at = pkv::round_up(
+        pkv_decode_workspace_bytes(batch->batch, q_heads, hd, max_seq_len, 0), 256);
+    const size_t need =
+        mass != nullptr
+            ? mass_at + pkv::mass_scratch_bytes(batch->batch, q_heads, segs_all, gv, max_seq_len)
+        : use_tc ? tws_static.total
+                 : ws.total;
     if (workspace == nullptr || workspace_bytes < need || ((uintptr_t)workspace % 256) != 0) {
         pkv_internal_set_error(error, error_capacity,
                                "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", what,
@@ -1634,6 +1669,12 @@ int paged_decode_impl(const char *what, const PkvPagedLayer *layer, const PkvBat
         t.kpool = static_cast<uint4 *>(layer->key_pool);
         t.vpool = static_cast<uint4 *>(layer->value_pool);
         t.row_vecs = (int32_t)(kvh * hd / 8);
+        pkv::MassScratch ms = {};
+        if (mass != nullptr)
+            ms = pkv::mass_scratch(wsb + mass_at, batch->batch, q_heads, segs_all, max_seq_len);
+        t.scores = ms.scores;
+        t.final_ml = ms.final_ml;
+        t.score_tiles = ms.tiles;
         // In-kernel merges need every segment to span at most
         // kInKernelMergeMax CTAs.  They also sit on the critical path of the
         // CTA that finishes last, so with few segments (each cut into many
@@ -1674,6 +1715,20 @@ int paged_decode_impl(const char *what, const PkvPagedLayer *layer, const PkvBat
                 sl.new_v += b0 * (size_t)t.row_vecs;
             }
             ok = pkv::dispatch_tc(sl, (int)group, pair, bf16, output_dtype, mp, ncta, s);
+            if (ok && mass != nullptr) {
+                const pkv::MassShape shape = {n,
+                                              q_heads,
+                                              kvh,
+                                              hd,
+                                              layer->block_size,
+                                              layer->block_count,
+                                              batch->table_stride,
+                                              max_seq_len,
+                                              gv,
+                                              1};
+                ok = pkv::mass_apply(shape, ms, sl.tile_prefix, sl.tables, sl.seq_lens, mass,
+                                     stream);
+            }
         }
     } else if (fused && !pkv_kv_append(layer, batch, nullptr, key_rows, value_rows, batch->batch,
                                        stream, error, error_capacity)) {
@@ -1705,7 +1760,25 @@ int pkv_paged_decode(const PkvPagedLayer *layer, const PkvBatch *batch, size_t q
     PKV_RANGE("pkv_paged_decode");
     return pkv::paged_decode_impl("pkv_paged_decode", layer, batch, nullptr, nullptr, q_heads,
                                   query, scale, output, output_dtype, max_seq_len, chunk_tokens,
-                                  workspace, workspace_bytes, stream, error, error_capacity);
+                                  nullptr, workspace, workspace_bytes, stream, error,
+                                  error_capacity);
+}
+
+int pkv_paged_decode_mass(const PkvPagedLayer *layer, const PkvBatch *batch, size_t q_heads,
+                          const void *query, float scale, void *output, PkvDType output_dtype,
+                          size_t max_seq_len, float *mass, void *workspace,
+                          size_t workspace_bytes, PkvStream stream, char *error,
+                          size_t error_capacity) {
+    PKV_RANGE("pkv_paged_decode_mass");
+    const char *what = "pkv_paged_decode_mass";
+    if (mass == nullptr || (uintptr_t)mass % 4 != 0) {
+        pkv_internal_set_error(error, error_capacity, "%s: mass is null or not 4-byte aligned",
+                               what);
+        return 0;
+    }
+    return pkv::paged_decode_impl(what, layer, batch, nullptr, nullptr, q_heads, query, scale,
+                                  output, output_dtype, max_seq_len, 0, mass, workspace,
+                                  workspace_bytes, stream, error, error_capacity);
 }
 
 int pkv_paged_decode_append(const PkvPagedLayer *layer, const PkvBatch *batch,
@@ -1721,8 +1794,8 @@ int pkv_paged_decode_append(const PkvPagedLayer *layer, const PkvBatch *batch,
         return 0;
     }
     return pkv::paged_decode_impl(what, layer, batch, key_rows, value_rows, q_heads, query, scale,
-                                  output, output_dtype, max_seq_len, chunk_tokens, workspace,
-                                  workspace_bytes, stream, error, error_capacity);
+                                  output, output_dtype, max_seq_len, chunk_tokens, nullptr,
+                                  workspace, workspace_bytes, stream, error, error_capacity);
 }
 
 int pkv_internal_take_decode_fault(uint32_t *code) {

@@ -55,6 +55,8 @@ int pkv_internal_take_sequence_fault(uint32_t *code);
 int pkv_internal_take_peer_fault(uint32_t *code);
 int pkv_internal_take_q8_copy_fault(uint32_t *code);
 int pkv_internal_take_q8_decode_fault(uint32_t *code);
+int pkv_internal_take_mass_fault(uint32_t *code);
+int pkv_internal_take_evict_fault(uint32_t *code);
 
 /* Tests on one GPU: makes `area` (a device buffer of
  * pkv_internal_peer_gather_area_bytes bytes on this GPU) stand in for the

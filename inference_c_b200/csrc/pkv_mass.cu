@@ -1,0 +1,135 @@
+// pkv_mass.cu -- attention weights of a decode step, added to the paged mass
+// (float32 [block_count][kv_heads][block_size]).
+//
+// One CTA takes kTiles tiles of 128 tokens of one lane (one KV head of
+// head_dim 128, two of 64) of one sequence: thread = token, a coalesced load
+// per query head, one read and write of the token's cell per KV head.  Each
+// cell belongs to one thread, so sums do not depend on any order of CTAs.
+// Bound by HBM: 4 bytes a token and query head (mostly L2 hits, just written)
+// and 8 bytes a token and KV head.
+#include "pkv_device.cuh"
+#include "pkv_mass.cuh"
+
+namespace pkv {
+namespace {
+
+__device__ uint32_t g_mass_fault;
+
+constexpr int kTiles = 4;
+
+struct MassArgs {
+    const float *scores;
+    const float *final_ml;
+    const int32_t *tile_prefix;
+    const uint32_t *tables;
+    const int32_t *seq_lens;
+    float *mass;
+    int64_t tiles;
+    int32_t table_stride, kv_heads, q_heads, group, block_size, gv, per, subs, segs;
+    uint32_t block_count;
+};
+
+template <bool PAIR>
+__global__ void __launch_bounds__(128) mass_kernel(const MassArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = blockIdx.y, b = blockIdx.z;
+    const int L = max(0, __ldg(a.seq_lens + b));
+    const int k0 = blockIdx.x * kTiles;
+    if (k0 * 128 >= L) return;
+    const int nt = (L + 127) / 128;
+    const int64_t first = a.tile_prefix[b];
+#pragma unroll
+    for (int half = 0; half < (PAIR ? 2 : 1); ++half) {
+        const int kvh = PAIR ? 2 * lane + half : lane;
+        if (kvh >= a.kv_heads) return;
+        float w[kTiles];
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) w[i] = 0.f;
+        for (int hh = 0; hh < a.group; ++hh) {
+            const float2 ml = __ldg(reinterpret_cast<const float2 *>(
+                a.final_ml + ((int64_t)b * a.q_heads + kvh * a.group + hh) * 2));
+            const float inv = ml.y == 0.f ? 0.f : 1.f / ml.y;
+            const int sub = hh / a.per, h = hh - sub * a.per + half * a.per;
+            const int64_t tile = first + (int64_t)(lane * a.subs + sub) * nt + k0;
+            float x[kTiles];
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+                const bool live = (k0 + i) * 128 + (int)threadIdx.x < L && tile + i < a.tiles;
+                x[i] = live ? __ldcg(a.scores + ((tile + i) * a.gv + h) * 128 + threadIdx.x)
+                            : -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i)
+                w[i] += x[i] == -INFINITY ? 0.f : exp2f(x[i] - ml.x) * inv;
+        }
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+            const int t = (k0 + i) * 128 + (int)threadIdx.x;
+            if (t >= L) continue;
+            const int page = t / a.block_size;
+            uint32_t pid = 0, fault = kFaultNone;
+            if (page >= a.table_stride) fault = kFaultPositionOutOfRange;
+            else if ((pid = __ldg(a.tables + (int64_t)b * a.table_stride + page)) >= a.block_count)
+                fault = kFaultPageOutOfRange;
+            else if (first + (int64_t)a.segs * nt > a.tiles)  // longer than the caller's bound
+                fault = kFaultPositionOutOfRange;
+            if (fault != kFaultNone) {
+                record_fault(&g_mass_fault, fault);
+                continue;
+            }
+            float *cell = a.mass + ((int64_t)pid * a.kv_heads + kvh) * a.block_size +
+                          (t - page * a.block_size);
+            *cell += w[i];
+        }
+    }
+}
+
+}  // namespace
+
+bool mass_apply(const MassShape &s, const MassScratch &scratch, const int32_t *tile_prefix,
+                const uint32_t *tables, const int32_t *seq_lens, float *mass, PkvStream stream) {
+    const bool pair = s.head_dim == 64;
+    MassArgs a;
+    a.scores = scratch.scores;
+    a.final_ml = scratch.final_ml;
+    a.tile_prefix = tile_prefix;
+    a.tables = tables;
+    a.seq_lens = seq_lens;
+    a.mass = mass;
+    a.tiles = scratch.tiles;
+    a.table_stride = (int32_t)s.table_stride;
+    a.kv_heads = (int32_t)s.kv_heads;
+    a.q_heads = (int32_t)s.q_heads;
+    a.group = (int32_t)(s.q_heads / s.kv_heads);
+    a.block_size = (int32_t)s.block_size;
+    a.gv = (int32_t)s.gv;
+    a.per = (int32_t)(pair ? s.gv / 2 : s.gv);
+    a.subs = (int32_t)s.subs;
+    const size_t lanes = mass_lanes(s.kv_heads, s.head_dim);
+    a.segs = (int32_t)(lanes * s.subs);
+    a.block_count = (uint32_t)s.block_count;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    const size_t tiles = (s.max_seq_len + 127) / 128;
+    cfg.gridDim = dim3((unsigned)((tiles + kTiles - 1) / kTiles), (unsigned)lanes,
+                       (unsigned)s.batch);
+    cfg.blockDim = dim3(128);
+    cfg.stream = (cudaStream_t)stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (tiles == 0) return true;
+    const cudaError_t st = pair ? cudaLaunchKernelEx(&cfg, mass_kernel<true>, a)
+                                : cudaLaunchKernelEx(&cfg, mass_kernel<false>, a);
+    return st == cudaSuccess && cudaGetLastError() == cudaSuccess;
+}
+
+}  // namespace pkv
+
+extern "C" int pkv_internal_take_mass_fault(uint32_t *code) {
+    uint32_t zero = 0;
+    if (cudaMemcpyFromSymbol(code, pkv::g_mass_fault, sizeof(uint32_t)) != cudaSuccess) return 0;
+    return cudaMemcpyToSymbol(pkv::g_mass_fault, &zero, sizeof(uint32_t)) == cudaSuccess;
+}

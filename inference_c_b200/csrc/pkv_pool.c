@@ -448,7 +448,8 @@ int pkv_device_fault(int device, uint32_t *code, char *error, size_t cap) {
         pkv_internal_take_copy_fault,     pkv_internal_take_decode_fault,
         pkv_internal_take_prefill_fault,  pkv_internal_take_sequence_fault,
         pkv_internal_take_peer_fault,     pkv_internal_take_q8_copy_fault,
-        pkv_internal_take_q8_decode_fault};
+        pkv_internal_take_q8_decode_fault, pkv_internal_take_mass_fault,
+        pkv_internal_take_evict_fault};
     uint32_t first = 0;
     int ok = st == cudaSuccess;
     for (size_t i = 0; ok && i < sizeof take / sizeof take[0]; ++i) {

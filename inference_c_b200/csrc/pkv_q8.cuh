@@ -22,44 +22,58 @@ inline size_t q8_lanes(size_t kv_heads, size_t head_dim) {
     return (kv_heads * head_dim + kQ8Lane - 1) / kQ8Lane;
 }
 
-// The checks every entry point over 8-bit pages makes on its layer and batch
-// (host; no device work).  Writes the reason and returns false.
-inline bool q8_check(const PkvQ8Layer *layer, const PkvBatch *batch, char *error, size_t cap,
-                     const char *what) {
-    if (layer == nullptr || batch == nullptr || layer->key_pool == nullptr ||
-        layer->value_pool == nullptr || layer->key_scales == nullptr ||
-        layer->value_scales == nullptr || batch->block_tables == nullptr ||
-        batch->seq_lens == nullptr) {
-        pkv_internal_set_error(error, cap, "%s: null argument", what);
-        return false;
-    }
-    if (layer->dtype != PKV_DTYPE_F16 && layer->dtype != PKV_DTYPE_BF16) {
+// The checks every entry point over 8-bit pages makes on its shapes (eviction
+// of 16-bit pages too), and on its layer and batch (host; no device work).
+// They write the reason and return false.
+inline bool page_shape_check(size_t bs, size_t block_count, size_t kv_heads, size_t head_dim,
+                             PkvDType dtype, const PkvBatch *batch, char *error, size_t cap,
+                             const char *what) {
+    if (dtype != PKV_DTYPE_F16 && dtype != PKV_DTYPE_BF16) {
         pkv_internal_set_error(error, cap, "%s: row dtype must be F16 or BF16", what);
         return false;
     }
-    const size_t bs = layer->block_size;
-    if ((bs != 16 && bs != 32 && bs != 64 && bs != 128) ||
-        (layer->head_dim != 64 && layer->head_dim != 128) || layer->kv_heads == 0 ||
-        layer->kv_heads > 1024) {
+    if ((bs != 16 && bs != 32 && bs != 64 && bs != 128) || (head_dim != 64 && head_dim != 128) ||
+        kv_heads == 0 || kv_heads > 1024) {
         pkv_internal_set_error(error, cap,
-                               "%s: 8-bit pages hold 16, 32, 64 or 128 tokens of 1..1024 KV heads "
-                               "of head_dim 64 or 128",
+                               "%s: pages hold 16, 32, 64 or 128 tokens of 1..1024 KV heads of "
+                               "head_dim 64 or 128",
                                what);
         return false;
     }
-    if (layer->block_count == 0 || layer->block_count > UINT32_MAX || batch->batch == 0 ||
+    if (block_count == 0 || block_count > UINT32_MAX || batch->batch == 0 ||
         batch->batch > INT32_MAX / 4 || batch->table_stride == 0 ||
         batch->table_stride > INT32_MAX / bs) {
         pkv_internal_set_error(error, cap, "%s: invalid block count, batch or table stride", what);
         return false;
     }
-    if (((uintptr_t)layer->key_pool | (uintptr_t)layer->value_pool) % 16 != 0 ||
-        ((uintptr_t)layer->key_scales | (uintptr_t)layer->value_scales) % 4 != 0) {
-        pkv_internal_set_error(error, cap,
-                               "%s: pools must be 16-byte aligned, scales 4-byte aligned", what);
+    return true;
+}
+inline bool pool_check(const void *key_pool, const void *value_pool, const PkvBatch *batch,
+                       char *error, size_t cap, const char *what) {
+    if (batch == nullptr || key_pool == nullptr || value_pool == nullptr ||
+        batch->block_tables == nullptr || batch->seq_lens == nullptr) {
+        pkv_internal_set_error(error, cap, "%s: null argument", what);
+        return false;
+    }
+    if (((uintptr_t)key_pool | (uintptr_t)value_pool) % 16 != 0) {
+        pkv_internal_set_error(error, cap, "%s: pools must be 16-byte aligned", what);
         return false;
     }
     return true;
+}
+inline bool q8_check(const PkvQ8Layer *layer, const PkvBatch *batch, char *error, size_t cap,
+                     const char *what) {
+    if (layer == nullptr || layer->key_scales == nullptr || layer->value_scales == nullptr) {
+        pkv_internal_set_error(error, cap, "%s: null argument", what);
+        return false;
+    }
+    if (((uintptr_t)layer->key_scales | (uintptr_t)layer->value_scales) % 4 != 0) {
+        pkv_internal_set_error(error, cap, "%s: scales must be 4-byte aligned", what);
+        return false;
+    }
+    return pool_check(layer->key_pool, layer->value_pool, batch, error, cap, what) &&
+           page_shape_check(layer->block_size, layer->block_count, layer->kv_heads,
+                            layer->head_dim, layer->dtype, batch, error, cap, what);
 }
 
 // Four int8 values of a word, as floats.

@@ -37,6 +37,7 @@
 
 #include <cudaTypedefs.h>
 
+#include "pkv_mass.cuh"
 #include "pkv_q8.cuh"
 #include "pkv_sched.cuh"
 #include "pkv_sm100.cuh"
@@ -100,6 +101,10 @@ struct Q8Args {
     float scale_log2;
     int32_t merge_in_kernel, min_unit;
     int32_t bf16, out_f32;   // row type; 32-bit outputs
+    // Mass (else null): every score by stream tile and slot, and every query
+    // head's final maximum and sum (pkv_mass.cuh).
+    float *scores, *final_ml;
+    int64_t score_tiles;
 };
 
 struct Workspace {
@@ -157,6 +162,10 @@ __device__ __forceinline__ int head_at(const Q8Args &a, int g, int h) {
 template <bool PAIR>
 __device__ __forceinline__ bool owns(int gv, int h, int row) {
     return !PAIR || (h >= gv / 2) == (row >= 64);
+}
+__device__ __forceinline__ void store_ml(const Q8Args &a, int b, int qh, float m, float l) {
+    *reinterpret_cast<float2 *>(a.final_ml + ((int64_t)b * a.q_heads + qh) * 2) =
+        make_float2(m, l);
 }
 template <bool PAIR>
 __device__ __forceinline__ int64_t out_at(const Q8Args &a, int b, int qh, int row) {
@@ -627,6 +636,8 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                         const int lo = __float_as_int(s[GV + h]) * 256 + __float_as_int(s[2 * GV + h]);
                         const float v = fmaf((float)__float_as_int(s[h]), 65536.f, (float)lo);
                         x[h] = live ? v * (qs[h] * ks[PAIR && h >= GV / 2 ? 1 : 0]) : -INFINITY;
+                        if (a.scores != nullptr && P.seg + k < a.score_tiles)
+                            a.scores[((P.seg + k) * GV + h) * 128 + row] = x[h];
                         const float wm = redux_max(x[h]);
                         if (lane == 0) myred[q4 * 16 + h] = wm;
                     }
@@ -708,6 +719,8 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                         if (qh >= 0 && owns<PAIR>(GV, h, row))
                             store_out(a, out_at<PAIR>(a, P.b, qh, row),
                                       l[h] == 0.f ? 0.f : acc[h] / l[h]);
+                        if (a.final_ml != nullptr && qh >= 0 && wt == h)
+                            store_ml(a, P.b, qh, m_run[h], l[h]);
                     }
                     continue;
                 }
@@ -756,6 +769,8 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                     }
                     const float inv = lt == 0.f ? 0.f : 1.f / lt;
                     for (int c = 0; c < np; ++c) mw[c * GV + wt] *= inv;
+                    const int qh = head_at<GV, PAIR>(a, P.g, wt);
+                    if (a.final_ml != nullptr && qh >= 0) store_ml(a, P.b, qh, mx, lt);
                 }
                 group_sync();
 #pragma unroll
@@ -828,6 +843,7 @@ __global__ void __launch_bounds__(kMergeThreads) q8_merge_kernel(const Q8Args a,
         lt = warp_sum(lt);
         const float inv = lt == 0.f ? 0.f : 1.f / lt;
         for (int c = threadIdx.x; c < np; c += 32) w[c] *= inv;
+        if (a.final_ml != nullptr && threadIdx.x == 0) store_ml(a, b, qh, mx, lt);
     }
     __syncthreads();
     const int row = threadIdx.x & 127, share = threadIdx.x >> 7;
@@ -915,26 +931,12 @@ size_t slots_of(size_t group, size_t head_dim) {
     return want <= 4 ? 4 : want <= 8 ? 8 : 16;
 }
 
-}  // namespace
-}  // namespace pkv
-
-extern "C" {
-
-size_t pkv_q8_decode_workspace_bytes(size_t batch, size_t q_heads, size_t kv_heads,
-                                     size_t head_dim, size_t max_seq_len) {
-    if (kv_heads == 0 || q_heads == 0 || q_heads % kv_heads != 0) return 0;
-    return pkv::workspace_of((size_t)pkv::decode_grid() * (1 + pkv::kMaxRounds),
-                             pkv::slots_of(q_heads / kv_heads, head_dim))
-        .total;
-}
-
-int pkv_q8_decode(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads,
-                  const void *query, float scale, void *output, PkvDType output_dtype,
-                  size_t max_seq_len, void *workspace, size_t workspace_bytes, PkvStream stream,
-                  char *error, size_t error_capacity) {
-    PKV_RANGE("pkv_q8_decode");
-    const char *what = "pkv_q8_decode";
-    if (!pkv::q8_check(layer, batch, error, error_capacity, what)) return 0;
+// pkv_q8_decode, and with `mass` pkv_q8_decode_mass.
+int q8_decode(const char *what, const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads,
+              const void *query, float scale, void *output, PkvDType output_dtype,
+              size_t max_seq_len, float *mass, void *workspace, size_t workspace_bytes,
+              PkvStream stream, char *error, size_t error_capacity) {
+    if (!q8_check(layer, batch, error, error_capacity, what)) return 0;
     if (query == nullptr || output == nullptr) {
         pkv_internal_set_error(error, error_capacity, "%s: null argument", what);
         return 0;
@@ -945,20 +947,20 @@ int pkv_q8_decode(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads
         return 0;
     }
     const size_t kvh = layer->kv_heads, hd = layer->head_dim;
-    if (q_heads == 0 || q_heads % kvh != 0 || q_heads / kvh > pkv::kQ8MaxGroup) {
+    if (q_heads == 0 || q_heads % kvh != 0 || q_heads / kvh > kQ8MaxGroup) {
         pkv_internal_set_error(error, error_capacity,
                                "%s: q_heads must be 1..%zu times kv_heads", what,
-                               pkv::kQ8MaxGroup);
+                               kQ8MaxGroup);
         return 0;
     }
-    const size_t lanes = pkv::q8_lanes(kvh, hd);
+    const size_t lanes = q8_lanes(kvh, hd);
     const size_t rows = layer->block_count * lanes * layer->block_size;
-    if (batch->batch > (size_t)pkv::kMaxBatch || !isfinite(scale) ||
+    if (batch->batch > (size_t)kMaxBatch || !isfinite(scale) ||
         max_seq_len > INT32_MAX / 2 || layer->block_count > INT32_MAX || rows > INT32_MAX) {
         pkv_internal_set_error(error, error_capacity,
                                "%s: invalid batch (1..%d), scale, length or pool (block_count * "
                                "lanes * block_size must be below 2^31)",
-                               what, pkv::kMaxBatch);
+                               what, kMaxBatch);
         return 0;
     }
     if ((uintptr_t)query % 16 != 0 || (uintptr_t)output % 4 != 0) {
@@ -966,26 +968,30 @@ int pkv_q8_decode(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads
                                "%s: query must be 16-byte, output 4-byte aligned", what);
         return 0;
     }
-    const size_t group = q_heads / kvh, gv = pkv::slots_of(group, hd);
+    const size_t group = q_heads / kvh, gv = slots_of(group, hd);
     const size_t per = hd == 64 ? gv / 2 : gv;         // slots per KV head
     const size_t subs = (group + per - 1) / per;
     const size_t segs = lanes * subs;
-    const int ncta = pkv::decode_grid();
-    const pkv::Workspace ws = pkv::workspace_of((size_t)ncta * (1 + pkv::kMaxRounds), gv);
-    if (workspace == nullptr || workspace_bytes < ws.total || (uintptr_t)workspace % 256 != 0) {
+    const int ncta = decode_grid();
+    const Workspace ws = workspace_of((size_t)ncta * (1 + kMaxRounds), gv);
+    const size_t need =
+        ws.total + (mass == nullptr ? 0
+                                    : mass_scratch_bytes(batch->batch, q_heads, segs, gv,
+                                                         max_seq_len));
+    if (workspace == nullptr || workspace_bytes < need || (uintptr_t)workspace % 256 != 0) {
         pkv_internal_set_error(error, error_capacity,
                                "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", what,
-                               ws.total, workspace_bytes);
+                               need, workspace_bytes);
         return 0;
     }
     CUtensorMap kmap, vmap;
-    if (!pkv::encode_q8_map(&kmap, layer->key_pool, rows, (uint32_t)layer->block_size) ||
-        !pkv::encode_q8_map(&vmap, layer->value_pool, rows, (uint32_t)layer->block_size)) {
+    if (!encode_q8_map(&kmap, layer->key_pool, rows, (uint32_t)layer->block_size) ||
+        !encode_q8_map(&vmap, layer->value_pool, rows, (uint32_t)layer->block_size)) {
         pkv_internal_set_error(error, error_capacity, "%s: tensor map encoding failed", what);
         return 0;
     }
     auto *base = static_cast<unsigned char *>(workspace);
-    pkv::Q8Args a;
+    Q8Args a;
     a.query = query;
     a.out = output;
     a.kscales = layer->key_scales;
@@ -1004,24 +1010,29 @@ int pkv_q8_decode(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads
     a.q_heads = (int32_t)q_heads;
     a.block_size = (int32_t)layer->block_size;
     a.block_count = (uint32_t)layer->block_count;
-    a.scale_log2 = scale * pkv::kLog2e;
+    a.scale_log2 = scale * kLog2e;
     a.bf16 = layer->dtype == PKV_DTYPE_BF16;
     a.out_f32 = output_dtype == PKV_DTYPE_F32;
+    MassScratch ms = {};
+    if (mass != nullptr) ms = mass_scratch(base + ws.total, batch->batch, q_heads, segs, max_seq_len);
+    a.scores = ms.scores;
+    a.final_ml = ms.final_ml;
+    a.score_tiles = ms.tiles;
     // The 16-bit decode's rules: join in the kernel when a segment meets few
     // CTAs and there are many segments; dynamic units only then, none so small
     // that a segment of max_seq_len meets more than kInKernelMergeMax of them.
-    const bool fits = ncta / (int)segs + 2 <= pkv::kInKernelMergeMax;
+    const bool fits = ncta / (int)segs + 2 <= kInKernelMergeMax;
     a.merge_in_kernel = fits && batch->batch * segs * 2 >= (size_t)ncta;
-    const size_t by_pieces = ((max_seq_len + pkv::kTcTile - 1) / pkv::kTcTile + 23) / 24;
-    a.min_unit = a.merge_in_kernel ? (int32_t)(by_pieces > pkv::kMinUnitTiles ? by_pieces
-                                                                              : pkv::kMinUnitTiles)
+    const size_t by_pieces = ((max_seq_len + kTcTile - 1) / kTcTile + 23) / 24;
+    a.min_unit = a.merge_in_kernel ? (int32_t)(by_pieces > kMinUnitTiles ? by_pieces
+                                                                              : kMinUnitTiles)
                                    : 0;
     const size_t osz = a.out_f32 ? 4 : 2;
     int ok = 1;
-    for (size_t b0 = 0; ok && b0 < batch->batch; b0 += pkv::kLaunchBatch) {
-        const size_t n = batch->batch - b0 < (size_t)pkv::kLaunchBatch ? batch->batch - b0
-                                                                       : (size_t)pkv::kLaunchBatch;
-        pkv::Q8Args s = a;
+    for (size_t b0 = 0; ok && b0 < batch->batch; b0 += kLaunchBatch) {
+        const size_t n = batch->batch - b0 < (size_t)kLaunchBatch ? batch->batch - b0
+                                                                       : (size_t)kLaunchBatch;
+        Q8Args s = a;
         s.batch = (int32_t)n;
         s.tables = batch->block_tables + b0 * batch->table_stride;
         s.seq_lens = batch->seq_lens + b0;
@@ -1029,13 +1040,18 @@ int pkv_q8_decode(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads
         s.out = static_cast<char *>(output) + b0 * q_heads * hd * osz;
         const cudaStream_t st = (cudaStream_t)stream;
         if (hd == 128)
-            ok = gv == 4   ? pkv::launch<4, false>(s, kmap, vmap, ncta, st)
-                 : gv == 8 ? pkv::launch<8, false>(s, kmap, vmap, ncta, st)
-                           : pkv::launch<16, false>(s, kmap, vmap, ncta, st);
+            ok = gv == 4   ? launch<4, false>(s, kmap, vmap, ncta, st)
+                 : gv == 8 ? launch<8, false>(s, kmap, vmap, ncta, st)
+                           : launch<16, false>(s, kmap, vmap, ncta, st);
         else
-            ok = gv == 4   ? pkv::launch<4, true>(s, kmap, vmap, ncta, st)
-                 : gv == 8 ? pkv::launch<8, true>(s, kmap, vmap, ncta, st)
-                           : pkv::launch<16, true>(s, kmap, vmap, ncta, st);
+            ok = gv == 4   ? launch<4, true>(s, kmap, vmap, ncta, st)
+                 : gv == 8 ? launch<8, true>(s, kmap, vmap, ncta, st)
+                           : launch<16, true>(s, kmap, vmap, ncta, st);
+        if (ok && mass != nullptr) {
+            const MassShape shape = {n, q_heads, kvh, hd, layer->block_size, layer->block_count,
+                                     batch->table_stride, max_seq_len, gv, subs};
+            ok = mass_apply(shape, ms, s.tile_prefix, s.tables, s.seq_lens, mass, stream);
+        }
     }
     if (!ok) {
         pkv_internal_set_error(error, error_capacity, "%s: launch failed: %s", what,
@@ -1043,6 +1059,62 @@ int pkv_q8_decode(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads
         return 0;
     }
     return 1;
+}
+
+}  // namespace
+}  // namespace pkv
+
+extern "C" {
+
+size_t pkv_q8_decode_workspace_bytes(size_t batch, size_t q_heads, size_t kv_heads,
+                                     size_t head_dim, size_t max_seq_len) {
+    if (kv_heads == 0 || q_heads == 0 || q_heads % kv_heads != 0) return 0;
+    return pkv::workspace_of((size_t)pkv::decode_grid() * (1 + pkv::kMaxRounds),
+                             pkv::slots_of(q_heads / kv_heads, head_dim))
+        .total;
+}
+
+int pkv_q8_decode(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads,
+                  const void *query, float scale, void *output, PkvDType output_dtype,
+                  size_t max_seq_len, void *workspace, size_t workspace_bytes, PkvStream stream,
+                  char *error, size_t error_capacity) {
+    PKV_RANGE("pkv_q8_decode");
+    return pkv::q8_decode("pkv_q8_decode", layer, batch, q_heads, query, scale, output,
+                          output_dtype, max_seq_len, nullptr, workspace, workspace_bytes, stream,
+                          error, error_capacity);
+}
+
+int pkv_q8_decode_mass(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads,
+                       const void *query, float scale, void *output, PkvDType output_dtype,
+                       size_t max_seq_len, float *mass, void *workspace, size_t workspace_bytes,
+                       PkvStream stream, char *error, size_t error_capacity) {
+    PKV_RANGE("pkv_q8_decode_mass");
+    const char *what = "pkv_q8_decode_mass";
+    if (mass == nullptr || (uintptr_t)mass % 4 != 0) {
+        pkv_internal_set_error(error, error_capacity, "%s: mass is null or not 4-byte aligned",
+                               what);
+        return 0;
+    }
+    return pkv::q8_decode(what, layer, batch, q_heads, query, scale, output, output_dtype,
+                          max_seq_len, mass, workspace, workspace_bytes, stream, error,
+                          error_capacity);
+}
+
+// Scratch of the larger of the two kernels behind the mass calls.
+size_t pkv_decode_mass_workspace_bytes(size_t batch, size_t q_heads, size_t kv_heads,
+                                       size_t head_dim, size_t max_seq_len) {
+    if (kv_heads == 0 || q_heads == 0 || q_heads % kv_heads != 0) return 0;
+    const size_t group = q_heads / kv_heads, lanes = pkv::mass_lanes(kv_heads, head_dim);
+    const size_t gv8 = pkv::slots_of(group, head_dim), per = head_dim == 64 ? gv8 / 2 : gv8;
+    const size_t q8 =
+        pkv_q8_decode_workspace_bytes(batch, q_heads, kv_heads, head_dim, max_seq_len) +
+        pkv::mass_scratch_bytes(batch, q_heads, lanes * ((group + per - 1) / per), gv8,
+                                max_seq_len);
+    const size_t half =
+        (pkv_decode_workspace_bytes(batch, q_heads, head_dim, max_seq_len, 0) + 255) / 256 * 256 +
+        pkv::mass_scratch_bytes(batch, q_heads, lanes, head_dim == 64 ? 2 * group : group,
+                                max_seq_len);
+    return q8 > half ? q8 : half;
 }
 
 int pkv_internal_take_q8_decode_fault(uint32_t *code) {

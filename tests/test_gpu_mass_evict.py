@@ -1,0 +1,378 @@
+"""Attention mass of decode steps and eviction by it, on 16-bit and 8-bit
+pages: weights against 64 bits, kept positions and moved rows exactly."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import inference_c_b200 as P
+from inference_c_b200 import workloads as W
+from tests.gpu_cases import PagedCase, to_host_bits, torch_dtype
+from tests.q8_cases import Q8Case, attend64, attend_tol, widen
+
+pytestmark = pytest.mark.gpu
+
+LENGTHS = [0, 1, 17, 128, 129, 400, 1031]
+
+
+def _mass(rng, pages, heads, bs):
+    return rng.random((pages, heads, bs)).astype(np.float32) * 0.05
+
+
+def _rows16(case, which, b, L):
+    pool = getattr(case, which + "pool").reshape(-1, case.block_size, case.kv_heads, case.head_dim)
+    t = np.arange(L)
+    bits = pool[case.tables[b][t // case.block_size].astype(np.int64), t % case.block_size]
+    return widen(bits, case.dtype).astype(np.float64)
+
+
+def _check_mass(tables, lengths, bs, hd, rows, q, scale, before, after, out, out_eps):
+    want_mass, slack = before.astype(np.float64), np.zeros(before.shape)
+    for b, L in enumerate(lengths):
+        L = int(L)
+        if L == 0:
+            assert not out[b].any()
+            continue
+        k, v = rows("k", b, L), rows("v", b, L)
+        want, w, worst = attend64(q[b:b + 1], k, v, scale)
+        vmax = float(np.abs(v).max())
+        assert np.all(np.abs(out[b] - want[0]) <= attend_tol(worst, hd, vmax, want, out_eps)[0])
+        Hkv = k.shape[1]
+        G = q.shape[1] // Hkv
+        # a weight is off by the factor of its score's error (attend_tol), the
+        # sum over the group and the addition by a rounding each
+        delta = (hd + 4) * 2.0 ** -24 * worst * 1.5 + 2.0 ** -21
+        t = np.arange(L)
+        page = tables[b][t // bs].astype(np.int64)
+        for g in range(Hkv):
+            add = w[0, g * G:(g + 1) * G].sum(axis=0)
+            want_mass[page, g, t % bs] += add
+            slack[page, g, t % bs] += add * (2 * delta + (G + 4) * 2.0 ** -24) + 2.0 ** -100
+    slack += np.abs(want_mass) * 2.0 ** -23
+    assert np.all(np.abs(after - want_mass) <= slack)
+    same = slack <= np.abs(want_mass) * 2.0 ** -23  # cells of no position: untouched
+    assert np.array_equal(after[same].view(np.uint32), before[same].view(np.uint32))
+
+
+@pytest.mark.parametrize("q_heads,kv_heads,hd,bs,dtype,out", [
+    (32, 8, 128, 16, "f16", "f32"), (8, 8, 64, 16, "f16", "f16"), (16, 1, 128, 64, "bf16", "f32"),
+    (16, 4, 64, 32, "bf16", "bf16"), (2, 2, 128, 128, "f16", "f32"),
+])
+def test_paged_decode_mass(lib, cuda, q_heads, kv_heads, hd, bs, dtype, out):
+    import torch
+    case = PagedCase(LENGTHS, q_heads, kv_heads, hd, bs, dtype, seed=61, device=cuda)
+    od = torch.float32 if out == "f32" else torch_dtype(out)
+    before = _mass(np.random.default_rng(5), case.pool_pages, kv_heads, bs)
+    mass = torch.from_numpy(before).to(cuda)
+    got = torch.full((len(LENGTHS), q_heads, hd), float("nan"), dtype=od, device=cuda)
+    ws = P.decode_mass_workspace(len(LENGTHS), q_heads, kv_heads, hd, max(LENGTHS))
+    P.paged_decode_mass(case.layer(), case.batch(), case.d_q, got, case.scale, max(LENGTHS), mass,
+                        ws)
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 0
+    # the output is the plain decode's, bit for bit
+    plain = torch.empty_like(got)
+    ws2 = P.decode_workspace(len(LENGTHS), q_heads, hd, max(LENGTHS))
+    P.paged_decode(case.layer(), case.batch(), case.d_q, plain, case.scale, max(LENGTHS), ws2)
+    assert torch.equal(plain, got)
+    q = widen(case.q, dtype).astype(np.float64)
+    # the 16-bit kernel keeps a weight as two 16-bit halves for the output
+    halves = 2.0 ** -16 if dtype == "bf16" else 2.0 ** -21
+    eps = (0 if out == "f32" else torch.finfo(od).eps) + 2 * halves * 4
+    _check_mass(case.tables, case.lengths, bs, hd, lambda w, b, L: _rows16(case, w, b, L), q,
+                case.scale, before, mass.cpu().numpy(), got.double().cpu().numpy(), eps + 2e-5)
+
+
+@pytest.mark.parametrize("q_heads,kv_heads,hd,bs,dtype,out", [
+    (32, 8, 128, 16, "f16", "f32"), (7, 1, 128, 32, "bf16", "bf16"), (15, 3, 64, 16, "f16", "f32"),
+    (48, 3, 64, 64, "bf16", "f32"), (16, 1, 128, 128, "f16", "f32"), (8, 8, 64, 16, "f16", "f16"),
+])
+def test_q8_decode_mass(lib, cuda, q_heads, kv_heads, hd, bs, dtype, out):
+    import torch
+    case = Q8Case(LENGTHS, q_heads, kv_heads, hd, bs, dtype, seed=63, device=cuda)
+    od = torch.float32 if out == "f32" else torch_dtype(out)
+    before = _mass(np.random.default_rng(6), case.k.q.shape[0], kv_heads, bs)
+    mass = torch.from_numpy(before).to(cuda)
+    got = torch.full((len(LENGTHS), q_heads, hd), float("nan"), dtype=od, device=cuda)
+    ws = P.decode_mass_workspace(len(LENGTHS), q_heads, kv_heads, hd, max(LENGTHS))
+    P.q8_decode_mass(case.layer(), case.batch(), case.d_q, got, case.scale, max(LENGTHS), mass, ws)
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 0
+    q = widen(case.qbits, dtype).astype(np.float64)
+    _check_mass(case.tables, case.lengths, bs, hd,
+                lambda w, b, L: getattr(case, w).read64(case.tables[b], L), q, case.scale, before,
+                mass.cpu().numpy(), got.double().cpu().numpy(),
+                0 if out == "f32" else torch.finfo(od).eps)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_mass_of_one_long_sequence_adds_up(lib, cuda, q8):
+    """Many pieces and the merge kernel; over three steps every head's mass
+    grows by three times its query heads (weights sum to one)."""
+    import torch
+    L, steps = 20011, 3
+    if q8:
+        case = Q8Case([L], 16, 2, 128, 16, "f16", seed=65, device=cuda)
+        pages, call, lens = case.k.q.shape[0], P.q8_decode_mass, [L]
+    else:
+        case = PagedCase([L], 16, 2, 128, 16, "f16", seed=65, device=cuda)
+        pages, call = case.pool_pages, P.paged_decode_mass
+    mass = torch.zeros(pages, 2, 16, device=cuda)
+    ws = P.decode_mass_workspace(1, 16, 2, 128, L)
+    out = torch.empty(1, 16, 128, dtype=torch.float32, device=cuda)
+    for _ in range(steps):
+        call(case.layer(), case.batch(), case.d_q, out, case.scale, L, mass, ws)
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 0
+    total = mass.double().sum(dim=(0, 2)).cpu().numpy()
+    # each weight is off by at most 2 delta (attend_tol with worst <= 30)
+    delta = 132 * 2.0 ** -24 * 45 + 2.0 ** -21
+    assert np.all(np.abs(total - steps * 8) <= steps * 8 * (2 * delta + 2.0 ** -20))
+    # a length past the declared bound adds nothing and is reported
+    before = mass.clone()
+    call(case.layer(), case.batch(), case.d_q, out, case.scale, 1000, mass, ws)
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 2 and torch.equal(mass, before)
+
+
+def test_paged_decode_mass_refuses_other_shapes(lib, cuda):
+    import torch
+    case = PagedCase([40], 3, 3, 64, 16, "f16", seed=5, device=cuda)  # odd KV heads of 64
+    ws = P.decode_mass_workspace(1, 3, 3, 64, 40)
+    out = torch.empty(1, 3, 64, dtype=torch.float32, device=cuda)
+    mass = torch.zeros(case.pool_pages, 3, 16, device=cuda)
+    with pytest.raises(P.PkvError, match="even number"):
+        P.paged_decode_mass(case.layer(), case.batch(), case.d_q, out, case.scale, 40, mass, ws)
+    with pytest.raises(ValueError, match="mass"):
+        P.paged_decode_mass(case.layer(), case.batch(), case.d_q, out, case.scale, 40,
+                            mass[:, :2], ws)
+
+
+# ---------------------------------------------------------------------------
+# Eviction
+# ---------------------------------------------------------------------------
+
+def keep_list(mass, L, keep, recent):
+    """mass [L] -> ascending kept positions."""
+    m = min(L, keep)
+    if L <= keep:
+        return np.arange(L)
+    old = L - recent
+    x = mass[:old].astype(np.float64) + 0.0
+    x = np.where(np.isnan(x), -np.inf, x)
+    nan = np.isnan(mass[:old])
+    # lowest last: NaN below everything, then by value, ties by position
+    order = np.lexsort((np.arange(old), -x, nan))
+    return np.sort(np.concatenate([order[:m - recent], np.arange(old, L)]))
+
+
+def _evict_case(q8, lengths, kv_heads, hd, bs, dtype, seed, cuda, keep, extra=3):
+    need = sum(-(-min(int(L), keep) // bs) for L in lengths)
+    if q8:
+        case = Q8Case(lengths, kv_heads, kv_heads, hd, bs, dtype, seed, cuda,
+                      extra_pages=need + extra)
+        pages = case.k.q.shape[0]
+    else:
+        pages = int(sum(-(-int(L) // bs) for L in lengths)) + need + extra
+        case = PagedCase(lengths, kv_heads, kv_heads, hd, bs, dtype, seed, cuda, pool_pages=pages)
+    return case, pages
+
+
+def _run_evict(case, pages, q8, kv_heads, hd, bs, keep, recent, mass, in_place, cuda, max_len):
+    import torch
+    lengths = case.lengths
+    n = len(lengths)
+    if in_place:
+        dst, d_dst = case.tables, None
+    else:
+        used = {int(p) for b, L in enumerate(lengths) for p in case.tables[b][:-(-int(L) // bs)]}
+        free = [p for p in range(pages) if p not in used]
+        width = max(1, max(-(-min(int(L), keep) // bs) for L in lengths))
+        dst, at = np.zeros((n, width), np.uint32), 0
+        for b, L in enumerate(lengths):
+            k = -(-min(int(L), keep) // bs)
+            dst[b, :k] = free[at:at + k]
+            at += k
+        d_dst = torch.from_numpy(dst.view(np.int32)).to(cuda)
+    d_mass = torch.from_numpy(mass).to(cuda)
+    kept = torch.full((n, kv_heads, keep), -7, dtype=torch.int32, device=cuda)
+    P.kv_evict(case.layer(), case.batch(), d_mass, keep, recent, kept, max_len, dst_tables=d_dst)
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 0
+    # ---- the same on the host ----
+    want_kept = np.full((n, kv_heads, keep), -1, np.int32)
+    want_mass = mass.copy()
+    if q8:
+        pools = [(p, p.q.copy(), p.s.copy()) for p in (case.k, case.v)]
+    else:
+        shape = (pages, bs, kv_heads, hd)
+        old = [case.kpool.reshape(shape), case.vpool.reshape(shape)]
+        new = [o.copy() for o in old]
+    for b, L in enumerate(lengths):
+        L = int(L)
+        t = np.arange(L)
+        src = case.tables[b].astype(np.int64)
+        to = dst[b].astype(np.int64)
+        for g in range(kv_heads):
+            pick = keep_list(mass[src[t // bs], g, t % bs], L, keep, recent)
+            m = len(pick)
+            want_kept[b, g, :m] = pick
+            i = np.arange(m)
+            want_mass[to[i // bs], g, i % bs] = mass[src[pick // bs], g, pick % bs]
+            if not q8:
+                for o, w in zip(old, new):
+                    w[to[i // bs], i % bs, g] = o[src[pick // bs], pick % bs, g]
+                continue
+            for pool, q, s in pools:
+                lane, cols = pool._cols(g)
+                for j in range(-(-m // bs)):
+                    idx = pick[j * bs:(j + 1) * bs]
+                    ss = pool.s[src[idx // bs], g]
+                    top = ss.max()
+                    x = pool.q[src[idx // bs], lane, idx % bs, cols].astype(np.float32)
+                    f = (ss / top)[:, None] if top > 0 else np.float32(0)
+                    q[to[j], lane, :len(idx), cols] = np.rint(x * f).astype(np.int8)
+                    s[to[j], g] = top
+    assert np.array_equal(kept.cpu().numpy(), want_kept)
+    assert np.array_equal(d_mass.cpu().numpy().view(np.uint32), want_mass.view(np.uint32))
+    if q8:
+        for (pool, q, s), d_q, d_s in zip(pools, (case.d_kq, case.d_vq), (case.d_ks, case.d_vs)):
+            assert np.array_equal(d_q.cpu().numpy(), q)
+            assert np.array_equal(d_s.cpu().numpy().view(np.uint32), s.view(np.uint32))
+    else:
+        for w, d in zip(new, (case.d_kpool, case.d_vpool)):
+            assert np.array_equal(to_host_bits(d).reshape(w.shape), w)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("kv_heads,hd,bs,dtype,keep,recent", [
+    (8, 128, 16, "f16", 100, 20), (3, 64, 16, "bf16", 64, 64), (2, 128, 64, "bf16", 130, 0),
+    (5, 64, 128, "f16", 1, 0), (1, 128, 32, "f16", 300, 299), (2, 64, 32, "f16", 33, 1),
+])
+def test_evict(lib, cuda, q8, in_place, kv_heads, hd, bs, dtype, keep, recent):
+    lengths = np.array([0, 1, keep, keep + 1, 700, 131, 1500])
+    case, pages = _evict_case(q8, lengths, kv_heads, hd, bs, dtype, 71, cuda, keep)
+    mass = np.random.default_rng(7).random((pages, kv_heads, bs)).astype(np.float32)
+    _run_evict(case, pages, q8, kv_heads, hd, bs, keep, recent, mass, in_place, cuda, 1500)
+
+
+@pytest.mark.parametrize("max_len", [4096, 9000, 1 << 20])  # one CTA, eight, keys not held
+def test_evict_ties_and_odd_masses(lib, cuda, max_len):
+    """Few distinct values (ties to the lower position), signed zeros,
+    infinities and NaN, over every way a list is shared."""
+    lengths = np.array([3000, 4096, 65])
+    case, pages = _evict_case(False, lengths, 2, 64, 16, "f16", 73, cuda, 777)
+    rng = np.random.default_rng(9)
+    mass = rng.choice(np.array([0.0, -0.0, 1.0, 0.5, np.inf, -np.inf, np.nan, -3.0, 1e-42],
+                               np.float32), (pages, 2, 16),
+                      p=[.3, .1, .1, .2, .02, .08, .1, .05, .05])
+    _run_evict(case, pages, False, 2, 64, 16, 777, 50, mass, False, cuda, max_len)
+
+
+def test_evict_long_sequence_shared_list(lib, cuda):
+    lengths = np.array([40000])
+    case, pages = _evict_case(True, lengths, 2, 128, 16, "bf16", 75, cuda, 5000)
+    mass = (np.random.default_rng(11).random((pages, 2, 16)) ** 3).astype(np.float32)
+    _run_evict(case, pages, True, 2, 128, 16, 5000, 128, mass, False, cuda, 40000)
+
+
+def test_evict_bad_pages_are_reported(lib, cuda):
+    import torch
+    case, pages = _evict_case(False, np.array([100]), 2, 128, 16, "f16", 77, cuda, 20)
+    mass = torch.ones(pages, 2, 16, device=cuda)
+    kept = torch.empty(1, 2, 20, dtype=torch.int32, device=cuda)
+    before = case.d_kpool.clone()
+    dst = torch.full((1, 2), pages + 9, dtype=torch.int32, device=cuda)
+    P.kv_evict(case.layer(), case.batch(), mass, 20, 4, kept, 100, dst_tables=dst)
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 1 and torch.equal(case.d_kpool, before)
+    P.kv_evict(case.layer(), case.batch(), mass, 20, 4, kept, 100, dst_tables=dst[:, :1] * 0)
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 2  # the result's second page has no entry
+
+
+def test_evict_refusals(lib, cuda):
+    import torch
+    case, pages = _evict_case(False, np.array([40]), 2, 128, 16, "f16", 79, cuda, 20)
+    mass = torch.ones(pages, 2, 16, device=cuda)
+    kept = torch.empty(1, 2, 20, dtype=torch.int32, device=cuda)
+    with pytest.raises(P.PkvError, match="recent"):
+        P.kv_evict(case.layer(), case.batch(), mass, 20, 21, kept, 40)
+    with pytest.raises(P.PkvError, match="keep"):
+        P.kv_evict(case.layer(), case.batch(), mass, 0, 0, kept[:, :, :0].contiguous(), 40)
+    with pytest.raises(ValueError, match="kept"):
+        P.kv_evict(case.layer(), case.batch(), mass, 19, 2, kept, 40)
+
+
+def test_steps_then_eviction_then_steps(lib, cuda):
+    """A sequence as a server runs it, on 8-bit pages: prompt imported, steps
+    that append, attend and add mass, an eviction in place, more steps."""
+    import torch
+    kv_heads, hd, bs, q_heads, dtype = 2, 128, 16, 8, "f16"
+    prompt, steps, keep = 230, 5, 96
+    case = Q8Case([prompt + steps], q_heads, kv_heads, hd, bs, dtype, seed=81, device=cuda)
+    host_k, host_v = case.k, case.v
+    table = case.tables[0]
+    mass = torch.zeros(case.k.q.shape[0], kv_heads, bs, device=cuda)
+    L_max = prompt + steps
+    ws = P.decode_mass_workspace(1, q_heads, kv_heads, hd, L_max)
+    rows = W.normal_bits(83, (L_max + steps, kv_heads * hd), dtype, stream=5)
+    qs = W.normal_bits(85, (2 * steps, 1, q_heads, hd), dtype, stream=6)
+    from tests.gpu_cases import to_device_bits
+    d_rows, d_q = to_device_bits(rows, dtype, cuda), to_device_bits(qs, dtype, cuda)
+    x = widen(rows, dtype).reshape(-1, kv_heads, hd)
+    lens = torch.tensor([prompt], dtype=torch.int32, device=cuda)
+    batch = P.make_batch(case.d_tables, lens)
+    offs = torch.tensor([0, prompt], dtype=torch.int32, device=cuda)
+    P.q8_import(case.layer(), batch, d_rows[:prompt], d_rows[:prompt], offs)
+    for pool in (host_k, host_v):
+        pool.write(table, 0, x[:prompt])
+    out = torch.empty(1, q_heads, hd, dtype=torch.float32, device=cuda)
+    want_mass = np.zeros((kv_heads, L_max))
+    L = prompt
+
+    def step(i):
+        nonlocal L
+        L += 1
+        lens.fill_(L)
+        r = prompt + i
+        P.q8_append(case.layer(), batch, d_rows[r:r + 1], d_rows[r:r + 1])
+        P.q8_decode_mass(case.layer(), batch, d_q[i], out, case.scale, L_max, mass, ws)
+        torch.cuda.synchronize()
+        for pool in (host_k, host_v):
+            pool.write(table, L - 1, x[r:r + 1])
+        k, v = host_k.read64(table, L), host_v.read64(table, L)
+        want, w, worst = attend64(widen(qs[i], dtype).astype(np.float64), k, v, case.scale)
+        tol = attend_tol(worst, hd, float(np.abs(v).max()), want, 0)
+        assert np.all(np.abs(out.double().cpu().numpy() - want) <= tol)
+        want_mass[:, :L] += w[0].reshape(kv_heads, -1, L).sum(axis=1)
+    for i in range(steps):
+        step(i)
+    case.same_pages()
+    t = np.arange(L)
+    pages = table[t // bs].astype(np.int64)
+    m = np.stack([mass.cpu().numpy()[pages, g, t % bs] for g in range(kv_heads)])
+    assert np.allclose(m, want_mass, rtol=1e-4, atol=1e-7)
+    kept = torch.empty(1, kv_heads, keep, dtype=torch.int32, device=cuda)
+    P.kv_evict(case.layer(), batch, mass, keep, 16, kept, L_max)
+    torch.cuda.synchronize()
+    got = kept.cpu().numpy()[0]
+    for g in range(kv_heads):  # by the device's own mass, then moved on the host
+        assert np.array_equal(got[g], keep_list(m[g], L, keep, 16))
+        for pool in (host_k, host_v):
+            lane, cols = pool._cols(g)
+            src = table[got[g] // bs].astype(np.int64)
+            q, s = pool.q[src, lane, got[g] % bs, cols].astype(np.float32), pool.s[src, g].copy()
+            for j in range(keep // bs):
+                sl = slice(j * bs, (j + 1) * bs)
+                top = s[sl].max()
+                pool.q[int(table[j]), lane, :, cols] = np.rint(q[sl] * (s[sl] / top)[:, None])
+                pool.s[int(table[j]), g] = top
+    case.same_pages()
+    L = keep
+    want_mass[:] = 0
+    for i in range(steps, 2 * steps):
+        step(i)
+    case.same_pages()
+    assert P.device_fault(0) == 0
