@@ -236,7 +236,6 @@ def _handles(st):
     elif c["op"] == "prefill":
         st["ws"] = P.q8_prefill_workspace(st["layer"], c["batch"], st["max_len"])
     elif c["op"] == "evict":
-        st["ws"] = P.evict_workspace(c["batch"], c["kv_heads"], st["max_len"])
         st["dst_batch"] = P.make_batch(st["dst_tables"], st["dst_lens"])
 
 
@@ -257,7 +256,7 @@ def _run_own(st):
         call = P.q8_decode_mass if _is_q8(c) else P.paged_decode_mass
         call(st["layer"], st["batch"], st["q"], st["out"], st["scale"], st["max_len"], st["mass"], st["ws"])
         return [st["out"], st["mass"]]
-    P.kv_evict(st["layer"], st["batch"], st["mass"], c["keep"], c["recent"], st["kept"], st["max_len"], st["ws"],
+    P.kv_evict(st["layer"], st["batch"], st["mass"], c["keep"], c["recent"], st["kept"], st["max_len"],
                dst_tables=st["dst_tables"])
     if _is_q8(c):
         P.q8_gather(st["layer"], st["dst_batch"], st["k_out"], st["v_out"], st["dst_offsets"])
