@@ -16,18 +16,26 @@
 // over tiles.  Bytes past a sequence's length are finite whatever they are and
 // meet digits of zero.
 //
-// Bound by HBM: 2 bytes a token, KV head and column.  One persistent 384-thread
+// Bound by HBM: 2 bytes a token, KV head and column.  One persistent 512-thread
 // CTA per SM:
-//   warp 0      K producer: one TMA box per page (block x 128 bytes, contiguous
-//               in the pool) and the page's scales by cp.async; claims units
-//   warp 1      one thread issues tcgen05.mma: S of tile j, then PV of j - 2
-//   warps 2-5   softmax group of even tiles, warps 6-9 of odd tiles: a 32 KiB
+//   warps 0-3   producers, each every fourth tile: one TMA box per page of K and
+//               of V (block x 128 bytes, contiguous in the pool) and the page's
+//               scales by cp.async.  16 boxes of 2 KiB and their bookkeeping
+//               take one warp some 2000 cycles, in which HBM delivers a tile
+//               and a half, so one warp (or one for K and one for V) cannot
+//               keep up; warp 0 also claims the units
+//   warps 4-7   softmax group of even tiles, warps 8-11 of odd tiles: a 32 KiB
 //               tile streams in half the time of a 16-bit one, and one group's
 //               chain of TMEM load, maximum, exp and digit stores would not
 //               keep up; each group carries its own running maximum, sum and
 //               output, joined when a piece ends
-//   warp 10     V producer
-//   warp 11     query warp: the digits of the next piece's query rows
+//   warps 12, 13 one thread each issues tcgen05.mma, S and PV: a barrier wait
+//               costs a thread some 90 cycles even when it is through and an
+//               issue some 40, nearly a tile's time for one thread with both
+//   warp 14     query warp: the digits of the next piece's query rows
+// Few barriers a tile: s_full(j) (S done) also frees K's slot, o_full(j) (PV
+// done) V's, and p_full(j) (weights written) also says that S(j) and O(j - 4)
+// have been read, which is what S(j + 4) and PV(j) overwrite.
 // Work split: stream-K with a dynamic tail (pkv_sched.cuh), as the 16-bit
 // decode.  A segment is one lane (128 columns) of one sequence: one KV head of
 // head_dim 128, or two of head_dim 64 whose query digits are zero in each
@@ -50,7 +58,10 @@ __device__ uint32_t g_q8_decode_fault;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr size_t kQ8MaxGroup = 16;
-constexpr int kThreads = 384;
+constexpr int kThreads = 512;
+constexpr int kProducers = 4;        // producer warps, one per K slot
+constexpr int kRegsControl = 64, kRegsSoftmax = 192;
+static_assert(256 * kRegsControl + 256 * kRegsSoftmax <= kThreads * 128, "register split");
 constexpr int kMaxBatch = 8192;
 constexpr int kLaunchBatch = 1024;   // sequences of one launch (their prefix lives in smem)
 constexpr int kMaxGrid = 256;
@@ -65,9 +76,11 @@ constexpr float kDigitMax = 8323072.f;  // 127 * 2^16: three signed digits hold 
 template <int GV>
 struct Cfg {
     static constexpr int N = GV == 4 ? 16 : GV == 8 ? 32 : 48;  // B rows (digit-major, padded)
-    static constexpr int STAGES = GV == 4 ? 6 : 5;
+    static constexpr int KS = 4;                // K tiles in the ring, and S and O buffers
+    static constexpr int VS = GV == 4 ? 8 : 6;  // V tiles
     static constexpr uint32_t BT = N * 128;                      // bytes of one B tile
-    static constexpr uint32_t Q_OFF = STAGES * 2 * kTileBytes;
+    static constexpr uint32_t V_OFF = KS * kTileBytes;
+    static constexpr uint32_t Q_OFF = V_OFF + VS * kTileBytes;
     static constexpr uint32_t P_OFF = Q_OFF + 2 * BT;
     static constexpr uint32_t X_OFF = P_OFF + 4 * BT;            // odd group's output
     static constexpr uint32_t SC_OFF = X_OFF + GV * 512;
@@ -178,16 +191,15 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                     const __grid_constant__ CUtensorMap vmap) {
     using namespace sm100;
     using C = Cfg<GV>;
-    constexpr int N = C::N, STAGES = C::STAGES;
+    constexpr int N = C::N, KS = C::KS, VS = C::VS;
     constexpr uint32_t kIdescQK = idesc_s8(128, N, false, false);
     constexpr uint32_t kIdescPV = idesc_s8(128, N, true, false);
     extern __shared__ unsigned char smem_raw[];
     unsigned char *sm = reinterpret_cast<unsigned char *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *bars = reinterpret_cast<uint64_t *>(sm + C::BAR_OFF);
-    uint64_t *kfull = bars, *kempty = bars + 6, *vfull = bars + 12, *vempty = bars + 18;
-    uint64_t *s_full = bars + 24, *s_empty = bars + 28, *p_full = bars + 32;
-    uint64_t *o_full = bars + 36, *o_empty = bars + 40;
+    uint64_t *kfull = bars, *vfull = bars + 8, *s_full = bars + 16, *p_full = bars + 24;
+    uint64_t *o_full = bars + 32;  // one per V slot
     uint64_t *q_full = bars + 44, *q_empty = bars + 46;
     uint64_t *x_full = bars + 48, *x_empty = bars + 49;
     uint64_t *ring_full = bars + 50, *ring_empty = bars + 54;  // .. 57
@@ -210,28 +222,26 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        for (int s = 0; s < STAGES; ++s) {
+        for (int s = 0; s < KS; ++s) {
             mbar_init(&kfull[s], 33);  // TMA bytes, and each lane's scale copies
-            mbar_init(&kempty[s], 1);
+        }
+        for (int s = 0; s < VS; ++s) {
             mbar_init(&vfull[s], 1);
-            mbar_init(&vempty[s], 1);
+            mbar_init(&o_full[s], 1);
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(&s_full[i], 2);
-            mbar_init(&s_empty[i], 128);
             mbar_init(&p_full[i], 128);
-            mbar_init(&o_full[i], 1);
-            mbar_init(&o_empty[i], 128);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&q_full[i], 32);
-            mbar_init(&q_empty[i], 257);  // last QK done, both groups read the scales
+            mbar_init(&q_empty[i], 256);  // both groups saw their last S of the piece
         }
         mbar_init(x_full, 128);
         mbar_init(x_empty, 128);
         for (int i = 0; i < kRing; ++i) {
             mbar_init(&ring_full[i], 1);
-            mbar_init(&ring_empty[i], 5);  // V producer, MMA, query warp, two groups
+            mbar_init(&ring_empty[i], 8);  // three producers, two MMA, query warp, two groups
         }
         *abort_flag = 0;
         fence_mbar_init();
@@ -239,7 +249,7 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
     // B rows past the digits (and, paired, the other head's columns) stay zero
     for (int i = tid; i < (int)(6 * C::BT / 16); i += kThreads)
         reinterpret_cast<uint4 *>(sm + C::Q_OFF)[i] = make_uint4(0, 0, 0, 0);
-    if (warp == 1) {
+    if (warp == 12) {
         tmem_alloc(tmem_slot, C::TMEM_COLS);
         tmem_relinquish();
     }
@@ -265,87 +275,98 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
     if (blockIdx.x == 0 && a.tile_prefix != nullptr)
         for (int b = tid; b <= a.batch; b += kThreads) a.tile_prefix[b] = prefix[b];
 
-    // Block-table entries, 32 at a time (one per lane), as the 16-bit decode.
-    struct Window {
-        int first;
-        uint32_t entry;
-    };
-    auto window_at = [&](const uint32_t *trow, int first) {
-        Window w;
-        w.first = first;
-        w.entry = first + lane < a.table_stride ? __ldg(trow + first + lane) : 0xffffffffu;
-        return w;
-    };
-    // The pages of one tile of one pool into `dst`; K also brings the scales of
-    // both pools (lane: kind = lane / 8, page = lane % 8).
-    auto load_tile = [&](const CUtensorMap *map, uint64_t *bar, unsigned char *dst,
-                         const uint32_t *trow, Window &win, int k, int L, int kl, float *slot) {
-        const int ts = k * kTcTile;
-        const int te = min(L, ts + kTcTile);
-        const int p0 = ts / a.block_size;
-        const int np = (te - ts + a.block_size - 1) / a.block_size;  // 1..8
-        if (p0 < win.first || p0 + np > win.first + 32) win = window_at(trow, p0);
-        const int page = lane & 7;
-        const uint32_t pid = __shfl_sync(0xffffffffu, win.entry, (p0 - win.first + page) & 31);
-        const bool good = page < np && p0 + page < a.table_stride && pid < a.block_count;
-        if (page < np && !good) record_fault(fault, kFaultPageOutOfRange);
-        const unsigned mask = __ballot_sync(0xffffffffu, good && lane < 8);
-        if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)__popc(mask) * a.block_size * 128u);
-        __syncwarp();
-        if (good && lane < 8)
-            tma_load_2d(dst + (uint32_t)page * a.block_size * 128u, map, bar, 0,
-                        (int32_t)((pid * (uint32_t)a.lanes + (uint32_t)kl) *
-                                  (uint32_t)a.block_size));
-        if (slot != nullptr) {
-            const int head = (PAIR ? 2 * kl : kl) + (lane >> 4);
-            const bool want = good && head < a.heads && (PAIR || lane < 16);
-            const float *src = (lane & 8) != 0 ? a.vscales : a.kscales;
-            cp_async4_or_zero(slot + lane, want ? src + (int64_t)pid * a.heads + head : src, want);
-            cp_async_mbar_arrive(bar);
-        }
-    };
-
-    if (warp == 0) {
-        // ---------------------------- K producer ----------------------------
+    const int page_shift = 31 - __clz(a.block_size);
+    if (warp < 4 || warp >= 12) {
+    setmaxnreg_dec<kRegsControl>();
+    if (warp < kProducers) {
+        // ----------------------------- producers -----------------------------
         uint32_t j = 0;
         bool ok = true;
         int u = works ? (int)blockIdx.x : -1;
         for (uint32_t ku = 0;; ++ku) {
             const int rs = (int)(ku % kRing);
-            if (!mbar_wait(&ring_empty[rs], ((ku / kRing) & 1) ^ 1, abort_flag, fault)) ok = false;
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) u = -1;
-            if (lane == 0) {
-                ring[rs] = u;
-                mbar_arrive(&ring_full[rs]);
+            if (warp == 0) {  // publish the unit (-1: no more) to the other roles
+                ok = __all_sync(0xffffffffu, mbar_wait(&ring_empty[rs], ((ku / kRing) & 1) ^ 1,
+                                                       abort_flag, fault)) && ok;
+                if (!ok) u = -1;
+                if (lane == 0) {
+                    ring[rs] = u;
+                    mbar_arrive(&ring_full[rs]);
+                }
+                __syncwarp();
+            } else {
+                if (lane == 0) {
+                    u = mbar_wait(&ring_full[rs], (ku / kRing) & 1, abort_flag, fault) ? ring[rs] : -1;
+                    mbar_arrive(&ring_empty[rs]);
+                }
+                u = __shfl_sync(0xffffffffu, u, 0);
             }
-            __syncwarp();
-            if (u < 0) break;
+            if (u < 0 || !ok) break;
             const int64_t ue = unit_start(sc, u + 1);
             for (int64_t t = unit_start(sc, u); ok && t < ue;) {
                 const Piece P = piece_at(t, ue, prefix, a);
                 t += P.k1 - P.k0;
                 const int L = __ldg(a.seq_lens + P.b);
                 const uint32_t *trow = a.tables + (int64_t)P.b * a.table_stride;
-                Window win = window_at(trow, P.k0 * kTcTile / a.block_size);
-                for (int k = P.k0; k < P.k1; ++k, ++j) {
-                    const int stage = (int)(j % STAGES);
-                    ok = __all_sync(0xffffffffu, mbar_wait(&kempty[stage], ((j / STAGES) & 1) ^ 1,
-                                                           abort_flag, fault));
+                const int kl = P.g / a.subs;
+                const int page = lane & 7;
+                // lane's page of tile k (an invalid id past the table row)
+                auto entry_at = [&](int k) -> uint32_t {
+                    const int at = (k * kTcTile >> page_shift) + page;
+                    return k < P.k1 && at < a.table_stride ? __ldg(trow + at) : 0xffffffffu;
+                };
+                const int first = (int)((warp - j) & 3u);  // this warp's first tile of the piece
+                uint32_t next = entry_at(P.k0 + first);
+                for (int k = P.k0 + first; k < P.k1; k += kProducers) {
+                    const uint32_t jj = j + (uint32_t)(k - P.k0);
+                    const uint32_t ks = jj % KS, vs = jj % VS;
+                    const uint32_t pid = next;
+                    next = entry_at(k + kProducers);
+                    const int rows = min(kTcTile, L - k * kTcTile);
+                    const int np = (rows + a.block_size - 1) >> page_shift;  // 1..8
+                    const bool good = page < np && pid < a.block_count;
+                    if (page < np && !good) record_fault(fault, kFaultPageOutOfRange);
+                    const uint32_t bytes =
+                        (uint32_t)__popc(__ballot_sync(0xffffffffu, good) & 0xffu)
+                        << (page_shift + 7);
+                    // S(j - KS) done: K's slot is free; PV(j - VS): V's
+                    ok = __all_sync(0xffffffffu,
+                                    mbar_wait(&s_full[ks], ((jj / KS) & 1) ^ 1, abort_flag, fault) &&
+                                        mbar_wait(&o_full[vs], ((jj / VS) & 1) ^ 1, abort_flag,
+                                                  fault));
                     if (!ok) break;
-                    load_tile(&kmap, &kfull[stage], sm + stage * 2 * kTileBytes, trow, win, k, L,
-                              P.g / a.subs, scales + (j % kScaleSlots) * 32);
+                    if (lane == 0) mbar_arrive_expect_tx(&kfull[ks], bytes);
+                    if (lane == 8) mbar_arrive_expect_tx(&vfull[vs], bytes);
+                    __syncwarp();
+                    // lanes 0-7 one page of K each, 8-15 of V
+                    const bool is_v = (lane & 8) != 0;
+                    if (good && lane < 16)
+                        tma_load_2d(sm + (is_v ? C::V_OFF + vs * kTileBytes : ks * kTileBytes) +
+                                        ((uint32_t)page << (page_shift + 7)),
+                                    is_v ? &vmap : &kmap, is_v ? &vfull[vs] : &kfull[ks], 0,
+                                    (int32_t)((pid * (uint32_t)a.lanes + (uint32_t)kl)
+                                              << page_shift));
+                    // scales: kind = lane / 8 (K0, V0, K1, V1 of the lane's heads)
+                    const int head = (PAIR ? 2 * kl : kl) + (lane >> 4);
+                    const bool want = good && head < a.heads && (PAIR || lane < 16);
+                    const float *src = is_v ? a.vscales : a.kscales;
+                    cp_async4_or_zero(scales + (jj % kScaleSlots) * 32 + lane,
+                                      want ? src + (int64_t)pid * a.heads + head : src, want);
+                    cp_async_mbar_arrive(&kfull[ks]);
                 }
+                j += (uint32_t)(P.k1 - P.k0);
             }
-            int next = -1;
-            if (ok && sc.rounds > 0 && lane == 0) {
-                const int c = sc.n + (int)atomicAdd(a.claim, 1u);
-                next = c < n_units ? c : -1;
+            if (warp == 0) {
+                int claimed = -1;
+                if (ok && sc.rounds > 0 && lane == 0) {
+                    const int c = sc.n + (int)atomicAdd(a.claim, 1u);
+                    claimed = c < n_units ? c : -1;
+                }
+                u = __shfl_sync(0xffffffffu, claimed, 0);
             }
-            u = __shfl_sync(0xffffffffu, next, 0);
         }
         // the last CTA done claiming zeroes the claim words for the next launch
-        if (sc.rounds > 0 && works && lane == 0) {
+        if (sc.rounds > 0 && works && tid == 0) {
             __threadfence();
             if (atomicAdd(a.claim + 1, 1u) == (uint32_t)sc.n - 1) {
                 atomicExch(a.claim, 0u);
@@ -353,9 +374,9 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
             }
         }
         asm volatile("cp.async.wait_all;\n" ::: "memory");
-    } else if (warp == 10 || warp == 11) {
-        // --------------------- V producer / query warp ---------------------
-        uint32_t j = 0, qi = 0;
+    } else if (warp == 14) {
+        // ----------------------------- query warp -----------------------------
+        uint32_t qi = 0;
         bool ok = true;
         for (uint32_t ku = 0; ok; ++ku) {
             const int rs = (int)(ku % kRing);
@@ -370,160 +391,149 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
             for (int64_t t = unit_start(sc, u); ok && t < ue;) {
                 const Piece P = piece_at(t, ue, prefix, a);
                 t += P.k1 - P.k0;
-                if (warp == 10) {
-                    const int L = __ldg(a.seq_lens + P.b);
-                    const uint32_t *trow = a.tables + (int64_t)P.b * a.table_stride;
-                    Window win = window_at(trow, P.k0 * kTcTile / a.block_size);
-                    for (int k = P.k0; k < P.k1; ++k, ++j) {
-                        const int stage = (int)(j % STAGES);
-                        ok = __all_sync(0xffffffffu,
-                                        mbar_wait(&vempty[stage], ((j / STAGES) & 1) ^ 1,
-                                                  abort_flag, fault));
-                        if (!ok) break;
-                        load_tile(&vmap, &vfull[stage],
-                                  sm + stage * 2 * kTileBytes + kTileBytes, trow, win, k, L,
-                                  P.g / a.subs, nullptr);
-                    }
-                    continue;
-                }
                 // Query digits: lane holds 4 columns of a row (head_dim 64: the
                 // first half warp, at the head's half of the 128 columns).
                 constexpr int HD = PAIR ? 64 : 128;
-                uint2 raw[GV];
-#pragma unroll
-                for (int h = 0; h < GV; ++h) {
-                    const int qh = head_at<GV, PAIR>(a, P.g, h);
-                    raw[h] = make_uint2(0, 0);
-                    if (qh >= 0 && lane * 4 < HD)
-                        raw[h] = __ldg(reinterpret_cast<const uint2 *>(
-                            static_cast<const uint16_t *>(a.query) +
-                            ((int64_t)P.b * a.q_heads + qh) * HD + lane * 4));
-                }
                 ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[qi & 1], ((qi >> 1) & 1) ^ 1,
                                                        abort_flag, fault));
                 if (!ok) break;
                 unsigned char *qb = sm + C::Q_OFF + (qi & 1) * C::BT;
+                for (int h0 = 0; h0 < GV; h0 += 4) {
+                    uint2 raw[4];
 #pragma unroll
-                for (int h = 0; h < GV; ++h) {
-                    float x[4];
-                    if (a.bf16) {
-                        x[0] = __uint_as_float(raw[h].x << 16);
-                        x[1] = __uint_as_float(raw[h].x & 0xffff0000u);
-                        x[2] = __uint_as_float(raw[h].y << 16);
-                        x[3] = __uint_as_float(raw[h].y & 0xffff0000u);
-                    } else {
-                        const float2 lo = __half22float2(*reinterpret_cast<__half2 *>(&raw[h].x));
-                        const float2 hi = __half22float2(*reinterpret_cast<__half2 *>(&raw[h].y));
-                        x[0] = lo.x; x[1] = lo.y; x[2] = hi.x; x[3] = hi.y;
+                    for (int i = 0; i < 4; ++i) {
+                        const int qh = head_at<GV, PAIR>(a, P.g, h0 + i);
+                        raw[i] = make_uint2(0, 0);
+                        if (qh >= 0 && lane * 4 < HD)
+                            raw[i] = __ldg(reinterpret_cast<const uint2 *>(
+                                static_cast<const uint16_t *>(a.query) +
+                                ((int64_t)P.b * a.q_heads + qh) * HD + lane * 4));
                     }
-                    // |x| as ordered integers: infinities and NaN stay the largest
-                    uint32_t top = 0;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(fabsf(x[e])));
-                    top = __reduce_max_sync(0xffffffffu, top);
-                    // f = 2^(21 - exponent of the largest): q f < 2^22, its bits
-                    // down to 2^-21 of the largest kept exactly
-                    const int ex = max((int)(top >> 23), 22);
-                    const float f = top == 0 ? 0.f : __uint_as_float((uint32_t)(275 - ex) << 23);
-                    const float back = __uint_as_float((uint32_t)(ex - 21) << 23);  // 1 / f
-                    uint32_t d[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) d[e] = digits(__float2int_rn(x[e] * f));
-                    if (lane * 4 < HD) {
-                        const uint32_t col = lane * 4 + (PAIR && h >= GV / 2 ? 64 : 0);
-#pragma unroll
-                        for (int k = 0; k < 3; ++k) {  // digit k: most significant first
-                            const int sh = 16 - 8 * k;
-                            uint32_t w = 0;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) w |= ((d[e] >> sh) & 255u) << (8 * e);
-                            *reinterpret_cast<uint32_t *>(qb + sw_byte(k * GV + h, col)) = w;
+                    for (int i = 0; i < 4; ++i) {
+                        const int h = h0 + i;
+                        float x[4];
+                        if (a.bf16) {
+                            x[0] = __uint_as_float(raw[i].x << 16);
+                            x[1] = __uint_as_float(raw[i].x & 0xffff0000u);
+                            x[2] = __uint_as_float(raw[i].y << 16);
+                            x[3] = __uint_as_float(raw[i].y & 0xffff0000u);
+                        } else {
+                            const float2 lo = __half22float2(*reinterpret_cast<__half2 *>(&raw[i].x));
+                            const float2 hi = __half22float2(*reinterpret_cast<__half2 *>(&raw[i].y));
+                            x[0] = lo.x; x[1] = lo.y; x[2] = hi.x; x[3] = hi.y;
                         }
+                        // |x| as ordered integers: infinities and NaN stay the largest
+                        uint32_t top = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(fabsf(x[e])));
+                        top = __reduce_max_sync(0xffffffffu, top);
+                        // f = 2^(21 - exponent of the largest): q f < 2^22, its bits
+                        // down to 2^-21 of the largest kept exactly
+                        const int ex = max((int)(top >> 23), 22);
+                        const float f = top == 0 ? 0.f : __uint_as_float((uint32_t)(275 - ex) << 23);
+                        const float back = __uint_as_float((uint32_t)(ex - 21) << 23);  // 1 / f
+                        uint32_t d[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) d[e] = digits(__float2int_rn(x[e] * f));
+                        if (lane * 4 < HD) {
+                            const uint32_t col = lane * 4 + (PAIR && h >= GV / 2 ? 64 : 0);
+#pragma unroll
+                            for (int k = 0; k < 3; ++k) {  // digit k: most significant first
+                                const int sh = 16 - 8 * k;
+                                uint32_t w = 0;
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) w |= ((d[e] >> sh) & 255u) << (8 * e);
+                                *reinterpret_cast<uint32_t *>(qb + sw_byte(k * GV + h, col)) = w;
+                            }
+                        }
+                        if (lane == 0)
+                            qscale[(qi & 1) * 16 + h] =
+                                top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : back * a.scale_log2;
                     }
-                    if (lane == 0)
-                        qscale[(qi & 1) * 16 + h] =
-                            top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : back * a.scale_log2;
                 }
                 fence_proxy_async_smem();
                 mbar_arrive(&q_full[qi & 1]);
                 ++qi;
             }
         }
-    } else if (warp == 1) {
-        // ------------------------------ MMA issuer ------------------------------
+    } else if (warp == 12 || warp == 13) {
+        // ------------------- MMA issuers: S (warp 12), PV (warp 13) -------------------
         if (lane == 0) {
+            const uint64_t kdesc = sw128_desc(smem_u32(sm), 16, 1024);
+            const uint64_t vdesc = sw128_desc(smem_u32(sm + C::V_OFF), kTileBytes, 1024);
+            const uint64_t qdesc = sw128_desc(smem_u32(sm + C::Q_OFF), 16, 1024);
+            const uint64_t pdesc = sw128_desc(smem_u32(sm + C::P_OFF), 16, 1024);
             uint32_t j = 0, qi = 0;
             bool ok = true;
-            auto issue_pv = [&](uint32_t jp) -> bool {
-                const int stage = (int)(jp % STAGES);
-                const uint32_t buf = jp & 3, par = (jp >> 2) & 1;
-                if (!mbar_wait(&vfull[stage], (jp / STAGES) & 1, abort_flag, fault) ||
-                    !mbar_wait(&p_full[buf], par, abort_flag, fault) ||
-                    !mbar_wait(&o_empty[buf], par ^ 1, abort_flag, fault))
-                    return false;
-                tc_fence_after();
-                const uint32_t vaddr = smem_u32(sm + stage * 2 * kTileBytes + kTileBytes);
-                const uint32_t paddr = smem_u32(sm + C::P_OFF + buf * C::BT);
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk)
-                    mma_i8_ss(tmem + (4 + buf) * N, sw128_desc(vaddr + kk * 4096, kTileBytes, 1024),
-                              sw128_desc(paddr + kk * 32, 16, 1024), kIdescPV, kk > 0);
-                mma_commit(&o_full[buf]);
-                mma_commit(&vempty[stage]);
-                return true;
-            };
             for (uint32_t ku = 0; ok; ++ku) {
                 const int rs = (int)(ku % kRing);
                 int u = -1;
                 if (mbar_wait(&ring_full[rs], (ku / kRing) & 1, abort_flag, fault)) u = ring[rs];
                 mbar_arrive(&ring_empty[rs]);
                 if (u < 0) break;
+                int64_t t = unit_start(sc, u);
                 const int64_t ue = unit_start(sc, u + 1);
-                for (int64_t t = unit_start(sc, u); ok && t < ue;) {
-                    const Piece P = piece_at(t, ue, prefix, a);
-                    t += P.k1 - P.k0;
-                    ok = mbar_wait(&q_full[qi & 1], (qi >> 1) & 1, abort_flag, fault);
-                    const uint32_t qaddr = smem_u32(sm + C::Q_OFF + (qi & 1) * C::BT);
-                    for (int k = P.k0; ok && k < P.k1; ++k, ++j) {
-                        const int stage = (int)(j % STAGES);
-                        const uint32_t buf = j & 3, par = (j >> 2) & 1;
-                        if (!mbar_wait(&kfull[stage], (j / STAGES) & 1, abort_flag, fault) ||
-                            !mbar_wait(&s_empty[buf], par ^ 1, abort_flag, fault)) {
+                if (warp == 13) {  // the pieces' bounds do not matter to PV
+                    for (; ok && t < ue; ++t, ++j) {
+                        const uint32_t stage = j % VS, buf = j & 3;
+                        if (!mbar_wait(&vfull[stage], (j / VS) & 1, abort_flag, fault) ||
+                            !mbar_wait(&p_full[buf], (j >> 2) & 1, abort_flag, fault)) {
                             ok = false;
                             break;
                         }
                         tc_fence_after();
-                        const uint32_t kaddr = smem_u32(sm + stage * 2 * kTileBytes);
-#pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)
-                            mma_i8_ss(tmem + buf * N, sw128_desc(kaddr + kk * 32, 16, 1024),
-                                      sw128_desc(qaddr + kk * 32, 16, 1024), kIdescQK, kk > 0);
+                        const uint64_t ad = vdesc + (uint64_t)(stage * (kTileBytes >> 4));
+                        const uint64_t bd = pdesc + (uint64_t)(buf * (C::BT >> 4));
+                        const uint32_t dst = tmem + (4 + buf) * N;
+                        mma_i8_ss_at<0, 0>(dst, ad, bd, kIdescPV, 0);
+                        mma_i8_ss_at<256, 2>(dst, ad, bd, kIdescPV, 1);
+                        mma_i8_ss_at<512, 4>(dst, ad, bd, kIdescPV, 1);
+                        mma_i8_ss_at<768, 6>(dst, ad, bd, kIdescPV, 1);
+                        mma_commit(&o_full[stage]);
+                    }
+                    continue;
+                }
+                while (ok && t < ue) {
+                    const Piece P = piece_at(t, ue, prefix, a);
+                    t += P.k1 - P.k0;
+                    ok = mbar_wait(&q_full[qi & 1], (qi >> 1) & 1, abort_flag, fault);
+                    const uint64_t bd = qdesc + (uint64_t)((qi & 1) * (C::BT >> 4));
+                    for (int k = P.k0; ok && k < P.k1; ++k, ++j) {
+                        const uint32_t buf = j & 3;
+                        if (!mbar_wait(&kfull[buf], (j >> 2) & 1, abort_flag, fault) ||
+                            !mbar_wait(&p_full[buf], ((j >> 2) & 1) ^ 1, abort_flag, fault)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint64_t ad = kdesc + (uint64_t)(buf * (kTileBytes >> 4));
+                        const uint32_t dst = tmem + buf * N;
+                        mma_i8_ss_at<0, 0>(dst, ad, bd, kIdescQK, 0);
+                        mma_i8_ss_at<2, 2>(dst, ad, bd, kIdescQK, 1);
+                        mma_i8_ss_at<4, 4>(dst, ad, bd, kIdescQK, 1);
+                        mma_i8_ss_at<6, 6>(dst, ad, bd, kIdescQK, 1);
                         mma_commit(&s_full[buf]);
                         // this thread saw the scales land: its own arrival passes
                         // them on to the softmax group
                         mbar_arrive(&s_full[buf]);
-                        mma_commit(&kempty[stage]);
-                        if (k == P.k1 - 1) mma_commit(&q_empty[qi & 1]);
-                        // the lag runs on over piece and unit ends
-                        if (j >= 2 && !issue_pv(j - 2)) ok = false;
                     }
                     ++qi;
                 }
             }
-            if (ok && j >= 2) ok = issue_pv(j - 2);
-            if (ok && j >= 1) ok = issue_pv(j - 1);
         }
         __syncwarp();
+    }
     } else {
+        setmaxnreg_inc<kRegsSoftmax>();
         // ------------------------ softmax group `grp` ------------------------
         // On an abort the groups keep running the same loops and barriers but
         // stop reading TMEM; the fault word already records the failure.
-        const int grp = warp >= 6 ? 1 : 0;
+        const int grp = warp >= 8 ? 1 : 0;
         const int q4 = warp & 3;        // TMEM lane quadrant
         const int row = q4 * 32 + lane; // token of S^T, column of O^T
-        const int wt = tid - 64 - grp * 128;
+        const int wt = tid - 128 - grp * 128;
         const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
-        const int page_shift = 31 - __clz(a.block_size);
         auto group_sync = [&] { named_barrier(1 + grp, 128); };
         uint32_t j = 0, qi = 0;
         bool aborted = false;
@@ -558,13 +568,11 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                     acc[h] = 0.f;
                     qs[h] = qscale[(qi & 1) * 16 + h];
                 }
-                mbar_arrive(&q_empty[qi & 1]);
-                ++qi;
                 // O of this group's previous tile, whose weights were relative
                 // to that tile's maximum and scaled by F = f_prev
                 auto fold = [&](uint32_t jp) {
                     const uint32_t buf = jp & 3;
-                    await(&o_full[buf], (jp >> 2) & 1);
+                    await(&o_full[jp % VS], (jp / VS) & 1);
                     float o[N];
 #pragma unroll
                     for (int i = 0; i < N; ++i) o[i] = 0.f;
@@ -581,7 +589,6 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                         tmem_wait_ld();
                         tc_fence_before();
                     }
-                    mbar_arrive(&o_empty[buf]);
 #pragma unroll
                     for (int h = 0; h < GV; ++h) {
                         const int lo = __float_as_int(o[GV + h]) * 256 + __float_as_int(o[2 * GV + h]);
@@ -625,7 +632,6 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                                           : 0.f;
                         f_cur[e] = top * (1.f / kDigitMax);
                     }
-                    mbar_arrive(&s_empty[buf]);
                     const bool live = row < L - k * kTcTile;
                     // two buffers: a warp writes a tile's maxima only after all
                     // read those of the group's tile before the last
@@ -667,6 +673,8 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
 #pragma unroll
                     for (int e = 0; e < (PAIR ? 2 : 1); ++e) f_prev[e] = f_cur[e];
                 }
+                mbar_arrive(&q_empty[qi & 1]);  // the piece's last S is done in both groups
+                ++qi;
                 if (mine >= 0) fold((uint32_t)mine);
                 // ---- join the groups ----
                 float l[GV];
@@ -798,7 +806,7 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 1) tmem_dealloc(tmem, C::TMEM_COLS);
+    if (warp == 12) tmem_dealloc(tmem, C::TMEM_COLS);
 }
 
 // Merges segments cut into more pieces than the decode kernel joins itself

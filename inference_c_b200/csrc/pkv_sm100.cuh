@@ -188,14 +188,17 @@ __device__ __forceinline__ void mma_f16_ts_at(uint32_t d_tmem, uint32_t a_tmem, 
         "r"(a_tmem), "l"(b_base), "r"(idesc), "r"(accumulate), "n"(ACOL), "n"(BOFF)
         : "memory");
 }
-// D[tmem] (+)= A[smem] * B[smem], kind::i8 (8-bit integers, exact 32-bit sums).
-__device__ __forceinline__ void mma_i8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
-                                          uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A[smem] * B[smem], kind::i8 (8-bit integers, exact 32-bit sums),
+// with k-step offsets as mma_f16_ss_at.
+template <uint32_t AOFF, uint32_t BOFF>
+__device__ __forceinline__ void mma_i8_ss_at(uint32_t d_tmem, uint64_t a_base, uint64_t b_base,
+                                             uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .b64 ad, bd;\n\t"
+        "add.s64 ad, %1, %5;\n\tadd.s64 bd, %2, %6;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], ad, bd, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "l"(a_base), "l"(b_base), "r"(idesc), "r"(accumulate), "n"(AOFF), "n"(BOFF)
         : "memory");
 }
 // Arrive on `bar` once every tcgen05 operation issued so far by this thread
