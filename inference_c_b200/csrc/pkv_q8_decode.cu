@@ -59,7 +59,7 @@ __device__ uint32_t g_q8_decode_fault;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr size_t kQ8MaxGroup = 16;
 constexpr int kThreads = 512;
-constexpr int kProducers = 4;        // producer warps, one per K slot
+constexpr int kProducers = 4;        // producer warps
 constexpr int kRegsControl = 64, kRegsSoftmax = 192;
 static_assert(256 * kRegsControl + 256 * kRegsSoftmax <= kThreads * 128, "register split");
 constexpr int kMaxBatch = 8192;
@@ -70,14 +70,15 @@ constexpr int kMaxUnits = kMaxGrid * (1 + kMaxRounds);
 constexpr size_t kMinUnitTiles = 8;  // smallest dynamic unit
 constexpr int kRing = 4;             // unit ids in flight between the roles
 constexpr int kScaleSlots = 16;      // tiles whose scales are in shared memory
+constexpr int kPending = 64;         // cut pieces a CTA keeps before it takes their tickets
 constexpr uint32_t kTileBytes = 16384;
 constexpr float kDigitMax = 8323072.f;  // 127 * 2^16: three signed digits hold +-this
 
 template <int GV>
 struct Cfg {
     static constexpr int N = GV == 4 ? 16 : GV == 8 ? 32 : 48;  // B rows (digit-major, padded)
-    static constexpr int KS = 4;                // K tiles in the ring, and S and O buffers
-    static constexpr int VS = GV == 4 ? 8 : 6;  // V tiles
+    static constexpr int KS = GV == 4 ? 6 : 5;  // K tiles in the ring
+    static constexpr int VS = GV == 4 ? 6 : 5;  // V tiles (S, P and O have four buffers)
     static constexpr uint32_t BT = N * 128;                      // bytes of one B tile
     static constexpr uint32_t V_OFF = KS * kTileBytes;
     static constexpr uint32_t Q_OFF = V_OFF + VS * kTileBytes;
@@ -86,7 +87,9 @@ struct Cfg {
     static constexpr uint32_t SC_OFF = X_OFF + GV * 512;
     static constexpr uint32_t BAR_OFF = SC_OFF + kScaleSlots * 128;
     static constexpr uint32_t MISC_OFF = BAR_OFF + 512;
-    static constexpr uint32_t PREFIX_OFF = MISC_OFF + 2048 + kInKernelMergeMax * (2 * GV + 1) * 4;
+    // per group: [kInKernelMergeMax][GV] maxima, then sums, then slots
+    static constexpr uint32_t MERGE_WORDS = kInKernelMergeMax * (2 * GV + 1);
+    static constexpr uint32_t PREFIX_OFF = MISC_OFF + 2560 + 2 * MERGE_WORDS * 4;
     static constexpr uint32_t TMEM_COLS = GV == 4 ? 128 : GV == 8 ? 256 : 512;
     static_assert(8 * N <= (int)TMEM_COLS, "tensor memory");
     static size_t smem(int batch) { return PREFIX_OFF + 4u * ((size_t)batch + 1u) + 1024u; }
@@ -206,7 +209,7 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
     unsigned char *misc = sm + C::MISC_OFF;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(misc);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(misc + 4);
-    int *ticket = reinterpret_cast<int *>(misc + 8);
+    int *pend_n = reinterpret_cast<int *>(misc + 8);
     volatile int *group_unit = reinterpret_cast<volatile int *>(misc + 16);  // [2]
     volatile int *ring = reinterpret_cast<volatile int *>(misc + 32);        // [kRing]
     int *scan = reinterpret_cast<int *>(misc + 64);                          // [12]
@@ -215,8 +218,8 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
     float *red = reinterpret_cast<float *>(misc + 384);                      // [2 groups][2][4][16]
     float *lred = reinterpret_cast<float *>(misc + 1408);                    // [2][4][16]
     float *xml = reinterpret_cast<float *>(misc + 1920);                     // [16][m, l]
-    float *mw = reinterpret_cast<float *>(misc + 2048);     // [kInKernelMergeMax][GV] m, then l
-    int *mslot = reinterpret_cast<int *>(mw + 2 * kInKernelMergeMax * GV);
+    int *pend = reinterpret_cast<int *>(misc + 2048);       // [kPending] b << 16 | segment
+    int *last = reinterpret_cast<int *>(misc + 2304);       // [kPending] this CTA merges it
     float *scales = reinterpret_cast<float *>(sm + C::SC_OFF);  // [slot][K0, V0, K1, V1][8]
     int *prefix = reinterpret_cast<int *>(sm + C::PREFIX_OFF);
 
@@ -224,13 +227,13 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
     if (tid == 0) {
         for (int s = 0; s < KS; ++s) {
             mbar_init(&kfull[s], 33);  // TMA bytes, and each lane's scale copies
+            mbar_init(&s_full[s], 2);  // the MMAs, and the issuer that saw the scales
         }
         for (int s = 0; s < VS; ++s) {
             mbar_init(&vfull[s], 1);
             mbar_init(&o_full[s], 1);
         }
         for (int i = 0; i < 4; ++i) {
-            mbar_init(&s_full[i], 2);
             mbar_init(&p_full[i], 128);
         }
         for (int i = 0; i < 2; ++i) {
@@ -500,23 +503,23 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                     ok = mbar_wait(&q_full[qi & 1], (qi >> 1) & 1, abort_flag, fault);
                     const uint64_t bd = qdesc + (uint64_t)((qi & 1) * (C::BT >> 4));
                     for (int k = P.k0; ok && k < P.k1; ++k, ++j) {
-                        const uint32_t buf = j & 3;
-                        if (!mbar_wait(&kfull[buf], (j >> 2) & 1, abort_flag, fault) ||
+                        const uint32_t stage = j % KS, buf = j & 3;
+                        if (!mbar_wait(&kfull[stage], (j / KS) & 1, abort_flag, fault) ||
                             !mbar_wait(&p_full[buf], ((j >> 2) & 1) ^ 1, abort_flag, fault)) {
                             ok = false;
                             break;
                         }
                         tc_fence_after();
-                        const uint64_t ad = kdesc + (uint64_t)(buf * (kTileBytes >> 4));
+                        const uint64_t ad = kdesc + (uint64_t)(stage * (kTileBytes >> 4));
                         const uint32_t dst = tmem + buf * N;
                         mma_i8_ss_at<0, 0>(dst, ad, bd, kIdescQK, 0);
                         mma_i8_ss_at<2, 2>(dst, ad, bd, kIdescQK, 1);
                         mma_i8_ss_at<4, 4>(dst, ad, bd, kIdescQK, 1);
                         mma_i8_ss_at<6, 6>(dst, ad, bd, kIdescQK, 1);
-                        mma_commit(&s_full[buf]);
+                        mma_commit(&s_full[stage]);
                         // this thread saw the scales land: its own arrival passes
                         // them on to the softmax group
-                        mbar_arrive(&s_full[buf]);
+                        mbar_arrive(&s_full[stage]);
                     }
                     ++qi;
                 }
@@ -539,6 +542,89 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
         bool aborted = false;
         auto await = [&](uint64_t *bar, uint32_t par) {
             aborted = aborted || !__all_sync(0xffffffffu, mbar_wait(bar, par, abort_flag, fault));
+        };
+        // Group 0: tickets of the pending pieces; last[i]: this CTA finished the
+        // segment of piece i (its partials are all in memory).
+        int pending = 0;
+        auto take_tickets = [&] {
+            group_sync();  // the group's partials and the list are written
+            if (wt < pending) {
+                const int b = pend[wt] >> 16, g = pend[wt] & 0xffff;
+                const int nt = (prefix[b + 1] - prefix[b]) / a.kv_heads;
+                const int64_t seg = prefix[b] + (int64_t)g * nt;
+                const int u0 = unit_of_tile(sc, seg);
+                const int np = unit_of_tile(sc, seg + nt - 1) - u0 + 1;
+                __threadfence();  // publishes the group's partials (bar.sync is cumulative)
+                last[wt] = atomicAdd(a.counters + u0, 1u) == (uint32_t)(np - 1);
+            }
+            group_sync();
+        };
+        float *mw = reinterpret_cast<float *>(misc + 2560) + grp * C::MERGE_WORDS;
+        int *mslot = reinterpret_cast<int *>(mw + 2 * kInKernelMergeMax * GV);
+        auto merge = [&](int i) {
+            const int b = pend[i] >> 16, g = pend[i] & 0xffff;
+            const int nt = (prefix[b + 1] - prefix[b]) / a.kv_heads;
+            const int64_t seg = prefix[b] + (int64_t)g * nt;
+            const int u0 = unit_of_tile(sc, seg);
+            const int np = unit_of_tile(sc, seg + nt - 1) - u0 + 1;
+            if (np > kInKernelMergeMax) {  // cannot happen with the host's choice of units
+                if (wt == 0) record_fault(fault, kFaultPositionOutOfRange);
+                return;
+            }
+            __threadfence();  // the other CTAs' partials, seen through the ticket
+            for (int e = wt; e < np * GV; e += 128) {
+                const int c = e / GV, h = e - c * GV;
+                const int slot = (u0 + c) * 2 + unit_slot(sc, u0 + c, seg);
+                const float2 ml = __ldcg(reinterpret_cast<const float2 *>(
+                    a.part_ml + ((int64_t)slot * GV + h) * 2));
+                mw[e] = ml.x;
+                mw[kInKernelMergeMax * GV + e] = ml.y;
+                if (h == 0) mslot[c] = slot;
+            }
+            group_sync();
+            if (wt < GV) {
+                float mx = -INFINITY, lt = 0.f;
+                for (int c = 0; c < np; ++c) mx = fmaxf(mx, mw[c * GV + wt]);
+                for (int c = 0; c < np; ++c) {
+                    const float mc = mw[c * GV + wt];
+                    const float f = mc == mx ? 1.f : exp2f(mc - mx);
+                    lt += mw[kInKernelMergeMax * GV + c * GV + wt] * f;
+                    mw[c * GV + wt] = f;
+                }
+                const float inv = lt == 0.f ? 0.f : 1.f / lt;
+                for (int c = 0; c < np; ++c) mw[c * GV + wt] *= inv;
+                const int qh = head_at<GV, PAIR>(a, g, wt);
+                if (a.final_ml != nullptr && qh >= 0) store_ml(a, b, qh, mx, lt);
+            }
+            // 16 loads in flight, the first of them before the weights are known
+            float o[GV];
+#pragma unroll
+            for (int h = 0; h < GV; ++h) o[h] = 0.f;
+            constexpr int AT_ONCE = 16 / GV;
+            for (int c0 = 0; c0 < np; c0 += AT_ONCE) {
+                float v[AT_ONCE][GV];
+#pragma unroll
+                for (int k = 0; k < AT_ONCE; ++k) {
+                    const float *src =
+                        a.part_o + (int64_t)mslot[min(c0 + k, np - 1)] * GV * 128 + row;
+#pragma unroll
+                    for (int h = 0; h < GV; ++h) v[k][h] = __ldcg(src + h * 128);
+                }
+                if (c0 == 0) group_sync();
+#pragma unroll
+                for (int k = 0; k < AT_ONCE; ++k)
+#pragma unroll
+                    for (int h = 0; h < GV; ++h)
+                        if (c0 + k < np) o[h] = fmaf(mw[(c0 + k) * GV + h], v[k][h], o[h]);
+            }
+#pragma unroll
+            for (int h = 0; h < GV; ++h) {
+                const int qh = head_at<GV, PAIR>(a, g, h);
+                if (qh >= 0 && owns<PAIR>(GV, h, row))
+                    store_out(a, out_at<PAIR>(a, b, qh, row), o[h]);
+            }
+            if (wt == 0) a.counters[u0] = 0u;
+            group_sync();  // the scratch is free again
         };
         for (uint32_t ku = 0;; ++ku) {
             const int rs = (int)(ku % kRing);
@@ -600,7 +686,7 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                 for (int k = P.k0; k < P.k1; ++k, ++j) {
                     if ((int)(j & 1) != grp) continue;
                     const uint32_t buf = j & 3;
-                    await(&s_full[buf], (j >> 2) & 1);
+                    await(&s_full[j % KS], (j / KS) & 1);
                     float s[N];
 #pragma unroll
                     for (int i = 0; i < N; ++i) s[i] = 0.f;
@@ -741,59 +827,27 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                             make_float2(m_run[h], l[h]);
                 }
                 if (!a.merge_in_kernel) continue;
-                const int u0 = unit_of_tile(sc, P.seg);
-                const int np = unit_of_tile(sc, P.seg + P.nt - 1) - u0 + 1;
-                group_sync();
-                if (wt == 0) {
-                    __threadfence();
-                    const uint32_t tk = atomicAdd(a.counters + u0, 1u);
-                    *ticket = tk == (uint32_t)(np - 1);
+                if (wt == 0) pend[pending] = P.b << 16 | P.g;
+                if (++pending == kPending) {
+                    take_tickets();
+                    for (int i = 0; i < pending; ++i)
+                        if (last[i]) merge(i);
+                    pending = 0;
                 }
-                group_sync();
-                if (!*ticket) continue;
-                __threadfence();
-                if (np > kInKernelMergeMax) {  // cannot happen with the host's choice of units
-                    if (wt == 0) record_fault(fault, kFaultPositionOutOfRange);
-                    continue;
-                }
-                for (int c = wt; c < np; c += 128) mslot[c] = unit_slot(sc, u0 + c, P.seg);
-                group_sync();
-                for (int i = wt; i < np * GV; i += 128) {
-                    const int c = i / GV, h = i - c * GV;
-                    const float2 ml = __ldcg(reinterpret_cast<const float2 *>(
-                        a.part_ml + (((int64_t)(u0 + c) * 2 + mslot[c]) * GV + h) * 2));
-                    mw[i] = ml.x;
-                    mw[kInKernelMergeMax * GV + i] = ml.y;
-                }
-                group_sync();
-                if (wt < GV) {
-                    float mx = -INFINITY, lt = 0.f;
-                    for (int c = 0; c < np; ++c) mx = fmaxf(mx, mw[c * GV + wt]);
-                    for (int c = 0; c < np; ++c) {
-                        const float mc = mw[c * GV + wt];
-                        const float f = mc == mx ? 1.f : exp2f(mc - mx);
-                        lt += mw[kInKernelMergeMax * GV + c * GV + wt] * f;
-                        mw[c * GV + wt] = f;
-                    }
-                    const float inv = lt == 0.f ? 0.f : 1.f / lt;
-                    for (int c = 0; c < np; ++c) mw[c * GV + wt] *= inv;
-                    const int qh = head_at<GV, PAIR>(a, P.g, wt);
-                    if (a.final_ml != nullptr && qh >= 0) store_ml(a, P.b, qh, mx, lt);
-                }
-                group_sync();
-#pragma unroll
-                for (int h = 0; h < GV; ++h) {
-                    const int qh = head_at<GV, PAIR>(a, P.g, h);
-                    if (qh < 0 || !owns<PAIR>(GV, h, row)) continue;
-                    float o = 0.f;
-                    for (int c = 0; c < np; ++c)
-                        o += mw[c * GV + h] *
-                             __ldcg(a.part_o + (((int64_t)(u0 + c) * 2 + mslot[c]) * GV + h) * 128 + row);
-                    store_out(a, out_at<PAIR>(a, P.b, qh, row), o);
-                }
-                group_sync();
-                if (wt == 0) a.counters[u0] = 0u;
             }
+        }
+        // The tickets of the cut pieces wait until the CTA's work is done: a
+        // fence, a ticket and a merge in mid-stream held both groups, and so
+        // the stream, for about 4 us a unit.
+        if (grp == 0) {
+            take_tickets();
+            if (wt == 0) *pend_n = pending;
+        }
+        named_barrier(3, 256);
+        {
+            int nth = 0;
+            for (int i = 0; i < *pend_n; ++i)
+                if (last[i] && (nth++ & 1) == grp) merge(i);
         }
         // empty sequences: zeros
         if (grp == 0)
