@@ -24,18 +24,20 @@
 //               take one warp some 2000 cycles, in which HBM delivers a tile
 //               and a half, so one warp (or one for K and one for V) cannot
 //               keep up; warp 0 also claims the units
-//   warps 4-7   softmax group of even tiles, warps 8-11 of odd tiles: a 32 KiB
-//               tile streams in half the time of a 16-bit one, and one group's
-//               chain of TMEM load, maximum, exp and digit stores would not
-//               keep up; each group carries its own running maximum, sum and
-//               output, joined when a piece ends
+//   warps 4-7   softmax group of even pairs of tiles, warps 8-11 of odd pairs.
+//               A 32 KiB tile streams in half the time of a 16-bit one, and a
+//               group's chain (TMEM load, maximum over its warps, exp, digit
+//               stores, O of the pair before) is latency: two groups overlap
+//               theirs, and a pair of tiles shares one chain and one O.  Each
+//               group carries its own running maximum, sum and output, a
+//               partial of its own that the merge kernel joins: joining them
+//               when a piece ends made each group wait for the other
 //   warps 12, 13 one thread each issues tcgen05.mma, S and PV: a barrier wait
 //               costs a thread some 90 cycles even when it is through and an
 //               issue some 40, nearly a tile's time for one thread with both
 //   warp 14     query warp: the digits of the next piece's query rows
-// Few barriers a tile: s_full(j) (S done) also frees K's slot, o_full(j) (PV
-// done) V's, and p_full(j) (weights written) also says that S(j) and O(j - 4)
-// have been read, which is what S(j + 4) and PV(j) overwrite.
+// p_full of a pair (weights written) also says that its S and the O of the pair
+// NB before have been read, which is what the next S and this PV overwrite.
 // Work split: stream-K with a dynamic tail (pkv_sched.cuh), as the 16-bit
 // decode.  A segment is one lane (128 columns) of one sequence: one KV head of
 // head_dim 128, or two of head_dim 64 whose query digits are zero in each
@@ -60,17 +62,16 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr size_t kQ8MaxGroup = 16;
 constexpr int kThreads = 512;
 constexpr int kProducers = 4;        // producer warps
-constexpr int kRegsControl = 64, kRegsSoftmax = 192;
+constexpr int kRegsControl = 72, kRegsSoftmax = 184;
 static_assert(256 * kRegsControl + 256 * kRegsSoftmax <= kThreads * 128, "register split");
 constexpr int kMaxBatch = 8192;
-constexpr int kLaunchBatch = 1024;   // sequences of one launch (their prefix lives in smem)
-constexpr int kMaxGrid = 256;
-constexpr int kInKernelMergeMax = 32;
-constexpr int kMaxUnits = kMaxGrid * (1 + kMaxRounds);
+constexpr int kLaunchBatch = 512;    // sequences of one launch: one a thread of the prologue
+static_assert(kLaunchBatch == kThreads && kLaunchBatch <= (int)kMassBatch, "launch");
+constexpr int kMaxGrid = 152;
+constexpr int kMaxPieces = 256;      // of one segment
 constexpr size_t kMinUnitTiles = 8;  // smallest dynamic unit
 constexpr int kRing = 4;             // unit ids in flight between the roles
 constexpr int kScaleSlots = 16;      // tiles whose scales are in shared memory
-constexpr int kPending = 64;         // cut pieces a CTA keeps before it takes their tickets
 constexpr uint32_t kTileBytes = 16384;
 constexpr float kDigitMax = 8323072.f;  // 127 * 2^16: three signed digits hold +-this
 
@@ -78,22 +79,23 @@ template <int GV>
 struct Cfg {
     static constexpr int N = GV == 4 ? 16 : GV == 8 ? 32 : 48;  // B rows (digit-major, padded)
     static constexpr int KS = GV == 4 ? 6 : 5;  // K tiles in the ring
-    static constexpr int VS = GV == 4 ? 6 : 5;  // V tiles (S, P and O have four buffers)
+    static constexpr int VS = GV == 4 ? 6 : 5;  // V tiles
+    static constexpr int NB = GV == 16 ? 2 : 4; // S, P and O buffers, one per pair of tiles
     static constexpr uint32_t BT = N * 128;                      // bytes of one B tile
     static constexpr uint32_t V_OFF = KS * kTileBytes;
     static constexpr uint32_t Q_OFF = V_OFF + VS * kTileBytes;
-    static constexpr uint32_t P_OFF = Q_OFF + 2 * BT;
-    static constexpr uint32_t X_OFF = P_OFF + 4 * BT;            // odd group's output
-    static constexpr uint32_t SC_OFF = X_OFF + GV * 512;
+    static constexpr int QB = GV == 16 ? 2 : 4;                  // query tiles ahead
+    static constexpr uint32_t P_OFF = Q_OFF + QB * BT;
+    static constexpr uint32_t SC_OFF = P_OFF + 2 * NB * BT;
     static constexpr uint32_t BAR_OFF = SC_OFF + kScaleSlots * 128;
     static constexpr uint32_t MISC_OFF = BAR_OFF + 512;
-    // per group: [kInKernelMergeMax][GV] maxima, then sums, then slots
-    static constexpr uint32_t MERGE_WORDS = kInKernelMergeMax * (2 * GV + 1);
-    static constexpr uint32_t PREFIX_OFF = MISC_OFF + 2560 + 2 * MERGE_WORDS * 4;
-    static constexpr uint32_t TMEM_COLS = GV == 4 ? 128 : GV == 8 ? 256 : 512;
-    static_assert(8 * N <= (int)TMEM_COLS, "tensor memory");
-    static size_t smem(int batch) { return PREFIX_OFF + 4u * ((size_t)batch + 1u) + 1024u; }
-    static_assert(PREFIX_OFF + 4u * (kLaunchBatch + 1u) + 1024u <= 232448u, "shared memory");
+    static constexpr uint32_t PREFIX_OFF = MISC_OFF + 2624;
+    static constexpr uint32_t O_COL = 2 * NB * N;                // S of two tiles, then O
+    static constexpr uint32_t TMEM_COLS = GV == 4 ? 256 : 512;
+    static_assert(3 * NB * N <= (int)TMEM_COLS, "tensor memory");
+    // tile prefix and lengths of the sequences
+    static size_t smem(int batch) { return PREFIX_OFF + 4u * (2u * (size_t)batch + 1u) + 1024u; }
+    static_assert(PREFIX_OFF + 4u * (2u * kLaunchBatch + 1u) + 1024u <= 232448u, "shared memory");
 };
 
 struct Q8Args {
@@ -102,11 +104,13 @@ struct Q8Args {
     const void *query;
     void *out;
     const float *kscales, *vscales;
-    uint32_t *counters;      // [kMaxUnits] merge tickets by first unit
     uint32_t *claim;         // [2]
-    float *part_ml;          // [units][2][GV][m, l]
-    float *part_o;           // [units][2][GV][128]
-    int32_t *tile_prefix;    // [batch + 1] for the merge kernel
+    // Partials: [slot][2 groups][GV] of (m, l) and of 128 columns; slots 2 u and
+    // 2 u + 1 are unit u's first and last piece, whole_slot + i segment i whole.
+    float *part_ml, *part_o;
+    int32_t whole_slot;
+    int32_t *tile_prefix;    // [batch + 1] for the merge and the mass kernels
+    Sched *sched;            // for the merge kernel
     int32_t table_stride, batch;
     int32_t kv_heads;        // segments of one sequence (the schedule's name for them)
     int32_t heads;           // KV heads
@@ -115,7 +119,7 @@ struct Q8Args {
     int32_t block_size;
     uint32_t block_count;
     float scale_log2;
-    int32_t merge_in_kernel, min_unit;
+    int32_t min_unit;
     int32_t bf16, out_f32;   // row type; 32-bit outputs
     // Mass (else null): every score by stream tile and slot, and every query
     // head's final maximum and sum (pkv_mass.cuh).
@@ -124,19 +128,21 @@ struct Q8Args {
 };
 
 struct Workspace {
-    size_t claim, counters, prefix, ml, o, total;
+    size_t claim, sched, prefix, ml, o, total;
 };
 
 size_t round_up(size_t v, size_t m) { return (v + m - 1) / m * m; }
 
-Workspace workspace_of(size_t units, size_t gv) {
+// `segments` of the launch's largest batch; a partial is two groups' GV heads.
+Workspace workspace_of(size_t units, size_t segments, size_t gv) {
+    const size_t partials = (2 * units + segments) * 2 * gv;
     Workspace w;
     w.claim = 0;
-    w.counters = 256;
-    w.prefix = w.counters + round_up((size_t)kMaxUnits * 4, 256);
+    w.sched = 256;
+    w.prefix = 512;
     w.ml = w.prefix + round_up(((size_t)kLaunchBatch + 1) * 4, 256);
-    w.o = w.ml + round_up(units * 2 * gv * 8, 256);
-    w.total = w.o + round_up(units * 2 * gv * 512, 256);
+    w.o = w.ml + round_up(partials * 8, 256);
+    w.total = w.o + round_up(partials * 512, 256);
     return w;
 }
 
@@ -194,63 +200,59 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                     const __grid_constant__ CUtensorMap vmap) {
     using namespace sm100;
     using C = Cfg<GV>;
-    constexpr int N = C::N, KS = C::KS, VS = C::VS;
+    constexpr int N = C::N, KS = C::KS, VS = C::VS, NB = C::NB, QB = C::QB;
     constexpr uint32_t kIdescQK = idesc_s8(128, N, false, false);
     constexpr uint32_t kIdescPV = idesc_s8(128, N, true, false);
     extern __shared__ unsigned char smem_raw[];
     unsigned char *sm = reinterpret_cast<unsigned char *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *bars = reinterpret_cast<uint64_t *>(sm + C::BAR_OFF);
-    uint64_t *kfull = bars, *vfull = bars + 8, *s_full = bars + 16, *p_full = bars + 24;
-    uint64_t *o_full = bars + 32;  // one per V slot
-    uint64_t *q_full = bars + 44, *q_empty = bars + 46;
-    uint64_t *x_full = bars + 48, *x_empty = bars + 49;
-    uint64_t *ring_full = bars + 50, *ring_empty = bars + 54;  // .. 57
+    uint64_t *kfull = bars, *kempty = bars + 6, *vfull = bars + 12, *vempty = bars + 18;
+    uint64_t *s_full = bars + 24, *p_full = bars + 28, *o_full = bars + 32;
+    uint64_t *q_full = bars + 36, *q_empty = bars + 40;  // a piece's digits and descriptor
+    uint64_t *ring_full = bars + 44, *ring_empty = bars + 48;
     unsigned char *misc = sm + C::MISC_OFF;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(misc);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(misc + 4);
-    int *pend_n = reinterpret_cast<int *>(misc + 8);
-    volatile int *group_unit = reinterpret_cast<volatile int *>(misc + 16);  // [2]
     volatile int *ring = reinterpret_cast<volatile int *>(misc + 32);        // [kRing]
     int *scan = reinterpret_cast<int *>(misc + 64);                          // [12]
     Sched *sched = reinterpret_cast<Sched *>(misc + 128);
-    float *qscale = reinterpret_cast<float *>(misc + 256);                   // [2][16]
-    float *red = reinterpret_cast<float *>(misc + 384);                      // [2 groups][2][4][16]
-    float *lred = reinterpret_cast<float *>(misc + 1408);                    // [2][4][16]
-    float *xml = reinterpret_cast<float *>(misc + 1920);                     // [16][m, l]
-    int *pend = reinterpret_cast<int *>(misc + 2048);       // [kPending] b << 16 | segment
-    int *last = reinterpret_cast<int *>(misc + 2304);       // [kPending] this CTA merges it
+    float *qscale = reinterpret_cast<float *>(misc + 256);                   // [QB][16]
+    volatile int4 *desc = reinterpret_cast<volatile int4 *>(misc + 512);     // [QB], see below
+    float *red = reinterpret_cast<float *>(misc + 576);                      // [2 groups][2][16][4]
+    float *lred = reinterpret_cast<float *>(misc + 1600);                    // [2 groups][2][4][16]
     float *scales = reinterpret_cast<float *>(sm + C::SC_OFF);  // [slot][K0, V0, K1, V1][8]
     int *prefix = reinterpret_cast<int *>(sm + C::PREFIX_OFF);
+    int *lens = prefix + a.batch + 1;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int s = 0; s < KS; ++s) {
             mbar_init(&kfull[s], 33);  // TMA bytes, and each lane's scale copies
-            mbar_init(&s_full[s], 2);  // the MMAs, and the issuer that saw the scales
+            mbar_init(&kempty[s], 1);
         }
         for (int s = 0; s < VS; ++s) {
             mbar_init(&vfull[s], 1);
-            mbar_init(&o_full[s], 1);
+            mbar_init(&vempty[s], 1);
         }
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < NB; ++i) {
+            mbar_init(&s_full[i], 2);  // the MMAs, and the issuer that saw the scales
+            mbar_init(&o_full[i], 1);
             mbar_init(&p_full[i], 128);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < QB; ++i) {
             mbar_init(&q_full[i], 32);
-            mbar_init(&q_empty[i], 256);  // both groups saw their last S of the piece
+            mbar_init(&q_empty[i], 258);  // both groups saw their last S, both issuers started
         }
-        mbar_init(x_full, 128);
-        mbar_init(x_empty, 128);
         for (int i = 0; i < kRing; ++i) {
             mbar_init(&ring_full[i], 1);
-            mbar_init(&ring_empty[i], 8);  // three producers, two MMA, query warp, two groups
+            mbar_init(&ring_empty[i], 4);  // three producers, query warp
         }
         *abort_flag = 0;
         fence_mbar_init();
     }
     // B rows past the digits (and, paired, the other head's columns) stay zero
-    for (int i = tid; i < (int)(6 * C::BT / 16); i += kThreads)
+    for (int i = tid; i < (int)((QB + 2 * NB) * C::BT / 16); i += kThreads)
         reinterpret_cast<uint4 *>(sm + C::Q_OFF)[i] = make_uint4(0, 0, 0, 0);
     if (warp == 12) {
         tmem_alloc(tmem_slot, C::TMEM_COLS);
@@ -260,23 +262,60 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
         tma_prefetch_desc(&kmap);
         tma_prefetch_desc(&vmap);
     }
+    // Lengths and block tables into L2 while the kernel before this one
+    // finishes (a hint: nothing is read before the wait).
+    {
+        const size_t bytes = (size_t)a.batch * (size_t)a.table_stride * 4u;
+        const char *tb = reinterpret_cast<const char *>(a.tables);
+        for (size_t off = ((size_t)blockIdx.x * kThreads + tid) * 128u; off < bytes;
+             off += (size_t)gridDim.x * kThreads * 128u)
+            prefetch_l2(tb + off);
+        if (tid < a.batch && tid % 32 == 0) prefetch_l2(a.seq_lens + tid);
+    }
     pdl_wait();
     pdl_launch_dependents();
-    build_tile_prefix(a, prefix, scan);
+    // Exclusive prefix of tiles (one sequence a thread), lengths and schedule.
+    {
+        const int len = tid < a.batch ? max(0, __ldg(a.seq_lens + tid)) : 0;
+        const int tiles = (len + kTcTile - 1) / kTcTile * a.kv_heads;
+        int incl = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (lane == 31) scan[warp] = incl;
+        __syncthreads();
+        int before = 0, total = 0;
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; ++w) {
+            const int v = scan[w];
+            if (w < warp) before += v;
+            total += v;
+        }
+        if (tid < a.batch) {
+            prefix[tid] = before + incl - tiles;
+            lens[tid] = len;
+        }
+        if (tid == 0) {
+            prefix[a.batch] = total;
+            make_sched(*sched, total, (int)gridDim.x, a.min_unit);
+        }
+    }
     fence_proxy_async_smem();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const int64_t total_tiles = prefix[a.batch];
-    if (tid == 0) make_sched(*sched, total_tiles, (int)gridDim.x, a.min_unit);
-    __syncthreads();
     const Sched &sc = *sched;
     const bool works = (int)blockIdx.x < sc.n && total_tiles > 0;
     const int n_units = sched_units(sc);
     uint32_t *fault = &g_q8_decode_fault;
-    if (blockIdx.x == 0 && a.tile_prefix != nullptr)
+    if (blockIdx.x == 0) {
         for (int b = tid; b <= a.batch; b += kThreads) a.tile_prefix[b] = prefix[b];
+        if (tid == 0) *a.sched = sc;
+    }
 
     const int page_shift = 31 - __clz(a.block_size);
     if (warp < 4 || warp >= 12) {
@@ -309,7 +348,7 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
             for (int64_t t = unit_start(sc, u); ok && t < ue;) {
                 const Piece P = piece_at(t, ue, prefix, a);
                 t += P.k1 - P.k0;
-                const int L = __ldg(a.seq_lens + P.b);
+                const int L = lens[P.b];
                 const uint32_t *trow = a.tables + (int64_t)P.b * a.table_stride;
                 const int kl = P.g / a.subs;
                 const int page = lane & 7;
@@ -332,30 +371,31 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                     const uint32_t bytes =
                         (uint32_t)__popc(__ballot_sync(0xffffffffu, good) & 0xffu)
                         << (page_shift + 7);
-                    // S(j - KS) done: K's slot is free; PV(j - VS): V's
-                    ok = __all_sync(0xffffffffu,
-                                    mbar_wait(&s_full[ks], ((jj / KS) & 1) ^ 1, abort_flag, fault) &&
-                                        mbar_wait(&o_full[vs], ((jj / VS) & 1) ^ 1, abort_flag,
-                                                  fault));
+                    // lanes 0-7 one page each
+                    const uint32_t off = (uint32_t)page << (page_shift + 7);
+                    const int32_t y =
+                        (int32_t)((pid * (uint32_t)a.lanes + (uint32_t)kl) << page_shift);
+                    ok = __all_sync(0xffffffffu, mbar_wait(&kempty[ks], ((jj / KS) & 1) ^ 1,
+                                                           abort_flag, fault));
                     if (!ok) break;
                     if (lane == 0) mbar_arrive_expect_tx(&kfull[ks], bytes);
-                    if (lane == 8) mbar_arrive_expect_tx(&vfull[vs], bytes);
                     __syncwarp();
-                    // lanes 0-7 one page of K each, 8-15 of V
-                    const bool is_v = (lane & 8) != 0;
-                    if (good && lane < 16)
-                        tma_load_2d(sm + (is_v ? C::V_OFF + vs * kTileBytes : ks * kTileBytes) +
-                                        ((uint32_t)page << (page_shift + 7)),
-                                    is_v ? &vmap : &kmap, is_v ? &vfull[vs] : &kfull[ks], 0,
-                                    (int32_t)((pid * (uint32_t)a.lanes + (uint32_t)kl)
-                                              << page_shift));
+                    if (good && lane < 8)
+                        tma_load_2d(sm + ks * kTileBytes + off, &kmap, &kfull[ks], 0, y);
                     // scales: kind = lane / 8 (K0, V0, K1, V1 of the lane's heads)
                     const int head = (PAIR ? 2 * kl : kl) + (lane >> 4);
                     const bool want = good && head < a.heads && (PAIR || lane < 16);
-                    const float *src = is_v ? a.vscales : a.kscales;
+                    const float *src = (lane & 8) != 0 ? a.vscales : a.kscales;
                     cp_async4_or_zero(scales + (jj % kScaleSlots) * 32 + lane,
                                       want ? src + (int64_t)pid * a.heads + head : src, want);
                     cp_async_mbar_arrive(&kfull[ks]);
+                    ok = __all_sync(0xffffffffu, mbar_wait(&vempty[vs], ((jj / VS) & 1) ^ 1,
+                                                           abort_flag, fault));
+                    if (!ok) break;
+                    if (lane == 0) mbar_arrive_expect_tx(&vfull[vs], bytes);
+                    __syncwarp();
+                    if (good && lane < 8)
+                        tma_load_2d(sm + C::V_OFF + vs * kTileBytes + off, &vmap, &vfull[vs], 0, y);
                 }
                 j += (uint32_t)(P.k1 - P.k0);
             }
@@ -379,6 +419,9 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
         asm volatile("cp.async.wait_all;\n" ::: "memory");
     } else if (warp == 14) {
         // ----------------------------- query warp -----------------------------
+        // Walks the pieces ahead of the issuers and the groups and hands each of
+        // them on as query digits, their scales and a descriptor: tiles (0: no
+        // more), positions left from its first tile, partial slot, stream tile.
         uint32_t qi = 0;
         bool ok = true;
         for (uint32_t ku = 0; ok; ++ku) {
@@ -389,18 +432,34 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                 mbar_arrive(&ring_empty[rs]);
             }
             u = __shfl_sync(0xffffffffu, u, 0);
-            if (u < 0) break;
-            const int64_t ue = unit_start(sc, u + 1);
-            for (int64_t t = unit_start(sc, u); ok && t < ue;) {
+            const int64_t us = u < 0 ? 0 : unit_start(sc, u), ue = u < 0 ? 1 : unit_start(sc, u + 1);
+            for (int64_t t = us; ok && t < ue;) {
+                const uint32_t qb_i = qi % QB;
+                ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[qb_i], ((qi / QB) & 1) ^ 1,
+                                                       abort_flag, fault));
+                if (!ok) break;
+                if (u < 0) {
+                    if (lane == 0) desc[qb_i].x = 0;
+                    mbar_arrive(&q_full[qb_i]);
+                    ok = false;
+                    break;
+                }
                 const Piece P = piece_at(t, ue, prefix, a);
+                if (lane == 0) {
+                    desc[qb_i].x = P.k1 - P.k0;
+                    desc[qb_i].y = lens[P.b] - P.k0 * kTcTile;
+                    // a cut piece is its unit's first or last; a whole segment has
+                    // its own place behind those
+                    desc[qb_i].z = P.k0 == 0 && P.k1 == P.nt
+                                       ? a.whole_slot + P.b * a.kv_heads + P.g
+                                       : u * 2 + (t == us ? 0 : 1);
+                    desc[qb_i].w = (int)t;
+                }
                 t += P.k1 - P.k0;
                 // Query digits: lane holds 4 columns of a row (head_dim 64: the
                 // first half warp, at the head's half of the 128 columns).
                 constexpr int HD = PAIR ? 64 : 128;
-                ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[qi & 1], ((qi >> 1) & 1) ^ 1,
-                                                       abort_flag, fault));
-                if (!ok) break;
-                unsigned char *qb = sm + C::Q_OFF + (qi & 1) * C::BT;
+                unsigned char *qb = sm + C::Q_OFF + qb_i * C::BT;
                 for (int h0 = 0; h0 < GV; h0 += 4) {
                     uint2 raw[4];
 #pragma unroll
@@ -451,12 +510,12 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                             }
                         }
                         if (lane == 0)
-                            qscale[(qi & 1) * 16 + h] =
+                            qscale[qb_i * 16 + h] =
                                 top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : back * a.scale_log2;
                     }
                 }
                 fence_proxy_async_smem();
-                mbar_arrive(&q_full[qi & 1]);
+                mbar_arrive(&q_full[qb_i]);
                 ++qi;
             }
         }
@@ -467,61 +526,55 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
             const uint64_t vdesc = sw128_desc(smem_u32(sm + C::V_OFF), kTileBytes, 1024);
             const uint64_t qdesc = sw128_desc(smem_u32(sm + C::Q_OFF), 16, 1024);
             const uint64_t pdesc = sw128_desc(smem_u32(sm + C::P_OFF), 16, 1024);
-            uint32_t j = 0, qi = 0;
+            uint32_t j = 0, pc = 0;  // tiles, pairs
             bool ok = true;
-            for (uint32_t ku = 0; ok; ++ku) {
-                const int rs = (int)(ku % kRing);
-                int u = -1;
-                if (mbar_wait(&ring_full[rs], (ku / kRing) & 1, abort_flag, fault)) u = ring[rs];
-                mbar_arrive(&ring_empty[rs]);
-                if (u < 0) break;
-                int64_t t = unit_start(sc, u);
-                const int64_t ue = unit_start(sc, u + 1);
-                if (warp == 13) {  // the pieces' bounds do not matter to PV
-                    for (; ok && t < ue; ++t, ++j) {
-                        const uint32_t stage = j % VS, buf = j & 3;
-                        if (!mbar_wait(&vfull[stage], (j / VS) & 1, abort_flag, fault) ||
-                            !mbar_wait(&p_full[buf], (j >> 2) & 1, abort_flag, fault)) {
-                            ok = false;
-                            break;
+            for (uint32_t qi = 0; ok; ++qi) {
+                const uint32_t qb_i = qi % QB;
+                if (!mbar_wait(&q_full[qb_i], (qi / QB) & 1, abort_flag, fault)) break;
+                const int n = desc[qb_i].x;
+                mbar_arrive(&q_empty[qb_i]);
+                if (n == 0) break;
+                const uint64_t qd = qdesc + (uint64_t)(qb_i * (C::BT >> 4));
+                for (int k = 0; ok && k < n; k += 2, ++pc) {
+                    const uint32_t buf = pc % NB;
+                    const int n2 = min(2, n - k);
+                    if (warp == 12) {
+                        ok = mbar_wait(&p_full[buf], ((pc / NB) & 1) ^ 1, abort_flag, fault);
+                        for (int i = 0; ok && i < n2; ++i, ++j) {
+                            const uint32_t stage = j % KS;
+                            ok = mbar_wait(&kfull[stage], (j / KS) & 1, abort_flag, fault);
+                            if (!ok) break;
+                            tc_fence_after();
+                            const uint64_t ad = kdesc + (uint64_t)(stage * (kTileBytes >> 4));
+                            const uint32_t dst = tmem + (2 * buf + i) * N;
+                            mma_i8_ss_at<0, 0>(dst, ad, qd, kIdescQK, 0);
+                            mma_i8_ss_at<2, 2>(dst, ad, qd, kIdescQK, 1);
+                            mma_i8_ss_at<4, 4>(dst, ad, qd, kIdescQK, 1);
+                            mma_i8_ss_at<6, 6>(dst, ad, qd, kIdescQK, 1);
+                            mma_commit(&kempty[stage]);
                         }
-                        tc_fence_after();
-                        const uint64_t ad = vdesc + (uint64_t)(stage * (kTileBytes >> 4));
-                        const uint64_t bd = pdesc + (uint64_t)(buf * (C::BT >> 4));
-                        const uint32_t dst = tmem + (4 + buf) * N;
-                        mma_i8_ss_at<0, 0>(dst, ad, bd, kIdescPV, 0);
-                        mma_i8_ss_at<256, 2>(dst, ad, bd, kIdescPV, 1);
-                        mma_i8_ss_at<512, 4>(dst, ad, bd, kIdescPV, 1);
-                        mma_i8_ss_at<768, 6>(dst, ad, bd, kIdescPV, 1);
-                        mma_commit(&o_full[stage]);
-                    }
-                    continue;
-                }
-                while (ok && t < ue) {
-                    const Piece P = piece_at(t, ue, prefix, a);
-                    t += P.k1 - P.k0;
-                    ok = mbar_wait(&q_full[qi & 1], (qi >> 1) & 1, abort_flag, fault);
-                    const uint64_t bd = qdesc + (uint64_t)((qi & 1) * (C::BT >> 4));
-                    for (int k = P.k0; ok && k < P.k1; ++k, ++j) {
-                        const uint32_t stage = j % KS, buf = j & 3;
-                        if (!mbar_wait(&kfull[stage], (j / KS) & 1, abort_flag, fault) ||
-                            !mbar_wait(&p_full[buf], ((j >> 2) & 1) ^ 1, abort_flag, fault)) {
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
-                        const uint64_t ad = kdesc + (uint64_t)(stage * (kTileBytes >> 4));
-                        const uint32_t dst = tmem + buf * N;
-                        mma_i8_ss_at<0, 0>(dst, ad, bd, kIdescQK, 0);
-                        mma_i8_ss_at<2, 2>(dst, ad, bd, kIdescQK, 1);
-                        mma_i8_ss_at<4, 4>(dst, ad, bd, kIdescQK, 1);
-                        mma_i8_ss_at<6, 6>(dst, ad, bd, kIdescQK, 1);
-                        mma_commit(&s_full[stage]);
+                        mma_commit(&s_full[buf]);
                         // this thread saw the scales land: its own arrival passes
                         // them on to the softmax group
-                        mbar_arrive(&s_full[stage]);
+                        mbar_arrive(&s_full[buf]);
+                    } else {
+                        ok = mbar_wait(&p_full[buf], (pc / NB) & 1, abort_flag, fault);
+                        const uint32_t dst = tmem + C::O_COL + buf * N;
+                        for (int i = 0; ok && i < n2; ++i, ++j) {
+                            const uint32_t stage = j % VS;
+                            ok = mbar_wait(&vfull[stage], (j / VS) & 1, abort_flag, fault);
+                            if (!ok) break;
+                            tc_fence_after();
+                            const uint64_t ad = vdesc + (uint64_t)(stage * (kTileBytes >> 4));
+                            const uint64_t bd = pdesc + (uint64_t)((2 * buf + i) * (C::BT >> 4));
+                            mma_i8_ss_at<0, 0>(dst, ad, bd, kIdescPV, i);
+                            mma_i8_ss_at<256, 2>(dst, ad, bd, kIdescPV, 1);
+                            mma_i8_ss_at<512, 4>(dst, ad, bd, kIdescPV, 1);
+                            mma_i8_ss_at<768, 6>(dst, ad, bd, kIdescPV, 1);
+                            mma_commit(&vempty[stage]);
+                        }
+                        mma_commit(&o_full[buf]);
                     }
-                    ++qi;
                 }
             }
         }
@@ -538,321 +591,183 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
         const int wt = tid - 128 - grp * 128;
         const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
         auto group_sync = [&] { named_barrier(1 + grp, 128); };
-        uint32_t j = 0, qi = 0;
+        uint32_t j = 0, pc = 0;  // tiles, pairs
         bool aborted = false;
         auto await = [&](uint64_t *bar, uint32_t par) {
             aborted = aborted || !__all_sync(0xffffffffu, mbar_wait(bar, par, abort_flag, fault));
         };
-        // Group 0: tickets of the pending pieces; last[i]: this CTA finished the
-        // segment of piece i (its partials are all in memory).
-        int pending = 0;
-        auto take_tickets = [&] {
-            group_sync();  // the group's partials and the list are written
-            if (wt < pending) {
-                const int b = pend[wt] >> 16, g = pend[wt] & 0xffff;
-                const int nt = (prefix[b + 1] - prefix[b]) / a.kv_heads;
-                const int64_t seg = prefix[b] + (int64_t)g * nt;
-                const int u0 = unit_of_tile(sc, seg);
-                const int np = unit_of_tile(sc, seg + nt - 1) - u0 + 1;
-                __threadfence();  // publishes the group's partials (bar.sync is cumulative)
-                last[wt] = atomicAdd(a.counters + u0, 1u) == (uint32_t)(np - 1);
-            }
-            group_sync();
-        };
-        float *mw = reinterpret_cast<float *>(misc + 2560) + grp * C::MERGE_WORDS;
-        int *mslot = reinterpret_cast<int *>(mw + 2 * kInKernelMergeMax * GV);
-        auto merge = [&](int i) {
-            const int b = pend[i] >> 16, g = pend[i] & 0xffff;
-            const int nt = (prefix[b + 1] - prefix[b]) / a.kv_heads;
-            const int64_t seg = prefix[b] + (int64_t)g * nt;
-            const int u0 = unit_of_tile(sc, seg);
-            const int np = unit_of_tile(sc, seg + nt - 1) - u0 + 1;
-            if (np > kInKernelMergeMax) {  // cannot happen with the host's choice of units
-                if (wt == 0) record_fault(fault, kFaultPositionOutOfRange);
-                return;
-            }
-            __threadfence();  // the other CTAs' partials, seen through the ticket
-            for (int e = wt; e < np * GV; e += 128) {
-                const int c = e / GV, h = e - c * GV;
-                const int slot = (u0 + c) * 2 + unit_slot(sc, u0 + c, seg);
-                const float2 ml = __ldcg(reinterpret_cast<const float2 *>(
-                    a.part_ml + ((int64_t)slot * GV + h) * 2));
-                mw[e] = ml.x;
-                mw[kInKernelMergeMax * GV + e] = ml.y;
-                if (h == 0) mslot[c] = slot;
-            }
-            group_sync();
-            if (wt < GV) {
-                float mx = -INFINITY, lt = 0.f;
-                for (int c = 0; c < np; ++c) mx = fmaxf(mx, mw[c * GV + wt]);
-                for (int c = 0; c < np; ++c) {
-                    const float mc = mw[c * GV + wt];
-                    const float f = mc == mx ? 1.f : exp2f(mc - mx);
-                    lt += mw[kInKernelMergeMax * GV + c * GV + wt] * f;
-                    mw[c * GV + wt] = f;
-                }
-                const float inv = lt == 0.f ? 0.f : 1.f / lt;
-                for (int c = 0; c < np; ++c) mw[c * GV + wt] *= inv;
-                const int qh = head_at<GV, PAIR>(a, g, wt);
-                if (a.final_ml != nullptr && qh >= 0) store_ml(a, b, qh, mx, lt);
-            }
-            // 16 loads in flight, the first of them before the weights are known
-            float o[GV];
-#pragma unroll
-            for (int h = 0; h < GV; ++h) o[h] = 0.f;
-            constexpr int AT_ONCE = 16 / GV;
-            for (int c0 = 0; c0 < np; c0 += AT_ONCE) {
-                float v[AT_ONCE][GV];
-#pragma unroll
-                for (int k = 0; k < AT_ONCE; ++k) {
-                    const float *src =
-                        a.part_o + (int64_t)mslot[min(c0 + k, np - 1)] * GV * 128 + row;
-#pragma unroll
-                    for (int h = 0; h < GV; ++h) v[k][h] = __ldcg(src + h * 128);
-                }
-                if (c0 == 0) group_sync();
-#pragma unroll
-                for (int k = 0; k < AT_ONCE; ++k)
-#pragma unroll
-                    for (int h = 0; h < GV; ++h)
-                        if (c0 + k < np) o[h] = fmaf(mw[(c0 + k) * GV + h], v[k][h], o[h]);
-            }
-#pragma unroll
-            for (int h = 0; h < GV; ++h) {
-                const int qh = head_at<GV, PAIR>(a, g, h);
-                if (qh >= 0 && owns<PAIR>(GV, h, row))
-                    store_out(a, out_at<PAIR>(a, b, qh, row), o[h]);
-            }
-            if (wt == 0) a.counters[u0] = 0u;
-            group_sync();  // the scratch is free again
-        };
-        for (uint32_t ku = 0;; ++ku) {
-            const int rs = (int)(ku % kRing);
-            if (wt == 0) {
-                int uu = -1;
-                if (mbar_wait(&ring_full[rs], (ku / kRing) & 1, abort_flag, fault)) uu = ring[rs];
-                group_unit[grp] = uu;
-                mbar_arrive(&ring_empty[rs]);
-            }
-            group_sync();
-            const int u = group_unit[grp];
-            group_sync();
-            if (u < 0) break;
-            const int64_t us = unit_start(sc, u), ue = unit_start(sc, u + 1);
-            for (int64_t t = us; t < ue;) {
-                const Piece P = piece_at(t, ue, prefix, a);
-                const bool first_piece = t == us;
-                t += P.k1 - P.k0;
-                const int L = __ldg(a.seq_lens + P.b);
+        for (uint32_t qi = 0;; ++qi) {
+                const uint32_t qb_i = qi % QB;
+                await(&q_full[qb_i], (qi / QB) & 1);
+                // all warps of the group leave together, also where only some
+                // of them saw a wait give up
+                aborted = named_barrier_or(1 + grp, 128, aborted);
+                const int n = desc[qb_i].x;
+                if (aborted || n == 0) break;
+                const int len = desc[qb_i].y, slot = desc[qb_i].z, tile0 = desc[qb_i].w;
                 float m_run[GV], l_part[GV], acc[GV], alpha_prev[GV], qs[GV];
                 float f_prev[PAIR ? 2 : 1];
-                await(&q_full[qi & 1], (qi >> 1) & 1);
 #pragma unroll
                 for (int h = 0; h < GV; ++h) {
                     m_run[h] = -INFINITY;
                     l_part[h] = 0.f;
                     acc[h] = 0.f;
-                    qs[h] = qscale[(qi & 1) * 16 + h];
+                    qs[h] = qscale[qb_i * 16 + h];
                 }
-                // O of this group's previous tile, whose weights were relative
-                // to that tile's maximum and scaled by F = f_prev
-                auto fold = [&](uint32_t jp) {
-                    const uint32_t buf = jp & 3;
-                    await(&o_full[jp % VS], (jp / VS) & 1);
-                    float o[N];
+                // N columns of TMEM at `col`, this thread's row
+                auto load_cols = [&](uint32_t col, float (&v)[N]) {
 #pragma unroll
-                    for (int i = 0; i < N; ++i) o[i] = 0.f;
-                    if (!aborted) {
-                        tc_fence_after();
-                        if constexpr (N == 48) {
-                            tmem_ld_32x32b<32>(tmem + (4 + buf) * N + lane_off,
-                                               *reinterpret_cast<float(*)[32]>(&o[0]));
-                            tmem_ld_32x32b<16>(tmem + (4 + buf) * N + 32 + lane_off,
-                                               *reinterpret_cast<float(*)[16]>(&o[32]));
-                        } else {
-                            tmem_ld_32x32b<N>(tmem + (4 + buf) * N + lane_off, o);
-                        }
-                        tmem_wait_ld();
-                        tc_fence_before();
-                    }
-#pragma unroll
-                    for (int h = 0; h < GV; ++h) {
-                        const int lo = __float_as_int(o[GV + h]) * 256 + __float_as_int(o[2 * GV + h]);
-                        const float v = fmaf((float)__float_as_int(o[h]), 65536.f, (float)lo);
-                        acc[h] = fmaf(v, f_prev[PAIR && h >= GV / 2 ? 1 : 0], acc[h] * alpha_prev[h]);
+                    for (int i = 0; i < N; ++i) v[i] = 0.f;
+                    if (aborted) return;
+                    if constexpr (N == 48) {
+                        tmem_ld_32x32b<32>(tmem + col + lane_off,
+                                           *reinterpret_cast<float(*)[32]>(&v[0]));
+                        tmem_ld_32x32b<16>(tmem + col + 32 + lane_off,
+                                           *reinterpret_cast<float(*)[16]>(&v[32]));
+                    } else {
+                        tmem_ld_32x32b<N>(tmem + col + lane_off, v);
                     }
                 };
-                int64_t mine = -1;  // this group's previous tile of the piece
-                for (int k = P.k0; k < P.k1; ++k, ++j) {
-                    if ((int)(j & 1) != grp) continue;
-                    const uint32_t buf = j & 3;
-                    await(&s_full[j % KS], (j / KS) & 1);
-                    float s[N];
+                // slot h's number from its three digit sums
+                auto number = [&](const float (&v)[N], int h) -> float {
+                    const int lo = __float_as_int(v[GV + h]) * 256 + __float_as_int(v[2 * GV + h]);
+                    return fmaf((float)__float_as_int(v[h]), 65536.f, (float)lo);
+                };
+                // O of this group's previous pair, whose weights were relative
+                // to that pair's maximum and scaled by F = f_prev
+                auto fold = [&](uint32_t pair) {
+                    const uint32_t buf = pair % NB;
+                    await(&o_full[buf], (pair / NB) & 1);
+                    float o[N];
+                    tc_fence_after();
+                    load_cols(C::O_COL + buf * N, o);
+                    tmem_wait_ld();
+                    tc_fence_before();
 #pragma unroll
-                    for (int i = 0; i < N; ++i) s[i] = 0.f;
-                    if (!aborted) {
-                        tc_fence_after();
-                        if constexpr (N == 48) {
-                            tmem_ld_32x32b<32>(tmem + buf * N + lane_off,
-                                               *reinterpret_cast<float(*)[32]>(&s[0]));
-                            tmem_ld_32x32b<16>(tmem + buf * N + 32 + lane_off,
-                                               *reinterpret_cast<float(*)[16]>(&s[32]));
-                        } else {
-                            tmem_ld_32x32b<N>(tmem + buf * N + lane_off, s);
-                        }
-                        tmem_wait_ld();
-                        tc_fence_before();
-                    }
-                    const float *sl = scales + (j % kScaleSlots) * 32;
-                    float ks[PAIR ? 2 : 1], pf[PAIR ? 2 : 1], f_cur[PAIR ? 2 : 1];
+                    for (int h = 0; h < GV; ++h)
+                        acc[h] = fmaf(number(o, h), f_prev[PAIR && h >= GV / 2 ? 1 : 0],
+                                      acc[h] * alpha_prev[h]);
+                };
+                int64_t mine = -1;  // this group's previous pair of the piece
+                for (int k = 0; k < n; k += 2, ++pc) {
+                    const int n2 = min(2, n - k);
+                    const uint32_t j0 = j;
+                    j += (uint32_t)n2;
+                    if ((int)(pc & 1) != grp) continue;
+                    const uint32_t buf = pc % NB;
+                    await(&s_full[buf], (pc / NB) & 1);
+                    float s[2][N];
+                    tc_fence_after();
+                    load_cols(2 * buf * N, s[0]);
+                    load_cols((2 * buf + 1) * N, s[1]);  // past an odd end: not used
+                    // scales: a token's own, and the largest V scale of the pair
+                    float ks[2][PAIR ? 2 : 1], pf[2][PAIR ? 2 : 1], f_cur[PAIR ? 2 : 1];
+                    const float *sl0 = scales + (j0 % kScaleSlots) * 32;
+                    const float *sl1 = n2 > 1 ? scales + ((j0 + 1) % kScaleSlots) * 32 : sl0;
 #pragma unroll
                     for (int e = 0; e < (PAIR ? 2 : 1); ++e) {
-                        ks[e] = sl[e * 16 + (row >> page_shift)];
-                        const float4 v0 = *reinterpret_cast<const float4 *>(sl + e * 16 + 8);
-                        const float4 v1 = *reinterpret_cast<const float4 *>(sl + e * 16 + 12);
-                        const float top = fmaxf(fmaxf(fmaxf(v0.x, v0.y), fmaxf(v0.z, v0.w)),
-                                                fmaxf(fmaxf(v1.x, v1.y), fmaxf(v1.z, v1.w)));
+                        const float4 v0 = *reinterpret_cast<const float4 *>(sl0 + e * 16 + 8);
+                        const float4 v1 = *reinterpret_cast<const float4 *>(sl0 + e * 16 + 12);
+                        const float4 v2 = *reinterpret_cast<const float4 *>(sl1 + e * 16 + 8);
+                        const float4 v3 = *reinterpret_cast<const float4 *>(sl1 + e * 16 + 12);
+                        const float top = fmaxf(
+                            fmaxf(fmaxf(fmaxf(v0.x, v0.y), fmaxf(v0.z, v0.w)),
+                                  fmaxf(fmaxf(v1.x, v1.y), fmaxf(v1.z, v1.w))),
+                            fmaxf(fmaxf(fmaxf(v2.x, v2.y), fmaxf(v2.z, v2.w)),
+                                  fmaxf(fmaxf(v3.x, v3.y), fmaxf(v3.z, v3.w))));
                         // weight digits: p * vs / top * kDigitMax
-                        pf[e] = top > 0.f ? __fdividef(sl[e * 16 + 8 + (row >> page_shift)], top) *
-                                                kDigitMax
-                                          : 0.f;
+                        const float f = top > 0.f ? __fdividef(kDigitMax, top) : 0.f;
+                        const int at = e * 16 + (row >> page_shift);
+                        ks[0][e] = sl0[at];
+                        ks[1][e] = sl1[at];
+                        pf[0][e] = sl0[at + 8] * f;
+                        pf[1][e] = sl1[at + 8] * f;
                         f_cur[e] = top * (1.f / kDigitMax);
                     }
-                    const bool live = row < L - k * kTcTile;
-                    // two buffers: a warp writes a tile's maxima only after all
-                    // read those of the group's tile before the last
-                    float *myred = red + grp * 128 + ((j >> 1) & 1) * 64;
-                    float x[GV];
+                    tmem_wait_ld();
+                    tc_fence_before();
+                    const int left = len - k * kTcTile;
+                    const bool live0 = row < left, live1 = row + kTcTile < left && n2 > 1;
+                    // two buffers: a warp writes a pair's maxima only after all
+                    // read those of the group's pair before the last
+                    float *myred = red + grp * 128 + ((pc >> 1) & 1) * 64;  // [slot][warp]
+                    float x[2][GV];
 #pragma unroll
                     for (int h = 0; h < GV; ++h) {
-                        const int lo = __float_as_int(s[GV + h]) * 256 + __float_as_int(s[2 * GV + h]);
-                        const float v = fmaf((float)__float_as_int(s[h]), 65536.f, (float)lo);
-                        x[h] = live ? v * (qs[h] * ks[PAIR && h >= GV / 2 ? 1 : 0]) : -INFINITY;
-                        if (a.scores != nullptr && P.seg + k < a.score_tiles)
-                            a.scores[((P.seg + k) * GV + h) * 128 + row] = x[h];
-                        const float wm = redux_max(x[h]);
-                        if (lane == 0) myred[q4 * 16 + h] = wm;
+                        const int e = PAIR && h >= GV / 2 ? 1 : 0;
+                        x[0][h] = live0 ? number(s[0], h) * (qs[h] * ks[0][e]) : -INFINITY;
+                        x[1][h] = live1 ? number(s[1], h) * (qs[h] * ks[1][e]) : -INFINITY;
+                        const float wm = redux_max(fmaxf(x[0][h], x[1][h]));
+                        if (lane == 0) myred[h * 4 + q4] = wm;
                     }
+                    if (a.scores != nullptr)
+                        for (int i = 0; i < n2; ++i)
+                            if (tile0 + k + i < a.score_tiles)
+#pragma unroll
+                                for (int h = 0; h < GV; ++h)
+                                    a.scores[((int64_t)(tile0 + k + i) * GV + h) * 128 + row] =
+                                        i == 0 ? x[0][h] : x[1][h];
+                    if constexpr (NB == 2)  // the weights below overwrite the previous pair's
+                        if (mine >= 0) fold((uint32_t)mine);
                     group_sync();
                     float alpha[GV];
-                    unsigned char *pb = sm + C::P_OFF + buf * C::BT;
+                    unsigned char *pb = sm + C::P_OFF + 2 * buf * C::BT;
 #pragma unroll
                     for (int h = 0; h < GV; ++h) {
-                        const float tmax = fmaxf(fmaxf(myred[h], myred[16 + h]),
-                                                 fmaxf(myred[32 + h], myred[48 + h]));
-                        const float m_new = fmaxf(m_run[h], tmax);
+                        const int e = PAIR && h >= GV / 2 ? 1 : 0;
+                        const float4 r = *reinterpret_cast<const float4 *>(myred + h * 4);
+                        const float m_new =
+                            fmaxf(m_run[h], fmaxf(fmaxf(r.x, r.y), fmaxf(r.z, r.w)));
                         alpha[h] = ex2_fast(m_run[h] - m_new);
                         m_run[h] = m_new;
-                        const float p = ex2_fast(x[h] - m_new);
-                        l_part[h] = fmaf(l_part[h], alpha[h], p);
-                        const uint32_t d = digits(__float2int_rn(p * pf[PAIR && h >= GV / 2 ? 1 : 0]));
-                        pb[sw_byte(h, row)] = (unsigned char)(d >> 16);
-                        pb[sw_byte(GV + h, row)] = (unsigned char)(d >> 8);
-                        pb[sw_byte(2 * GV + h, row)] = (unsigned char)d;
+                        const float p0 = ex2_fast(x[0][h] - m_new);
+                        const float p1 = ex2_fast(x[1][h] - m_new);
+                        l_part[h] = fmaf(l_part[h], alpha[h], p0 + p1);
+                        const uint32_t d0 = digits(__float2int_rn(p0 * pf[0][e]));
+                        const uint32_t d1 = digits(__float2int_rn(p1 * pf[1][e]));
+#pragma unroll
+                        for (int i = 0; i < 3; ++i) {
+                            const uint32_t at = sw_byte(i * GV + h, row);
+                            pb[at] = (unsigned char)(d0 >> (16 - 8 * i));
+                            pb[C::BT + at] = (unsigned char)(d1 >> (16 - 8 * i));
+                        }
                     }
                     fence_proxy_async_smem();
                     mbar_arrive(&p_full[buf]);
-                    if (mine >= 0) fold((uint32_t)mine);
-                    mine = j;
+                    if constexpr (NB != 2)
+                        if (mine >= 0) fold((uint32_t)mine);
+                    mine = pc;
 #pragma unroll
                     for (int h = 0; h < GV; ++h) alpha_prev[h] = alpha[h];
 #pragma unroll
                     for (int e = 0; e < (PAIR ? 2 : 1); ++e) f_prev[e] = f_cur[e];
                 }
-                mbar_arrive(&q_empty[qi & 1]);  // the piece's last S is done in both groups
-                ++qi;
-                if (mine >= 0) fold((uint32_t)mine);
-                // ---- join the groups ----
-                float l[GV];
+                mbar_arrive(&q_empty[qb_i]);  // the piece's last S is done in both groups
+                // ---- this group's partial: the merge kernel joins the groups' ----
+                // (a group without a pair in the piece leaves m = -inf, and no O)
+                float *my_l = lred + grp * 128 + (qi & 1) * 64;
 #pragma unroll
                 for (int h = 0; h < GV; ++h) {
                     const float ls = warp_sum(l_part[h]);
-                    if (lane == 0) lred[grp * 64 + q4 * 16 + h] = ls;
+                    if (lane == 0) my_l[q4 * 16 + h] = ls;
+                }
+                const int64_t at = ((int64_t)slot * 2 + grp) * GV;
+                if (mine >= 0) {
+                    fold((uint32_t)mine);
+#pragma unroll
+                    for (int h = 0; h < GV; ++h) a.part_o[(at + h) * 128 + row] = acc[h];
                 }
                 group_sync();
 #pragma unroll
-                for (int h = 0; h < GV; ++h) {
-                    const float *r = lred + grp * 64 + h;
-                    l[h] = (r[0] + r[16]) + (r[32] + r[48]);
-                }
-                group_sync();
-                float *xo = reinterpret_cast<float *>(sm + C::X_OFF);  // [GV][128]
-                const uint32_t xpar = (qi - 1) & 1;
-                if (grp == 1) {
-                    await(x_empty, xpar ^ 1);
-#pragma unroll
-                    for (int h = 0; h < GV; ++h) {
-                        xo[h * 128 + row] = acc[h];
-                        if (wt == h) {
-                            xml[h * 2] = m_run[h];
-                            xml[h * 2 + 1] = l[h];
-                        }
-                    }
-                    mbar_arrive(x_full);
-                    continue;
-                }
-                await(x_full, xpar);
-#pragma unroll
-                for (int h = 0; h < GV; ++h) {
-                    const float mb = xml[h * 2], lb = xml[h * 2 + 1];
-                    const float m = fmaxf(m_run[h], mb);
-                    // equal maxima keep a factor of 1, both -inf (a query that
-                    // is not a number) included
-                    const float fa = m_run[h] == m ? 1.f : ex2_fast(m_run[h] - m);
-                    const float fb = mb == m ? 1.f : ex2_fast(mb - m);
-                    acc[h] = acc[h] * fa + xo[h * 128 + row] * fb;
-                    l[h] = l[h] * fa + lb * fb;
-                    m_run[h] = m;
-                }
-                mbar_arrive(x_empty);
-                // ---- the piece's output or partial ----
-                if (P.k0 == 0 && P.k1 == P.nt) {
-#pragma unroll
-                    for (int h = 0; h < GV; ++h) {
-                        const int qh = head_at<GV, PAIR>(a, P.g, h);
-                        if (qh >= 0 && owns<PAIR>(GV, h, row))
-                            store_out(a, out_at<PAIR>(a, P.b, qh, row),
-                                      l[h] == 0.f ? 0.f : acc[h] / l[h]);
-                        if (a.final_ml != nullptr && qh >= 0 && wt == h)
-                            store_ml(a, P.b, qh, m_run[h], l[h]);
-                    }
-                    continue;
-                }
-                const int64_t slot = ((int64_t)u * 2 + (first_piece ? 0 : 1)) * GV;
-#pragma unroll
-                for (int h = 0; h < GV; ++h) {
-                    a.part_o[(slot + h) * 128 + row] = acc[h];
+                for (int h = 0; h < GV; ++h)
                     if (wt == h)
-                        *reinterpret_cast<float2 *>(a.part_ml + (slot + h) * 2) =
-                            make_float2(m_run[h], l[h]);
-                }
-                if (!a.merge_in_kernel) continue;
-                if (wt == 0) pend[pending] = P.b << 16 | P.g;
-                if (++pending == kPending) {
-                    take_tickets();
-                    for (int i = 0; i < pending; ++i)
-                        if (last[i]) merge(i);
-                    pending = 0;
-                }
-            }
-        }
-        // The tickets of the cut pieces wait until the CTA's work is done: a
-        // fence, a ticket and a merge in mid-stream held both groups, and so
-        // the stream, for about 4 us a unit.
-        if (grp == 0) {
-            take_tickets();
-            if (wt == 0) *pend_n = pending;
-        }
-        named_barrier(3, 256);
-        {
-            int nth = 0;
-            for (int i = 0; i < *pend_n; ++i)
-                if (last[i] && (nth++ & 1) == grp) merge(i);
+                        *reinterpret_cast<float2 *>(a.part_ml + (at + h) * 2) = make_float2(
+                            m_run[h], (my_l[h] + my_l[16 + h]) + (my_l[32 + h] + my_l[48 + h]));
         }
         // empty sequences: zeros
         if (grp == 0)
             for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
-                if (__ldg(a.seq_lens + b) > 0) continue;
+                if (lens[b] > 0) continue;
                 const int n = a.q_heads * (PAIR ? 64 : 128);
                 for (int i = wt; i < n; i += 128) store_out(a, (int64_t)b * n + i, 0.f);
             }
@@ -863,60 +778,123 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
     if (warp == 12) tmem_dealloc(tmem, C::TMEM_COLS);
 }
 
-// Merges segments cut into more pieces than the decode kernel joins itself
-// (few segments: one long sequence).  Grid (segments * GV, batch), one slot's
-// query head per CTA: four threads a column, each every fourth piece.
-constexpr int kMergeThreads = 512;
-template <int GV, bool PAIR>
-__global__ void __launch_bounds__(kMergeThreads) q8_merge_kernel(const Q8Args a, int grid) {
-    pdl_wait();
+// Joins a segment's partials (two groups' for each of its pieces) into its
+// output; a CTA takes HPC of a segment's query heads: all of them where there
+// are segments enough, one where few long segments have many pieces each.  A merge inside the decode kernel (a fence, a
+// ticket, two rounds of dependent loads: about 5 us) falls to the CTA that ends
+// last, after its own work and once for each of its pieces: 27 us of 200 at 64
+// sequences of 512-32k.  Here all run at once, their CTAs wait on the SMs as the
+// decode's leave them, and the partials' loads go out with those of the weights.
+constexpr int kMergeThreads = 256;
+template <int GV, bool PAIR, int HPC>
+__global__ void __launch_bounds__(kMergeThreads) q8_merge_kernel(const Q8Args a) {
     pdl_launch_dependents();
-    __shared__ float w[kMaxGrid], lsum[kMaxGrid];
-    __shared__ int slot[kMaxGrid];
-    __shared__ float part[4][128];
+    pdl_wait();
+    __shared__ float w[2 * kMaxPieces * HPC];
+    __shared__ int slot[2 * kMaxPieces];
+    __shared__ float4 part[kMergeThreads];
     __shared__ Sched sc;
-    const int b = blockIdx.y, g = blockIdx.x / GV, h = blockIdx.x - g * GV;
-    const int qh = head_at<GV, PAIR>(a, g, h);
-    const int64_t T = a.tile_prefix[a.batch];
-    if (threadIdx.x == 0) make_sched(sc, T, grid, a.min_unit);
+    const int tid = threadIdx.x, lane = tid & 31, b = blockIdx.y;
+    const int g = blockIdx.x / (GV / HPC), h0 = blockIdx.x % (GV / HPC) * HPC;
+    if (HPC == 1 && head_at<GV, PAIR>(a, g, h0) < 0) return;
+    const int first = __ldcg(a.tile_prefix + b), next = __ldcg(a.tile_prefix + b + 1);
+    if (tid < (int)(sizeof(Sched) / 4))
+        reinterpret_cast<int *>(&sc)[tid] = __ldcg(reinterpret_cast<const int *>(a.sched) + tid);
+    if (next == first) return;
     __syncthreads();
-    const int nt = (a.tile_prefix[b + 1] - a.tile_prefix[b]) / a.kv_heads;
-    if (qh < 0 || nt == 0 || T == 0) return;
-    const int64_t seg = a.tile_prefix[b] + (int64_t)g * nt;
+    const int nt = (next - first) / a.kv_heads;
+    const int64_t seg = first + (int64_t)g * nt;
     const int u0 = unit_of_tile(sc, seg);
-    const int np = unit_of_tile(sc, seg + nt - 1) - u0 + 1;
-    if (np == 1 || np > kMaxGrid) return;  // one piece: the decode kernel wrote it
-    for (int c = threadIdx.x; c < np; c += kMergeThreads) {
-        slot[c] = (int)(((int64_t)(u0 + c) * 2 + unit_slot(sc, u0 + c, seg)) * GV + h);
-        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.part_ml + (int64_t)slot[c] * 2));
-        w[c] = ml.x;
-        lsum[c] = ml.y;
+    const int np = (unit_of_tile(sc, seg + nt - 1) - u0 + 1) * 2;  // partials
+    if (np > 2 * kMaxPieces) {  // cannot happen with the host's choice of units
+        if (tid == 0) record_fault(&g_q8_decode_fault, kFaultPositionOutOfRange);
+        return;
     }
+    for (int c = tid; c < np; c += kMergeThreads)
+        slot[c] = (np == 2 ? a.whole_slot + b * a.kv_heads + g
+                           : (u0 + c / 2) * 2 + unit_slot(sc, u0 + c / 2, seg)) *
+                      2 +
+                  (c & 1);
     __syncthreads();
-    if (threadIdx.x < 32) {
-        float mx = -INFINITY, lt = 0.f;
-        for (int c = threadIdx.x; c < np; c += 32) mx = fmaxf(mx, w[c]);
-        mx = warp_max(mx);
-        for (int c = threadIdx.x; c < np; c += 32) {
-            const float f = w[c] == mx ? 1.f : exp2f(w[c] - mx);
-            lt += lsum[c] * f;
-            w[c] = f;
+    // thread: one float4 of the HPC x 128 columns, every SHARES-th partial
+    constexpr int COLS = HPC * 32;
+    constexpr int SHARES = COLS < kMergeThreads ? kMergeThreads / COLS : 1;
+    constexpr int AHEAD = 4;  // partials loaded before the weights are known
+    for (int f0 = 0; f0 < COLS; f0 += kMergeThreads) {
+        const int f = f0 + tid % COLS, share = tid / COLS;
+        auto load = [&](int i) {
+            const int c = share + i * SHARES;
+            return c < np ? __ldcg(reinterpret_cast<const float4 *>(
+                                       a.part_o + ((int64_t)slot[c] * GV + h0) * 128) + f)
+                          : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
+        float4 v[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) v[i] = load(i);
+        if (f0 == 0) {
+            for (int h = tid >> 5; h < HPC; h += kMergeThreads / 32) {  // a warp a head
+                auto ml_at = [&](int c) {
+                    return __ldcg(reinterpret_cast<const float2 *>(
+                        a.part_ml + ((int64_t)slot[c] * GV + h0 + h) * 2));
+                };
+                float mx = -INFINITY, lt = 0.f;
+                for (int c = lane; c < np; c += 32) mx = fmaxf(mx, ml_at(c).x);
+                mx = warp_max(mx);
+                for (int c = lane; c < np; c += 32) {
+                    const float2 ml = ml_at(c);
+                    // a query that is not a number: every m is -inf, l is not 0
+                    const float k = ml.x == mx ? 1.f : exp2f(ml.x - mx);
+                    lt += ml.y == 0.f ? 0.f : ml.y * k;
+                    w[c * HPC + h] = ml.y == 0.f ? 0.f : k;  // nothing there: O was not written
+                }
+                lt = warp_sum(lt);
+                const float inv = lt == 0.f ? 0.f : 1.f / lt;
+                for (int c = lane; c < np; c += 32) w[c * HPC + h] *= inv;
+                const int qh = head_at<GV, PAIR>(a, g, h0 + h);
+                if (a.final_ml != nullptr && qh >= 0 && lane == 0) store_ml(a, b, qh, mx, lt);
+            }
+            __syncthreads();
         }
-        lt = warp_sum(lt);
-        const float inv = lt == 0.f ? 0.f : 1.f / lt;
-        for (int c = threadIdx.x; c < np; c += 32) w[c] *= inv;
-        if (a.final_ml != nullptr && threadIdx.x == 0) store_ml(a, b, qh, mx, lt);
+        const int h = f >> 5;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i0 = 0; share + i0 * SHARES < np; i0 += AHEAD) {
+            if (i0 > 0) {
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) v[i] = load(i0 + i);
+            }
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const int c = share + (i0 + i) * SHARES;
+                const float k = c < np ? w[c * HPC + h] : 0.f;
+                if (k == 0.f) continue;
+                o.x = fmaf(k, v[i].x, o.x);
+                o.y = fmaf(k, v[i].y, o.y);
+                o.z = fmaf(k, v[i].z, o.z);
+                o.w = fmaf(k, v[i].w, o.w);
+            }
+        }
+        if constexpr (SHARES > 1) {
+            part[tid] = o;
+            __syncthreads();
+            if (share > 0) return;
+#pragma unroll
+            for (int k = 1; k < SHARES; ++k) {
+                const float4 r = part[k * COLS + tid];
+                o.x += r.x;
+                o.y += r.y;
+                o.z += r.z;
+                o.w += r.w;
+            }
+        }
+        const int qh = head_at<GV, PAIR>(a, g, h0 + h), d = (f & 31) * 4;
+        if (qh >= 0 && owns<PAIR>(GV, h0 + h, d)) {
+            const int64_t at = out_at<PAIR>(a, b, qh, d);
+            store_out(a, at, o.x);
+            store_out(a, at + 1, o.y);
+            store_out(a, at + 2, o.z);
+            store_out(a, at + 3, o.w);
+        }
     }
-    __syncthreads();
-    const int row = threadIdx.x & 127, share = threadIdx.x >> 7;
-    float o = 0.f;
-#pragma unroll 8
-    for (int c = share; c < np; c += 4) o += w[c] * __ldcg(a.part_o + (int64_t)slot[c] * 128 + row);
-    part[share][row] = o;
-    __syncthreads();
-    if (share == 0 && owns<PAIR>(GV, h, row))
-        store_out(a, out_at<PAIR>(a, b, qh, row),
-                  (part[0][row] + part[1][row]) + (part[2][row] + part[3][row]));
 }
 
 int sm_count() {
@@ -977,12 +955,17 @@ int launch(const Q8Args &a, const CUtensorMap &k, const CUtensorMap &v, int ncta
     cfg.attrs = pdl;
     cfg.numAttrs = 1;
     if (cudaLaunchKernelEx(&cfg, kern, a, k, v) != cudaSuccess) return 0;
-    if (!a.merge_in_kernel) {
-        cfg.gridDim = dim3(a.kv_heads * GV, a.batch);
-        cfg.blockDim = dim3(kMergeThreads);
-        cfg.dynamicSmemBytes = 0;
-        if (cudaLaunchKernelEx(&cfg, q8_merge_kernel<GV, PAIR>, a, ncta) != cudaSuccess) return 0;
-    }
+    // One head a CTA where that makes two CTAs an SM or fewer (one sequence of
+    // 131072, 64 heads: 57 us against 67), else the start of more CTAs costs
+    // more than their parallelism gives (32 sequences, 256 segments: 45 us
+    // against 41 with all heads in one).
+    const bool all_heads = (int64_t)a.kv_heads * GV * a.batch > 2 * ncta;
+    cfg.gridDim = dim3(all_heads ? a.kv_heads : a.kv_heads * GV, a.batch);
+    cfg.blockDim = dim3(kMergeThreads);
+    cfg.dynamicSmemBytes = 0;
+    if ((all_heads ? cudaLaunchKernelEx(&cfg, q8_merge_kernel<GV, PAIR, GV>, a)
+                   : cudaLaunchKernelEx(&cfg, q8_merge_kernel<GV, PAIR, 1>, a)) != cudaSuccess)
+        return 0;
     return cudaGetLastError() == cudaSuccess;
 }
 
@@ -991,6 +974,19 @@ int launch(const Q8Args &a, const CUtensorMap &k, const CUtensorMap &v, int ncta
 size_t slots_of(size_t group, size_t head_dim) {
     const size_t want = head_dim == 64 ? 2 * group : group;
     return want <= 4 ? 4 : want <= 8 ? 8 : 16;
+}
+
+// Segments of one lane: groups above a segment's slots take several.
+size_t subs_of(size_t group, size_t head_dim) {
+    const size_t gv = slots_of(group, head_dim), per = head_dim == 64 ? gv / 2 : gv;
+    return (group + per - 1) / per;
+}
+
+Workspace decode_space(size_t batch, size_t group, size_t kv_heads, size_t head_dim) {
+    const size_t n = batch < (size_t)kLaunchBatch ? batch : (size_t)kLaunchBatch;
+    return workspace_of((size_t)decode_grid() * (1 + kMaxRounds),
+                        n * q8_lanes(kv_heads, head_dim) * subs_of(group, head_dim),
+                        slots_of(group, head_dim));
 }
 
 // pkv_q8_decode, and with `mass` pkv_q8_decode_mass.
@@ -1031,11 +1027,10 @@ int q8_decode(const char *what, const PkvQ8Layer *layer, const PkvBatch *batch, 
         return 0;
     }
     const size_t group = q_heads / kvh, gv = slots_of(group, hd);
-    const size_t per = hd == 64 ? gv / 2 : gv;         // slots per KV head
-    const size_t subs = (group + per - 1) / per;
+    const size_t subs = subs_of(group, hd);
     const size_t segs = lanes * subs;
     const int ncta = decode_grid();
-    const Workspace ws = workspace_of((size_t)ncta * (1 + kMaxRounds), gv);
+    const Workspace ws = decode_space(batch->batch, group, kvh, hd);
     const size_t need =
         ws.total + (mass == nullptr ? 0
                                     : mass_scratch_bytes(batch->batch, q_heads, segs, gv,
@@ -1059,10 +1054,11 @@ int q8_decode(const char *what, const PkvQ8Layer *layer, const PkvBatch *batch, 
     a.kscales = layer->key_scales;
     a.vscales = layer->value_scales;
     a.claim = reinterpret_cast<uint32_t *>(base + ws.claim);
-    a.counters = reinterpret_cast<uint32_t *>(base + ws.counters);
     a.part_ml = reinterpret_cast<float *>(base + ws.ml);
     a.part_o = reinterpret_cast<float *>(base + ws.o);
+    a.whole_slot = 2 * ncta * (1 + kMaxRounds);
     a.tile_prefix = reinterpret_cast<int32_t *>(base + ws.prefix);
+    a.sched = reinterpret_cast<Sched *>(base + ws.sched);
     a.table_stride = (int32_t)batch->table_stride;
     a.kv_heads = (int32_t)segs;
     a.heads = (int32_t)kvh;
@@ -1080,15 +1076,12 @@ int q8_decode(const char *what, const PkvQ8Layer *layer, const PkvBatch *batch, 
     a.scores = ms.scores;
     a.final_ml = ms.final_ml;
     a.score_tiles = ms.tiles;
-    // The 16-bit decode's rules: join in the kernel when a segment meets few
-    // CTAs and there are many segments; dynamic units only then, none so small
-    // that a segment of max_seq_len meets more than kInKernelMergeMax of them.
-    const bool fits = ncta / (int)segs + 2 <= kInKernelMergeMax;
-    a.merge_in_kernel = fits && batch->batch * segs * 2 >= (size_t)ncta;
-    const size_t by_pieces = ((max_seq_len + kTcTile - 1) / kTcTile + 23) / 24;
-    a.min_unit = a.merge_in_kernel ? (int32_t)(by_pieces > kMinUnitTiles ? by_pieces
-                                                                              : kMinUnitTiles)
-                                   : 0;
+    // Pieces of one segment: the dynamic tail is at most a quarter of the
+    // stream, so static units hold 3/4 of T / ncta tiles or more and a segment
+    // meets at most 4/3 ncta + 2 <= 205 of them; min_unit is chosen so that a
+    // segment of max_seq_len meets at most 42 dynamic ones: kMaxPieces holds.
+    const size_t by_pieces = (max_seq_len + kTcTile - 1) / kTcTile / 40 + 1;
+    a.min_unit = (int32_t)(by_pieces > kMinUnitTiles ? by_pieces : kMinUnitTiles);
     const size_t osz = a.out_f32 ? 4 : 2;
     int ok = 1;
     for (size_t b0 = 0; ok && b0 < batch->batch; b0 += kLaunchBatch) {
@@ -1131,9 +1124,7 @@ extern "C" {
 size_t pkv_q8_decode_workspace_bytes(size_t batch, size_t q_heads, size_t kv_heads,
                                      size_t head_dim, size_t max_seq_len) {
     if (kv_heads == 0 || q_heads == 0 || q_heads % kv_heads != 0) return 0;
-    return pkv::workspace_of((size_t)pkv::decode_grid() * (1 + pkv::kMaxRounds),
-                             pkv::slots_of(q_heads / kv_heads, head_dim))
-        .total;
+    return pkv::decode_space(batch, q_heads / kv_heads, kv_heads, head_dim).total;
 }
 
 int pkv_q8_decode(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads,
@@ -1167,11 +1158,10 @@ size_t pkv_decode_mass_workspace_bytes(size_t batch, size_t q_heads, size_t kv_h
                                        size_t head_dim, size_t max_seq_len) {
     if (kv_heads == 0 || q_heads == 0 || q_heads % kv_heads != 0) return 0;
     const size_t group = q_heads / kv_heads, lanes = pkv::mass_lanes(kv_heads, head_dim);
-    const size_t gv8 = pkv::slots_of(group, head_dim), per = head_dim == 64 ? gv8 / 2 : gv8;
     const size_t q8 =
         pkv_q8_decode_workspace_bytes(batch, q_heads, kv_heads, head_dim, max_seq_len) +
-        pkv::mass_scratch_bytes(batch, q_heads, lanes * ((group + per - 1) / per), gv8,
-                                max_seq_len);
+        pkv::mass_scratch_bytes(batch, q_heads, lanes * pkv::subs_of(group, head_dim),
+                                pkv::slots_of(group, head_dim), max_seq_len);
     const size_t half =
         (pkv_decode_workspace_bytes(batch, q_heads, head_dim, max_seq_len, 0) + 255) / 256 * 256 +
         pkv::mass_scratch_bytes(batch, q_heads, lanes, head_dim == 64 ? 2 * group : group,
