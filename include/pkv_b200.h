@@ -311,10 +311,10 @@ int pkv_q8_evict(const PkvQ8Layer *layer, const PkvBatch *batch, float *mass, si
                  size_t recent, const uint32_t *dst_tables, size_t dst_stride, int32_t *kept,
                  size_t max_seq_len, PkvStream stream, char *error, size_t error_capacity);
 
-/* pkv_paged_prefill over 8-bit pages; max_seq_len bounds seq_lens (fault
- * code 2 and no keys for a longer sequence).  The pages are widened to
- * layer->dtype (q * s, one rounding) in the workspace first, so scores and
- * outputs are those of a 16-bit cache of the gathered rows.  The byte count is
+/* pkv_paged_prefill over 8-bit pages; scale must be positive.  max_seq_len
+ * bounds seq_lens (fault code 2 and no keys for a longer sequence).  The pages'
+ * 8-bit numbers are widened to 16-bit rows in the workspace first (exact) and
+ * the scales applied to scores and weights.  The byte count is
  * for the whole batch; a smaller workspace that holds at least one sequence
  * (the count for batch 1) also works and runs the batch in parts. */
 size_t pkv_q8_prefill_workspace_bytes(size_t batch, size_t kv_heads, size_t head_dim,

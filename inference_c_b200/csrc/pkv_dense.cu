@@ -291,7 +291,8 @@ int pkv_sdpa_f16(const void *query, const void *key, const void *value,
                                          (size_t)(S * (int64_t)q_len), q_len, scale, causal,
                                          output, PKV_DTYPE_F16,
                                          static_cast<const uint16_t *>(additive_mask), kv_len,
-                                         q_len > kv_len, 1, stream, error, error_capacity, what);
+                                         q_len > kv_len, 1, nullptr, stream, error, error_capacity,
+                                         what);
 }
 
 int pkv_sdpa_f16_host(const uint16_t *query, const uint16_t *key, const uint16_t *value,

@@ -76,20 +76,30 @@ int pkv_internal_plant_prefill_fault(uint32_t code);
 void pkv_internal_comm_set_probe(PkvComm *comm, int (*probe)(void *arg, PkvStream stream),
                                  void *arg);
 
+/* 8-bit pages widened to whole numbers in 16-bit rows (exact), for the prefill:
+ * per sequence, KV head and 16 keys the K scale, log2 of the V scale and its
+ * inverse ([batch][kv_heads][stride]; scales of 0 stand as 1, their rows are
+ * zeros).  Device pointers, 16-byte aligned rows, stride a multiple of 8. */
+typedef struct {
+    const float *k, *v_log2, *v_inverse;
+    size_t stride;
+} PkvRowScales;
+
 /* pkv_paged_prefill with the general options the dense SDPA needs: an
  * additive FP16 mask [query row of the chunk][key] with a row stride in
  * elements (NULL: none), dense mode (a chunk may be longer than its
  * sequence; the causal offset kv_len - q_len clamps at 0), and the dense
  * layout (query and output are [sequences * q_heads][max_query_len][128],
  * every sequence holding max_query_len rows, read and written in place).
- * Errors name `what`. */
+ * `scales` non-null: K and V are 8-bit rows widened to 16 bits (no mask, not
+ * dense, scale > 0).  Errors name `what`. */
 int pkv_internal_paged_prefill_ex(const PkvPagedLayer *layer, const PkvBatch *batch,
                                   size_t q_heads, const int32_t *query_offsets, const void *query,
                                   size_t total_query_rows, size_t max_query_len, float scale,
                                   int causal, void *output, PkvDType output_dtype,
                                   const uint16_t *mask, size_t mask_stride, int dense,
-                                  int dense_layout, PkvStream stream, char *error,
-                                  size_t error_capacity, const char *what);
+                                  int dense_layout, const PkvRowScales *scales, PkvStream stream,
+                                  char *error, size_t error_capacity, const char *what);
 
 /* Writes a message into a caller error buffer (NULL-safe). */
 void pkv_internal_set_error(char *error, size_t capacity, const char *fmt, ...);

@@ -94,7 +94,10 @@ struct PfArgs {
     // read and written in place instead of token-major rows.
     int32_t dense_layout;
     int32_t dense_rows;
-    int32_t seq0;  // dense layout: the launch's first sequence (launches hold <= kPfMaxBatch)
+    int32_t seq0;  // the launch's first sequence (launches hold <= kPfMaxBatch)
+    // Q8 instantiation only
+    const float *k_scale, *v_log2, *v_inverse;
+    int32_t scale_stride;
 };
 
 struct Item {
@@ -337,8 +340,14 @@ __device__ __forceinline__ void add_mask_chunk(uint32_t (&v)[32], const uint16_t
 // taken over raw scores and scaled once).  GEN = true: scores are scaled (and
 // masked) before the max, any finite scale, and rows whose running max
 // becomes +inf give zeros (the SDK CUDA backend's rule for a non-finite max).
+// Q8: K and V are whole numbers kq, vq with scales per 16 keys (PkvRowScales).
+// With c = ks * scale and e = log2 vs of a key's block, the weight the PV takes
+// is vs 2^(c s - m) = 2^(c s + e - m): the scales sit in the multiplier and the
+// addend of the exponent and cost nothing per score.  m is the running maximum
+// of c s + e, and the softmax sum is the blocks' sums times 1 / vs, so scores,
+// weights and sums are those of the exact values kq ks and vq vs.
 // HD = head_dim (64 or 128).
-template <typename T, typename OT, bool GEN, int HD>
+template <typename T, typename OT, bool GEN, bool Q8, int HD>
 __global__ void __launch_bounds__(kPfThreads, 1)
 paged_prefill_tc_kernel(const PfArgs a, const __grid_constant__ CUtensorMap qmap,
                         const __grid_constant__ CUtensorMap kmap,
@@ -599,9 +608,44 @@ paged_prefill_tc_kernel(const PfArgs a, const __grid_constant__ CUtensorMap qmap
 #pragma unroll
                     for (int c = 0; c < 4; ++c) mask_chunk(v[c], k0 + c * 32, limit);
                 }
+                // Q8: scales of the tile's eight 16-key blocks
+                const int64_t sc_at =
+                    Q8 ? ((int64_t)(a.seq0 + I.b) * a.kv_heads + I.g) * a.scale_stride + k0 / 16
+                       : 0;
+                float cb[Q8 ? 8 : 1], eb[Q8 ? 8 : 1];
                 float mc[4];  // one running max per chunk: four short chains
+                if constexpr (Q8) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                    for (int i = 0; i < 2; ++i) {
+                        const float4 c4 = __ldg(reinterpret_cast<const float4 *>(a.k_scale + sc_at) + i);
+                        const float4 e4 = __ldg(reinterpret_cast<const float4 *>(a.v_log2 + sc_at) + i);
+                        cb[4 * i] = c4.x * a.scale_log2;
+                        cb[4 * i + 1] = c4.y * a.scale_log2;
+                        cb[4 * i + 2] = c4.z * a.scale_log2;
+                        cb[4 * i + 3] = c4.w * a.scale_log2;
+                        eb[4 * i] = e4.x;
+                        eb[4 * i + 1] = e4.y;
+                        eb[4 * i + 2] = e4.z;
+                        eb[4 * i + 3] = e4.w;
+                    }
+                }
+#pragma unroll
+                for (int c = 0; Q8 && c < 4; ++c) {
+                    float mb[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        mb[k] = __uint_as_float(v[c][16 * k]);
+#pragma unroll
+                        for (int i = 1; i < 15; i += 2)
+                            mb[k] = max3(mb[k], __uint_as_float(v[c][16 * k + i]),
+                                         __uint_as_float(v[c][16 * k + i + 1]));
+                        mb[k] = fmaxf(mb[k], __uint_as_float(v[c][16 * k + 15]));
+                    }
+                    mc[c] = fmaxf(fmaf(mb[0], cb[2 * c], eb[2 * c]),
+                                  fmaf(mb[1], cb[2 * c + 1], eb[2 * c + 1]));
+                }
+#pragma unroll
+                for (int c = 0; !Q8 && c < 4; ++c) {
                     mc[c] = max3(__uint_as_float(v[c][0]), __uint_as_float(v[c][1]),
                                  __uint_as_float(v[c][2]));
 #pragma unroll
@@ -610,7 +654,7 @@ paged_prefill_tc_kernel(const PfArgs a, const __grid_constant__ CUtensorMap qmap
                     mc[c] = fmaxf(mc[c], __uint_as_float(v[c][31]));
                 }
                 float mx = max3(mc[0], mc[1], fmaxf(mc[2], mc[3]));
-                if constexpr (!GEN) mx *= a.scale_log2;  // scale > 0 commutes with max
+                if constexpr (!GEN && !Q8) mx *= a.scale_log2;  // scale > 0 commutes with max
                 float alpha = 1.f;
                 bool rescale = false;
                 if (mx > m_run + kRescaleThreshold) {  // first tile: m_run = -inf
@@ -675,16 +719,31 @@ paged_prefill_tc_kernel(const PfArgs a, const __grid_constant__ CUtensorMap qmap
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     uint32_t hi[16], lo[16];
+                    float2 bsum[Q8 ? 2 : 1];  // the chunk's two blocks
+                    if constexpr (Q8) bsum[0] = bsum[1] = make_float2(0.f, 0.f);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
+                        float2 mul = sc2, add = nm2;
+                        if constexpr (Q8) {
+                            const int k = 2 * c + i / 8;
+                            mul = make_float2(cb[k], cb[k]);
+                            add = make_float2(nm + eb[k], nm + eb[k]);
+                        }
                         const float2 x = ffma2(make_float2(__uint_as_float(v[c][2 * i]),
                                                            __uint_as_float(v[c][2 * i + 1])),
-                                               sc2, nm2);
+                                               mul, add);
                         const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
                         hi[i] = pack2<T>(e.x, e.y);
                         const float2 rem = ffma2(unpack2<T>(hi[i]), neg1, e);  // exact
                         lo[i] = pack2<T>(rem.x, rem.y);
-                        lsum2 = fadd2(lsum2, e);
+                        if constexpr (Q8) bsum[i / 8] = fadd2(bsum[i / 8], e);
+                        else lsum2 = fadd2(lsum2, e);
+                    }
+                    if constexpr (Q8) {
+                        const float2 inv2 = __ldg(
+                            reinterpret_cast<const float2 *>(a.v_inverse + sc_at) + c);
+                        lsum2 = ffma2(bsum[0], make_float2(inv2.x, inv2.x), lsum2);
+                        lsum2 = ffma2(bsum[1], make_float2(inv2.y, inv2.y), lsum2);
                     }
                     tmem_st_32x32b_x16(scol + c * 32, hi);
                     tmem_st_32x32b_x16(scol + c * 32 + 16, lo);
@@ -747,10 +806,10 @@ int sms() {
     return g_sms[dev];
 }
 
-template <typename T, typename OT, bool GEN, int HD>
+template <typename T, typename OT, bool GEN, bool Q8, int HD>
 int launch(const PfArgs &args, const CUtensorMap &qm, const CUtensorMap &km,
            const CUtensorMap &vm, cudaStream_t s) {
-    auto kern = paged_prefill_tc_kernel<T, OT, GEN, HD>;
+    auto kern = paged_prefill_tc_kernel<T, OT, GEN, Q8, HD>;
     static int configured[64];
     int dev = 0;
     cudaGetDevice(&dev);
@@ -767,8 +826,9 @@ int launch(const PfArgs &args, const CUtensorMap &qm, const CUtensorMap &km,
 template <typename T, typename OT, int HD>
 int launch_gen(bool gen, const PfArgs &args, const CUtensorMap &qm, const CUtensorMap &km,
                const CUtensorMap &vm, cudaStream_t s) {
-    return gen ? launch<T, OT, true, HD>(args, qm, km, vm, s)
-               : launch<T, OT, false, HD>(args, qm, km, vm, s);
+    if (args.k_scale != nullptr) return launch<T, OT, false, true, HD>(args, qm, km, vm, s);
+    return gen ? launch<T, OT, true, false, HD>(args, qm, km, vm, s)
+               : launch<T, OT, false, false, HD>(args, qm, km, vm, s);
 }
 
 template <int HD>
@@ -795,7 +855,7 @@ int pkv_paged_prefill(const PkvPagedLayer *layer, const PkvBatch *batch, size_t 
     PKV_RANGE("pkv_paged_prefill");
     return pkv_internal_paged_prefill_ex(layer, batch, q_heads, query_offsets, query,
                                          total_query_rows, max_query_len, scale, causal, output,
-                                         output_dtype, nullptr, 0, 0, 0, stream, error,
+                                         output_dtype, nullptr, 0, 0, 0, nullptr, stream, error,
                                          error_capacity, "pkv_paged_prefill");
 }
 
@@ -804,8 +864,8 @@ int pkv_internal_paged_prefill_ex(const PkvPagedLayer *layer, const PkvBatch *ba
                                   size_t total_query_rows, size_t max_query_len, float scale,
                                   int causal, void *output, PkvDType output_dtype,
                                   const uint16_t *mask, size_t mask_stride, int dense,
-                                  int dense_layout, PkvStream stream, char *error,
-                                  size_t error_capacity, const char *what) {
+                                  int dense_layout, const PkvRowScales *scales, PkvStream stream,
+                                  char *error, size_t error_capacity, const char *what) {
     if (layer == nullptr || batch == nullptr || query_offsets == nullptr || query == nullptr ||
         output == nullptr || layer->key_pool == nullptr || layer->value_pool == nullptr ||
         batch->block_tables == nullptr || batch->seq_lens == nullptr) {
@@ -905,6 +965,10 @@ int pkv_internal_paged_prefill_ex(const PkvPagedLayer *layer, const PkvBatch *ba
     args.dense_layout = dense_layout != 0;
     args.dense_rows = (int32_t)max_query_len;
     args.seq0 = 0;
+    args.k_scale = scales != nullptr ? scales->k : nullptr;
+    args.v_log2 = scales != nullptr ? scales->v_log2 : nullptr;
+    args.v_inverse = scales != nullptr ? scales->v_inverse : nullptr;
+    args.scale_stride = scales != nullptr ? (int32_t)scales->stride : 0;
     // the general instantiation: a mask, or a scale <= 0 (the max is then
     // taken after scaling); dense mode works in both
     const bool gen = mask != nullptr || !(scale > 0.f);

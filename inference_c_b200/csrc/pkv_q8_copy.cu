@@ -16,8 +16,8 @@
 // runs the paged prefill kernel on them: a chunk's pages are read by every
 // 128-row query tile and head pair, so widening them inside the attention
 // kernel would repeat each conversion that many times, while the expansion is
-// one pass of 3 bytes a value.  K and V are rounded to the row type there, as
-// a 16-bit cache holds them.
+// one pass of 3 bytes a value.  The rows it writes are the whole numbers q, exact
+// in either 16-bit type; the scales go beside them and enter the exponent.
 #include <math.h>
 
 #include "pkv_q8.cuh"
@@ -42,10 +42,12 @@ struct Q8RowArgs {
     int32_t units;            // upper bound of pages touched
     int32_t row_vecs;         // uint4 per contiguous row
     int32_t tail;             // rows are the sequence's last (append) or first positions
-    // > 0: every sequence's first seq_lens[b] rows go to rows b * pad_rows on,
-    // and table_out gets the identity table of those rows in pages of 128
+    // > 0: every sequence's first seq_lens[b] rows go to rows b * pad_rows on as
+    // whole numbers, their scales per 16 rows to `wide` (PkvRowScales), and
+    // table_out gets the identity table of those rows in pages of 128
     int32_t pad_rows;
     uint32_t *table_out;
+    float *wide_k, *wide_log2, *wide_inverse;
 };
 
 struct Q8Unit {
@@ -142,8 +144,21 @@ q8_rows_kernel(const Q8RowArgs a) {
     uint4 *row = a.rows[kv] + ((int64_t)row0 + (pos0 - first)) * a.row_vecs + col_lane * 16 + chunk;
 
     if constexpr (!WRITE) {
+        float s = live ? __ldg(sp) : 1.f;
+        if (a.pad_rows > 0) {
+            if (unit_live && head < a.kv_heads && (lane == 0 || (HD == 64 && lane == 8))) {
+                const float t = s == 0.f ? 1.f : s;  // a block of zeros, or none
+                const int64_t at = ((int64_t)b * a.kv_heads + head) * (a.pad_rows / 16) +
+                                   (page * a.block_size) / 16 + part;
+                if (kv == 0) a.wide_k[at] = t;
+                else {
+                    a.wide_log2[at] = log2f(t);
+                    a.wide_inverse[at] = __fdiv_rn(1.f, t);
+                }
+            }
+            s = 1.f;
+        }
         if (!live) return;
-        const float s = __ldg(sp);
         uint2 q[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -258,7 +273,8 @@ cudaError_t launch_q8(const Q8RowArgs &a, cudaStream_t s) {
 template <bool WRITE>
 int q8_rows(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *offsets,
             const void *krows, const void *vrows, size_t total_rows, bool tail, size_t pad_rows,
-            uint32_t *table_out, PkvStream stream, char *error, size_t cap, const char *what) {
+            uint32_t *table_out, const PkvRowScales *wide, PkvStream stream, char *error,
+            size_t cap, const char *what) {
     if (!q8_check(layer, batch, error, cap, what)) return 0;
     if (krows == nullptr || vrows == nullptr) {
         pkv_internal_set_error(error, cap, "%s: null rows", what);
@@ -301,6 +317,9 @@ int q8_rows(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *offse
     a.tail = tail ? 1 : 0;
     a.pad_rows = (int32_t)pad_rows;
     a.table_out = table_out;
+    a.wide_k = wide == nullptr ? nullptr : const_cast<float *>(wide->k);
+    a.wide_log2 = wide == nullptr ? nullptr : const_cast<float *>(wide->v_log2);
+    a.wide_inverse = wide == nullptr ? nullptr : const_cast<float *>(wide->v_inverse);
     if (pad_rows > 0) a.units = (int32_t)(total_rows / layer->block_size);
     const cudaStream_t s = (cudaStream_t)stream;
     cudaError_t st;
@@ -321,7 +340,8 @@ int q8_rows(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *offse
 // Scratch of the prefill: 16-bit rows of every sequence, padded to whole pages
 // of 128, and their identity table.
 struct PrefillSpace {
-    size_t pad, k, v, table, total;
+    size_t pad, k, v, table, scales, total;  // scales: three arrays of scale_bytes
+    size_t scale_bytes;
 };
 
 PrefillSpace prefill_space(size_t batch, size_t kv_heads, size_t head_dim, size_t max_seq_len) {
@@ -331,7 +351,9 @@ PrefillSpace prefill_space(size_t batch, size_t kv_heads, size_t head_dim, size_
     w.k = 0;
     w.v = bytes;
     w.table = 2 * bytes;
-    w.total = w.table + (batch * (w.pad / 128) * 4 + 255) / 256 * 256;
+    w.scales = w.table + (batch * (w.pad / 128) * 4 + 255) / 256 * 256;
+    w.scale_bytes = (batch * kv_heads * (w.pad / 16) * 4 + 255) / 256 * 256;
+    w.total = w.scales + 3 * w.scale_bytes;
     return w;
 }
 
@@ -345,7 +367,7 @@ int pkv_q8_append(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t 
                   PkvStream stream, char *error, size_t error_capacity) {
     PKV_RANGE("pkv_q8_append");
     return pkv::q8_rows<true>(layer, batch, row_offsets, key_rows, value_rows, total_rows, true,
-                              0, nullptr, stream, error, error_capacity, "pkv_q8_append");
+                              0, nullptr, nullptr, stream, error, error_capacity, "pkv_q8_append");
 }
 
 int pkv_q8_import(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *row_offsets,
@@ -353,7 +375,7 @@ int pkv_q8_import(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t 
                   PkvStream stream, char *error, size_t error_capacity) {
     PKV_RANGE("pkv_q8_import");
     return pkv::q8_rows<true>(layer, batch, row_offsets, key_rows, value_rows, total_rows, false,
-                              0, nullptr, stream, error, error_capacity, "pkv_q8_import");
+                              0, nullptr, nullptr, stream, error, error_capacity, "pkv_q8_import");
 }
 
 int pkv_q8_gather(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *row_offsets,
@@ -361,7 +383,7 @@ int pkv_q8_gather(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t 
                   size_t error_capacity) {
     PKV_RANGE("pkv_q8_gather");
     return pkv::q8_rows<false>(layer, batch, row_offsets, key_out, value_out, total_rows, false,
-                               0, nullptr, stream, error, error_capacity, "pkv_q8_gather");
+                               0, nullptr, nullptr, stream, error, error_capacity, "pkv_q8_gather");
 }
 
 size_t pkv_q8_prefill_workspace_bytes(size_t batch, size_t kv_heads, size_t head_dim,
@@ -396,17 +418,19 @@ int pkv_q8_prefill(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_head
         return 0;
     }
     if (max_seq_len == 0 || max_seq_len > INT32_MAX / 4 || max_query_len > INT32_MAX ||
-        total_query_rows >= (size_t(1) << 31) || !isfinite(scale) ||
+        total_query_rows >= (size_t(1) << 31) || !isfinite(scale) || !(scale > 0.f) ||
         (causal != 0 && causal != 1)) {
         pkv_internal_set_error(error, error_capacity,
-                               "%s: invalid max_seq_len, sizes, scale or causal", what);
+                               "%s: invalid max_seq_len, sizes, scale (positive) or causal", what);
         return 0;
     }
     if (total_query_rows == 0) return 1;
     const pkv::PrefillSpace one = pkv::prefill_space(1, kvh, hd, max_seq_len);
     // as many sequences at a time as the workspace holds (rows below 2^31)
-    size_t most = workspace_bytes / one.total;
-    if (most > batch->batch) most = batch->batch;
+    size_t most = workspace_bytes / one.total;  // (one's padding counted each time)
+    if (most > batch->batch ||
+        workspace_bytes >= pkv::prefill_space(batch->batch, kvh, hd, max_seq_len).total)
+        most = batch->batch;
     if (most > (size_t)INT32_MAX / 4 / one.pad) most = (size_t)INT32_MAX / 4 / one.pad;
     if (workspace == nullptr || most == 0 || (uintptr_t)workspace % 256 != 0) {
         pkv_internal_set_error(error, error_capacity,
@@ -437,11 +461,17 @@ int pkv_q8_prefill(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_head
         rows.table_stride = w.pad / 128;
         rows.seq_lens = part.seq_lens;
         rows.batch = n;
+        PkvRowScales scales;
+        scales.k = reinterpret_cast<float *>(base + w.scales);
+        scales.v_log2 = reinterpret_cast<float *>(base + w.scales + w.scale_bytes);
+        scales.v_inverse = reinterpret_cast<float *>(base + w.scales + 2 * w.scale_bytes);
+        scales.stride = w.pad / 16;
         if (!pkv::q8_rows<false>(layer, &part, nullptr, wide.key_pool, wide.value_pool, n * w.pad,
-                                 false, w.pad, table, stream, error, error_capacity, what) ||
+                                 false, w.pad, table, &scales, stream, error, error_capacity,
+                                 what) ||
             !pkv_internal_paged_prefill_ex(&wide, &rows, q_heads, query_offsets + b0, query,
                                            total_query_rows, max_query_len, scale, causal, output,
-                                           output_dtype, nullptr, 0, 0, 0, stream, error,
+                                           output_dtype, nullptr, 0, 0, 0, &scales, stream, error,
                                            error_capacity, what))
             return 0;
     }

@@ -186,8 +186,7 @@ def test_decode(lib, cuda, q_heads, kv_heads, hd, bs, dtype, out):
 ])
 @pytest.mark.parametrize("parts", [False, True])
 def test_prefill(lib, cuda, q_heads, kv_heads, hd, bs, dtype, out, causal, parts):
-    """Chunks of none, one and many rows; the attention is that over the
-    gathered 16-bit rows, so the reference rounds K and V once."""
+    """Chunks of none, one and many rows, over the exact values q * s."""
     import torch
     lengths = np.array([1, 129, 0, 300, 131, 17])
     rows = np.array([1, 129, 0, 40, 0, 5])
@@ -209,8 +208,7 @@ def test_prefill(lib, cuda, q_heads, kv_heads, hd, bs, dtype, out, causal, parts
         L, n = int(L), int(rows[b])
         if n == 0:
             continue
-        k, v = (widen(W.storage_bits(p.read(case.tables[b], L), dtype), dtype).astype(np.float64)
-                for p in (case.k, case.v))
+        k, v = case.k.read64(case.tables[b], L), case.v.read64(case.tables[b], L)
         limits = L - n + 1 + np.arange(n) if causal else np.full(n, L)
         want, _, worst = attend64(q[offs[b]:offs[b + 1]], k, v, case.scale, limits)
         # the 16-bit prefill keeps weights as two 16-bit halves: bf16 2^-16,
