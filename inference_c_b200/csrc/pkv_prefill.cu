@@ -223,6 +223,13 @@ __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
     return r;
 }
 
+// The c-th two floats at `p` (read-only data), loaded here and not earlier.
+__device__ __forceinline__ float2 load_pair(const float *p, int c) {
+    float2 v;
+    asm volatile("ld.global.nc.v2.f32 {%0, %1}, [%2];\n" : "=f"(v.x), "=f"(v.y) : "l"(p + 2 * c));
+    return v;
+}
+
 // Scores of keys at or past `limit` in the 32-key chunk starting at key kc
 // become -inf (their weight is exactly 0).
 __device__ __forceinline__ void mask_chunk(uint32_t (&v)[32], int kc, int limit) {
@@ -612,23 +619,7 @@ paged_prefill_tc_kernel(const PfArgs a, const __grid_constant__ CUtensorMap qmap
                 const int64_t sc_at =
                     Q8 ? ((int64_t)(a.seq0 + I.b) * a.kv_heads + I.g) * a.scale_stride + k0 / 16
                        : 0;
-                float cb[Q8 ? 8 : 1], eb[Q8 ? 8 : 1];
                 float mc[4];  // one running max per chunk: four short chains
-                if constexpr (Q8) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float4 c4 = __ldg(reinterpret_cast<const float4 *>(a.k_scale + sc_at) + i);
-                        const float4 e4 = __ldg(reinterpret_cast<const float4 *>(a.v_log2 + sc_at) + i);
-                        cb[4 * i] = c4.x * a.scale_log2;
-                        cb[4 * i + 1] = c4.y * a.scale_log2;
-                        cb[4 * i + 2] = c4.z * a.scale_log2;
-                        cb[4 * i + 3] = c4.w * a.scale_log2;
-                        eb[4 * i] = e4.x;
-                        eb[4 * i + 1] = e4.y;
-                        eb[4 * i + 2] = e4.z;
-                        eb[4 * i + 3] = e4.w;
-                    }
-                }
 #pragma unroll
                 for (int c = 0; Q8 && c < 4; ++c) {
                     float mb[2];
@@ -641,8 +632,10 @@ paged_prefill_tc_kernel(const PfArgs a, const __grid_constant__ CUtensorMap qmap
                                          __uint_as_float(v[c][16 * k + i + 1]));
                         mb[k] = fmaxf(mb[k], __uint_as_float(v[c][16 * k + 15]));
                     }
-                    mc[c] = fmaxf(fmaf(mb[0], cb[2 * c], eb[2 * c]),
-                                  fmaf(mb[1], cb[2 * c + 1], eb[2 * c + 1]));
+                    const float2 cb = load_pair(a.k_scale + sc_at, c);
+                    const float2 eb = load_pair(a.v_log2 + sc_at, c);
+                    mc[c] = fmaxf(fmaf(mb[0], cb.x * a.scale_log2, eb.x),
+                                  fmaf(mb[1], cb.y * a.scale_log2, eb.y));
                 }
 #pragma unroll
                 for (int c = 0; !Q8 && c < 4; ++c) {
@@ -720,14 +713,24 @@ paged_prefill_tc_kernel(const PfArgs a, const __grid_constant__ CUtensorMap qmap
                 for (int c = 0; c < 4; ++c) {
                     uint32_t hi[16], lo[16];
                     float2 bsum[Q8 ? 2 : 1];  // the chunk's two blocks
-                    if constexpr (Q8) bsum[0] = bsum[1] = make_float2(0.f, 0.f);
+                    // the chunk's scales again from L1: held over both loops they
+                    // spilled
+                    float2 cb = make_float2(0.f, 0.f), eb = cb;
+                    if constexpr (Q8) {
+                        bsum[0] = bsum[1] = make_float2(0.f, 0.f);
+                        cb = load_pair(a.k_scale + sc_at, c);
+                        eb = load_pair(a.v_log2 + sc_at, c);
+                        cb.x *= a.scale_log2;
+                        cb.y *= a.scale_log2;
+                        eb.x += nm;
+                        eb.y += nm;
+                    }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         float2 mul = sc2, add = nm2;
                         if constexpr (Q8) {
-                            const int k = 2 * c + i / 8;
-                            mul = make_float2(cb[k], cb[k]);
-                            add = make_float2(nm + eb[k], nm + eb[k]);
+                            mul = i < 8 ? make_float2(cb.x, cb.x) : make_float2(cb.y, cb.y);
+                            add = i < 8 ? make_float2(eb.x, eb.x) : make_float2(eb.y, eb.y);
                         }
                         const float2 x = ffma2(make_float2(__uint_as_float(v[c][2 * i]),
                                                            __uint_as_float(v[c][2 * i + 1])),
@@ -740,8 +743,7 @@ paged_prefill_tc_kernel(const PfArgs a, const __grid_constant__ CUtensorMap qmap
                         else lsum2 = fadd2(lsum2, e);
                     }
                     if constexpr (Q8) {
-                        const float2 inv2 = __ldg(
-                            reinterpret_cast<const float2 *>(a.v_inverse + sc_at) + c);
+                        const float2 inv2 = load_pair(a.v_inverse + sc_at, c);
                         lsum2 = ffma2(bsum[0], make_float2(inv2.x, inv2.x), lsum2);
                         lsum2 = ffma2(bsum[1], make_float2(inv2.y, inv2.y), lsum2);
                     }
