@@ -264,7 +264,7 @@ int pkv_q8_decode(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads
                   char *error, size_t error_capacity);
 
 /* Decode that also adds up attention weights, for eviction:  mass is float32
- * [block_count][kv_heads][block_size], laid out like the pages, and beside the
+ * [block_count][kv_heads][block_size] (16-byte aligned), and beside the
  * output of pkv_paged_decode (pkv_q8_decode) every position t < seq_lens[b]
  * and KV head g of the batch gets
  *     mass[table[t / block_size]][g][t % block_size] += sum over the query

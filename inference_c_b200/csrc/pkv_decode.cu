@@ -1126,8 +1126,6 @@ paged_decode_tc_kernel(const TcArgs a, const __grid_constant__ CUtensorMap kmap,
                 for (int h = 0; h < GV; ++h) {
                     const int col = PAIR && h >= G ? 8 + h - G : h;  // S^T column of head h
                     x[h] = live ? s[col] * a.scale_log2 : -INFINITY;
-                    if (a.scores != nullptr && P.seg + k < a.score_tiles)
-                        a.scores[((P.seg + k) * GV + h) * 128 + row] = x[h];
                     const float wm = warp_max(x[h]);
                     if (lane == 0) red[buf * 64 + q4 * 16 + h] = wm;
                 }
@@ -1162,6 +1160,12 @@ paged_decode_tc_kernel(const TcArgs a, const __grid_constant__ CUtensorMap kmap,
                 }
                 fence_proxy_async_smem();
                 mbar_arrive(&p_full[buf]);
+                // scores for the mass, behind the fence above (it waits for stores)
+                if (a.scores != nullptr && P.seg + k < a.score_tiles) {
+                    float *sp = a.scores + (P.seg + k) * GV * 128 + row;
+#pragma unroll
+                    for (int h = 0; h < GV; ++h) sp[h * 128] = x[h];
+                }
                 if (k > P.k0) fold(j - 1);
 #pragma unroll
                 for (int h = 0; h < GV; ++h) alpha_prev[h] = alpha[h];
@@ -1771,8 +1775,8 @@ int pkv_paged_decode_mass(const PkvPagedLayer *layer, const PkvBatch *batch, siz
                           size_t error_capacity) {
     PKV_RANGE("pkv_paged_decode_mass");
     const char *what = "pkv_paged_decode_mass";
-    if (mass == nullptr || (uintptr_t)mass % 4 != 0) {
-        pkv_internal_set_error(error, error_capacity, "%s: mass is null or not 4-byte aligned",
+    if (mass == nullptr || (uintptr_t)mass % 16 != 0) {
+        pkv_internal_set_error(error, error_capacity, "%s: mass is null or not 16-byte aligned",
                                what);
         return 0;
     }

@@ -1,12 +1,13 @@
 // pkv_mass.cu -- attention weights of a decode step, added to the paged mass
 // (float32 [block_count][kv_heads][block_size]).
 //
-// One CTA takes kTiles tiles of 128 tokens of one lane (one KV head of
-// head_dim 128, two of 64) of one sequence: thread = token, a coalesced load
-// per query head, one read and write of the token's cell per KV head.  Each
+// One warp takes one tile of 128 tokens of one lane (one KV head of head_dim
+// 128, two of 64): thread = 4 tokens, a 16-byte load per query head, eight of
+// them in flight, one read and write of the tokens' cells per KV head.  Each
 // cell belongs to one thread, so sums do not depend on any order of CTAs.
 // Bound by HBM: 4 bytes a token and query head (mostly L2 hits, just written)
-// and 8 bytes a token and KV head.
+// and 8 bytes a token and KV head.  One load of 4 bytes a step took 27 us for
+// 131072 tokens of 64 heads.
 #include "pkv_device.cuh"
 #include "pkv_mass.cuh"
 
@@ -15,7 +16,7 @@ namespace {
 
 __device__ uint32_t g_mass_fault;
 
-constexpr int kTiles = 4;
+constexpr int kTiles = 8;  // tiles (warps) of a CTA
 
 struct MassArgs {
     const float *scores;
@@ -30,57 +31,66 @@ struct MassArgs {
 };
 
 template <bool PAIR>
-__global__ void __launch_bounds__(128) mass_kernel(const MassArgs a) {
+__global__ void __launch_bounds__(kTiles * 32) mass_kernel(const MassArgs a) {
     pdl_launch_dependents();
     pdl_wait();
     const int lane = blockIdx.y, b = blockIdx.z;
     const int L = max(0, __ldg(a.seq_lens + b));
-    const int k0 = blockIdx.x * kTiles;
-    if (k0 * 128 >= L) return;
+    const int k = blockIdx.x * kTiles + (threadIdx.x >> 5);
+    const int t = k * 128 + (threadIdx.x & 31) * 4;  // this thread's first token
+    if (t >= L) return;
     const int nt = (L + 127) / 128;
-    const int64_t first = a.tile_prefix[b];
+    const int64_t first = __ldcg(a.tile_prefix + b);
+    const int page = t / a.block_size;  // its 4 tokens share a page
+    uint32_t pid = 0, fault = kFaultNone;
+    if (page >= a.table_stride) fault = kFaultPositionOutOfRange;
+    else if ((pid = __ldg(a.tables + (int64_t)b * a.table_stride + page)) >= a.block_count)
+        fault = kFaultPageOutOfRange;
+    else if (first + (int64_t)a.segs * nt > a.tiles)  // longer than the caller's bound
+        fault = kFaultPositionOutOfRange;
+    if (fault != kFaultNone) {
+        record_fault(&g_mass_fault, fault);
+        return;
+    }
 #pragma unroll
     for (int half = 0; half < (PAIR ? 2 : 1); ++half) {
         const int kvh = PAIR ? 2 * lane + half : lane;
         if (kvh >= a.kv_heads) return;
-        float w[kTiles];
+        float4 *cell = reinterpret_cast<float4 *>(
+            a.mass + ((int64_t)pid * a.kv_heads + kvh) * a.block_size + (t - page * a.block_size));
+        const float4 old = *cell;
+        float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int h0 = 0; h0 < a.group; h0 += 8) {
+            float4 x[8];
+            float2 ml[8];
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) w[i] = 0.f;
-        for (int hh = 0; hh < a.group; ++hh) {
-            const float2 ml = __ldg(reinterpret_cast<const float2 *>(
-                a.final_ml + ((int64_t)b * a.q_heads + kvh * a.group + hh) * 2));
-            const float inv = ml.y == 0.f ? 0.f : 1.f / ml.y;
-            const int sub = hh / a.per, h = hh - sub * a.per + half * a.per;
-            const int64_t tile = first + (int64_t)(lane * a.subs + sub) * nt + k0;
-            float x[kTiles];
-#pragma unroll
-            for (int i = 0; i < kTiles; ++i) {
-                const bool live = (k0 + i) * 128 + (int)threadIdx.x < L && tile + i < a.tiles;
-                x[i] = live ? __ldcg(a.scores + ((tile + i) * a.gv + h) * 128 + threadIdx.x)
-                            : -INFINITY;
+            for (int i = 0; i < 8; ++i) {
+                const int hh = min(h0 + i, a.group - 1);
+                const int sub = hh / a.per, h = hh - sub * a.per + half * a.per;
+                const int64_t tile = first + (int64_t)(lane * a.subs + sub) * nt + k;
+                x[i] = __ldcg(reinterpret_cast<const float4 *>(a.scores + (tile * a.gv + h) * 128) +
+                              (threadIdx.x & 31));
+                ml[i] = __ldcg(reinterpret_cast<const float2 *>(
+                    a.final_ml + ((int64_t)b * a.q_heads + kvh * a.group + hh) * 2));
             }
 #pragma unroll
-            for (int i = 0; i < kTiles; ++i)
-                w[i] += x[i] == -INFINITY ? 0.f : exp2f(x[i] - ml.x) * inv;
+            for (int i = 0; i < 8; ++i) {
+                if (h0 + i >= a.group) break;
+                const float inv = ml[i].y == 0.f ? 0.f : 1.f / ml[i].y;
+                w.x += exp2f(x[i].x - ml[i].x) * inv;
+                w.y += exp2f(x[i].y - ml[i].x) * inv;
+                w.z += exp2f(x[i].z - ml[i].x) * inv;
+                w.w += exp2f(x[i].w - ml[i].x) * inv;
+            }
         }
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
-            const int t = (k0 + i) * 128 + (int)threadIdx.x;
-            if (t >= L) continue;
-            const int page = t / a.block_size;
-            uint32_t pid = 0, fault = kFaultNone;
-            if (page >= a.table_stride) fault = kFaultPositionOutOfRange;
-            else if ((pid = __ldg(a.tables + (int64_t)b * a.table_stride + page)) >= a.block_count)
-                fault = kFaultPageOutOfRange;
-            else if (first + (int64_t)a.segs * nt > a.tiles)  // longer than the caller's bound
-                fault = kFaultPositionOutOfRange;
-            if (fault != kFaultNone) {
-                record_fault(&g_mass_fault, fault);
-                continue;
-            }
-            float *cell = a.mass + ((int64_t)pid * a.kv_heads + kvh) * a.block_size +
-                          (t - page * a.block_size);
-            *cell += w[i];
+        // the last tokens one by one: cells past the length stay as they are
+        if (t + 4 <= L) {
+            *cell = make_float4(old.x + w.x, old.y + w.y, old.z + w.z, old.w + w.w);
+        } else {
+            float *c = reinterpret_cast<float *>(cell);
+            c[0] = old.x + w.x;
+            if (t + 1 < L) c[1] = old.y + w.y;
+            if (t + 2 < L) c[2] = old.z + w.z;
         }
     }
 }
@@ -116,7 +126,7 @@ bool mass_apply(const MassShape &s, const MassScratch &scratch, const int32_t *t
     const size_t tiles = (s.max_seq_len + 127) / 128;
     cfg.gridDim = dim3((unsigned)((tiles + kTiles - 1) / kTiles), (unsigned)lanes,
                        (unsigned)s.batch);
-    cfg.blockDim = dim3(128);
+    cfg.blockDim = dim3(kTiles * 32);
     cfg.stream = (cudaStream_t)stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;

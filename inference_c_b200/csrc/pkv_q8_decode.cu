@@ -322,6 +322,9 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
     setmaxnreg_dec<kRegsControl>();
     if (warp < kProducers) {
         // ----------------------------- producers -----------------------------
+        // pages leave L2 first: the partials and the scores stay for the kernels
+        // behind this one
+        const uint64_t once = policy_evict_first();
         uint32_t j = 0;
         bool ok = true;
         int u = works ? (int)blockIdx.x : -1;
@@ -381,7 +384,8 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                     if (lane == 0) mbar_arrive_expect_tx(&kfull[ks], bytes);
                     __syncwarp();
                     if (good && lane < 8)
-                        tma_load_2d(sm + ks * kTileBytes + off, &kmap, &kfull[ks], 0, y);
+                        tma_load_2d_policy(sm + ks * kTileBytes + off, &kmap, &kfull[ks], 0, y,
+                                           once);
                     // scales: kind = lane / 8 (K0, V0, K1, V1 of the lane's heads)
                     const int head = (PAIR ? 2 * kl : kl) + (lane >> 4);
                     const bool want = good && head < a.heads && (PAIR || lane < 16);
@@ -395,7 +399,8 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                     if (lane == 0) mbar_arrive_expect_tx(&vfull[vs], bytes);
                     __syncwarp();
                     if (good && lane < 8)
-                        tma_load_2d(sm + C::V_OFF + vs * kTileBytes + off, &vmap, &vfull[vs], 0, y);
+                        tma_load_2d_policy(sm + C::V_OFF + vs * kTileBytes + off, &vmap, &vfull[vs],
+                                           0, y, once);
                 }
                 j += (uint32_t)(P.k1 - P.k0);
             }
@@ -700,13 +705,6 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                         const float wm = redux_max(fmaxf(x[0][h], x[1][h]));
                         if (lane == 0) myred[h * 4 + q4] = wm;
                     }
-                    if (a.scores != nullptr)
-                        for (int i = 0; i < n2; ++i)
-                            if (tile0 + k + i < a.score_tiles)
-#pragma unroll
-                                for (int h = 0; h < GV; ++h)
-                                    a.scores[((int64_t)(tile0 + k + i) * GV + h) * 128 + row] =
-                                        i == 0 ? x[0][h] : x[1][h];
                     if constexpr (NB == 2)  // the weights below overwrite the previous pair's
                         if (mine >= 0) fold((uint32_t)mine);
                     group_sync();
@@ -734,6 +732,16 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                     }
                     fence_proxy_async_smem();
                     mbar_arrive(&p_full[buf]);
+                    // scores for the mass: behind the fence, which would wait for
+                    // these stores (one sequence of 131072, 64 heads: 84 us so)
+                    if (a.scores != nullptr && tile0 + k + n2 <= a.score_tiles) {
+                        float *sp = a.scores + (int64_t)(tile0 + k) * GV * 128 + row;
+#pragma unroll
+                        for (int h = 0; h < GV; ++h) {
+                            sp[h * 128] = x[0][h];
+                            if (n2 > 1) sp[(GV + h) * 128] = x[1][h];
+                        }
+                    }
                     if constexpr (NB != 2)
                         if (mine >= 0) fold((uint32_t)mine);
                     mine = pc;
@@ -1143,8 +1151,8 @@ int pkv_q8_decode_mass(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_
                        PkvStream stream, char *error, size_t error_capacity) {
     PKV_RANGE("pkv_q8_decode_mass");
     const char *what = "pkv_q8_decode_mass";
-    if (mass == nullptr || (uintptr_t)mass % 4 != 0) {
-        pkv_internal_set_error(error, error_capacity, "%s: mass is null or not 4-byte aligned",
+    if (mass == nullptr || (uintptr_t)mass % 16 != 0) {
+        pkv_internal_set_error(error, error_capacity, "%s: mass is null or not 16-byte aligned",
                                what);
         return 0;
     }

@@ -97,6 +97,22 @@ __device__ __forceinline__ void tma_load_2d(void *smem_dst, const CUtensorMap *m
         "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y)
         : "memory");
 }
+// L2 policy for bytes that are read once: first to be evicted.
+__device__ __forceinline__ uint64_t policy_evict_first() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;\n" : "=l"(p));
+    return p;
+}
+// tma_load_2d under an L2 policy.
+__device__ __forceinline__ void tma_load_2d_policy(void *smem_dst, const CUtensorMap *map,
+                                                   uint64_t *bar, int32_t x, int32_t y,
+                                                   uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%3, %4}], [%2], %5;\n" ::"r"(smem_u32(smem_dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "l"(policy)
+        : "memory");
+}
 // Brings the 128-byte line holding `p` into L2 (a hint: no register or L1
 // copy, so a later write to the line by any kernel is still seen).
 __device__ __forceinline__ void prefetch_l2(const void *p) {
