@@ -31,6 +31,7 @@ __device__ uint32_t g_evict_fault;
 
 constexpr int kSelThreads = 1024;
 constexpr int kBins = 2048;
+constexpr int kMoveRows = 128;  // rows a move CTA takes at a time: its threads
 
 struct EvictArgs {
     const uint32_t *tables, *dst_tables;
@@ -70,16 +71,32 @@ __device__ __forceinline__ bool page_at(const EvictArgs &a, const uint32_t *trow
     return true;
 }
 
-// Grid (cluster size * kv_heads, batch), clusters along x.
+// Place of the i-th held key: a gap every 32 words, so that threads that read
+// runs of their own (strides of a few powers of two) meet different banks.
+__device__ __forceinline__ int key_slot(int i) { return i + (i >> 5); }
+
+// Grid (CS * kv_heads, batch), clusters of CS CTAs along x.
+template <int CS>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictArgs a) {
     cg::cluster_group cluster = cg::this_cluster();
+    auto list_sync = [&] {
+        if constexpr (CS > 1) cluster.sync();
+        else __syncthreads();
+    };
+    // the same variable in the list's r-th CTA
+    auto of_rank = [&](uint32_t *p, int r) {
+        if constexpr (CS > 1) return cluster.map_shared_rank(p, r);
+        else return p;
+    };
     extern __shared__ uint32_t keys[];
     __shared__ __align__(8) uint32_t hist[kBins];
     __shared__ uint32_t wsum[32];
     __shared__ uint32_t found[2];     // bin, keys above it
     __shared__ uint32_t count[2];     // this CTA's keys above / equal to the threshold
+    __shared__ uint32_t wgt[32], weq[32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int cs = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    constexpr int cs = CS;
+    const int rank = CS > 1 ? (int)cluster.block_rank() : 0;
     const int g = blockIdx.x / cs, b = blockIdx.y;
     const int32_t L = max(0, __ldg(a.seq_lens + b));
     const int32_t n = min(L, a.keep);
@@ -95,7 +112,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
         kept[need + i] = old + i;
     if (need == 0) return;
     const uint32_t *trow = a.tables + (int64_t)b * a.table_stride;
-    const int32_t span = (old + cs - 1) / cs;
+    const int32_t span = ((old + cs - 1) / cs + 3) & ~3;
     const int32_t lo = min(old, rank * span), hi = min(old, lo + span);
     auto gather = [&](int32_t t) -> uint32_t {
         uint32_t pid;
@@ -104,9 +121,36 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
                               (t & (a.block_size - 1))));
     };
     const bool held = hi - lo <= a.cached;
-    if (held)
-        for (int32_t t = lo + tid; t < hi; t += kSelThreads) keys[t - lo] = gather(t);
-    auto key = [&](int32_t t) { return held ? keys[t - lo] : gather(t); };
+    if (held) {
+        // four tokens a load (a page holds a multiple of 16, lo a multiple of
+        // 4), four loads in flight
+        const int quads = (hi - lo + 3) / 4;
+        for (int q0 = tid; q0 < quads; q0 += 4 * kSelThreads) {
+            float4 m[4];
+            bool good[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int q = q0 + i * kSelThreads;
+                uint32_t pid = 0;
+                good[i] = q < quads && page_at(a, trow, a.table_stride, lo + 4 * q, pid);
+                m[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (good[i])
+                    m[i] = __ldg(reinterpret_cast<const float4 *>(
+                        a.mass + ((int64_t)pid * a.kv_heads + g) * a.block_size +
+                        ((lo + 4 * q) & (a.block_size - 1))));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int k = 4 * (q0 + i * kSelThreads);  // (past hi: never read)
+                if (k >= hi - lo) continue;
+                keys[key_slot(k)] = good[i] ? mass_key(m[i].x) : 0u;
+                keys[key_slot(k + 1)] = good[i] ? mass_key(m[i].y) : 0u;
+                keys[key_slot(k + 2)] = good[i] ? mass_key(m[i].z) : 0u;
+                keys[key_slot(k + 3)] = good[i] ? mass_key(m[i].w) : 0u;
+            }
+        }
+    }
+    auto key = [&](int32_t t) { return held ? keys[key_slot(t - lo)] : gather(t); };
 
     uint32_t prefix = 0, want = (uint32_t)need;  // the want-th largest of those with `prefix`
     uint32_t above = 0;
@@ -117,16 +161,23 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
         __syncthreads();
         for (int32_t t = lo + tid; t < hi; t += kSelThreads) {
             const uint32_t k = key(t);
-            if (pass == 0 || (k >> (shift + bits)) == prefix)
-                atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1u)], 1u);
+            if (pass == 0 || (k >> (shift + bits)) == prefix) {
+                // masses crowd into few bins: one atomic a bin and warp
+                const uint32_t bin = (k >> shift) & ((1u << bits) - 1u);
+                const uint32_t same = __match_any_sync(__activemask(), bin);
+                if ((__ffs(same) - 1) == lane) atomicAdd(&hist[bin], (uint32_t)__popc(same));
+            }
         }
-        cluster.sync();
+        list_sync();
         // bins 2 tid and 2 tid + 1 of the whole list, then keys above each
         uint32_t c0 = 0, c1 = 0;
-        for (int r = 0; r < cs; ++r) {
-            const uint2 v = reinterpret_cast<const uint2 *>(cluster.map_shared_rank(hist, r))[tid];
-            c0 += v.x;
-            c1 += v.y;
+        uint2 part[CS];
+#pragma unroll
+        for (int r = 0; r < CS; ++r) part[r] = reinterpret_cast<const uint2 *>(of_rank(hist, r))[tid];
+#pragma unroll
+        for (int r = 0; r < CS; ++r) {
+            c0 += part[r].x;
+            c1 += part[r].y;
         }
         uint32_t incl = c0 + c1;  // suffix sums: over this and higher lanes, then warps
 #pragma unroll
@@ -136,8 +187,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
         }
         if (lane == 0) wsum[warp] = incl;
         __syncthreads();
-        uint32_t higher = 0;
-        for (int w = warp + 1; w < 32; ++w) higher += wsum[w];
+        const uint32_t higher = __reduce_add_sync(0xffffffffu, lane > warp ? wsum[lane] : 0u);
         const uint32_t top1 = higher + incl - c0 - c1;  // keys in bins above 2 tid + 1
         const uint32_t top0 = top1 + c1;
         if (top1 < want && want <= top1 + c1) {
@@ -148,74 +198,89 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
             found[0] = 2 * tid;
             found[1] = top0;
         }
-        cluster.sync();  // also: every CTA has read every histogram
+        list_sync();  // also: every CTA has read every histogram
         prefix = (prefix << bits) | found[0];
         above += found[1];
         want -= found[1];
         __syncthreads();
     }
-    // keys above `prefix` are all kept, of those equal to it the first `want`
+    // Keys above `prefix` are all kept, of those equal to it the first `want`.
+    // Each thread takes a run of positions: its counts, one scan over the CTA and
+    // the CTAs before it, then its positions in order.
+    const int32_t run = (hi - lo + kSelThreads - 1) / kSelThreads;
+    const int32_t r0 = min(hi, lo + tid * run), r1 = min(hi, r0 + run);
     uint32_t gt = 0, eq = 0;
-    for (int32_t t = lo + tid; t < hi; t += kSelThreads) {
+    for (int32_t t = r0; t < r1; ++t) {
         const uint32_t k = key(t);
         gt += k > prefix;
         eq += k == prefix;
     }
-    if (tid < 2) count[tid] = 0;
-    __syncthreads();
-    gt = __reduce_add_sync(0xffffffffu, gt);
-    eq = __reduce_add_sync(0xffffffffu, eq);
-    if (lane == 0) {
-        atomicAdd(&count[0], gt);
-        atomicAdd(&count[1], eq);
-    }
-    cluster.sync();
-    uint32_t gt0 = 0, eq0 = 0;  // before this CTA's run
-    for (int r = 0; r < rank; ++r) {
-        const uint32_t *c = cluster.map_shared_rank(count, r);
-        gt0 += c[0];
-        eq0 += c[1];
-    }
-    cluster.sync();  // no CTA leaves while its counts are read
-    for (int32_t t0 = lo; t0 < hi; t0 += kSelThreads) {
-        const int32_t t = t0 + tid;
-        const uint32_t k = t < hi ? key(t) : 0u;
-        const bool is_gt = t < hi && k > prefix, is_eq = t < hi && k == prefix;
-        const uint32_t bg = __ballot_sync(0xffffffffu, is_gt);
-        const uint32_t be = __ballot_sync(0xffffffffu, is_eq);
-        if (lane == 0) wsum[warp] = (uint32_t)__popc(bg) | (uint32_t)__popc(be) << 16;
-        __syncthreads();
-        uint32_t before = 0, all = 0;  // packed counts of at most 1024 each
-        for (int w = 0; w < 32; ++w) {
-            if (w < warp) before += wsum[w];
-            all += wsum[w];
+    uint32_t gi = gt, ei = eq;  // inclusive over the warp
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(0xffffffffu, gi, o);
+        const uint32_t y = __shfl_up_sync(0xffffffffu, ei, o);
+        if (lane >= o) {
+            gi += x;
+            ei += y;
         }
-        const uint32_t below = (1u << lane) - 1u;
-        const uint32_t g_at = gt0 + (before & 0xffffu) + __popc(bg & below);
-        const uint32_t e_at = eq0 + (before >> 16) + __popc(be & below);
-        if (is_gt) kept[g_at + min(e_at, want)] = t;
-        if (is_eq && e_at < want) kept[g_at + e_at] = t;
-        gt0 += all & 0xffffu;
-        eq0 += all >> 16;
-        __syncthreads();
     }
+    if (lane == 31) {
+        wgt[warp] = gi;
+        weq[warp] = ei;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        uint32_t x = wgt[lane], y = weq[lane];
+        const uint32_t x0 = x, y0 = y;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t p = __shfl_up_sync(0xffffffffu, x, o);
+            const uint32_t q = __shfl_up_sync(0xffffffffu, y, o);
+            if (lane >= o) {
+                x += p;
+                y += q;
+            }
+        }
+        wgt[lane] = x - x0;
+        weq[lane] = y - y0;
+        if (lane == 31) {
+            count[0] = x;
+            count[1] = y;
+        }
+    }
+    list_sync();
+    uint32_t g_at = wgt[warp] + gi - gt, e_at = weq[warp] + ei - eq;
+    for (int r = 0; r < rank; ++r) {
+        const uint32_t *c = of_rank(count, r);
+        g_at += c[0];
+        e_at += c[1];
+    }
+    for (int32_t t = r0; t < r1; ++t) {
+        const uint32_t k = key(t);
+        if (k > prefix) kept[g_at++ + min(e_at, want)] = t;
+        else if (k == prefix) {
+            if (e_at < want) kept[g_at + e_at] = t;
+            ++e_at;
+        }
+    }
+    list_sync();  // no CTA leaves while its counts are read
 }
 
 // VEC: uint4 of one head's row (16-bit 8 or 16, 8-bit 4 or 8).
 template <int VEC, bool Q8, bool IN_PLACE>
-__global__ void __launch_bounds__(128) evict_move_kernel(const EvictArgs a) {
+__global__ void __launch_bounds__(kMoveRows) evict_move_kernel(const EvictArgs a) {
     pdl_launch_dependents();
     pdl_wait();
-    __shared__ int64_t from[128];   // uint4 index of the source row, -1: none
-    __shared__ float moved[128];    // its mass
-    __shared__ float ratio[2][128];
-    __shared__ float top[2];
-    constexpr int ITEMS = 16 * VEC * 2 / 128;
+    __shared__ int64_t from[kMoveRows];  // uint4 index of the source row, -1: none
+    __shared__ int64_t to[kMoveRows];    // and of its place
+    __shared__ float ratio[2][kMoveRows];
+    __shared__ float wtop[2][kMoveRows / 32];
+    constexpr int ITEMS = 16 * VEC * 2 / kMoveRows;
     const int tid = threadIdx.x;
     const int g = blockIdx.y, b = blockIdx.z;
     const int32_t L = max(0, __ldg(a.seq_lens + b));
     const int32_t n = min(L, a.keep);
-    const int32_t blocks = (n + a.block_size - 1) >> a.block_shift;
     const int32_t *kept = a.kept + ((int64_t)b * a.kv_heads + g) * a.keep;
     const uint32_t *trow = a.tables + (int64_t)b * a.table_stride;
     const uint32_t *drow = a.dst_tables + (int64_t)b * a.dst_stride;
@@ -228,57 +293,60 @@ __global__ void __launch_bounds__(128) evict_move_kernel(const EvictArgs a) {
             return ((int64_t)pid * a.block_size + in) * a.row_vecs + (int64_t)g * VEC;
         }
     };
-    for (int32_t j = blockIdx.x; j < blocks; j += gridDim.x) {
-        const int32_t rows = min(a.block_size, n - (j << a.block_shift));
-        uint32_t dpid;
-        if (!page_at(a, drow, a.dst_stride, j << a.block_shift, dpid)) return;  // whole CTA
-        float s[2] = {0.f, 0.f};
-        if (tid < 128) from[tid] = -1;
-        if (tid < rows) {
-            const int32_t t = kept[(j << a.block_shift) + tid];
-            uint32_t pid;
+    for (int32_t i0 = blockIdx.x * kMoveRows; i0 < n; i0 += gridDim.x * kMoveRows) {
+        // thread: one row of the result, i0 + tid
+        const int32_t row = i0 + tid, in = row & (a.block_size - 1);
+        float s[2] = {0.f, 0.f}, mass = 0.f;
+        uint32_t pid = 0, dpid = 0;
+        int64_t src = -1;
+        if (row < n && page_at(a, drow, a.dst_stride, row, dpid)) {
+            const int32_t t = __ldcg(kept + row);
             if (t >= 0 && page_at(a, trow, a.table_stride, t, pid)) {
-                const int32_t in = t & (a.block_size - 1);
-                from[tid] = row_at(pid, in);
-                moved[tid] = a.mass[((int64_t)pid * a.kv_heads + g) * a.block_size + in];
+                const int32_t tin = t & (a.block_size - 1);
+                src = row_at(pid, tin);
+                mass = a.mass[((int64_t)pid * a.kv_heads + g) * a.block_size + tin];
                 if (Q8) {
                     s[0] = a.scales[0][(int64_t)pid * a.kv_heads + g];
                     s[1] = a.scales[1][(int64_t)pid * a.kv_heads + g];
                 }
             }
         }
-        if (Q8) {
-            ratio[0][tid] = s[0];
-            ratio[1][tid] = s[1];
+        from[tid] = src;
+        to[tid] = row_at(dpid, in);
+        float top[2] = {s[0], s[1]};
+        if (Q8) {  // the largest scale of the row's block
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+                for (int o = 1; o < 32 && o < a.block_size; o <<= 1)
+                    top[kv] = fmaxf(top[kv], __shfl_xor_sync(0xffffffffu, top[kv], o));
+                if ((tid & 31) == 0) wtop[kv][tid >> 5] = top[kv];
+            }
         }
         __syncthreads();
         if (Q8) {
-            if (tid < 64) {  // warp kv: the largest scale of the block's rows
-                float m = 0.f;
-                for (int i = tid & 31; i < 128; i += 32) m = fmaxf(m, ratio[tid >> 5][i]);
-                m = warp_max(m);
-                if ((tid & 31) == 0) top[tid >> 5] = m;
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+                const int w0 = (tid >> 5) & ~(a.block_size / 32 - 1);  // the block's warps
+                for (int w = 0; w < a.block_size / 32; ++w) top[kv] = fmaxf(top[kv], wtop[kv][w0 + w]);
+                ratio[kv][tid] = top[kv] > 0.f ? __fdiv_rn(s[kv], top[kv]) : 0.f;
             }
             __syncthreads();
-            ratio[0][tid] = top[0] > 0.f ? __fdiv_rn(s[0], top[0]) : 0.f;
-            ratio[1][tid] = top[1] > 0.f ? __fdiv_rn(s[1], top[1]) : 0.f;
-            __syncthreads();
         }
-        const int64_t to = row_at(dpid, 0);
-        const int32_t step = Q8 ? 8 : a.row_vecs;  // uint4 between rows of a page
+        const int32_t rows = min(kMoveRows, n - i0);
+#pragma unroll 2
         for (int32_t r0 = 0; r0 < rows; r0 += 16) {
             uint4 x[ITEMS];
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
-                const int it = i * 128 + tid;
+                const int it = i * kMoveRows + tid;
                 const int kv = it / (16 * VEC), r = r0 + it / VEC % 16, c = it % VEC;
                 x[i] = make_uint4(0, 0, 0, 0);
-                if (from[r] >= 0) x[i] = (kv == 0 ? a.pools[0] : a.pools[1])[from[r] + c];
+                if (from[r] >= 0) x[i] = __ldcg((kv == 0 ? a.pools[0] : a.pools[1]) + from[r] + c);
             }
             if (IN_PLACE) __syncthreads();
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
-                const int it = i * 128 + tid;
+                const int it = i * kMoveRows + tid;
                 const int kv = it / (16 * VEC), r = r0 + it / VEC % 16, c = it % VEC;
                 if (from[r] < 0) continue;
                 if (Q8 && ratio[kv][r] != 1.f) {
@@ -295,14 +363,17 @@ __global__ void __launch_bounds__(128) evict_move_kernel(const EvictArgs a) {
                     }
                     x[i] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
-                (kv == 0 ? a.pools[0] : a.pools[1])[to + (int64_t)r * step + c] = x[i];
+                (kv == 0 ? a.pools[0] : a.pools[1])[to[r] + c] = x[i];
             }
         }
-        if (tid < rows && from[tid] >= 0)
-            a.mass[((int64_t)dpid * a.kv_heads + g) * a.block_size + tid] = moved[tid];
-        if (Q8 && tid < 2)
-            (tid == 0 ? a.scales[0] : a.scales[1])[(int64_t)dpid * a.kv_heads + g] = top[tid];
-        if (IN_PLACE) __syncthreads();
+        if (src >= 0) {
+            a.mass[((int64_t)dpid * a.kv_heads + g) * a.block_size + in] = mass;
+            if (Q8 && in == 0) {
+                a.scales[0][(int64_t)dpid * a.kv_heads + g] = top[0];
+                a.scales[1][(int64_t)dpid * a.kv_heads + g] = top[1];
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -312,9 +383,8 @@ cudaError_t launch_move(const EvictArgs &a, size_t batch, bool in_place, cudaStr
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    const int32_t blocks = (a.keep + a.block_size - 1) / a.block_size;
-    cfg.gridDim = dim3(in_place ? 1u : (unsigned)blocks, (unsigned)a.kv_heads, (unsigned)batch);
-    cfg.blockDim = dim3(128);
+    cfg.gridDim = dim3(in_place ? 1u : (unsigned)((a.keep + kMoveRows - 1) / kMoveRows), (unsigned)a.kv_heads, (unsigned)batch);
+    cfg.blockDim = dim3(kMoveRows);
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
@@ -322,7 +392,7 @@ cudaError_t launch_move(const EvictArgs &a, size_t batch, bool in_place, cudaStr
                     : cudaLaunchKernelEx(&cfg, evict_move_kernel<VEC, Q8, false>, a);
 }
 
-constexpr int32_t kCachedMax = 49152;  // keys of a select CTA: 192 KiB
+constexpr int32_t kCachedMax = 49152;  // keys of a select CTA: 198 KiB with the gaps
 
 int evict(EvictArgs &a, const PkvBatch *batch, size_t head_dim, bool q8, float *mass, size_t keep,
           size_t recent, const uint32_t *dst_tables, size_t dst_stride, int32_t *kept,
@@ -333,8 +403,11 @@ int evict(EvictArgs &a, const PkvBatch *batch, size_t head_dim, bool q8, float *
                                what);
         return 0;
     }
-    if (mass == nullptr || kept == nullptr || ((uintptr_t)mass | (uintptr_t)kept) % 4 != 0) {
-        pkv_internal_set_error(error, cap, "%s: mass or kept is null or not 4-byte aligned", what);
+    if (mass == nullptr || kept == nullptr || (uintptr_t)mass % 16 != 0 ||
+        (uintptr_t)kept % 4 != 0) {
+        pkv_internal_set_error(error, cap,
+                               "%s: mass (16-byte aligned) or kept (4-byte) is null or misaligned",
+                               what);
         return 0;
     }
     if (batch->batch > 65535) {
@@ -367,8 +440,8 @@ int evict(EvictArgs &a, const PkvBatch *batch, size_t head_dim, bool q8, float *
     // (four a thread) and the lists alone do not fill the SMs.
     const size_t lists = batch->batch * (size_t)a.kv_heads;
     const unsigned cs = max_seq_len > 4096 && lists <= 148 ? 8 : 1;
-    const size_t span = (max_seq_len + cs - 1) / cs;
-    a.cached = (int32_t)(span < (size_t)kCachedMax ? span : 0);
+    const size_t span = ((max_seq_len + cs - 1) / cs + 3) / 4 * 4;
+    a.cached = (int32_t)(span <= (size_t)kCachedMax ? span : 0);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cs;
@@ -377,7 +450,7 @@ int evict(EvictArgs &a, const PkvBatch *batch, size_t head_dim, bool q8, float *
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(cs * (unsigned)a.kv_heads, (unsigned)batch->batch);
     cfg.blockDim = dim3(kSelThreads);
-    cfg.dynamicSmemBytes = (size_t)a.cached * 4;
+    cfg.dynamicSmemBytes = ((size_t)a.cached + a.cached / 32 + 1) * 4;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
@@ -386,11 +459,17 @@ int evict(EvictArgs &a, const PkvBatch *batch, size_t head_dim, bool q8, float *
     cudaGetDevice(&dev);
     cudaError_t st = cudaSuccess;
     if (dev >= 0 && dev < 64 && !configured[dev]) {
-        st = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  kCachedMax * 4);
+        const int most = (kCachedMax + kCachedMax / 32 + 1) * 4;
+        st = cudaFuncSetAttribute(evict_select_kernel<1>,
+                                  cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        if (st == cudaSuccess)
+            st = cudaFuncSetAttribute(evict_select_kernel<8>,
+                                      cudaFuncAttributeMaxDynamicSharedMemorySize, most);
         if (st == cudaSuccess) configured[dev] = 1;
     }
-    if (st == cudaSuccess) st = cudaLaunchKernelEx(&cfg, evict_select_kernel, a);
+    if (st == cudaSuccess)
+        st = cs == 1 ? cudaLaunchKernelEx(&cfg, evict_select_kernel<1>, a)
+                     : cudaLaunchKernelEx(&cfg, evict_select_kernel<8>, a);
     if (st == cudaSuccess) {
         if (q8)
             st = head_dim == 128 ? launch_move<8, true>(a, batch->batch, in_place, s)

@@ -73,14 +73,13 @@ q8_rows_kernel(const Q8RowArgs a) {
     const int per = a.block_size / 16;              // warps of one unit
     const int u = blockIdx.x * (kQ8Warps / per) + warp / per;
     const int part = warp % per;                    // this warp's 16 rows of the page
-    const int col_lane = blockIdx.y >> 1, kv = blockIdx.y & 1;
+    const int kv = blockIdx.y & 1;
     constexpr int kHeads = 128 / HD;                // heads of a lane
     const int chunk = lane & 15;                    // this thread's 8 columns
     const int hl = HD == 64 ? chunk >> 3 : 0;       // its head within the lane
-    const int head = col_lane * kHeads + hl;
 
     // ---- which page ----
-    bool live = u < a.units && head < a.kv_heads;
+    bool live = u < a.units;
     const bool unit_live = u < a.units;
     int b = 0;
     int32_t first = 0, end = 0, row0 = 0, page = 0;
@@ -106,10 +105,15 @@ q8_rows_kernel(const Q8RowArgs a) {
             b = u;
             row0 = u;
         } else {
-            int lo = 0, hi = a.batch - 1;
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (q8_first_unit(a, mid) <= u) lo = mid; else hi = mid - 1;
+            // the warp tries 32 sequences at a time: one round of loads up to 32
+            int lo = 0, n = a.batch;  // the answer is in [lo, lo + n)
+            while (n > 1) {
+                const int step = (n + 31) / 32, at = lo + min(lane * step, n - 1);
+                const uint32_t below = __ballot_sync(0xffffffffu, q8_first_unit(a, at) <= u);
+                const int k = 31 - __clz(below);  // lane 0's always is
+                lo += min(k * step, n - 1);
+                n = min(step, a.batch - lo);
+                if (step == 1) break;
             }
             b = lo;
             row0 = __ldg(a.offsets + b);
@@ -136,122 +140,127 @@ q8_rows_kernel(const Q8RowArgs a) {
         }
         held = page * a.block_size < first;
     }
-    // ---- the page's rows: i-th is row part*16 + 2 i + lane/16 ----
-    const int64_t base = (((int64_t)pid * a.lanes + col_lane) * a.block_size + part * 16 + (lane >> 4)) * 16 + chunk;
-    uint2 *cell = a.pools[kv] + base;
-    float *sp = a.scales[kv] + (int64_t)pid * a.kv_heads + head;
-    const int32_t pos0 = page * a.block_size + part * 16 + (lane >> 4);
-    uint4 *row = a.rows[kv] + ((int64_t)row0 + (pos0 - first)) * a.row_vecs + col_lane * 16 + chunk;
+    // the page's columns, a lane at a time: one lookup serves several
+    for (int col_lane = blockIdx.y >> 1; col_lane < a.lanes; col_lane += gridDim.y >> 1) {
+        const int head = col_lane * kHeads + hl;
+        // ---- the page's rows: i-th is row part*16 + 2 i + lane/16 ----
+        const bool on = live && head < a.kv_heads;
+        const int64_t base = (((int64_t)pid * a.lanes + col_lane) * a.block_size + part * 16 + (lane >> 4)) * 16 + chunk;
+        uint2 *cell = a.pools[kv] + base;
+        float *sp = a.scales[kv] + (int64_t)pid * a.kv_heads + head;
+        const int32_t pos0 = page * a.block_size + part * 16 + (lane >> 4);
+        uint4 *row = a.rows[kv] + ((int64_t)row0 + (pos0 - first)) * a.row_vecs + col_lane * 16 + chunk;
 
-    if constexpr (!WRITE) {
-        float s = live ? __ldg(sp) : 1.f;
-        if (a.pad_rows > 0) {
-            if (unit_live && head < a.kv_heads && (lane == 0 || (HD == 64 && lane == 8))) {
-                const float t = s == 0.f ? 1.f : s;  // a block of zeros, or none
-                const int64_t at = ((int64_t)b * a.kv_heads + head) * (a.pad_rows / 16) +
-                                   (page * a.block_size) / 16 + part;
-                if (kv == 0) a.wide_k[at] = t;
-                else {
-                    a.wide_log2[at] = log2f(t);
-                    a.wide_inverse[at] = __fdiv_rn(1.f, t);
+        if constexpr (!WRITE) {
+            float s = on ? __ldg(sp) : 1.f;
+            if (a.pad_rows > 0) {
+                if (unit_live && head < a.kv_heads && (lane == 0 || (HD == 64 && lane == 8))) {
+                    const float t = s == 0.f ? 1.f : s;  // a block of zeros, or none
+                    const int64_t at = ((int64_t)b * a.kv_heads + head) * (a.pad_rows / 16) +
+                                       (page * a.block_size) / 16 + part;
+                    if (kv == 0) a.wide_k[at] = t;
+                    else {
+                        a.wide_log2[at] = log2f(t);
+                        a.wide_inverse[at] = __fdiv_rn(1.f, t);
+                    }
                 }
+                s = 1.f;
             }
-            s = 1.f;
-        }
-        if (!live) return;
-        uint2 q[8];
+            if (!on) continue;
+            uint2 q[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            q[i] = pos0 + 2 * i < end ? __ldg(cell + i * 32) : make_uint2(0, 0);
+            for (int i = 0; i < 8; ++i)
+                q[i] = pos0 + 2 * i < end ? __ldg(cell + i * 32) : make_uint2(0, 0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (pos0 + 2 * i >= end) continue;
+                float lo[4], hi[4];
+                q8_unpack4(q[i].x, lo);
+                q8_unpack4(q[i].y, hi);
+                T o[8];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    o[k] = from_f32<T>(lo[k] * s);
+                    o[4 + k] = from_f32<T>(hi[k] * s);
+                }
+                row[(int64_t)i * 2 * a.row_vecs] = *reinterpret_cast<uint4 *>(o);
+            }
+            continue;
+        }
+
+        uint4 x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            if (pos0 + 2 * i >= end) continue;
-            float lo[4], hi[4];
-            q8_unpack4(q[i].x, lo);
-            q8_unpack4(q[i].y, hi);
-            T o[8];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                o[k] = from_f32<T>(lo[k] * s);
-                o[4 + k] = from_f32<T>(hi[k] * s);
-            }
-            row[(int64_t)i * 2 * a.row_vecs] = *reinterpret_cast<uint4 *>(o);
+            const int32_t p = pos0 + 2 * i;
+            x[i] = on && p >= first && p < end ? __ldg(row + (int64_t)i * 2 * a.row_vecs)
+                                                 : make_uint4(0, 0, 0, 0);
         }
-        return;
-    }
-
-    uint4 x[8];
+        float m = 0.f;
+        bool odd = false;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int32_t p = pos0 + 2 * i;
-        x[i] = live && p >= first && p < end ? __ldg(row + (int64_t)i * 2 * a.row_vecs)
-                                             : make_uint4(0, 0, 0, 0);
-    }
-    float m = 0.f;
-    bool odd = false;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float f[8];
-        unpack8<T>(x[i], f);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float v = fabsf(f[k]);
-            if (v < INFINITY) m = fmaxf(m, v);
-            else odd = true;  // NaN or infinity
-        }
-    }
-    if (odd) record_fault(&g_q8_copy_fault, kFaultNotFinite);
-    // head_dim 64: lanes 0-7 and 16-23 hold one head, the others the second
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-    if (HD == 128) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    if (per > 1) {
-        if ((lane & 15) == (HD == 64 ? hl * 8 : 0) && lane < 16) top[warp][hl] = m;
-        __syncthreads();
-        const int w0 = warp - part;
-        for (int w = 0; w < per; ++w) m = fmaxf(m, top[w0 + w][hl]);
-    }
-    // every thread of the unit reads the old scale before one of them stores
-    // the new one
-    const float s_old = live && held ? *sp : 0.f;
-    __syncthreads();
-    if (!live) return;
-    float s = fmaxf(s_old, __fdiv_rn(m, 127.f));
-    if (s < kQ8MinScale) s = 0.f;
-    const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
-    if (part == 0 && lane < 16 && (lane & (HD == 64 ? 7 : 15)) == 0) *sp = s;
-    const bool rescale = held && s > s_old;
-    const float ratio = s > 0.f ? __fdiv_rn(s_old, s) : 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int32_t p = pos0 + 2 * i;
-        int lo[4], hi[4];
-        if (p >= first) {
-            if (p >= end) continue;
+        for (int i = 0; i < 8; ++i) {
             float f[8];
             unpack8<T>(x[i], f);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                // an infinity times a zero inverse (all others zero) is not a number
-                lo[k] = q8_round(fabsf(f[k]) == INFINITY ? copysignf(127.f, f[k]) : f[k] * inv);
-                hi[k] = q8_round(fabsf(f[4 + k]) == INFINITY ? copysignf(127.f, f[4 + k])
-                                                             : f[4 + k] * inv);
-            }
-        } else {
-            if (!rescale) continue;
-            const uint2 q = cell[i * 32];
-            float g[4], h[4];
-            q8_unpack4(q.x, g);
-            q8_unpack4(q.y, h);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                lo[k] = q8_round(g[k] * ratio);
-                hi[k] = q8_round(h[k] * ratio);
+            for (int k = 0; k < 8; ++k) {
+                const float v = fabsf(f[k]);
+                if (v < INFINITY) m = fmaxf(m, v);
+                else odd = true;  // NaN or infinity
             }
         }
-        cell[i * 32] = make_uint2(q8_pack4(lo), q8_pack4(hi));
+        if (odd) record_fault(&g_q8_copy_fault, kFaultNotFinite);
+        // head_dim 64: lanes 0-7 and 16-23 hold one head, the others the second
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+        if (HD == 128) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        if (per > 1) {
+            if ((lane & 15) == (HD == 64 ? hl * 8 : 0) && lane < 16) top[warp][hl] = m;
+            __syncthreads();
+            const int w0 = warp - part;
+            for (int w = 0; w < per; ++w) m = fmaxf(m, top[w0 + w][hl]);
+        }
+        // every thread of the unit reads the old scale before one of them stores
+        // the new one
+        const float s_old = on && held ? *sp : 0.f;
+        __syncthreads();
+        if (!on) continue;
+        float s = fmaxf(s_old, __fdiv_rn(m, 127.f));
+        if (s < kQ8MinScale) s = 0.f;
+        const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+        if (part == 0 && lane < 16 && (lane & (HD == 64 ? 7 : 15)) == 0) *sp = s;
+        const bool rescale = held && s > s_old;
+        const float ratio = s > 0.f ? __fdiv_rn(s_old, s) : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int32_t p = pos0 + 2 * i;
+            int lo[4], hi[4];
+            if (p >= first) {
+                if (p >= end) continue;
+                float f[8];
+                unpack8<T>(x[i], f);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    // an infinity times a zero inverse (all others zero) is not a number
+                    lo[k] = q8_round(fabsf(f[k]) == INFINITY ? copysignf(127.f, f[k]) : f[k] * inv);
+                    hi[k] = q8_round(fabsf(f[4 + k]) == INFINITY ? copysignf(127.f, f[4 + k])
+                                                                 : f[4 + k] * inv);
+                }
+            } else {
+                if (!rescale) continue;
+                const uint2 q = cell[i * 32];
+                float g[4], h[4];
+                q8_unpack4(q.x, g);
+                q8_unpack4(q.y, h);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    lo[k] = q8_round(g[k] * ratio);
+                    hi[k] = q8_round(h[k] * ratio);
+                }
+            }
+            cell[i * 32] = make_uint2(q8_pack4(lo), q8_pack4(hi));
+        }
     }
 }
 
@@ -262,7 +271,13 @@ cudaError_t launch_q8(const Q8RowArgs &a, cudaStream_t s) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     const int per_cta = kQ8Warps / (a.block_size / 16);
-    cfg.gridDim = dim3((unsigned)((a.units + per_cta - 1) / per_cta), (unsigned)(a.lanes * 2));
+    // Lanes of a page in CTAs of their own while the SMs (148, 8 CTAs each) are
+    // not full twice; then a warp takes several, so that finding the sequence
+    // and the page (three dependent loads) is paid once for them.
+    const int64_t ctas = (a.units + per_cta - 1) / per_cta;
+    int lanes = a.lanes;
+    while (lanes > 1 && ctas * lanes * 2 > 2 * 8 * 148) lanes = (lanes + 1) / 2;
+    cfg.gridDim = dim3((unsigned)ctas, (unsigned)(lanes * 2));
     cfg.blockDim = dim3(kQ8Warps * 32);
     cfg.stream = s;
     cfg.attrs = attr;
