@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import pathlib
+import threading
 from typing import Optional, Sequence
 
 LIB_PATH = pathlib.Path(__file__).resolve().parent / "lib" / "libpkv_b200.so"
@@ -237,10 +238,17 @@ class PkvError(RuntimeError):
     """A C entry point returned 0."""
 
 
+_tls = threading.local()  # one error buffer a thread
+
+
 def _call(name: str, *args):
-    lib = load()
-    err = ctypes.create_string_buffer(512)
-    ok = getattr(lib, name)(*args, err, len(err))
+    lib = _lib or load()
+    try:
+        err = _tls.err
+    except AttributeError:
+        err = _tls.err = ctypes.create_string_buffer(512)
+    err[0] = 0
+    ok = getattr(lib, name)(*args, err, 512)
     if not ok:
         raise PkvError(f"{name}: {err.value.decode(errors='replace')}")
     return ok
@@ -335,16 +343,36 @@ def _ptr(x) -> Optional[int]:
     return x.data_ptr()
 
 
+_dtype_codes: dict = {}
+
+
 def _dtype_code(t) -> int:
-    import torch
-    return {torch.float16: PKV_DTYPE_F16, torch.bfloat16: PKV_DTYPE_BF16,
-            torch.float32: PKV_DTYPE_F32}[t.dtype]
+    if not _dtype_codes:
+        import torch
+        _dtype_codes.update({torch.float16: PKV_DTYPE_F16, torch.bfloat16: PKV_DTYPE_BF16,
+                             torch.float32: PKV_DTYPE_F32})
+    return _dtype_codes[t.dtype]
+
+
+_raw_stream = None
 
 
 def _stream_ptr(stream) -> int:
-    import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    """The given stream, or torch's current one of the current device.  The
+    stream object torch.cuda.current_stream builds costs 3 us a call; the raw
+    lookup a few tenths."""
+    global _raw_stream
+    if stream is not None:
+        return stream.cuda_stream
+    if _raw_stream is None:
+        import torch
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        device = torch.cuda.current_device
+        if raw is not None:
+            _raw_stream = lambda: raw(device())  # noqa: E731
+        else:
+            _raw_stream = lambda: torch.cuda.current_stream().cuda_stream  # noqa: E731
+    return _raw_stream()
 
 
 def make_layer(key_pool, value_pool, block_size: int, kv_heads: int, head_dim: int) -> PkvPagedLayer:

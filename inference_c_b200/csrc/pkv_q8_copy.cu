@@ -50,10 +50,46 @@ struct Q8RowArgs {
     float *wide_k, *wide_log2, *wide_inverse;
 };
 
-struct Q8Unit {
-    int b;
-    int32_t first, count, page0;  // first new position, new rows, first page touched
-};
+// Largest |x| of 64 values, as a float; NaN if one is not a number.
+template <typename T>
+__device__ __forceinline__ float abs_max(const uint4 (&x)[8]);
+template <>
+__device__ __forceinline__ float abs_max<__half>(const uint4 (&x)[8]) {
+    __half2 m = __float2half2_rn(0.f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const __half2 *h = reinterpret_cast<const __half2 *>(&x[i]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m = __hmax2_nan(m, __habs2(h[k]));
+    }
+    const float2 f = __half22float2(m);
+    return f.x != f.x ? f.x : (f.y != f.y ? f.y : fmaxf(f.x, f.y));
+}
+template <>
+__device__ __forceinline__ float abs_max<__nv_bfloat16>(const uint4 (&x)[8]) {
+    __nv_bfloat162 m = __float2bfloat162_rn(0.f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&x[i]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m = __hmax2_nan(m, __habs2(h[k]));
+    }
+    const float2 f = __bfloat1622float2(m);
+    return f.x != f.x ? f.x : (f.y != f.y ? f.y : fmaxf(f.x, f.y));
+}
+
+// rint(x * inv) of four finite values within +-127 as the bytes of a word.
+// Adding 1.5 * 2^23 rounds to a whole number, ties to even, and leaves it in
+// two's complement in the sum's low bits: no conversion, whose unit takes a
+// quarter of a warp a cycle.
+__device__ __forceinline__ uint32_t q8_quantise4(float a, float b, float c, float d, float inv) {
+    constexpr float kRound = 12582912.f;
+    const uint32_t w = __float_as_uint(__fadd_rn(__fmul_rn(a, inv), kRound));
+    const uint32_t x = __float_as_uint(__fadd_rn(__fmul_rn(b, inv), kRound));
+    const uint32_t y = __float_as_uint(__fadd_rn(__fmul_rn(c, inv), kRound));
+    const uint32_t z = __float_as_uint(__fadd_rn(__fmul_rn(d, inv), kRound));
+    return __byte_perm(__byte_perm(w, x, 0x0040), __byte_perm(y, z, 0x0040), 0x5410);
+}
 
 // Sequence b touches at most floor((n_b - 1) / block) + 2 pages, so giving it
 // the units from floor(offsets[b] / block) + 2 b on needs no scan: unit u
@@ -195,20 +231,19 @@ q8_rows_kernel(const Q8RowArgs a) {
             x[i] = on && p >= first && p < end ? __ldg(row + (int64_t)i * 2 * a.row_vecs)
                                                  : make_uint4(0, 0, 0, 0);
         }
-        float m = 0.f;
-        bool odd = false;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float f[8];
-            unpack8<T>(x[i], f);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float v = fabsf(f[k]);
-                if (v < INFINITY) m = fmaxf(m, v);
-                else odd = true;  // NaN or infinity
+        float m = abs_max<T>(x);
+        const bool odd = !(m < INFINITY);  // a NaN or an infinity among them
+        if (odd) {
+            record_fault(&g_q8_copy_fault, kFaultNotFinite);
+            m = 0.f;
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i) {
+                float f[8];
+                unpack8<T>(x[i], f);
+                for (int k = 0; k < 8; ++k)
+                    if (fabsf(f[k]) < INFINITY) m = fmaxf(m, fabsf(f[k]));
             }
         }
-        if (odd) record_fault(&g_q8_copy_fault, kFaultNotFinite);
         // head_dim 64: lanes 0-7 and 16-23 hold one head, the others the second
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
         if (HD == 128) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
@@ -235,20 +270,28 @@ q8_rows_kernel(const Q8RowArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int32_t p = pos0 + 2 * i;
-            int lo[4], hi[4];
             if (p >= first) {
                 if (p >= end) continue;
                 float f[8];
                 unpack8<T>(x[i], f);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    // an infinity times a zero inverse (all others zero) is not a number
-                    lo[k] = q8_round(fabsf(f[k]) == INFINITY ? copysignf(127.f, f[k]) : f[k] * inv);
-                    hi[k] = q8_round(fabsf(f[4 + k]) == INFINITY ? copysignf(127.f, f[4 + k])
-                                                                 : f[4 + k] * inv);
+                if (odd) {  // infinities +-127, NaN (and 0 times a zero scale) 0
+                    int lo[4], hi[4];
+                    for (int k = 0; k < 4; ++k) {
+                        lo[k] = q8_round(fabsf(f[k]) == INFINITY ? copysignf(127.f, f[k])
+                                                                 : f[k] * inv);
+                        hi[k] = q8_round(fabsf(f[4 + k]) == INFINITY ? copysignf(127.f, f[4 + k])
+                                                                     : f[4 + k] * inv);
+                    }
+                    cell[i * 32] = make_uint2(q8_pack4(lo), q8_pack4(hi));
+                } else {
+                    cell[i * 32] = make_uint2(q8_quantise4(f[0], f[1], f[2], f[3], inv),
+                                              q8_quantise4(f[4], f[5], f[6], f[7], inv));
                 }
-            } else {
-                if (!rescale) continue;
+                continue;
+            }
+            if (!rescale) continue;
+            int lo[4], hi[4];
+            {
                 const uint2 q = cell[i * 32];
                 float g[4], h[4];
                 q8_unpack4(q.x, g);
