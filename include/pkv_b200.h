@@ -255,7 +255,14 @@ int pkv_q8_gather(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t 
                   size_t error_capacity);
 
 /* pkv_paged_decode over 8-bit pages: q_heads 1 to 16 times kv_heads (any
- * whole group), query in layer->dtype, output F32 or layer->dtype. */
+ * whole group), query in layer->dtype (16-byte aligned), output F32 or
+ * layer->dtype.  K and V are used exactly (q * s); the query is kept to 2^-22
+ * of its head's largest element, a softmax weight to 2^-23.  max_seq_len
+ * bounds seq_lens: a longer sequence is cut there and fault code 2 recorded.
+ * block_count * lanes * block_size must be below 2^31.  The workspace starts
+ * zeroed once (pkv_decode_workspace_init) and serves any batch it was sized
+ * for; calls that overlap on the GPU need one each.  As pkv_paged_decode, the
+ * kernels release programmatic dependents early. */
 size_t pkv_q8_decode_workspace_bytes(size_t batch, size_t q_heads, size_t kv_heads,
                                      size_t head_dim, size_t max_seq_len);
 int pkv_q8_decode(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads,
@@ -269,8 +276,10 @@ int pkv_q8_decode(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads
  * and KV head g of the batch gets
  *     mass[table[t / block_size]][g][t % block_size] += sum over the query
  *     heads of g of their softmax weight of t.
- * Cells of other positions are left as they are; a sequence's new positions
- * start from what the cell holds, so clear a page's cells when it is taken.
+ * Cells of other positions are left as they are; a new position starts from
+ * what its cell holds, so its cell is cleared when its row is written:
+ * pkv_mass_clear zeroes those of every sequence's last n_b positions
+ * (row_offsets as in pkv_kv_append, NULL: one each).
  * pkv_paged_decode_mass takes the shapes of the tensor-core decode (pages of
  * 16 to 128 tokens; an even number of KV heads with head_dim 64).  Sequences
  * of a batch share no page.  max_seq_len bounds seq_lens (a longer sequence
@@ -283,6 +292,9 @@ int pkv_paged_decode_mass(const PkvPagedLayer *layer, const PkvBatch *batch, siz
                           size_t max_seq_len, float *mass, void *workspace,
                           size_t workspace_bytes, PkvStream stream, char *error,
                           size_t error_capacity);
+int pkv_mass_clear(size_t block_size, size_t block_count, size_t kv_heads,
+                   const PkvBatch *batch, const int32_t *row_offsets, float *mass,
+                   PkvStream stream, char *error, size_t error_capacity);
 int pkv_q8_decode_mass(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads,
                        const void *query, float scale, void *output, PkvDType output_dtype,
                        size_t max_seq_len, float *mass, void *workspace, size_t workspace_bytes,
@@ -450,6 +462,19 @@ int pkv_pool_create(TensorPagedKVCache *cache, int device, PkvDType dtype,
                     size_t layer_count, size_t kv_heads, size_t head_dim,
                     size_t max_batch, size_t max_pages_per_seq,
                     PkvPool **pool, char *error, size_t error_capacity);
+/* The same pool of 8-bit pages: int8 K and V pages with their scales, zeroed,
+ * and with `mass` non-zero the attention mass of every layer; dtype is that of
+ * rows and queries (F16 or BF16), and the cache's block size 16, 32, 64 or 128.
+ * Steps, tables and lengths work as with 16-bit pages; pkv_pool_layer refuses
+ * such a pool, pkv_pool_q8_layer any other. */
+int pkv_pool_create_q8(TensorPagedKVCache *cache, int device, PkvDType dtype, size_t layer_count,
+                       size_t kv_heads, size_t head_dim, size_t max_batch,
+                       size_t max_pages_per_seq, int mass, PkvPool **pool, char *error,
+                       size_t error_capacity);
+int pkv_pool_q8_layer(PkvPool *pool, size_t layer, PkvQ8Layer *out);
+/* Mass of one layer of an 8-bit pool ([block_count][kv_heads][block_size]), or
+ * NULL. */
+float *pkv_pool_mass(PkvPool *pool, size_t layer);
 /* The pool attached to `cache`, or NULL. */
 PkvPool *pkv_pool_from_cache(TensorPagedKVCache *cache);
 /* Device view of one layer. */

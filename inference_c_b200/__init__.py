@@ -167,6 +167,7 @@ EXPORTS = {
     "pkv_q8_decode": (_c_int, [_QP, _BP, _c_size, _c_ptr, ctypes.c_float, _c_ptr, _c_int, _c_size,
                                _c_ptr, _c_size, _c_ptr, *_ERR]),
     "pkv_decode_mass_workspace_bytes": (_c_size, [_c_size] * 5),
+    "pkv_mass_clear": (_c_int, [_c_size, _c_size, _c_size, _BP, _c_ptr, _c_ptr, _c_ptr, *_ERR]),
     "pkv_paged_decode_mass": (_c_int, [_LP, _BP, _c_size, _c_ptr, ctypes.c_float, _c_ptr, _c_int,
                                        _c_size, _c_ptr, _c_ptr, _c_size, _c_ptr, *_ERR]),
     "pkv_q8_decode_mass": (_c_int, [_QP, _BP, _c_size, _c_ptr, ctypes.c_float, _c_ptr, _c_int,
@@ -191,6 +192,10 @@ EXPORTS = {
     # include/pkv_b200.h -- host transaction layer
     "pkv_pool_create": (_c_int, [_c_ptr, _c_int, _c_int, _c_size, _c_size, _c_size, _c_size,
                                  _c_size, ctypes.POINTER(_c_ptr), *_ERR]),
+    "pkv_pool_create_q8": (_c_int, [_c_ptr, _c_int, _c_int, _c_size, _c_size, _c_size, _c_size,
+                                    _c_size, _c_int, ctypes.POINTER(_c_ptr), *_ERR]),
+    "pkv_pool_q8_layer": (_c_int, [_c_ptr, _c_size, _QP]),
+    "pkv_pool_mass": (_c_ptr, [_c_ptr, _c_size]),
     "pkv_pool_from_cache": (_c_ptr, [_c_ptr]),
     "pkv_pool_layer": (_c_int, [_c_ptr, _c_size, _LP]),
     "pkv_step_begin": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_size, _c_ptr, *_ERR]),
@@ -537,14 +542,28 @@ def decode_mass_workspace(batch: int, q_heads: int, kv_heads: int, head_dim: int
     return ws
 
 
-def _decode_mass(name: str, layer, batch: PkvBatch, query, output, scale: float,
-                 max_seq_len: int, mass, workspace, stream) -> None:
+def _check_mass(mass, layer) -> int:
+    """Address of a mass tensor of this layer (an address passes through)."""
+    if isinstance(mass, int):
+        return mass
     if mass.shape != (layer.block_count, layer.kv_heads, layer.block_size) or \
             not mass.is_contiguous():
         raise ValueError("mass is a contiguous [block_count, kv_heads, block_size] tensor")
+    return mass.data_ptr()
+
+
+def mass_clear(layer, batch: PkvBatch, mass, row_offsets=None, stream=None) -> None:
+    """Zeroes the mass of every sequence's last n_b positions (row_offsets as
+    in kv_append; None: one each)."""
+    _call("pkv_mass_clear", layer.block_size, layer.block_count, layer.kv_heads,
+          ctypes.byref(batch), _ptr(row_offsets), _check_mass(mass, layer), _stream_ptr(stream))
+
+
+def _decode_mass(name: str, layer, batch: PkvBatch, query, output, scale: float,
+                 max_seq_len: int, mass, workspace, stream) -> None:
     _call(name, ctypes.byref(layer), ctypes.byref(batch), query.shape[-2], query.data_ptr(),
           ctypes.c_float(scale), output.data_ptr(), _dtype_code(output), max_seq_len,
-          mass.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream_ptr(stream))
+          _check_mass(mass, layer), workspace.data_ptr(), workspace.numel(), _stream_ptr(stream))
 
 
 def paged_decode_mass(layer: PkvPagedLayer, batch: PkvBatch, query, output, scale: float,
@@ -569,14 +588,11 @@ def kv_evict(layer, batch: PkvBatch, mass, keep: int, recent: int, kept, max_seq
     (None: in place)."""
     if kept.shape != (batch.batch, layer.kv_heads, keep) or not kept.is_contiguous():
         raise ValueError("kept is a contiguous [batch, kv_heads, keep] tensor")
-    if mass.shape != (layer.block_count, layer.kv_heads, layer.block_size) or \
-            not mass.is_contiguous():
-        raise ValueError("mass is a contiguous [block_count, kv_heads, block_size] tensor")
     if dst_tables is not None and (dst_tables.shape[0] != batch.batch or
                                    not dst_tables.is_contiguous()):
         raise ValueError("dst_tables is a contiguous [batch, stride] tensor")
     name = "pkv_q8_evict" if isinstance(layer, PkvQ8Layer) else "pkv_kv_evict"
-    _call(name, ctypes.byref(layer), ctypes.byref(batch), mass.data_ptr(), keep, recent,
+    _call(name, ctypes.byref(layer), ctypes.byref(batch), _check_mass(mass, layer), keep, recent,
           _ptr(dst_tables), 0 if dst_tables is None else dst_tables.shape[1], kept.data_ptr(),
           max_seq_len, _stream_ptr(stream))
 
@@ -627,6 +643,30 @@ class PagedPool:
         self.cache = cache
         self.max_batch = max_batch
         self._lib = load()
+
+    @classmethod
+    def q8(cls, cache: PagedKVCache, device: int, dtype: int, layer_count: int, kv_heads: int,
+           head_dim: int, max_batch: int, max_pages_per_seq: int, mass: bool = False):
+        """A pool of 8-bit pages (pkv_pool_create_q8); use q8_layer and mass."""
+        self = cls.__new__(cls)
+        h = _c_ptr()
+        _call("pkv_pool_create_q8", cache.handle, device, dtype, layer_count, kv_heads, head_dim,
+              max_batch, max_pages_per_seq, int(mass), ctypes.byref(h))
+        self.handle = h.value
+        self.cache = cache
+        self.max_batch = max_batch
+        self._lib = load()
+        return self
+
+    def q8_layer(self, index: int) -> PkvQ8Layer:
+        out = PkvQ8Layer()
+        if not self._lib.pkv_pool_q8_layer(self.handle, index, ctypes.byref(out)):
+            raise PkvError(f"pkv_pool_q8_layer({index}) failed")
+        return out
+
+    def mass(self, index: int) -> Optional[int]:
+        """Device address of a layer's mass, or None."""
+        return self._lib.pkv_pool_mass(self.handle, index)
 
     def layer(self, index: int) -> PkvPagedLayer:
         out = PkvPagedLayer()

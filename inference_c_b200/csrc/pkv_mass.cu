@@ -10,6 +10,7 @@
 // 131072 tokens of 64 heads.
 #include "pkv_device.cuh"
 #include "pkv_mass.cuh"
+#include "pkv_trace.h"
 
 namespace pkv {
 namespace {
@@ -95,6 +96,33 @@ __global__ void __launch_bounds__(kTiles * 32) mass_kernel(const MassArgs a) {
     }
 }
 
+// Zeroes the cells of every sequence's last n_b positions: one warp a sequence
+// and KV head, thread = position.
+__global__ void __launch_bounds__(128)
+mass_clear_kernel(const uint32_t *tables, const int32_t *seq_lens, const int32_t *offsets,
+                  float *mass, int table_stride, int block_size, uint32_t block_count,
+                  int kv_heads, int batch) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int g = blockIdx.y * 4 + (threadIdx.x >> 5), b = blockIdx.x;
+    if (g >= kv_heads) return;
+    const int L = __ldg(seq_lens + b);
+    const int n = offsets == nullptr ? 1 : __ldg(offsets + b + 1) - __ldg(offsets + b);
+    if (n > L) {
+        record_fault(&g_mass_fault, kFaultRowsMismatch);
+        return;
+    }
+    for (int t = L - n + (int)(threadIdx.x & 31); t < L; t += 32) {
+        const int page = t / block_size;
+        uint32_t pid = 0, fault = kFaultNone;
+        if (page >= table_stride) fault = kFaultPositionOutOfRange;
+        else if ((pid = __ldg(tables + (int64_t)b * table_stride + page)) >= block_count)
+            fault = kFaultPageOutOfRange;
+        if (fault != kFaultNone) record_fault(&g_mass_fault, fault);
+        else mass[((int64_t)pid * kv_heads + g) * block_size + (t - page * block_size)] = 0.f;
+    }
+}
+
 }  // namespace
 
 bool mass_apply(const MassShape &s, const MassScratch &scratch, const int32_t *tile_prefix,
@@ -137,6 +165,45 @@ bool mass_apply(const MassShape &s, const MassScratch &scratch, const int32_t *t
 }
 
 }  // namespace pkv
+
+extern "C" int pkv_mass_clear(size_t block_size, size_t block_count, size_t kv_heads,
+                              const PkvBatch *batch, const int32_t *row_offsets, float *mass,
+                              PkvStream stream, char *error, size_t error_capacity) {
+    PKV_RANGE("pkv_mass_clear");
+    const char *what = "pkv_mass_clear";
+    if (batch == nullptr || mass == nullptr || batch->block_tables == nullptr ||
+        batch->seq_lens == nullptr || (uintptr_t)mass % 4 != 0) {
+        pkv_internal_set_error(error, error_capacity, "%s: null argument or misaligned mass", what);
+        return 0;
+    }
+    if (block_size == 0 || block_size > INT32_MAX || block_count == 0 ||
+        block_count > UINT32_MAX || kv_heads == 0 || kv_heads > 1024 || batch->batch == 0 ||
+        batch->batch > INT32_MAX / 4 || batch->table_stride == 0 ||
+        batch->table_stride > INT32_MAX) {
+        pkv_internal_set_error(error, error_capacity, "%s: invalid shape", what);
+        return 0;
+    }
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)batch->batch, (unsigned)((kv_heads + 3) / 4));
+    cfg.blockDim = dim3(128);
+    cfg.stream = (cudaStream_t)stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t st = cudaLaunchKernelEx(
+        &cfg, pkv::mass_clear_kernel, batch->block_tables, batch->seq_lens, row_offsets, mass,
+        (int)batch->table_stride, (int)block_size, (uint32_t)block_count, (int)kv_heads,
+        (int)batch->batch);
+    if (st == cudaSuccess) st = cudaGetLastError();
+    if (st != cudaSuccess) {
+        pkv_internal_set_error(error, error_capacity, "%s: launch failed: %s", what,
+                               cudaGetErrorString(st));
+        return 0;
+    }
+    return 1;
+}
 
 extern "C" int pkv_internal_take_mass_fault(uint32_t *code) {
     uint32_t zero = 0;

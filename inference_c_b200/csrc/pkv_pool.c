@@ -43,6 +43,9 @@ struct PkvPool {
     TensorPagedKVCache *cache;
     int device;
     PkvDType dtype;
+    int q8, has_mass;       /* 8-bit pages; with the attention mass */
+    float **scales;         /* 8-bit pages, per layer: K scales, V scales, mass */
+    size_t mass_offset;     /* floats before the mass */
     size_t layer_count, kv_heads, head_dim, block_size, block_count;
     size_t max_batch, max_pages;
     void **kpools;
@@ -80,6 +83,8 @@ static void pool_free_device(PkvPool *p) {
         for (size_t l = 0; l < p->layer_count; ++l) cudaFree(p->kpools[l]);
     if (p->vpools)
         for (size_t l = 0; l < p->layer_count; ++l) cudaFree(p->vpools[l]);
+    if (p->scales)
+        for (size_t l = 0; l < p->layer_count; ++l) cudaFree(p->scales[l]);
     cudaFree(p->d_tables);
     for (int s = 0; s < kStageSlots; ++s) {
         cudaFreeHost(p->h_stage[s]);
@@ -95,6 +100,7 @@ static void pool_destroy(void *state) {
     pool_free_device(p);
     free(p->kpools);
     free(p->vpools);
+    free(p->scales);
     free(p->rows);
     free(p->tmp_pages);
     free(p->step_seq);
@@ -110,15 +116,25 @@ static void pool_release_sequence(void *state, TensorPagedKVSequence sequence) {
         if (p->rows[r].seq == sequence) p->rows[r].seq = 0;
 }
 
-int pkv_pool_create(TensorPagedKVCache *cache, int device, PkvDType dtype,
-                    size_t layer_count, size_t kv_heads, size_t head_dim,
-                    size_t max_batch, size_t max_pages_per_seq, PkvPool **pool,
-                    char *error, size_t cap) {
+/* pkv_pool_create, and with q8 pkv_pool_create_q8 (mass: with the mass). */
+static int pool_create(TensorPagedKVCache *cache, int device, PkvDType dtype,
+                       size_t layer_count, size_t kv_heads, size_t head_dim,
+                       size_t max_batch, size_t max_pages_per_seq, int q8, int mass,
+                       PkvPool **pool, char *error, size_t cap) {
     if (pool == NULL || cache == NULL) {
         pkv_internal_set_error(error, cap, "pkv_pool_create: null argument");
         return 0;
     }
     *pool = NULL;
+    const size_t bs = tensor_paged_kv_cache_block_size(cache);
+    if (q8 && ((dtype != PKV_DTYPE_F16 && dtype != PKV_DTYPE_BF16) || kv_heads > 1024 ||
+               (head_dim != 64 && head_dim != 128) ||
+               (bs != 16 && bs != 32 && bs != 64 && bs != 128))) {
+        pkv_internal_set_error(error, cap,
+                               "pkv_pool_create_q8: needs F16 or BF16 rows, pages of 16, 32, 64 "
+                               "or 128 tokens and 1..1024 KV heads of head_dim 64 or 128");
+        return 0;
+    }
     if ((dtype != PKV_DTYPE_F16 && dtype != PKV_DTYPE_BF16 && dtype != PKV_DTYPE_F32) ||
         layer_count == 0 || kv_heads == 0 || head_dim == 0 ||
         max_batch == 0 || max_batch > INT32_MAX || max_pages_per_seq == 0 ||
@@ -144,12 +160,14 @@ int pkv_pool_create(TensorPagedKVCache *cache, int device, PkvDType dtype,
     p->max_pages = max_pages_per_seq;
     p->kpools = (void **)calloc(layer_count, sizeof(void *));
     p->vpools = (void **)calloc(layer_count, sizeof(void *));
+    p->q8 = q8;
+    p->scales = q8 ? (float **)calloc(layer_count, sizeof(float *)) : NULL;
     p->rows = (RowState *)calloc(max_batch, sizeof(RowState));
     p->tmp_pages = (uint32_t *)malloc(max_pages_per_seq * sizeof(uint32_t));
     p->step_seq = (TensorPagedKVSequence *)calloc(max_batch, sizeof(TensorPagedKVSequence));
     p->step_current = (size_t *)calloc(max_batch, sizeof(size_t));
     p->step_target = (size_t *)calloc(max_batch, sizeof(size_t));
-    if (!p->kpools || !p->vpools || !p->rows || !p->tmp_pages || !p->step_seq ||
+    if (!p->kpools || !p->vpools || (q8 && !p->scales) || !p->rows || !p->tmp_pages || !p->step_seq ||
         !p->step_current || !p->step_target) {
         pool_destroy(p);
         pkv_internal_set_error(error, cap, "pkv_pool_create: out of host memory");
@@ -160,12 +178,22 @@ int pkv_pool_create(TensorPagedKVCache *cache, int device, PkvDType dtype,
     cudaError_t st = cudaSetDevice(device);
     const size_t kv_width = kv_heads * head_dim;
     const size_t elem = dtype == PKV_DTYPE_F32 ? 4u : 2u;
-    const size_t pool_bytes = p->block_count * p->block_size * kv_width * elem;
+    /* 8-bit pages hold whole 128-column lanes of a token's row */
+    const size_t row_bytes = q8 ? (kv_width + 127) / 128 * 128 : kv_width * elem;
+    const size_t pool_bytes = p->block_count * p->block_size * row_bytes;
+    /* per layer: K scales, V scales, then the mass on a 16-byte boundary */
+    const size_t scale_floats = p->block_count * kv_heads;
+    p->mass_offset = align_up(2 * scale_floats, 4);
+    p->has_mass = mass != 0;
+    const size_t extra_bytes =
+        (p->mass_offset + (mass ? scale_floats * p->block_size : 0)) * sizeof(float);
     for (size_t l = 0; st == cudaSuccess && l < layer_count; ++l) {
         st = cudaMalloc(&p->kpools[l], pool_bytes);
         if (st == cudaSuccess) st = cudaMalloc(&p->vpools[l], pool_bytes);
         if (st == cudaSuccess) st = cudaMemset(p->kpools[l], 0, pool_bytes);
         if (st == cudaSuccess) st = cudaMemset(p->vpools[l], 0, pool_bytes);
+        if (q8 && st == cudaSuccess) st = cudaMalloc((void **)&p->scales[l], extra_bytes);
+        if (q8 && st == cudaSuccess) st = cudaMemset(p->scales[l], 0, extra_bytes);
     }
     const size_t table_bytes = max_batch * max_pages_per_seq * sizeof(uint32_t);
     if (st == cudaSuccess) st = cudaMalloc((void **)&p->d_tables, table_bytes);
@@ -208,12 +236,47 @@ int pkv_pool_create(TensorPagedKVCache *cache, int device, PkvDType dtype,
     return 1;
 }
 
+int pkv_pool_create(TensorPagedKVCache *cache, int device, PkvDType dtype,
+                    size_t layer_count, size_t kv_heads, size_t head_dim,
+                    size_t max_batch, size_t max_pages_per_seq, PkvPool **pool,
+                    char *error, size_t cap) {
+    return pool_create(cache, device, dtype, layer_count, kv_heads, head_dim, max_batch,
+                       max_pages_per_seq, 0, 0, pool, error, cap);
+}
+
+int pkv_pool_create_q8(TensorPagedKVCache *cache, int device, PkvDType dtype, size_t layer_count,
+                       size_t kv_heads, size_t head_dim, size_t max_batch,
+                       size_t max_pages_per_seq, int mass, PkvPool **pool, char *error,
+                       size_t cap) {
+    return pool_create(cache, device, dtype, layer_count, kv_heads, head_dim, max_batch,
+                       max_pages_per_seq, 1, mass, pool, error, cap);
+}
+
+int pkv_pool_q8_layer(PkvPool *pool, size_t layer, PkvQ8Layer *out) {
+    if (pool == NULL || out == NULL || !pool->q8 || layer >= pool->layer_count) return 0;
+    out->key_pool = (int8_t *)pool->kpools[layer];
+    out->value_pool = (int8_t *)pool->vpools[layer];
+    out->key_scales = pool->scales[layer];
+    out->value_scales = pool->scales[layer] + pool->block_count * pool->kv_heads;
+    out->block_size = pool->block_size;
+    out->block_count = pool->block_count;
+    out->kv_heads = pool->kv_heads;
+    out->head_dim = pool->head_dim;
+    out->dtype = pool->dtype;
+    return 1;
+}
+
+float *pkv_pool_mass(PkvPool *pool, size_t layer) {
+    if (pool == NULL || !pool->q8 || !pool->has_mass || layer >= pool->layer_count) return NULL;
+    return pool->scales[layer] + pool->mass_offset;
+}
+
 PkvPool *pkv_pool_from_cache(TensorPagedKVCache *cache) {
     return (PkvPool *)tensor_paged_kv_cache_backend_state(cache, TENSOR_PAGED_KV_BACKEND_CUDA);
 }
 
 int pkv_pool_layer(PkvPool *pool, size_t layer, PkvPagedLayer *out) {
-    if (pool == NULL || out == NULL || layer >= pool->layer_count) return 0;
+    if (pool == NULL || out == NULL || pool->q8 || layer >= pool->layer_count) return 0;
     out->key_pool = pool->kpools[layer];
     out->value_pool = pool->vpools[layer];
     out->block_size = pool->block_size;

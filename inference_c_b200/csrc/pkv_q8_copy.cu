@@ -40,6 +40,7 @@ struct Q8RowArgs {
     int32_t table_stride, batch, kv_heads, lanes, block_size;
     uint32_t block_count;
     int32_t units;            // upper bound of pages touched
+    int32_t total_rows;       // of the contiguous buffers
     int32_t row_vecs;         // uint4 per contiguous row
     int32_t tail;             // rows are the sequence's last (append) or first positions
     // > 0: every sequence's first seq_lens[b] rows go to rows b * pad_rows on as
@@ -161,8 +162,10 @@ q8_rows_kernel(const Q8RowArgs a) {
         first = a.tail ? L - count : 0;
         end = first + count;
         page = first / a.block_size + slot;
-        if (count > L) fault = slot == 0 ? kFaultRowsMismatch : kFaultNone;
-        if (count > L || count <= 0 || (int64_t)page * a.block_size >= end) live = false;
+        // more rows than the sequence has, or offsets outside the buffers
+        const bool bad = count > L || row0 < 0 || row0 > a.total_rows - count;
+        if (bad && count > 0) fault = slot == 0 ? kFaultRowsMismatch : kFaultNone;
+        if (bad || count <= 0 || (int64_t)page * a.block_size >= end) live = false;
         if (live) {
             if (page >= a.table_stride) fault = kFaultPositionOutOfRange;
             else {
@@ -371,6 +374,7 @@ int q8_rows(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *offse
     a.units = offsets == nullptr
                   ? (int32_t)batch->batch
                   : (int32_t)(total_rows / layer->block_size + 2 * batch->batch);
+    a.total_rows = (int32_t)total_rows;
     a.row_vecs = (int32_t)(layer->kv_heads * layer->head_dim / 8);
     a.tail = tail ? 1 : 0;
     a.pad_rows = (int32_t)pad_rows;

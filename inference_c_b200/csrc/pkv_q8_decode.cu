@@ -120,6 +120,7 @@ struct Q8Args {
     uint32_t block_count;
     float scale_log2;
     int32_t min_unit;
+    int32_t max_len;         // longer sequences are cut there, with a fault
     int32_t bf16, out_f32;   // row type; 32-bit outputs
     // Mass (else null): every score by stream tile and slot, and every query
     // head's final maximum and sum (pkv_mass.cuh).
@@ -276,7 +277,11 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
     pdl_launch_dependents();
     // Exclusive prefix of tiles (one sequence a thread), lengths and schedule.
     {
-        const int len = tid < a.batch ? max(0, __ldg(a.seq_lens + tid)) : 0;
+        int len = tid < a.batch ? max(0, __ldg(a.seq_lens + tid)) : 0;
+        if (len > a.max_len) {
+            if (blockIdx.x == 0) record_fault(&g_q8_decode_fault, kFaultPositionOutOfRange);
+            len = a.max_len;
+        }
         const int tiles = (len + kTcTile - 1) / kTcTile * a.kv_heads;
         int incl = tiles;
 #pragma unroll
@@ -1029,6 +1034,13 @@ int q8_decode(const char *what, const PkvQ8Layer *layer, const PkvBatch *batch, 
                                what, kMaxBatch);
         return 0;
     }
+    // the stream's tiles are counted in 32 bits
+    if (lanes * subs_of(q_heads / kvh, hd) * ((max_seq_len + 127) / 128) >
+        (size_t)INT32_MAX / kLaunchBatch) {
+        pkv_internal_set_error(error, error_capacity,
+                               "%s: max_seq_len times KV heads is too large", what);
+        return 0;
+    }
     if ((uintptr_t)query % 16 != 0 || (uintptr_t)output % 4 != 0) {
         pkv_internal_set_error(error, error_capacity,
                                "%s: query must be 16-byte, output 4-byte aligned", what);
@@ -1077,6 +1089,7 @@ int q8_decode(const char *what, const PkvQ8Layer *layer, const PkvBatch *batch, 
     a.block_size = (int32_t)layer->block_size;
     a.block_count = (uint32_t)layer->block_count;
     a.scale_log2 = scale * kLog2e;
+    a.max_len = (int32_t)max_seq_len;
     a.bf16 = layer->dtype == PKV_DTYPE_BF16;
     a.out_f32 = output_dtype == PKV_DTYPE_F32;
     MassScratch ms = {};

@@ -105,3 +105,64 @@ def test_prefill_arguments_are_checked(lib):
                      (dict(causal=2), "invalid"), (dict(scale=float("nan")), "invalid")):
         ok, got = call(**kw)
         assert ok == 0 and text in got and "pkv_q8_prefill" in got, (kw, got)
+
+
+def test_mass_and_evict_arguments_are_checked(lib):
+    f = ctypes.c_float
+    L, B = _layer(), _batch()
+    H = P.PkvPagedLayer(256, 256, 16, 4, 2, 128, P.PKV_DTYPE_F16)
+
+    def mass(name, layer, mass=256, q_heads=4, ws_bytes=1 << 40, max_len=64):
+        e = _err()
+        ok = getattr(lib, name)(ctypes.byref(layer), ctypes.byref(B), q_heads, 256, f(1), 256,
+                                P.PKV_DTYPE_F32, max_len, mass, 256, ws_bytes, None, e, len(e))
+        return ok, e.value.decode()
+    for name, layer in (("pkv_q8_decode_mass", L), ("pkv_paged_decode_mass", H)):
+        for kw, text in ((dict(mass=None), "mass"), (dict(mass=260), "mass"),
+                         (dict(ws_bytes=1 << 12), "workspace"), (dict(q_heads=3), "kv_heads")):
+            ok, got = mass(name, layer, **kw)
+            assert ok == 0 and text in got and name in got, (name, kw, got)
+    ok, got = mass("pkv_paged_decode_mass", P.PkvPagedLayer(256, 256, 12, 4, 2, 128, 1))
+    assert ok == 0 and "pages of 16, 32, 64 or 128" in got
+
+    def evict(name, layer, batch=B, mass=256, keep=8, recent=2, dst=None, stride=0, kept=256,
+              max_len=64):
+        e = _err()
+        ok = getattr(lib, name)(ctypes.byref(layer), ctypes.byref(batch), mass, keep, recent, dst,
+                                stride, kept, max_len, None, e, len(e))
+        return ok, e.value.decode()
+    for name, layer in (("pkv_q8_evict", L), ("pkv_kv_evict", H)):
+        for kw, text in ((dict(mass=None), "mass"), (dict(mass=264), "mass"),
+                         (dict(kept=None), "kept"), (dict(keep=0), "keep"),
+                         (dict(recent=9), "recent"), (dict(dst=512, stride=0), "stride"),
+                         (dict(batch=_batch(batch=0)), "batch"),
+                         (dict(batch=_batch(batch=65536)), "65535"),
+                         (dict(batch=_batch(seq_lens=None)), "null")):
+            ok, got = evict(name, layer, **kw)
+            assert ok == 0 and text in got and name in got, (name, kw, got)
+    ok, got = evict("pkv_kv_evict", P.PkvPagedLayer(256, 256, 16, 4, 2, 96, 1))
+    assert ok == 0 and "head_dim" in got
+    e = _err()
+    assert lib.pkv_mass_clear(16, 4, 2, ctypes.byref(B), None, None, None, e, len(e)) == 0
+    assert b"null" in e.value
+    assert lib.pkv_mass_clear(0, 4, 2, ctypes.byref(B), None, 256, None, e, len(e)) == 0
+    assert b"shape" in e.value
+
+
+def test_workspaces_grow_with_what_they_hold(lib):
+    a = lib.pkv_q8_decode_workspace_bytes(1, 32, 8, 128, 4096)
+    b = lib.pkv_q8_decode_workspace_bytes(64, 32, 8, 128, 4096)
+    assert 0 < a < b and a % 256 == 0 and b % 256 == 0
+    m = lib.pkv_decode_mass_workspace_bytes(64, 32, 8, 128, 4096)
+    # every score of every query head, and the decode's own scratch
+    assert m >= b + 64 * 32 * 4096 * 4
+    assert lib.pkv_q8_decode_workspace_bytes(1, 3, 2, 128, 64) == 0
+
+
+def test_q8_pool_shapes_are_checked(lib):
+    for bs, hd, kv, dtype in ((12, 128, 2, P.PKV_DTYPE_F16), (16, 96, 2, P.PKV_DTYPE_F16),
+                              (16, 128, 2000, P.PKV_DTYPE_F16), (16, 128, 2, P.PKV_DTYPE_F32)):
+        cache = P.PagedKVCache(bs, 4, 1)
+        with pytest.raises(P.PkvError, match="8|pages"):
+            P.PagedPool.q8(cache, 0, dtype, 1, kv, hd, 1, 4)
+        cache.free()
