@@ -315,7 +315,8 @@ int pkv_q8_decode_mass(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_
  * Positions of the destination past the result, and the source when it is
  * another place, are left as they are.  8-bit rows that meet in one block take
  * the largest s of their scales, q' = rint(q * (s_row / s)).  max_seq_len
- * should bound seq_lens (it only sizes the launch); mass is 16-byte aligned. */
+ * bounds seq_lens: a longer sequence is left as it is, its list all -1 and
+ * fault code 2 recorded.  mass is 16-byte aligned. */
 int pkv_kv_evict(const PkvPagedLayer *layer, const PkvBatch *batch, float *mass, size_t keep,
                  size_t recent, const uint32_t *dst_tables, size_t dst_stride, int32_t *kept,
                  size_t max_seq_len, PkvStream stream, char *error, size_t error_capacity);

@@ -40,6 +40,7 @@ struct EvictArgs {
     int32_t *kept;          // [batch][kv_heads][keep]
     int32_t table_stride, dst_stride, kv_heads, lanes, block_size, block_shift;
     int32_t keep, recent;
+    int32_t max_len;        // longer sequences are left alone, with a fault
     uint32_t block_count;
     int32_t cached;         // keys a CTA of the select kernel holds
     // pools: 16-bit rows [.][kv_heads * head_dim], or 8-bit pages
@@ -75,8 +76,10 @@ __device__ __forceinline__ bool page_at(const EvictArgs &a, const uint32_t *trow
 // runs of their own (strides of a few powers of two) meet different banks.
 __device__ __forceinline__ int key_slot(int i) { return i + (i >> 5); }
 
-// Grid (CS * kv_heads, batch), clusters of CS CTAs along x.
-template <int CS>
+// Grid (CS * kv_heads, batch), clusters of CS CTAs along x.  RUN > 0: a thread
+// holds its run of at most RUN positions (a multiple of 4) in registers; 0:
+// runs of any length, keys in shared memory or, past that, gathered each time.
+template <int CS, int RUN>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictArgs a) {
     cg::cluster_group cluster = cg::this_cluster();
     auto list_sync = [&] {
@@ -99,9 +102,13 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
     const int rank = CS > 1 ? (int)cluster.block_rank() : 0;
     const int g = blockIdx.x / cs, b = blockIdx.y;
     const int32_t L = max(0, __ldg(a.seq_lens + b));
-    const int32_t n = min(L, a.keep);
+    const int32_t n = L > a.max_len ? 0 : min(L, a.keep);
     int32_t *kept = a.kept + ((int64_t)b * a.kv_heads + g) * a.keep;
     for (int32_t i = n + rank * kSelThreads + tid; i < a.keep; i += cs * kSelThreads) kept[i] = -1;
+    if (L > a.max_len) {
+        if (tid == 0) record_fault(&g_evict_fault, kFaultPositionOutOfRange);
+        return;
+    }
     if (L <= a.keep) {
         for (int32_t i = rank * kSelThreads + tid; i < n; i += cs * kSelThreads) kept[i] = i;
         return;  // the whole cluster: L is the sequence's
@@ -120,8 +127,32 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
         return mass_key(__ldg(a.mass + ((int64_t)pid * a.kv_heads + g) * a.block_size +
                               (t & (a.block_size - 1))));
     };
-    const bool held = hi - lo <= a.cached;
-    if (held) {
+    // This thread's run of positions [r0, r1).
+    const int32_t run = RUN > 0 ? RUN : (hi - lo + kSelThreads - 1) / kSelThreads;
+    const int32_t r0 = min(hi, lo + tid * run), r1 = min(hi, r0 + run);
+    const bool held = RUN > 0 || hi - lo <= a.cached;
+    uint32_t reg[RUN > 0 ? RUN : 1];
+    if constexpr (RUN > 0) {  // all loads in flight; four tokens share a page
+        float4 m[RUN / 4];
+#pragma unroll
+        for (int i = 0; i < RUN / 4; ++i) {
+            uint32_t pid = 0;
+            m[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            const int32_t t = r0 + 4 * i;
+            if (t < r1 && page_at(a, trow, a.table_stride, t, pid))
+                m[i] = __ldg(reinterpret_cast<const float4 *>(
+                    a.mass + ((int64_t)pid * a.kv_heads + g) * a.block_size +
+                    (t & (a.block_size - 1))));
+        }
+#pragma unroll
+        for (int i = 0; i < RUN / 4; ++i) {
+            reg[4 * i] = mass_key(m[i].x);
+            reg[4 * i + 1] = mass_key(m[i].y);
+            reg[4 * i + 2] = mass_key(m[i].z);
+            reg[4 * i + 3] = mass_key(m[i].w);
+        }
+    }
+    if (RUN == 0 && held) {
         // four tokens a load (a page holds a multiple of 16, lo a multiple of
         // 4), four loads in flight
         const int quads = (hi - lo + 3) / 4;
@@ -151,6 +182,16 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
         }
     }
     auto key = [&](int32_t t) { return held ? keys[key_slot(t - lo)] : gather(t); };
+    // f(position, key) over this thread's run, in order
+    auto each = [&](auto f) {
+        if constexpr (RUN > 0) {
+#pragma unroll
+            for (int i = 0; i < RUN; ++i)
+                if (r0 + i < r1) f(r0 + i, reg[i]);
+        } else {
+            for (int32_t t = r0; t < r1; ++t) f(t, key(t));
+        }
+    };
 
     uint32_t prefix = 0, want = (uint32_t)need;  // the want-th largest of those with `prefix`
     uint32_t above = 0;
@@ -159,15 +200,14 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
         const int bits = pass == 2 ? 10 : 11;
         for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
         __syncthreads();
-        for (int32_t t = lo + tid; t < hi; t += kSelThreads) {
-            const uint32_t k = key(t);
-            if (pass == 0 || (k >> (shift + bits)) == prefix) {
-                // masses crowd into few bins: one atomic a bin and warp
-                const uint32_t bin = (k >> shift) & ((1u << bits) - 1u);
-                const uint32_t same = __match_any_sync(__activemask(), bin);
-                if ((__ffs(same) - 1) == lane) atomicAdd(&hist[bin], (uint32_t)__popc(same));
-            }
-        }
+        auto tally = [&](int32_t, uint32_t k) {
+            if (pass != 0 && (k >> (shift + bits)) != prefix) return;
+            // masses crowd into few bins: one atomic a bin and warp
+            const uint32_t bin = (k >> shift) & ((1u << bits) - 1u);
+            const uint32_t same = __match_any_sync(__activemask(), bin);
+            if ((__ffs(same) - 1) == lane) atomicAdd(&hist[bin], (uint32_t)__popc(same));
+        };
+        each(tally);
         list_sync();
         // bins 2 tid and 2 tid + 1 of the whole list, then keys above each
         uint32_t c0 = 0, c1 = 0;
@@ -207,14 +247,11 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
     // Keys above `prefix` are all kept, of those equal to it the first `want`.
     // Each thread takes a run of positions: its counts, one scan over the CTA and
     // the CTAs before it, then its positions in order.
-    const int32_t run = (hi - lo + kSelThreads - 1) / kSelThreads;
-    const int32_t r0 = min(hi, lo + tid * run), r1 = min(hi, r0 + run);
     uint32_t gt = 0, eq = 0;
-    for (int32_t t = r0; t < r1; ++t) {
-        const uint32_t k = key(t);
+    each([&](int32_t, uint32_t k) {
         gt += k > prefix;
         eq += k == prefix;
-    }
+    });
     uint32_t gi = gt, ei = eq;  // inclusive over the warp
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -256,14 +293,13 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
         g_at += c[0];
         e_at += c[1];
     }
-    for (int32_t t = r0; t < r1; ++t) {
-        const uint32_t k = key(t);
+    each([&](int32_t t, uint32_t k) {
         if (k > prefix) kept[g_at++ + min(e_at, want)] = t;
         else if (k == prefix) {
             if (e_at < want) kept[g_at + e_at] = t;
             ++e_at;
         }
-    }
+    });
     list_sync();  // no CTA leaves while its counts are read
 }
 
@@ -280,7 +316,7 @@ __global__ void __launch_bounds__(kMoveRows) evict_move_kernel(const EvictArgs a
     const int tid = threadIdx.x;
     const int g = blockIdx.y, b = blockIdx.z;
     const int32_t L = max(0, __ldg(a.seq_lens + b));
-    const int32_t n = min(L, a.keep);
+    const int32_t n = L > a.max_len ? 0 : min(L, a.keep);
     const int32_t *kept = a.kept + ((int64_t)b * a.kv_heads + g) * a.keep;
     const uint32_t *trow = a.tables + (int64_t)b * a.table_stride;
     const uint32_t *drow = a.dst_tables + (int64_t)b * a.dst_stride;
@@ -434,6 +470,7 @@ int evict(EvictArgs &a, const PkvBatch *batch, size_t head_dim, bool q8, float *
     while ((1 << a.block_shift) < a.block_size) ++a.block_shift;
     a.keep = (int32_t)keep;
     a.recent = (int32_t)recent;
+    a.max_len = (int32_t)max_seq_len;
     const cudaStream_t s = (cudaStream_t)stream;
 
     // A list is shared by eight CTAs where one would hold more than 4096 keys
@@ -441,7 +478,10 @@ int evict(EvictArgs &a, const PkvBatch *batch, size_t head_dim, bool q8, float *
     const size_t lists = batch->batch * (size_t)a.kv_heads;
     const unsigned cs = max_seq_len > 4096 && lists <= 148 ? 8 : 1;
     const size_t span = ((max_seq_len + cs - 1) / cs + 3) / 4 * 4;
-    a.cached = (int32_t)(span <= (size_t)kCachedMax ? span : 0);
+    // keys a thread: 4 or 16 in registers (one sequence of 131072: 36 us with the
+    // keys in shared memory, read through a bounds check and a gap each time)
+    const int held = span <= 4 * kSelThreads ? 4 : span <= 16 * kSelThreads ? 16 : 0;
+    a.cached = (int32_t)(held == 0 && span <= (size_t)kCachedMax ? span : 0);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cs;
@@ -450,26 +490,21 @@ int evict(EvictArgs &a, const PkvBatch *batch, size_t head_dim, bool q8, float *
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(cs * (unsigned)a.kv_heads, (unsigned)batch->batch);
     cfg.blockDim = dim3(kSelThreads);
-    cfg.dynamicSmemBytes = ((size_t)a.cached + a.cached / 32 + 1) * 4;
+    cfg.dynamicSmemBytes = a.cached > 0 ? ((size_t)a.cached + a.cached / 32 + 1) * 4 : 0;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    static int configured[64];
-    int dev = 0;
-    cudaGetDevice(&dev);
+    auto kern = cs == 1 ? (held == 4    ? evict_select_kernel<1, 4>
+                           : held == 16 ? evict_select_kernel<1, 16>
+                                        : evict_select_kernel<1, 0>)
+                        : (held == 4    ? evict_select_kernel<8, 4>
+                           : held == 16 ? evict_select_kernel<8, 16>
+                                        : evict_select_kernel<8, 0>);
     cudaError_t st = cudaSuccess;
-    if (dev >= 0 && dev < 64 && !configured[dev]) {
-        const int most = (kCachedMax + kCachedMax / 32 + 1) * 4;
-        st = cudaFuncSetAttribute(evict_select_kernel<1>,
-                                  cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-        if (st == cudaSuccess)
-            st = cudaFuncSetAttribute(evict_select_kernel<8>,
-                                      cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-        if (st == cudaSuccess) configured[dev] = 1;
-    }
-    if (st == cudaSuccess)
-        st = cs == 1 ? cudaLaunchKernelEx(&cfg, evict_select_kernel<1>, a)
-                     : cudaLaunchKernelEx(&cfg, evict_select_kernel<8>, a);
+    if (cfg.dynamicSmemBytes > 0)
+        st = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  (int)cfg.dynamicSmemBytes);
+    if (st == cudaSuccess) st = cudaLaunchKernelEx(&cfg, kern, a);
     if (st == cudaSuccess) {
         if (q8)
             st = head_dim == 128 ? launch_move<8, true>(a, batch->batch, in_place, s)

@@ -257,7 +257,7 @@ def test_evict(lib, cuda, q8, in_place, kv_heads, hd, bs, dtype, keep, recent):
     _run_evict(case, pages, q8, kv_heads, hd, bs, keep, recent, mass, in_place, cuda, 1500)
 
 
-@pytest.mark.parametrize("max_len", [4096, 9000, 1 << 20])  # one CTA, eight, keys not held
+@pytest.mark.parametrize("max_len", [4096, 9000, 100000, 200000, 1 << 20])  # 4 or 16 keys a thread, one CTA or eight, in shared memory, gathered
 def test_evict_ties_and_odd_masses(lib, cuda, max_len):
     """Few distinct values (ties to the lower position), signed zeros,
     infinities and NaN, over every way a list is shared."""
@@ -290,6 +290,21 @@ def test_evict_bad_pages_are_reported(lib, cuda):
     P.kv_evict(case.layer(), case.batch(), mass, 20, 4, kept, 100, dst_tables=dst[:, :1] * 0)
     torch.cuda.synchronize()
     assert P.device_fault(0) == 2  # the result's second page has no entry
+
+
+def test_evict_leaves_a_sequence_past_the_bound_alone(lib, cuda):
+    import torch
+    case, pages = _evict_case(False, np.array([5000, 60]), 2, 128, 16, "f16", 78, cuda, 20)
+    mass = torch.rand(pages, 2, 16, device=cuda)
+    kept = torch.full((2, 2, 20), 7, dtype=torch.int32, device=cuda)
+    before = case.d_kpool.clone()
+    P.kv_evict(case.layer(), case.batch(), mass, 20, 4, kept, 4096)
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 2
+    assert (kept[0] == -1).all() and (kept[1] >= 0).all()
+    own = case.d_tables[0].long()
+    rows = (own[:, None] * 16 + torch.arange(16, device=cuda)).reshape(-1)
+    assert torch.equal(case.d_kpool[rows], before[rows])
 
 
 def test_evict_refusals(lib, cuda):
