@@ -260,8 +260,8 @@ int pkv_q8_gather(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t 
  * of its head's largest element, a softmax weight to 2^-23.  max_seq_len
  * bounds seq_lens: a longer sequence is cut there and fault code 2 recorded.
  * block_count * lanes * block_size must be below 2^31.  The workspace starts
- * zeroed once (pkv_decode_workspace_init) and serves any batch it was sized
- * for; calls that overlap on the GPU need one each.  As pkv_paged_decode, the
+ * zeroed once (pkv_decode_workspace_init), and again after a fault code 4, and
+ * serves any batch it was sized for; calls that overlap on the GPU need one each.  As pkv_paged_decode, the
  * kernels release programmatic dependents early. */
 size_t pkv_q8_decode_workspace_bytes(size_t batch, size_t q_heads, size_t kv_heads,
                                      size_t head_dim, size_t max_seq_len);
@@ -312,6 +312,7 @@ int pkv_q8_decode_mass(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_
  * Keys keep the rotary position they were stored with.
  * dst_tables ([batch][dst_stride]): pages of the result, none of them a
  * source page of the batch; or NULL (or batch->block_tables): in place.
+ * In place, sequences of the batch share no page.
  * Positions of the destination past the result, and the source when it is
  * another place, are left as they are.  8-bit rows that meet in one block take
  * the largest s of their scales, q' = rint(q * (s_row / s)).  max_seq_len
@@ -325,7 +326,8 @@ int pkv_q8_evict(const PkvQ8Layer *layer, const PkvBatch *batch, float *mass, si
                  size_t max_seq_len, PkvStream stream, char *error, size_t error_capacity);
 
 /* pkv_paged_prefill over 8-bit pages; scale must be positive.  max_seq_len
- * bounds seq_lens (fault code 2 and no keys for a longer sequence).  The pages'
+ * bounds seq_lens (a longer sequence gets no output and records fault code 2
+ * or 3).  The pages'
  * 8-bit numbers are widened to 16-bit rows in the workspace first (exact) and
  * the scales applied to scores and weights.  The byte count is
  * for the whole batch; a smaller workspace that holds at least one sequence

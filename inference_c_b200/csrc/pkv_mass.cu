@@ -40,14 +40,16 @@ __global__ void __launch_bounds__(kTiles * 32) mass_kernel(const MassArgs a) {
     const int k = blockIdx.x * kTiles + (threadIdx.x >> 5);
     const int t = k * 128 + (threadIdx.x & 31) * 4;  // this thread's first token
     if (t >= L) return;
-    const int nt = (L + 127) / 128;
+    // the decode's tiles of this sequence (it may have cut a longer one)
     const int64_t first = __ldcg(a.tile_prefix + b);
+    const int nt = (__ldcg(a.tile_prefix + b + 1) - (int)first) / a.segs;
     const int page = t / a.block_size;  // its 4 tokens share a page
     uint32_t pid = 0, fault = kFaultNone;
     if (page >= a.table_stride) fault = kFaultPositionOutOfRange;
     else if ((pid = __ldg(a.tables + (int64_t)b * a.table_stride + page)) >= a.block_count)
         fault = kFaultPageOutOfRange;
-    else if (first + (int64_t)a.segs * nt > a.tiles)  // longer than the caller's bound
+    else if (nt != (L + 127) / 128 || first + (int64_t)a.segs * nt > a.tiles)
+        // longer than the caller's bound
         fault = kFaultPositionOutOfRange;
     if (fault != kFaultNone) {
         record_fault(&g_mass_fault, fault);

@@ -44,10 +44,13 @@ struct Q8RowArgs {
     int32_t row_vecs;         // uint4 per contiguous row
     int32_t tail;             // rows are the sequence's last (append) or first positions
     // > 0: every sequence's first seq_lens[b] rows go to rows b * pad_rows on as
-    // whole numbers, their scales per 16 rows to `wide` (PkvRowScales), and
-    // table_out gets the identity table of those rows in pages of 128
+    // whole numbers, their scales per 16 rows to `wide` (PkvRowScales);
+    // table_out gets the identity table of those rows in pages of 128 and
+    // lens_out the lengths, 0 for a sequence longer than max_len
     int32_t pad_rows;
     uint32_t *table_out;
+    int32_t *lens_out;
+    int32_t max_len;
     float *wide_k, *wide_log2, *wide_inverse;
 };
 
@@ -134,10 +137,11 @@ q8_rows_kernel(const Q8RowArgs a) {
                 const int at = (row0 + slot * a.block_size) / 128;
                 a.table_out[at] = (uint32_t)at;
             }
-            if (count > a.pad_rows) {  // longer than the caller's bound
+            if (count > a.max_len) {  // longer than the caller's bound
                 if (lane == 0) record_fault(&g_q8_copy_fault, kFaultPositionOutOfRange);
                 count = 0;
             }
+            if (blockIdx.y == 0 && part == 0 && lane == 0 && slot == 0) a.lens_out[b] = count;
         } else if (a.offsets == nullptr) {
             b = u;
             row0 = u;
@@ -334,8 +338,8 @@ cudaError_t launch_q8(const Q8RowArgs &a, cudaStream_t s) {
 template <bool WRITE>
 int q8_rows(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *offsets,
             const void *krows, const void *vrows, size_t total_rows, bool tail, size_t pad_rows,
-            uint32_t *table_out, const PkvRowScales *wide, PkvStream stream, char *error,
-            size_t cap, const char *what) {
+            uint32_t *table_out, int32_t *lens_out, size_t max_len, const PkvRowScales *wide,
+            PkvStream stream, char *error, size_t cap, const char *what) {
     if (!q8_check(layer, batch, error, cap, what)) return 0;
     if (krows == nullptr || vrows == nullptr) {
         pkv_internal_set_error(error, cap, "%s: null rows", what);
@@ -379,6 +383,8 @@ int q8_rows(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *offse
     a.tail = tail ? 1 : 0;
     a.pad_rows = (int32_t)pad_rows;
     a.table_out = table_out;
+    a.lens_out = lens_out;
+    a.max_len = (int32_t)max_len;
     a.wide_k = wide == nullptr ? nullptr : const_cast<float *>(wide->k);
     a.wide_log2 = wide == nullptr ? nullptr : const_cast<float *>(wide->v_log2);
     a.wide_inverse = wide == nullptr ? nullptr : const_cast<float *>(wide->v_inverse);
@@ -402,7 +408,7 @@ int q8_rows(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *offse
 // Scratch of the prefill: 16-bit rows of every sequence, padded to whole pages
 // of 128, and their identity table.
 struct PrefillSpace {
-    size_t pad, k, v, table, scales, total;  // scales: three arrays of scale_bytes
+    size_t pad, k, v, table, lens, scales, total;  // scales: three arrays of scale_bytes
     size_t scale_bytes;
 };
 
@@ -413,7 +419,8 @@ PrefillSpace prefill_space(size_t batch, size_t kv_heads, size_t head_dim, size_
     w.k = 0;
     w.v = bytes;
     w.table = 2 * bytes;
-    w.scales = w.table + (batch * (w.pad / 128) * 4 + 255) / 256 * 256;
+    w.lens = w.table + (batch * (w.pad / 128) * 4 + 255) / 256 * 256;
+    w.scales = w.lens + (batch * 4 + 255) / 256 * 256;
     w.scale_bytes = (batch * kv_heads * (w.pad / 16) * 4 + 255) / 256 * 256;
     w.total = w.scales + 3 * w.scale_bytes;
     return w;
@@ -429,7 +436,7 @@ int pkv_q8_append(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t 
                   PkvStream stream, char *error, size_t error_capacity) {
     PKV_RANGE("pkv_q8_append");
     return pkv::q8_rows<true>(layer, batch, row_offsets, key_rows, value_rows, total_rows, true,
-                              0, nullptr, nullptr, stream, error, error_capacity, "pkv_q8_append");
+                              0, nullptr, nullptr, 0, nullptr, stream, error, error_capacity, "pkv_q8_append");
 }
 
 int pkv_q8_import(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *row_offsets,
@@ -437,7 +444,7 @@ int pkv_q8_import(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t 
                   PkvStream stream, char *error, size_t error_capacity) {
     PKV_RANGE("pkv_q8_import");
     return pkv::q8_rows<true>(layer, batch, row_offsets, key_rows, value_rows, total_rows, false,
-                              0, nullptr, nullptr, stream, error, error_capacity, "pkv_q8_import");
+                              0, nullptr, nullptr, 0, nullptr, stream, error, error_capacity, "pkv_q8_import");
 }
 
 int pkv_q8_gather(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *row_offsets,
@@ -445,7 +452,7 @@ int pkv_q8_gather(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t 
                   size_t error_capacity) {
     PKV_RANGE("pkv_q8_gather");
     return pkv::q8_rows<false>(layer, batch, row_offsets, key_out, value_out, total_rows, false,
-                               0, nullptr, nullptr, stream, error, error_capacity, "pkv_q8_gather");
+                               0, nullptr, nullptr, 0, nullptr, stream, error, error_capacity, "pkv_q8_gather");
 }
 
 size_t pkv_q8_prefill_workspace_bytes(size_t batch, size_t kv_heads, size_t head_dim,
@@ -521,7 +528,8 @@ int pkv_q8_prefill(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_head
         PkvBatch rows;
         rows.block_tables = table;
         rows.table_stride = w.pad / 128;
-        rows.seq_lens = part.seq_lens;
+        auto *lens = reinterpret_cast<int32_t *>(base + w.lens);
+        rows.seq_lens = lens;
         rows.batch = n;
         PkvRowScales scales;
         scales.k = reinterpret_cast<float *>(base + w.scales);
@@ -529,8 +537,8 @@ int pkv_q8_prefill(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_head
         scales.v_inverse = reinterpret_cast<float *>(base + w.scales + 2 * w.scale_bytes);
         scales.stride = w.pad / 16;
         if (!pkv::q8_rows<false>(layer, &part, nullptr, wide.key_pool, wide.value_pool, n * w.pad,
-                                 false, w.pad, table, &scales, stream, error, error_capacity,
-                                 what) ||
+                                 false, w.pad, table, lens, max_seq_len, &scales, stream, error,
+                                 error_capacity, what) ||
             !pkv_internal_paged_prefill_ex(&wide, &rows, q_heads, query_offsets + b0, query,
                                            total_query_rows, max_query_len, scale, causal, output,
                                            output_dtype, nullptr, 0, 0, 0, &scales, stream, error,

@@ -263,10 +263,11 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
         tma_prefetch_desc(&kmap);
         tma_prefetch_desc(&vmap);
     }
-    // Lengths and block tables into L2 while the kernel before this one
-    // finishes (a hint: nothing is read before the wait).
+    // Lengths and block tables (the first 2 MiB) into L2 while the kernel before
+    // this one finishes (a hint: nothing is read before the wait).
     {
-        const size_t bytes = (size_t)a.batch * (size_t)a.table_stride * 4u;
+        const size_t all = (size_t)a.batch * (size_t)a.table_stride * 4u;
+        const size_t bytes = all < (size_t(2) << 20) ? all : (size_t(2) << 20);
         const char *tb = reinterpret_cast<const char *>(a.tables);
         for (size_t off = ((size_t)blockIdx.x * kThreads + tid) * 128u; off < bytes;
              off += (size_t)gridDim.x * kThreads * 128u)

@@ -135,6 +135,34 @@ def test_mass_of_one_long_sequence_adds_up(lib, cuda, q8):
     assert P.device_fault(0) == 2 and torch.equal(mass, before)
 
 
+@pytest.mark.parametrize("q8", [False, True])
+def test_mass_past_the_bound_beside_short_sequences(lib, cuda, q8):
+    """The scratch would hold the scores, the bound is broken all the same."""
+    import torch
+    lens = [300, 10, 10, 10]
+    if q8:
+        case = Q8Case(lens, 4, 2, 128, 16, "f16", seed=67, device=cuda)
+        pages, call = case.k.q.shape[0], P.q8_decode_mass
+    else:
+        case = PagedCase(lens, 4, 2, 128, 16, "f16", seed=67, device=cuda)
+        pages, call = case.pool_pages, P.paged_decode_mass
+    mass = torch.zeros(pages, 2, 16, device=cuda)
+    ws = P.decode_mass_workspace(4, 4, 2, 128, 300)
+    out = torch.empty(4, 4, 128, dtype=torch.float32, device=cuda)
+    call(case.layer(), case.batch(), case.d_q, out, case.scale, 128, mass, ws)
+    torch.cuda.synchronize()
+    fault = P.device_fault(0)
+    t = mass.double().cpu().numpy()
+    # each sequence's weights are there whole or not at all, and it is reported;
+    # the 8-bit decode cuts the long one, so the others always fit
+    assert fault == 2
+    for b, L in enumerate(lens):
+        own = t[case.tables[b][:-(-L // 16)].astype(np.int64)].sum(axis=(0, 2))
+        full = np.allclose(own, 2, atol=1e-4)
+        assert full or not own.any()
+        assert not q8 or full == (b > 0)
+
+
 def test_paged_decode_mass_refuses_other_shapes(lib, cuda):
     import torch
     case = PagedCase([40], 3, 3, 64, 16, "f16", seed=5, device=cuda)  # odd KV heads of 64

@@ -221,12 +221,21 @@ def test_prefill(lib, cuda, q_heads, kv_heads, hd, bs, dtype, out, causal, parts
 
 
 def test_prefill_longer_than_bound_is_reported(lib, cuda):
+    """Such a sequence gets no output, whatever its length says; the others do."""
     import torch
     case = Q8Case([200, 20], 4, 2, 128, 16, "f16", seed=3, device=cuda)
     offs = torch.tensor([0, 1, 2], dtype=torch.int32, device=cuda)
     ws = P.q8_prefill_workspace(case.layer(), 2, 100)
-    out = torch.empty(2, 4, 128, dtype=torch.float16, device=cuda)
-    P.q8_prefill(case.layer(), case.batch(), case.d_q, offs, out, case.scale, 1, 100, ws)
-    torch.cuda.synchronize()
-    assert P.device_fault(0) != 0
-    assert P.device_fault(0) == 0
+    for long in (200, 101, 1 << 28):
+        lens = torch.tensor([long, 20], dtype=torch.int32, device=cuda)
+        out = torch.full((2, 4, 128), 7.0, device=cuda)
+        P.q8_prefill(case.layer(), P.make_batch(case.d_tables, lens), case.d_q, offs, out,
+                     case.scale, 1, 100, ws)
+        torch.cuda.synchronize()
+        assert P.device_fault(0) in (2, 3)
+        assert P.device_fault(0) == 0
+        assert (out[0] == 7.0).all()
+        q = widen(case.qbits, "f16").astype(np.float64)
+        want, _, _ = attend64(q[1:2], case.k.read64(case.tables[1], 20),
+                              case.v.read64(case.tables[1], 20), case.scale)
+        assert np.abs(out[1].double().cpu().numpy() - want[0]).max() < 1e-4
