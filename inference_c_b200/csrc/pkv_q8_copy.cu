@@ -151,7 +151,7 @@ q8_rows_kernel(const Q8RowArgs a) {
             while (n > 1) {
                 const int step = (n + 31) / 32, at = lo + min(lane * step, n - 1);
                 const uint32_t below = __ballot_sync(0xffffffffu, q8_first_unit(a, at) <= u);
-                const int k = 31 - __clz(below);  // lane 0's always is
+                const int k = max(0, 31 - __clz(below));
                 lo += min(k * step, n - 1);
                 n = min(step, a.batch - lo);
                 if (step == 1) break;
@@ -159,7 +159,7 @@ q8_rows_kernel(const Q8RowArgs a) {
             b = lo;
             row0 = __ldg(a.offsets + b);
             count = __ldg(a.offsets + b + 1) - row0;
-            slot = u - q8_first_unit(a, b);
+            slot = u - q8_first_unit(a, b);  // below 0: before offsets[0], nobody's
         }
         const int32_t L = !WRITE && a.pad_rows > 0 ? count : __ldg(a.seq_lens + b);
         uint32_t fault = kFaultNone;
@@ -169,7 +169,7 @@ q8_rows_kernel(const Q8RowArgs a) {
         // more rows than the sequence has, or offsets outside the buffers
         const bool bad = count > L || row0 < 0 || row0 > a.total_rows - count;
         if (bad && count > 0) fault = slot == 0 ? kFaultRowsMismatch : kFaultNone;
-        if (bad || count <= 0 || (int64_t)page * a.block_size >= end) live = false;
+        if (bad || count <= 0 || slot < 0 || (int64_t)page * a.block_size >= end) live = false;
         if (live) {
             if (page >= a.table_stride) fault = kFaultPositionOutOfRange;
             else {

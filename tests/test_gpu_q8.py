@@ -78,6 +78,43 @@ def test_append_rescale_import_gather(lib, cuda, kv_heads, hd, bs, dtype):
     assert P.device_fault(0) == 0
 
 
+@pytest.mark.parametrize("batch", [1, 5, 70])
+def test_offsets_that_start_behind_the_first_row(lib, cuda, batch):
+    """The rows of a call may be any run of a longer buffer: append, import and
+    gather with row_offsets[0] > 0 do as with the run by itself."""
+    import torch
+    skip, kv_heads, hd, bs, dtype = 75, 3, 64, 16, "f16"
+    lengths = 20 + (np.arange(batch) * 7) % 31
+    case = Q8Case(lengths, kv_heads, kv_heads, hd, bs, dtype, seed=15, device=cuda)
+    offs = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32)
+    n = int(offs[-1])
+    bits = [_rows(17, skip + n, kv_heads, hd, dtype, s) for s in (4, 5)]
+    dev = [to_device_bits(x, dtype, cuda) for x in bits]
+    d_offs = torch.from_numpy(offs + skip).to(cuda)
+    x = [widen(b, dtype).reshape(-1, kv_heads, hd)[skip:] for b in bits]
+    for call, tail in ((P.q8_import, 0), (P.q8_append, 1)):
+        take = np.minimum(lengths, 9) if tail else lengths
+        at = np.concatenate([[0], np.cumsum(take)]).astype(np.int32)
+        rows = [torch.cat([d[:skip], d[skip:skip + int(at[-1])]]) for d in dev]
+        call(case.layer(), case.batch(), *rows, torch.from_numpy(at + skip).to(cuda))
+        for pool, r in zip((case.k, case.v), x):
+            for b, L in enumerate(lengths):
+                pool.write(case.tables[b], int(L - take[b]), r[at[b]:at[b + 1]])
+        torch.cuda.synchronize()
+        assert P.device_fault(0) == 0
+        case.same_pages()
+    outs = [torch.full((skip + n, kv_heads * hd), 7.0, dtype=torch.float16, device=cuda)
+            for _ in range(2)]
+    P.q8_gather(case.layer(), case.batch(), *outs, d_offs)
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 0
+    for pool, out in zip((case.k, case.v), outs):
+        want = np.concatenate([pool.read(case.tables[b], int(L)).reshape(int(L), -1)
+                               for b, L in enumerate(lengths)])
+        assert (out[:skip] == 7.0).all()
+        assert np.array_equal(to_host_bits(out[skip:]), W.storage_bits(want, dtype))
+
+
 @pytest.mark.parametrize("kv_heads,hd,bs,dtype", SHAPES[::3])
 def test_import_equals_write_at_zero(lib, cuda, kv_heads, hd, bs, dtype):
     import torch
