@@ -260,9 +260,11 @@ int pkv_q8_gather(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t 
  * of its head's largest element, a softmax weight to 2^-23.  max_seq_len
  * bounds seq_lens: a longer sequence is cut there and fault code 2 recorded.
  * block_count * lanes * block_size must be below 2^31.  The workspace starts
- * zeroed once (pkv_decode_workspace_init), and again after a fault code 4, and
- * serves any batch it was sized for; calls that overlap on the GPU need one each.  As pkv_paged_decode, the
- * kernels release programmatic dependents early. */
+ * zeroed once (pkv_decode_workspace_init), and again after a fault code 4.  It
+ * serves any batch it was sized for and, if large enough, the tensor-core
+ * shapes of pkv_paged_decode in turn; calls that overlap on the GPU need one
+ * each.  As pkv_paged_decode, the kernels release programmatic dependents
+ * early. */
 size_t pkv_q8_decode_workspace_bytes(size_t batch, size_t q_heads, size_t kv_heads,
                                      size_t head_dim, size_t max_seq_len);
 int pkv_q8_decode(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads,
@@ -283,8 +285,8 @@ int pkv_q8_decode(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads
  * pkv_paged_decode_mass takes the shapes of the tensor-core decode (pages of
  * 16 to 128 tokens; an even number of KV heads with head_dim 64).  Sequences
  * of a batch share no page.  max_seq_len bounds seq_lens (a longer sequence
- * records fault code 2 and adds nothing).  One workspace size serves both
- * calls; it must start zeroed once (pkv_decode_workspace_init). */
+ * records fault code 2 and adds nothing).  One workspace serves both
+ * calls, in any order; it must start zeroed once (pkv_decode_workspace_init). */
 size_t pkv_decode_mass_workspace_bytes(size_t batch, size_t q_heads, size_t kv_heads,
                                        size_t head_dim, size_t max_seq_len);
 int pkv_paged_decode_mass(const PkvPagedLayer *layer, const PkvBatch *batch, size_t q_heads,

@@ -476,9 +476,7 @@ size_t round_up(size_t v, size_t m) { return (v + m - 1) / m * m; }
 constexpr int kTcThreads = 224;
 constexpr int kTcStages = 3;
 constexpr int kTcMaxBatch = 1024;
-constexpr int kTcMaxGrid = 256;
 constexpr int kInKernelMergeMax = 32;
-constexpr int kTcMaxUnits = kTcMaxGrid * (1 + kMaxRounds);  // work units of one launch
 constexpr int kRing = 4;  // unit ids in flight from the K producer to the other roles
 constexpr size_t kMinUnitTiles = 8;  // smallest dynamic unit
 constexpr uint32_t kTcStageBytes = 65536;
@@ -551,8 +549,8 @@ struct TcWorkspace {
 TcWorkspace tc_workspace(size_t units, size_t heads) {
     TcWorkspace w;
     w.claim = 0;
-    w.counters = 256;
-    w.prefix = w.counters + round_up((size_t)kTcMaxUnits * sizeof(uint32_t), 256);
+    w.counters = kTicketsAt;
+    w.prefix = kZeroBytes;
     w.ml = w.prefix + round_up(((size_t)kTcMaxBatch + 1) * sizeof(int32_t), 256);
     w.o = w.ml + round_up(units * 2 * heads * 2 * sizeof(float), 256);
     w.total = w.o + round_up(units * 2 * heads * 128 * sizeof(float), 256);

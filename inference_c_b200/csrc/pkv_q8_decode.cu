@@ -139,8 +139,8 @@ Workspace workspace_of(size_t units, size_t segments, size_t gv) {
     const size_t partials = (2 * units + segments) * 2 * gv;
     Workspace w;
     w.claim = 0;
-    w.sched = 256;
-    w.prefix = 512;
+    w.sched = kZeroBytes;
+    w.prefix = w.sched + 256;
     w.ml = w.prefix + round_up(((size_t)kLaunchBatch + 1) * 4, 256);
     w.o = w.ml + round_up(partials * 8, 256);
     w.total = w.o + round_up(partials * 512, 256);

@@ -7,12 +7,22 @@
 // sequence) are read.
 #pragma once
 
+#include <stddef.h>
+
 #include "pkv_device.cuh"
 
 namespace pkv {
 
 constexpr int kTcTile = 128;    // tokens of one tile
 constexpr int kMaxRounds = 5;   // dynamic rounds
+constexpr int kTcMaxGrid = 256;
+constexpr int kTcMaxUnits = kTcMaxGrid * (1 + kMaxRounds);  // work units of one launch
+
+// Both decode kernels keep what must be zero between launches in the first
+// kZeroBytes of their workspace (two claim words, then the 16-bit decode's
+// merge tickets, by unit), so one workspace serves either in turn.
+constexpr size_t kTicketsAt = 256;
+constexpr size_t kZeroBytes = kTicketsAt + (kTcMaxUnits * 4 + 255) / 256 * 256;
 
 // a / b for a >= 0, b > 0.  A 64-bit division costs a GPU thread several
 // hundred cycles, and a handful of them precede every CTA's first load and its

@@ -105,6 +105,41 @@ def test_q8_decode_mass(lib, cuda, q_heads, kv_heads, hd, bs, dtype, out):
                 0 if out == "f32" else torch.finfo(od).eps)
 
 
+@pytest.mark.parametrize("q_heads,kv_heads,hd", [(32, 8, 128), (4, 2, 64)])
+def test_one_workspace_serves_both_decodes_in_turn(lib, cuda, q_heads, kv_heads, hd):
+    """A model with 16-bit and 8-bit layers: whatever ran before in the
+    workspace, each call gives the bits it gives in a fresh one."""
+    import torch
+    lens = [1031, 5, 700]  # segments in several pieces
+    a = PagedCase(lens, q_heads, kv_heads, hd, 16, "f16", seed=64, device=cuda)
+    b = Q8Case(lens, q_heads, kv_heads, hd, 16, "f16", seed=65, device=cuda)
+
+    def run(half, ws, with_mass):
+        case = a if half else b
+        pages = a.pool_pages if half else b.k.q.shape[0]
+        mass = torch.zeros(pages, kv_heads, 16, device=cuda)
+        out = torch.full((3, q_heads, hd), float("nan"), device=cuda)
+        args = (case.layer(), case.batch(), case.d_q, out, case.scale, 1031)
+        if with_mass:
+            (P.paged_decode_mass if half else P.q8_decode_mass)(*args, mass, ws)
+        else:
+            (P.paged_decode if half else P.q8_decode)(*args, ws)
+        return out, mass
+
+    def fresh():
+        return P.decode_mass_workspace(3, q_heads, kv_heads, hd, 1031)
+
+    calls = [(h, m) for h in (True, False) for m in (True, False)]
+    want = {c: run(c[0], fresh(), c[1]) for c in calls}
+    ws = fresh()
+    for first in calls:
+        for second in calls:
+            for c in (first, second):
+                out, mass = run(c[0], ws, c[1])
+                assert torch.equal(out, want[c][0]) and torch.equal(mass, want[c][1]), (c, first)
+    assert P.device_fault(0) == 0
+
+
 @pytest.mark.parametrize("q8", [False, True])
 def test_mass_of_one_long_sequence_adds_up(lib, cuda, q8):
     """Many pieces and the merge kernel; over three steps every head's mass
