@@ -198,7 +198,12 @@ q8_rows_kernel(const Q8RowArgs a) {
             float s = on ? __ldg(sp) : 1.f;
             if (a.pad_rows > 0) {
                 if (unit_live && head < a.kv_heads && (lane == 0 || (HD == 64 && lane == 8))) {
-                    const float t = s == 0.f ? 1.f : s;  // a block of zeros, or none
+                    // A block of zeros, or none.  Its weights meet zeros of V and only
+                    // enter the softmax sum, in FP32, but they also enter the maximum
+                    // that the others are relative to: 2^-31 is below every scale of
+                    // fp16 rows, whose weights would else run out of fp16's exponents
+                    // (V near 1e-3 beside one block of zeros).
+                    const float t = s != 0.f ? s : kv == 0 ? 1.f : 4.65661287e-10f;
                     const int64_t at = ((int64_t)b * a.kv_heads + head) * (a.pad_rows / 16) +
                                        (page * a.block_size) / 16 + part;
                     if (kv == 0) a.wide_k[at] = t;

@@ -257,6 +257,45 @@ def test_prefill(lib, cuda, q_heads, kv_heads, hd, bs, dtype, out, causal, parts
         assert np.all(diff <= tol + halves * vmax), (b, float(diff.max()))
 
 
+@pytest.mark.parametrize("dtype,amp", [("f16", 1e-3), ("f16", 2e-5), ("bf16", 1e-12)])
+def test_small_values_beside_pages_of_zeros(lib, cuda, dtype, amp):
+    """A page of zeros in V does not cost the other pages' weights their bits:
+    the error stays in proportion to the values (bounds of test_prefill and
+    test_decode with vmax the case's own)."""
+    import torch
+    L, n = 700, 40
+    case = Q8Case([L], 4, 2, 128, 16, dtype, seed=57, device=cuda)
+    for pool, a in ((case.k, 1.0), (case.v, amp)):
+        x = widen(W.storage_bits(W.normal(58, L * 256) * np.float32(a), dtype), dtype)
+        x = x.reshape(L, 2, 128)
+        x[:32] = 0
+        x[320:336, 1] = 0
+        pool.write(case.tables[0], 0, x)
+    case.upload()
+    qbits = W.normal_bits(59, (n, 4, 128), dtype, stream=9)
+    q = widen(qbits, dtype).astype(np.float64)
+    got = torch.full((n, 4, 128), float("nan"), device=cuda)
+    offs = torch.tensor([0, n], dtype=torch.int32, device=cuda)
+    P.q8_prefill(case.layer(), case.batch(), to_device_bits(qbits, dtype, cuda), offs, got,
+                 case.scale, n, L, P.q8_prefill_workspace(case.layer(), 1, L))
+    one = torch.full((1, 4, 128), float("nan"), device=cuda)
+    P.q8_decode(case.layer(), case.batch(), to_device_bits(qbits[-1:], dtype, cuda), one,
+                case.scale, L, P.q8_decode_workspace(1, 4, 2, 128, L))
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 0
+    k, v = case.k.read64(case.tables[0], L), case.v.read64(case.tables[0], L)
+    want, _, worst = attend64(q, k, v, case.scale, L - n + 1 + np.arange(n))
+    vmax = float(np.abs(v).max())
+    tol = attend_tol(worst, 128, vmax, want, 0)
+    assert np.all(np.abs(one.double().cpu().numpy()[0] - want[-1]) <= tol[-1])
+    # A weight is kept relative to the row's largest p vs, in fp16 halves with an
+    # error of 2^-25 at most, and multiplies a whole number up to 127; the sum
+    # it is divided by is sum(p) / max(p vs) >= 1 / max(vs).  So L keys are off
+    # by at most L 2^-25 127 max(vs) = L 2^-25 vmax.
+    halves = 2.0 ** -16 if dtype == "bf16" else 2.0 ** -21 + L * 2.0 ** -25
+    assert np.all(np.abs(got.double().cpu().numpy() - want) <= tol + halves * vmax)
+
+
 def test_prefill_longer_than_bound_is_reported(lib, cuda):
     """Such a sequence gets no output, whatever its length says; the others do."""
     import torch
