@@ -74,6 +74,9 @@ constexpr int kRing = 4;             // unit ids in flight between the roles
 constexpr int kScaleSlots = 16;      // tiles whose scales are in shared memory
 constexpr uint32_t kTileBytes = 16384;
 constexpr float kDigitMax = 8323072.f;  // 127 * 2^16: three signed digits hold +-this
+// 2^-103, the least V scale that weights are cut against: kDigitMax over a
+// smaller one would leave FP32's range.
+constexpr float kLeastTop = 9.86076132e-32f;
 
 template <int GV>
 struct Cfg {
@@ -682,12 +685,13 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                         const float4 v2 = *reinterpret_cast<const float4 *>(sl1 + e * 16 + 8);
                         const float4 v3 = *reinterpret_cast<const float4 *>(sl1 + e * 16 + 12);
                         const float top = fmaxf(
-                            fmaxf(fmaxf(fmaxf(v0.x, v0.y), fmaxf(v0.z, v0.w)),
-                                  fmaxf(fmaxf(v1.x, v1.y), fmaxf(v1.z, v1.w))),
-                            fmaxf(fmaxf(fmaxf(v2.x, v2.y), fmaxf(v2.z, v2.w)),
-                                  fmaxf(fmaxf(v3.x, v3.y), fmaxf(v3.z, v3.w))));
+                            kLeastTop,
+                            fmaxf(fmaxf(fmaxf(fmaxf(v0.x, v0.y), fmaxf(v0.z, v0.w)),
+                                        fmaxf(fmaxf(v1.x, v1.y), fmaxf(v1.z, v1.w))),
+                                  fmaxf(fmaxf(fmaxf(v2.x, v2.y), fmaxf(v2.z, v2.w)),
+                                        fmaxf(fmaxf(v3.x, v3.y), fmaxf(v3.z, v3.w)))));
                         // weight digits: p * vs / top * kDigitMax
-                        const float f = top > 0.f ? __fdividef(kDigitMax, top) : 0.f;
+                        const float f = __fdividef(kDigitMax, top);
                         const int at = e * 16 + (row >> page_shift);
                         ks[0][e] = sl0[at];
                         ks[1][e] = sl1[at];

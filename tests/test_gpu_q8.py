@@ -296,6 +296,30 @@ def test_small_values_beside_pages_of_zeros(lib, cuda, dtype, amp):
     assert np.all(np.abs(got.double().cpu().numpy() - want) <= tol + halves * vmax)
 
 
+@pytest.mark.parametrize("hd,kv", [(128, 2), (64, 2)])
+def test_decode_of_the_smallest_scales(lib, cuda, hd, kv):
+    """bf16 V near 2^-100, with scales that a weight's digits divided by them
+    would leave FP32: digits are cut against 2^-103 there, half a step of which
+    (2^-103 / (127 2^16) / 2) times 127 for each of the keys bounds the error."""
+    import torch
+    L = 300
+    case = Q8Case([L], 4, kv, hd, 16, "bf16", seed=57, device=cuda)
+    x = W.normal(58, L * kv * hd).astype(np.float64) * 2.0 ** -100
+    x = widen(W.storage_bits(x.astype(np.float32), "bf16"), "bf16").reshape(L, kv, hd)
+    case.v.write(case.tables[0], 0, x)
+    assert 0 < case.v.s[case.tables[0][:19]].max() < 2.0 ** -104
+    case.upload()
+    got = torch.full((1, 4, hd), float("nan"), device=cuda)
+    P.q8_decode(case.layer(), case.batch(), case.d_q, got, case.scale, L,
+                P.q8_decode_workspace(1, 4, kv, hd, L))
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 0
+    k, v = case.k.read64(case.tables[0], L), case.v.read64(case.tables[0], L)
+    want, _, worst = attend64(widen(case.qbits, "bf16").astype(np.float64), k, v, case.scale)
+    tol = attend_tol(worst, hd, float(np.abs(v).max()), want, 0) + L * 2.0 ** -120
+    assert np.all(np.abs(got.double().cpu().numpy() - want) <= tol)
+
+
 def test_prefill_longer_than_bound_is_reported(lib, cuda):
     """Such a sequence gets no output, whatever its length says; the others do."""
     import torch
