@@ -547,8 +547,8 @@ def _check_mass(mass, layer) -> int:
     if isinstance(mass, int):
         return mass
     if mass.shape != (layer.block_count, layer.kv_heads, layer.block_size) or \
-            not mass.is_contiguous():
-        raise ValueError("mass is a contiguous [block_count, kv_heads, block_size] tensor")
+            not mass.is_contiguous() or mass.element_size() != 4:
+        raise ValueError("mass is a contiguous float32 [block_count, kv_heads, block_size] tensor")
     return mass.data_ptr()
 
 
@@ -586,11 +586,13 @@ def kv_evict(layer, batch: PkvBatch, mass, keep: int, recent: int, kept, max_seq
     positions of every sequence and KV head stay, listed in kept (int32
     [batch, kv_heads, keep]); dst_tables [batch, stride]: pages of the result
     (None: in place)."""
-    if kept.shape != (batch.batch, layer.kv_heads, keep) or not kept.is_contiguous():
-        raise ValueError("kept is a contiguous [batch, kv_heads, keep] tensor")
+    if kept.shape != (batch.batch, layer.kv_heads, keep) or not kept.is_contiguous() or \
+            kept.element_size() != 4:
+        raise ValueError("kept is a contiguous int32 [batch, kv_heads, keep] tensor")
     if dst_tables is not None and (dst_tables.shape[0] != batch.batch or
-                                   not dst_tables.is_contiguous()):
-        raise ValueError("dst_tables is a contiguous [batch, stride] tensor")
+                                   not dst_tables.is_contiguous() or
+                                   dst_tables.element_size() != 4):
+        raise ValueError("dst_tables is a contiguous int32 [batch, stride] tensor")
     name = "pkv_q8_evict" if isinstance(layer, PkvQ8Layer) else "pkv_kv_evict"
     _call(name, ctypes.byref(layer), ctypes.byref(batch), _check_mass(mass, layer), keep, recent,
           _ptr(dst_tables), 0 if dst_tables is None else dst_tables.shape[1], kept.data_ptr(),

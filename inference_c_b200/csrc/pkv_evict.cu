@@ -5,9 +5,9 @@
 // the lower position.  A radix select over the mass as ordered 32-bit keys
 // (11 + 11 + 10 bits, most significant first) finds the smallest key kept,
 // then one scan in position order writes the list.  A cluster of CTAs shares
-// one list: each CTA keeps its run of positions in shared memory, so the
-// paged mass is gathered once, and the histograms are summed over distributed
-// shared memory.  Counts and ranks are whole numbers: the result does not
+// one list: each CTA gathers the mass of its run of positions once (into
+// registers, longer runs into shared memory, the longest each time anew), and
+// the histograms are summed over distributed shared memory.  Counts and ranks are whole numbers: the result does not
 // depend on the order of the atomics.
 //
 // evict_move_kernel: rows, mass and (8-bit) scales to their new places.
@@ -317,6 +317,7 @@ __global__ void __launch_bounds__(kMoveRows) evict_move_kernel(const EvictArgs a
     const int g = blockIdx.y, b = blockIdx.z;
     const int32_t L = max(0, __ldg(a.seq_lens + b));
     const int32_t n = L > a.max_len ? 0 : min(L, a.keep);
+    if (IN_PLACE && L <= a.keep) return;  // every row is where it stays
     const int32_t *kept = a.kept + ((int64_t)b * a.kv_heads + g) * a.keep;
     const uint32_t *trow = a.tables + (int64_t)b * a.table_stride;
     const uint32_t *drow = a.dst_tables + (int64_t)b * a.dst_stride;
@@ -419,7 +420,9 @@ cudaError_t launch_move(const EvictArgs &a, size_t batch, bool in_place, cudaStr
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(in_place ? 1u : (unsigned)((a.keep + kMoveRows - 1) / kMoveRows), (unsigned)a.kv_heads, (unsigned)batch);
+    const int32_t rows = a.keep < a.max_len ? a.keep : a.max_len;  // of the longest result
+    cfg.gridDim = dim3(in_place || rows == 0 ? 1u : (unsigned)((rows + kMoveRows - 1) / kMoveRows),
+                       (unsigned)a.kv_heads, (unsigned)batch);
     cfg.blockDim = dim3(kMoveRows);
     cfg.stream = s;
     cfg.attrs = attr;

@@ -25,8 +25,8 @@ struct MassShape {
     size_t gv, subs;  // slots of a segment, segments of a lane
 };
 
-// Sequences of one decode launch (the schedule's prefix lives in shared
-// memory), so also of one mass pass.
+// Most sequences of one decode launch (1024 over 16-bit pages, 512 over 8-bit
+// ones: the schedule's prefix lives in shared memory), so also of a mass pass.
 constexpr size_t kMassBatch = 1024;
 
 inline size_t mass_lanes(size_t kv_heads, size_t head_dim) {

@@ -454,3 +454,29 @@ def test_steps_then_eviction_then_steps(lib, cuda):
         step(i)
     case.same_pages()
     assert P.device_fault(0) == 0
+
+
+def test_tensors_of_other_types_are_refused(lib, cuda):
+    import torch
+    case = Q8Case([40], 4, 2, 128, 16, "f16", seed=3, device=cuda)
+    pages = case.k.q.shape[0]
+    mass = torch.zeros(pages, 2, 16, device=cuda)
+    kept = torch.zeros(1, 2, 8, dtype=torch.int32, device=cuda)
+    with pytest.raises(ValueError, match="float32"):
+        P.mass_clear(case.layer(), case.batch(), mass.half())
+    with pytest.raises(ValueError, match="float32"):
+        P.kv_evict(case.layer(), case.batch(), mass.double(), 8, 2, kept, 40)
+    with pytest.raises(ValueError, match="int32"):
+        P.kv_evict(case.layer(), case.batch(), mass, 8, 2, kept.long(), 40)
+    with pytest.raises(ValueError, match="int32"):
+        P.kv_evict(case.layer(), case.batch(), mass, 8, 2, kept, 40,
+                   dst_tables=torch.zeros(1, 1, dtype=torch.int64, device=cuda))
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_keep_far_above_the_lengths(lib, cuda, in_place):
+    """The list is filled to its end, the rows are those there are."""
+    import torch
+    case, pages = _evict_case(True, [40, 0, 300], 2, 128, 16, "f16", 87, cuda, 100000)
+    mass = _mass(np.random.default_rng(7), pages, 2, 16)
+    _run_evict(case, pages, True, 2, 128, 16, 100000, 3, mass, in_place, cuda, 300)
