@@ -81,6 +81,8 @@ __device__ __forceinline__ int key_slot(int i) { return i + (i >> 5); }
 // runs of any length, keys in shared memory or, past that, gathered each time.
 template <int CS, int RUN>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictArgs a) {
+    pdl_wait();
+    pdl_launch_dependents();
     cg::cluster_group cluster = cg::this_cluster();
     auto list_sync = [&] {
         if constexpr (CS > 1) cluster.sync();
@@ -202,10 +204,11 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
         __syncthreads();
         auto tally = [&](int32_t, uint32_t k) {
             if (pass != 0 && (k >> (shift + bits)) != prefix) return;
-            // masses crowd into few bins: one atomic a bin and warp
+            // Masses crowd into few bins, even so an atomic for each is fastest:
+            // adding up a warp's equal bins first took 7 of 74 us at 131072
+            // positions, with all masses equal 4 of 69.
             const uint32_t bin = (k >> shift) & ((1u << bits) - 1u);
-            const uint32_t same = __match_any_sync(__activemask(), bin);
-            if ((__ffs(same) - 1) == lane) atomicAdd(&hist[bin], (uint32_t)__popc(same));
+            atomicAdd(&hist[bin], 1u);
         };
         each(tally);
         list_sync();
@@ -312,7 +315,10 @@ __global__ void __launch_bounds__(kMoveRows) evict_move_kernel(const EvictArgs a
     __shared__ int64_t to[kMoveRows];    // and of its place
     __shared__ float ratio[2][kMoveRows];
     __shared__ float wtop[2][kMoveRows / 32];
-    constexpr int ITEMS = 16 * VEC * 2 / kMoveRows;
+    // rows of a step: eight 16-byte loads a thread in flight (in place fewer, a
+    // row's read must precede the writes behind it by a barrier each step)
+    constexpr int ROWS = IN_PLACE ? 16 : 8 * kMoveRows / (2 * VEC);
+    constexpr int ITEMS = ROWS * VEC * 2 / kMoveRows;
     const int tid = threadIdx.x;
     const int g = blockIdx.y, b = blockIdx.z;
     const int32_t L = max(0, __ldg(a.seq_lens + b));
@@ -370,13 +376,12 @@ __global__ void __launch_bounds__(kMoveRows) evict_move_kernel(const EvictArgs a
             __syncthreads();
         }
         const int32_t rows = min(kMoveRows, n - i0);
-#pragma unroll 2
-        for (int32_t r0 = 0; r0 < rows; r0 += 16) {
+        for (int32_t r0 = 0; r0 < rows; r0 += ROWS) {
             uint4 x[ITEMS];
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
                 const int it = i * kMoveRows + tid;
-                const int kv = it / (16 * VEC), r = r0 + it / VEC % 16, c = it % VEC;
+                const int kv = it / (ROWS * VEC), r = r0 + it / VEC % ROWS, c = it % VEC;
                 x[i] = make_uint4(0, 0, 0, 0);
                 if (from[r] >= 0) x[i] = __ldcg((kv == 0 ? a.pools[0] : a.pools[1]) + from[r] + c);
             }
@@ -384,7 +389,7 @@ __global__ void __launch_bounds__(kMoveRows) evict_move_kernel(const EvictArgs a
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
                 const int it = i * kMoveRows + tid;
-                const int kv = it / (16 * VEC), r = r0 + it / VEC % 16, c = it % VEC;
+                const int kv = it / (ROWS * VEC), r = r0 + it / VEC % ROWS, c = it % VEC;
                 if (from[r] < 0) continue;
                 if (Q8 && ratio[kv][r] != 1.f) {
                     const float f = ratio[kv][r];
@@ -485,7 +490,9 @@ int evict(EvictArgs &a, const PkvBatch *batch, size_t head_dim, bool q8, float *
     // keys in shared memory, read through a bounds check and a gap each time)
     const int held = span <= 4 * kSelThreads ? 4 : span <= 16 * kSelThreads ? 16 : 0;
     a.cached = (int32_t)(held == 0 && span <= (size_t)kCachedMax ? span : 0);
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cs;
     attr[0].val.clusterDim.y = 1;
@@ -496,7 +503,7 @@ int evict(EvictArgs &a, const PkvBatch *batch, size_t head_dim, bool q8, float *
     cfg.dynamicSmemBytes = a.cached > 0 ? ((size_t)a.cached + a.cached / 32 + 1) * 4 : 0;
     cfg.stream = s;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     auto kern = cs == 1 ? (held == 4    ? evict_select_kernel<1, 4>
                            : held == 16 ? evict_select_kernel<1, 16>
                                         : evict_select_kernel<1, 0>)
