@@ -6,15 +6,22 @@
 // with one scale per (page, KV head).  The pages go to the tensor cores as
 // they lie: q . k_t = ks (q . kq_t) and p v = (p vs) vq, so a scale multiplies
 // a score and a softmax weight, never an element, and no byte of K or V is
-// converted.  The other operand is cut into three signed base-256 digits:
+// converted.  The other operand is cut into signed base-256 digits:
 //   q = f (d0 2^16 + d1 2^8 + d2), f a power of two per query head (22 bits),
-//   p vs = F (d0 2^16 + d1 2^8 + d2), F per tile and head (23 bits),
+//   p vs = F (d0 2^24 + d1 2^16 + d2 2^8 + d3), F the largest V scale of a pair
+//   of tiles and a KV head over 127 * 2^24 (31 bits),
 // each digit one row of the B operand of tcgen05.mma kind::i8, whose sums are
 // exact 32-bit integers.  So a tile costs
-//   S^T[128 tok][3 GV] = K . Qd^T   and   O^T[128 dim][3 GV] = V^T . Pd^T
+//   S^T[128 tok][3 GV] = K . Qd^T   and   O^T[128 dim][4 GV] = V^T . Pd^T
 // and the only roundings are those of the digits, of exp and of FP32 sums
-// over tiles.  Bytes past a sequence's length are finite whatever they are and
-// meet digits of zero.
+// over tiles.  p is relative to the pair's own maximum (the step to the running
+// one goes into the FP32 factor of the pair's O), so what the digits round off
+// is 2^-32 of the pair's largest weight and not of the largest of all: with one
+// dominant token (an attention sink) the other 10^5 together carry an output
+// that digits relative to it would lose, 1% of it with the sink 16 nats up.
+// Three digits would lose the sink's own pair: 255 weights of 2^-24.
+// Bytes past a sequence's length are finite whatever they are and meet digits
+// of zero.
 //
 // Bound by HBM: 2 bytes a token, KV head and column.  One persistent 512-thread
 // CTA per SM:
@@ -73,29 +80,31 @@ constexpr size_t kMinUnitTiles = 8;  // smallest dynamic unit
 constexpr int kRing = 4;             // unit ids in flight between the roles
 constexpr int kScaleSlots = 16;      // tiles whose scales are in shared memory
 constexpr uint32_t kTileBytes = 16384;
-constexpr float kDigitMax = 8323072.f;  // 127 * 2^16: three signed digits hold +-this
-// 2^-103, the least V scale that weights are cut against: kDigitMax over a
-// smaller one would leave FP32's range.
-constexpr float kLeastTop = 9.86076132e-32f;
+constexpr float kDigitMax = 2130706432.f;  // 127 * 2^24: four signed digits hold +-this
+// 2^-94, the least V scale that weights are cut against: kDigitMax over it and
+// it over kDigitMax are normal FP32 numbers.
+constexpr float kLeastTop = 5.04870979e-29f;
+constexpr float kLowest = -3.40282347e38f;  // FP32's lowest finite number
 
 template <int GV>
 struct Cfg {
-    static constexpr int N = GV == 4 ? 16 : GV == 8 ? 32 : 48;  // B rows (digit-major, padded)
+    // B rows, digit-major, padded to 16: three digits a query, four a weight
+    static constexpr int NQ = GV == 4 ? 16 : GV == 8 ? 32 : 48, NP = 4 * GV;
     static constexpr int KS = GV == 4 ? 6 : 5;  // K tiles in the ring
     static constexpr int VS = GV == 4 ? 6 : 5;  // V tiles
     static constexpr int NB = GV == 16 ? 2 : 4; // S, P and O buffers, one per pair of tiles
-    static constexpr uint32_t BT = N * 128;                      // bytes of one B tile
+    static constexpr uint32_t QT = NQ * 128, PT = NP * 128;      // bytes of one B tile
     static constexpr uint32_t V_OFF = KS * kTileBytes;
     static constexpr uint32_t Q_OFF = V_OFF + VS * kTileBytes;
     static constexpr int QB = GV == 16 ? 2 : 4;                  // query tiles ahead
-    static constexpr uint32_t P_OFF = Q_OFF + QB * BT;
-    static constexpr uint32_t SC_OFF = P_OFF + 2 * NB * BT;
+    static constexpr uint32_t P_OFF = Q_OFF + QB * QT;
+    static constexpr uint32_t SC_OFF = P_OFF + 2 * NB * PT;
     static constexpr uint32_t BAR_OFF = SC_OFF + kScaleSlots * 128;
     static constexpr uint32_t MISC_OFF = BAR_OFF + 512;
     static constexpr uint32_t PREFIX_OFF = MISC_OFF + 2624;
-    static constexpr uint32_t O_COL = 2 * NB * N;                // S of two tiles, then O
+    static constexpr uint32_t O_COL = 2 * NB * NQ;               // S of two tiles, then O
     static constexpr uint32_t TMEM_COLS = GV == 4 ? 256 : 512;
-    static_assert(3 * NB * N <= (int)TMEM_COLS, "tensor memory");
+    static_assert(NB * (2 * NQ + NP) <= (int)TMEM_COLS, "tensor memory");
     // tile prefix and lengths of the sequences
     static size_t smem(int batch) { return PREFIX_OFF + 4u * (2u * (size_t)batch + 1u) + 1024u; }
     static_assert(PREFIX_OFF + 4u * (2u * kLaunchBatch + 1u) + 1024u <= 232448u, "shared memory");
@@ -157,9 +166,10 @@ __device__ __forceinline__ float redux_max(float v) {
     return r;
 }
 
-// The three signed base-256 digits of u as the bytes of a word: adding 128 to
-// the two lower digits makes the carries, flipping their top bits takes it off.
-__device__ __forceinline__ uint32_t digits(int u) { return (uint32_t)(u + 0x8080) ^ 0x8080u; }
+// The signed base-256 digits of u as the bytes of a word: adding 128 to the
+// lower digits makes the carries, flipping their top bits takes it off.
+__device__ __forceinline__ uint32_t digits3(int u) { return (uint32_t)(u + 0x8080) ^ 0x8080u; }
+__device__ __forceinline__ uint32_t digits4(int u) { return ((uint32_t)u + 0x808080u) ^ 0x808080u; }
 
 // Byte offset of (row, col) in a tile of 128-byte rows, 128-byte swizzle.
 __device__ __forceinline__ uint32_t sw_byte(uint32_t row, uint32_t col) {
@@ -204,9 +214,9 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                     const __grid_constant__ CUtensorMap vmap) {
     using namespace sm100;
     using C = Cfg<GV>;
-    constexpr int N = C::N, KS = C::KS, VS = C::VS, NB = C::NB, QB = C::QB;
-    constexpr uint32_t kIdescQK = idesc_s8(128, N, false, false);
-    constexpr uint32_t kIdescPV = idesc_s8(128, N, true, false);
+    constexpr int NQ = C::NQ, NP = C::NP, KS = C::KS, VS = C::VS, NB = C::NB, QB = C::QB;
+    constexpr uint32_t kIdescQK = idesc_s8(128, NQ, false, false);
+    constexpr uint32_t kIdescPV = idesc_s8(128, NP, true, false);
     extern __shared__ unsigned char smem_raw[];
     unsigned char *sm = reinterpret_cast<unsigned char *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -256,7 +266,7 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
         fence_mbar_init();
     }
     // B rows past the digits (and, paired, the other head's columns) stay zero
-    for (int i = tid; i < (int)((QB + 2 * NB) * C::BT / 16); i += kThreads)
+    for (int i = tid; i < (int)((QB * C::QT + 2 * NB * C::PT) / 16); i += kThreads)
         reinterpret_cast<uint4 *>(sm + C::Q_OFF)[i] = make_uint4(0, 0, 0, 0);
     if (warp == 12) {
         tmem_alloc(tmem_slot, C::TMEM_COLS);
@@ -473,7 +483,7 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                 // Query digits: lane holds 4 columns of a row (head_dim 64: the
                 // first half warp, at the head's half of the 128 columns).
                 constexpr int HD = PAIR ? 64 : 128;
-                unsigned char *qb = sm + C::Q_OFF + qb_i * C::BT;
+                unsigned char *qb = sm + C::Q_OFF + qb_i * C::QT;
                 for (int h0 = 0; h0 < GV; h0 += 4) {
                     uint2 raw[4];
 #pragma unroll
@@ -511,7 +521,7 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                         const float back = __uint_as_float((uint32_t)(ex - 21) << 23);  // 1 / f
                         uint32_t d[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) d[e] = digits(__float2int_rn(x[e] * f));
+                        for (int e = 0; e < 4; ++e) d[e] = digits3(__float2int_rn(x[e] * f));
                         if (lane * 4 < HD) {
                             const uint32_t col = lane * 4 + (PAIR && h >= GV / 2 ? 64 : 0);
 #pragma unroll
@@ -548,7 +558,7 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                 const int n = desc[qb_i].x;
                 mbar_arrive(&q_empty[qb_i]);
                 if (n == 0) break;
-                const uint64_t qd = qdesc + (uint64_t)(qb_i * (C::BT >> 4));
+                const uint64_t qd = qdesc + (uint64_t)(qb_i * (C::QT >> 4));
                 for (int k = 0; ok && k < n; k += 2, ++pc) {
                     const uint32_t buf = pc % NB;
                     const int n2 = min(2, n - k);
@@ -560,7 +570,7 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                             if (!ok) break;
                             tc_fence_after();
                             const uint64_t ad = kdesc + (uint64_t)(stage * (kTileBytes >> 4));
-                            const uint32_t dst = tmem + (2 * buf + i) * N;
+                            const uint32_t dst = tmem + (2 * buf + i) * NQ;
                             mma_i8_ss_at<0, 0>(dst, ad, qd, kIdescQK, 0);
                             mma_i8_ss_at<2, 2>(dst, ad, qd, kIdescQK, 1);
                             mma_i8_ss_at<4, 4>(dst, ad, qd, kIdescQK, 1);
@@ -573,14 +583,14 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                         mbar_arrive(&s_full[buf]);
                     } else {
                         ok = mbar_wait(&p_full[buf], (pc / NB) & 1, abort_flag, fault);
-                        const uint32_t dst = tmem + C::O_COL + buf * N;
+                        const uint32_t dst = tmem + C::O_COL + buf * NP;
                         for (int i = 0; ok && i < n2; ++i, ++j) {
                             const uint32_t stage = j % VS;
                             ok = mbar_wait(&vfull[stage], (j / VS) & 1, abort_flag, fault);
                             if (!ok) break;
                             tc_fence_after();
                             const uint64_t ad = vdesc + (uint64_t)(stage * (kTileBytes >> 4));
-                            const uint64_t bd = pdesc + (uint64_t)((2 * buf + i) * (C::BT >> 4));
+                            const uint64_t bd = pdesc + (uint64_t)((2 * buf + i) * (C::PT >> 4));
                             mma_i8_ss_at<0, 0>(dst, ad, bd, kIdescPV, i);
                             mma_i8_ss_at<256, 2>(dst, ad, bd, kIdescPV, 1);
                             mma_i8_ss_at<512, 4>(dst, ad, bd, kIdescPV, 1);
@@ -619,8 +629,7 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                 const int n = desc[qb_i].x;
                 if (aborted || n == 0) break;
                 const int len = desc[qb_i].y, slot = desc[qb_i].z, tile0 = desc[qb_i].w;
-                float m_run[GV], l_part[GV], acc[GV], alpha_prev[GV], qs[GV];
-                float f_prev[PAIR ? 2 : 1];
+                float m_run[GV], l_part[GV], acc[GV], alpha_prev[GV], f_prev[GV], qs[GV];
 #pragma unroll
                 for (int h = 0; h < GV; ++h) {
                     m_run[h] = -INFINITY;
@@ -628,39 +637,45 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                     acc[h] = 0.f;
                     qs[h] = qscale[qb_i * 16 + h];
                 }
-                // N columns of TMEM at `col`, this thread's row
-                auto load_cols = [&](uint32_t col, float (&v)[N]) {
+                // COLS columns of TMEM at `col`, this thread's row
+                auto load_cols = [&](uint32_t col, auto &v) {
+                    constexpr int COLS = sizeof(v) / sizeof(v[0]);
 #pragma unroll
-                    for (int i = 0; i < N; ++i) v[i] = 0.f;
+                    for (int i = 0; i < COLS; ++i) v[i] = 0.f;
                     if (aborted) return;
-                    if constexpr (N == 48) {
+                    if constexpr (COLS > 32) {
                         tmem_ld_32x32b<32>(tmem + col + lane_off,
                                            *reinterpret_cast<float(*)[32]>(&v[0]));
-                        tmem_ld_32x32b<16>(tmem + col + 32 + lane_off,
-                                           *reinterpret_cast<float(*)[16]>(&v[32]));
+                        tmem_ld_32x32b<COLS - 32>(tmem + col + 32 + lane_off,
+                                                  *reinterpret_cast<float(*)[COLS - 32]>(&v[32]));
                     } else {
-                        tmem_ld_32x32b<N>(tmem + col + lane_off, v);
+                        tmem_ld_32x32b<COLS>(tmem + col + lane_off, v);
                     }
                 };
-                // slot h's number from its three digit sums
-                auto number = [&](const float (&v)[N], int h) -> float {
-                    const int lo = __float_as_int(v[GV + h]) * 256 + __float_as_int(v[2 * GV + h]);
-                    return fmaf((float)__float_as_int(v[h]), 65536.f, (float)lo);
+                // two digit sums as one whole number (a sum is 2^22 at most)
+                auto two = [](float hi, float lo) {
+                    return __float_as_int(hi) * 256 + __float_as_int(lo);
                 };
-                // O of this group's previous pair, whose weights were relative
-                // to that pair's maximum and scaled by F = f_prev
+                // slot h's score from its three digit sums
+                auto number = [&](const float (&v)[NQ], int h) -> float {
+                    return fmaf((float)__float_as_int(v[h]), 65536.f,
+                                (float)two(v[GV + h], v[2 * GV + h]));
+                };
+                // O of this group's previous pair from its four digit sums; its
+                // weights were cut by a factor that f_prev takes back
                 auto fold = [&](uint32_t pair) {
                     const uint32_t buf = pair % NB;
                     await(&o_full[buf], (pair / NB) & 1);
-                    float o[N];
+                    float o[NP];
                     tc_fence_after();
-                    load_cols(C::O_COL + buf * N, o);
+                    load_cols(C::O_COL + buf * NP, o);
                     tmem_wait_ld();
                     tc_fence_before();
 #pragma unroll
                     for (int h = 0; h < GV; ++h)
-                        acc[h] = fmaf(number(o, h), f_prev[PAIR && h >= GV / 2 ? 1 : 0],
-                                      acc[h] * alpha_prev[h]);
+                        acc[h] = fmaf(fmaf((float)two(o[h], o[GV + h]), 65536.f,
+                                           (float)two(o[2 * GV + h], o[3 * GV + h])),
+                                      f_prev[h], acc[h] * alpha_prev[h]);
                 };
                 int64_t mine = -1;  // this group's previous pair of the piece
                 for (int k = 0; k < n; k += 2, ++pc) {
@@ -670,12 +685,12 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                     if ((int)(pc & 1) != grp) continue;
                     const uint32_t buf = pc % NB;
                     await(&s_full[buf], (pc / NB) & 1);
-                    float s[2][N];
+                    float s[2][NQ];
                     tc_fence_after();
-                    load_cols(2 * buf * N, s[0]);
-                    load_cols((2 * buf + 1) * N, s[1]);  // past an odd end: not used
+                    load_cols(2 * buf * NQ, s[0]);
+                    load_cols((2 * buf + 1) * NQ, s[1]);  // past an odd end: not used
                     // scales: a token's own, and the largest V scale of the pair
-                    float ks[2][PAIR ? 2 : 1], pf[2][PAIR ? 2 : 1], f_cur[PAIR ? 2 : 1];
+                    float ks[2][PAIR ? 2 : 1], pf[2][PAIR ? 2 : 1], top[PAIR ? 2 : 1];
                     const float *sl0 = scales + (j0 % kScaleSlots) * 32;
                     const float *sl1 = n2 > 1 ? scales + ((j0 + 1) % kScaleSlots) * 32 : sl0;
 #pragma unroll
@@ -684,20 +699,19 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                         const float4 v1 = *reinterpret_cast<const float4 *>(sl0 + e * 16 + 12);
                         const float4 v2 = *reinterpret_cast<const float4 *>(sl1 + e * 16 + 8);
                         const float4 v3 = *reinterpret_cast<const float4 *>(sl1 + e * 16 + 12);
-                        const float top = fmaxf(
+                        top[e] = fmaxf(
                             kLeastTop,
                             fmaxf(fmaxf(fmaxf(fmaxf(v0.x, v0.y), fmaxf(v0.z, v0.w)),
                                         fmaxf(fmaxf(v1.x, v1.y), fmaxf(v1.z, v1.w))),
                                   fmaxf(fmaxf(fmaxf(v2.x, v2.y), fmaxf(v2.z, v2.w)),
                                         fmaxf(fmaxf(v3.x, v3.y), fmaxf(v3.z, v3.w)))));
                         // weight digits: p * vs / top * kDigitMax
-                        const float f = __fdividef(kDigitMax, top);
+                        const float f = __fdividef(kDigitMax, top[e]);
                         const int at = e * 16 + (row >> page_shift);
                         ks[0][e] = sl0[at];
                         ks[1][e] = sl1[at];
                         pf[0][e] = sl0[at + 8] * f;
                         pf[1][e] = sl1[at + 8] * f;
-                        f_cur[e] = top * (1.f / kDigitMax);
                     }
                     tmem_wait_ld();
                     tc_fence_before();
@@ -718,26 +732,30 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                     if constexpr (NB == 2)  // the weights below overwrite the previous pair's
                         if (mine >= 0) fold((uint32_t)mine);
                     group_sync();
-                    float alpha[GV];
-                    unsigned char *pb = sm + C::P_OFF + 2 * buf * C::BT;
+                    float alpha[GV], f_cur[GV];
+                    unsigned char *pb = sm + C::P_OFF + 2 * buf * C::PT;
 #pragma unroll
                     for (int h = 0; h < GV; ++h) {
                         const int e = PAIR && h >= GV / 2 ? 1 : 0;
                         const float4 r = *reinterpret_cast<const float4 *>(myred + h * 4);
-                        const float m_new =
-                            fmaxf(m_run[h], fmaxf(fmaxf(r.x, r.y), fmaxf(r.z, r.w)));
+                        // the pair's maximum (finite, should every score be -inf)
+                        const float m_pair =
+                            fmaxf(kLowest, fmaxf(fmaxf(r.x, r.y), fmaxf(r.z, r.w)));
+                        const float m_new = fmaxf(m_run[h], m_pair);
+                        const float step = ex2_fast(m_pair - m_new);
                         alpha[h] = ex2_fast(m_run[h] - m_new);
                         m_run[h] = m_new;
-                        const float p0 = ex2_fast(x[0][h] - m_new);
-                        const float p1 = ex2_fast(x[1][h] - m_new);
-                        l_part[h] = fmaf(l_part[h], alpha[h], p0 + p1);
-                        const uint32_t d0 = digits(__float2int_rn(p0 * pf[0][e]));
-                        const uint32_t d1 = digits(__float2int_rn(p1 * pf[1][e]));
+                        const float p0 = ex2_fast(x[0][h] - m_pair);
+                        const float p1 = ex2_fast(x[1][h] - m_pair);
+                        l_part[h] = fmaf(l_part[h], alpha[h], (p0 + p1) * step);
+                        f_cur[h] = top[e] * (1.f / kDigitMax) * step;
+                        const uint32_t d0 = digits4(__float2int_rn(p0 * pf[0][e]));
+                        const uint32_t d1 = digits4(__float2int_rn(p1 * pf[1][e]));
 #pragma unroll
-                        for (int i = 0; i < 3; ++i) {
+                        for (int i = 0; i < 4; ++i) {
                             const uint32_t at = sw_byte(i * GV + h, row);
-                            pb[at] = (unsigned char)(d0 >> (16 - 8 * i));
-                            pb[C::BT + at] = (unsigned char)(d1 >> (16 - 8 * i));
+                            pb[at] = (unsigned char)(d0 >> (24 - 8 * i));
+                            pb[C::PT + at] = (unsigned char)(d1 >> (24 - 8 * i));
                         }
                     }
                     fence_proxy_async_smem();
@@ -756,9 +774,10 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                         if (mine >= 0) fold((uint32_t)mine);
                     mine = pc;
 #pragma unroll
-                    for (int h = 0; h < GV; ++h) alpha_prev[h] = alpha[h];
-#pragma unroll
-                    for (int e = 0; e < (PAIR ? 2 : 1); ++e) f_prev[e] = f_cur[e];
+                    for (int h = 0; h < GV; ++h) {
+                        alpha_prev[h] = alpha[h];
+                        f_prev[h] = f_cur[h];
+                    }
                 }
                 mbar_arrive(&q_empty[qb_i]);  // the piece's last S is done in both groups
                 // ---- this group's partial: the merge kernel joins the groups' ----
