@@ -286,8 +286,9 @@ int pkv_q8_decode(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_heads
  * (row_offsets as in pkv_kv_append, NULL: one each).
  * pkv_paged_decode_mass takes the shapes of the tensor-core decode (pages of
  * 16 to 128 tokens; an even number of KV heads with head_dim 64).  Sequences
- * of a batch share no page.  max_seq_len bounds seq_lens (a longer sequence
- * records fault code 2 and adds nothing).  One workspace serves both
+ * of a batch share no page.  max_seq_len bounds seq_lens: a longer sequence
+ * adds nothing, its output is that of its first max_seq_len positions, and
+ * fault code 2 is recorded.  One workspace serves both
  * calls, in any order; it must start zeroed once (pkv_decode_workspace_init). */
 size_t pkv_decode_mass_workspace_bytes(size_t batch, size_t q_heads, size_t kv_heads,
                                        size_t head_dim, size_t max_seq_len);

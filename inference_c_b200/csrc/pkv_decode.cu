@@ -530,6 +530,7 @@ struct TcArgs {
     // head's final maximum and sum (pkv_mass.cuh).
     float *scores, *final_ml;
     int64_t score_tiles;
+    int32_t max_len;  // with the mass longer sequences are cut there, with a fault
 };
 
 // Tensor maps of one launch: K and V pools (one page x 64 columns per box)
@@ -792,7 +793,11 @@ paged_decode_tc_kernel(const TcArgs a, const __grid_constant__ CUtensorMap kmap,
     const int q_heads = a.kv_heads * GV;
     uint32_t *fault = &g_decode_fault;
     if (blockIdx.x == 0 && a.tile_prefix != nullptr)
-        for (int b = tid; b <= a.batch; b += kTcThreads) a.tile_prefix[b] = prefix[b];
+        for (int b = tid; b <= a.batch; b += kTcThreads) {
+            a.tile_prefix[b] = prefix[b];
+            if (a.scores != nullptr && b < a.batch && __ldg(a.seq_lens + b) > a.max_len)
+                record_fault(fault, kFaultPositionOutOfRange);
+        }
 
     // Block-table entries of a piece, 32 pages at a time, one per lane of a
     // producer warp: one load round trip serves the pages of several tiles
@@ -875,7 +880,7 @@ paged_decode_tc_kernel(const TcArgs a, const __grid_constant__ CUtensorMap kmap,
         for (int64_t t = unit_start(sc, u); ok && t < ue;) {
             const Piece P = piece_at(t, ue, prefix, a);
             t += P.k1 - P.k0;
-            const int L = __ldg(a.seq_lens + P.b);
+            const int L = length_of(a, P.b);
             // fused append: this piece ends its segment, so it loads the tile
             // holding the new row; fetch the row now, store it at that tile
             const bool app = a.new_k != nullptr && P.k1 == P.nt;
@@ -952,7 +957,7 @@ paged_decode_tc_kernel(const TcArgs a, const __grid_constant__ CUtensorMap kmap,
         for (int64_t t = unit_start(sc, u); ok && t < ue;) {
             const Piece P = piece_at(t, ue, prefix, a);
             t += P.k1 - P.k0;
-            const int L = __ldg(a.seq_lens + P.b);
+            const int L = length_of(a, P.b);
             const bool app = a.new_v != nullptr && P.k1 == P.nt;  // as the K producer
             uint4 nrow = make_uint4(0, 0, 0, 0);
             if (app && lane < 16)
@@ -1073,7 +1078,7 @@ paged_decode_tc_kernel(const TcArgs a, const __grid_constant__ CUtensorMap kmap,
             const Piece P = piece_at(t, ue, prefix, a);
             const bool first_piece = t == us;
             t += P.k1 - P.k0;
-            const int L = __ldg(a.seq_lens + P.b);
+            const int L = length_of(a, P.b);
             float m_run[GV], l_part[GV], acc[GV];
 #pragma unroll
             for (int h = 0; h < GV; ++h) {
@@ -1230,7 +1235,7 @@ paged_decode_tc_kernel(const TcArgs a, const __grid_constant__ CUtensorMap kmap,
         }
         // empty sequences: no tile, zero output (the SDK's all-masked rule)
         for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
-            if (__ldg(a.seq_lens + b) > 0) continue;
+            if (length_of(a, b) > 0) continue;
             // a fused append needs room for its row (pkv_kv_append's rule)
             if (a.new_k != nullptr && wt == 0) record_fault(fault, kFaultRowsMismatch);
             OT *ob = static_cast<OT *>(a.out) + (int64_t)b * q_heads * OD;
@@ -1677,6 +1682,7 @@ int paged_decode_impl(const char *what, const PkvPagedLayer *layer, const PkvBat
         t.scores = ms.scores;
         t.final_ml = ms.final_ml;
         t.score_tiles = ms.tiles;
+        t.max_len = mass != nullptr ? (int32_t)max_seq_len : INT32_MAX;
         // In-kernel merges need every segment to span at most
         // kInKernelMergeMax CTAs.  They also sit on the critical path of the
         // CTA that finishes last, so with few segments (each cut into many

@@ -27,6 +27,7 @@ struct MassArgs {
     const int32_t *seq_lens;
     float *mass;
     int64_t tiles;
+    int32_t max_len;  // longer sequences add nothing; the decode recorded the fault
     int32_t table_stride, kv_heads, q_heads, group, block_size, gv, per, subs, segs;
     uint32_t block_count;
 };
@@ -39,8 +40,8 @@ __global__ void __launch_bounds__(kTiles * 32) mass_kernel(const MassArgs a) {
     const int L = max(0, __ldg(a.seq_lens + b));
     const int k = blockIdx.x * kTiles + (threadIdx.x >> 5);
     const int t = k * 128 + (threadIdx.x & 31) * 4;  // this thread's first token
-    if (t >= L) return;
-    // the decode's tiles of this sequence (it may have cut a longer one)
+    if (t >= L || L > a.max_len) return;
+    // the decode's tiles of this sequence
     const int64_t first = __ldcg(a.tile_prefix + b);
     const int nt = (__ldcg(a.tile_prefix + b + 1) - (int)first) / a.segs;
     const int page = t / a.block_size;  // its 4 tokens share a page
@@ -49,7 +50,7 @@ __global__ void __launch_bounds__(kTiles * 32) mass_kernel(const MassArgs a) {
     else if ((pid = __ldg(a.tables + (int64_t)b * a.table_stride + page)) >= a.block_count)
         fault = kFaultPageOutOfRange;
     else if (nt != (L + 127) / 128 || first + (int64_t)a.segs * nt > a.tiles)
-        // longer than the caller's bound
+        // not the lengths of the decode
         fault = kFaultPositionOutOfRange;
     if (fault != kFaultNone) {
         record_fault(&g_mass_fault, fault);
@@ -137,6 +138,7 @@ bool mass_apply(const MassShape &s, const MassScratch &scratch, const int32_t *t
     a.tables = tables;
     a.seq_lens = seq_lens;
     a.mass = mass;
+    a.max_len = (int32_t)s.max_seq_len;
     a.tiles = scratch.tiles;
     a.table_stride = (int32_t)s.table_stride;
     a.kv_heads = (int32_t)s.kv_heads;

@@ -3,8 +3,8 @@
 // The 128-token tiles of all (sequence, segment) pairs form one stream.  Most
 // of it is cut evenly over the CTAs (static units); on long launches the last
 // part is cut into smaller units that CTAs claim as they finish.  Args is a
-// kernel's argument struct: batch, seq_lens and kv_heads (the segments of one
-// sequence) are read.
+// kernel's argument struct: batch, seq_lens, kv_heads (the segments of one
+// sequence) and max_len (longer sequences are cut there) are read.
 #pragma once
 
 #include <stddef.h>
@@ -97,6 +97,12 @@ __device__ __forceinline__ int unit_slot(const Sched &s, int u, int64_t seg) {
     return unit_start(s, u) < seg ? 1 : 0;
 }
 
+// Sequence b's length as the launch sees it.
+template <typename Args>
+__device__ __forceinline__ int length_of(const Args &a, int b) {
+    return min(max(0, __ldg(a.seq_lens + b)), a.max_len);
+}
+
 // Exclusive prefix of tiles per sequence times kv_heads (0 for empty ones).
 template <typename Args>
 __device__ void build_tile_prefix(const Args &a, int *prefix, int *scratch) {
@@ -107,7 +113,7 @@ __device__ void build_tile_prefix(const Args &a, int *prefix, int *scratch) {
     for (int k = 0; k < per; ++k) {
         const int b = tid * per + k;
         if (b < a.batch)
-            local += (max(0, __ldg(a.seq_lens + b)) + kTcTile - 1) / kTcTile * a.kv_heads;
+            local += (length_of(a, b) + kTcTile - 1) / kTcTile * a.kv_heads;
     }
     int incl = local;
 #pragma unroll
@@ -124,7 +130,7 @@ __device__ void build_tile_prefix(const Args &a, int *prefix, int *scratch) {
         const int b = tid * per + k;
         if (b < a.batch) {
             prefix[b] = run;
-            run += (max(0, __ldg(a.seq_lens + b)) + kTcTile - 1) / kTcTile * a.kv_heads;
+            run += (length_of(a, b) + kTcTile - 1) / kTcTile * a.kv_heads;
         }
     }
     if (tid == nthr - 1) prefix[a.batch] = before + incl;

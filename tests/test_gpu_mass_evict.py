@@ -480,3 +480,55 @@ def test_keep_far_above_the_lengths(lib, cuda, in_place):
     case, pages = _evict_case(True, [40, 0, 300], 2, 128, 16, "f16", 87, cuda, 100000)
     mass = _mass(np.random.default_rng(7), pages, 2, 16)
     _run_evict(case, pages, True, 2, 128, 16, 100000, 3, mass, in_place, cuda, 300)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("lens,bound", [
+    ([2000] + [0] * 15, 128),           # the long one's scores would fit the scratch
+    ([2000, 0], 1000), ([10, 300, 10, 40, 0, 128, 129], 128),
+    ([1010, 999, 1000, 1001], 1000),    # the same number of tiles as the bound
+    ([50, 7], 0),
+])
+def test_mass_and_output_of_lengths_past_the_bound(lib, cuda, q8, lens, bound):
+    """A sequence past the bound adds nothing and is reported, its output that
+    of its first positions; those beside it keep theirs."""
+    import torch
+    q_heads, kv_heads, hd = 4, 2, 128
+    make = Q8Case if q8 else PagedCase
+    case = make(lens, q_heads, kv_heads, hd, 16, "f16", seed=89, device=cuda)
+    pages = case.k.q.shape[0] if q8 else case.pool_pages
+    before = _mass(np.random.default_rng(8), pages, kv_heads, 16)
+    mass = torch.from_numpy(before).to(cuda)
+    out = torch.full((len(lens), q_heads, hd), float("nan"), device=cuda)
+    # the scratch of a far larger bound: what is refused is not for want of room
+    ws = P.decode_mass_workspace(len(lens), q_heads, kv_heads, hd, 4096)
+    (P.q8_decode_mass if q8 else P.paged_decode_mass)(
+        case.layer(), case.batch(), case.d_q, out, case.scale, bound, mass, ws)
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 2 and P.device_fault(0) == 0
+    rows = (lambda w, b, L: getattr(case, w).read64(case.tables[b], L)) if q8 else \
+        (lambda w, b, L: _rows16(case, w, b, L))
+    q = widen(case.qbits if q8 else case.q, "f16").astype(np.float64)
+    want = before.astype(np.float64)
+    got = out.double().cpu().numpy()
+    for b, L in enumerate(lens):
+        seen = min(L, bound)
+        if seen == 0:
+            assert not got[b].any()
+            continue
+        k, v = rows("k", b, seen), rows("v", b, seen)
+        o, w, worst = attend64(q[b:b + 1], k, v, case.scale)
+        vmax = float(np.abs(v).max())
+        tol = attend_tol(worst, hd, vmax, o, 0) + (0 if q8 else 2.0 ** -21 * vmax)
+        assert np.all(np.abs(got[b] - o[0]) <= tol[0]), b
+        if L > bound:
+            continue
+        t = np.arange(L)
+        for g in range(kv_heads):
+            want[case.tables[b][t // 16].astype(np.int64), g, t % 16] += \
+                w[0, 2 * g:2 * g + 2].sum(axis=0)
+    after = mass.cpu().numpy()
+    # weights as in _check_mass (worst score error below 2^-11, sums of two)
+    assert np.all(np.abs(after - want) <= (want - before) * 2.0 ** -10 + np.abs(want) * 2.0 ** -22)
+    same = want == before
+    assert np.array_equal(after[same].view(np.uint32), before[same].view(np.uint32))
