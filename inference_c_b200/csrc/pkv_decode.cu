@@ -676,7 +676,10 @@ __device__ __forceinline__ void merge_segment(const TcArgs &a, int h0, int nh, i
 // 2g, Q rows zero in dims 64-127) and 8..8+G-1 (KV head 2g+1, Q rows zero in
 // dims 0-63), so one K . Q^T gives every head its own scores; O^T rows 0-63
 // are the dims of KV head 2g, rows 64-127 those of 2g+1.
-template <int G, typename T, typename OT, bool PAIR>
+// MASS: with the attention mass, an instance of its own: a choice at run time
+// cost the plain decode 22 registers with 16 heads (32 sequences of 1k-4k,
+// GQA 128/8: 98 us against 95).
+template <int G, typename T, typename OT, bool PAIR, bool MASS>
 __global__ void __launch_bounds__(kTcThreads, 1)
 paged_decode_tc_kernel(const TcArgs a, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap,
@@ -795,7 +798,7 @@ paged_decode_tc_kernel(const TcArgs a, const __grid_constant__ CUtensorMap kmap,
     if (blockIdx.x == 0 && a.tile_prefix != nullptr)
         for (int b = tid; b <= a.batch; b += kTcThreads) {
             a.tile_prefix[b] = prefix[b];
-            if (a.scores != nullptr && b < a.batch && __ldg(a.seq_lens + b) > a.max_len)
+            if (MASS && b < a.batch && __ldg(a.seq_lens + b) > a.max_len)
                 record_fault(fault, kFaultPositionOutOfRange);
         }
 
@@ -1164,7 +1167,7 @@ paged_decode_tc_kernel(const TcArgs a, const __grid_constant__ CUtensorMap kmap,
                 fence_proxy_async_smem();
                 mbar_arrive(&p_full[buf]);
                 // scores for the mass, behind the fence above (it waits for stores)
-                if (a.scores != nullptr && P.seg + k < a.score_tiles) {
+                if (MASS && P.seg + k < a.score_tiles) {
                     float *sp = a.scores + (P.seg + k) * GV * 128 + row;
 #pragma unroll
                     for (int h = 0; h < GV; ++h) sp[h * 128] = x[h];
@@ -1186,9 +1189,8 @@ paged_decode_tc_kernel(const TcArgs a, const __grid_constant__ CUtensorMap kmap,
             for (int h = 0; h < GV; ++h) l[h] = lred[h] + lred[16 + h] + lred[32 + h] + lred[48 + h];
             group_sync();
             OT *out = static_cast<OT *>(a.out) + ((int64_t)P.b * q_heads + (int64_t)P.g * GV) * OD;
-            float *fml = a.final_ml == nullptr
-                             ? nullptr
-                             : a.final_ml + ((int64_t)P.b * q_heads + (int64_t)P.g * GV) * 2;
+            float *fml = !MASS ? nullptr
+                               : a.final_ml + ((int64_t)P.b * q_heads + (int64_t)P.g * GV) * 2;
             if (P.k0 == 0 && P.k1 == P.nt) {  // the whole segment ran here
 #pragma unroll
                 for (int h = 0; h < GV; ++h) {
@@ -1198,7 +1200,7 @@ paged_decode_tc_kernel(const TcArgs a, const __grid_constant__ CUtensorMap kmap,
                     } else {
                         out[h * 128 + row] = from_f32<OT>(v);
                     }
-                    if (fml != nullptr && wt == h)
+                    if (MASS && wt == h)
                         reinterpret_cast<float2 *>(fml)[h] = make_float2(m_run[h], l[h]);
                 }
                 continue;
@@ -1254,7 +1256,7 @@ paged_decode_tc_kernel(const TcArgs a, const __grid_constant__ CUtensorMap kmap,
 // sixteen per output float4 (each summing every sixteenth piece), so the
 // ~150 partial rows of a segment cut across every SM load in one round.
 constexpr int kMergeThreads = 512;
-template <typename OT>
+template <typename OT, bool MASS>
 __global__ void __launch_bounds__(kMergeThreads)
 pkv_tc_merge_kernel(const TcArgs a, int group, int grid) {
     pdl_wait();
@@ -1276,9 +1278,8 @@ pkv_tc_merge_kernel(const TcArgs a, int group, int grid) {
     OT *out = static_cast<OT *>(a.out) +
               ((int64_t)b * a.kv_heads * group + (int64_t)g * group + h) *
                   (a.pair_split != 0 ? 64 : 128);
-    float *fml = a.final_ml == nullptr
-                     ? nullptr
-                     : a.final_ml + ((int64_t)b * a.kv_heads * group + (int64_t)g * group + h) * 2;
+    float *fml = !MASS ? nullptr
+                       : a.final_ml + ((int64_t)b * a.kv_heads * group + (int64_t)g * group + h) * 2;
     merge_segment<OT>(a, h, 1, group, seg, nt, sc, threadIdx.x, kMergeThreads, kMergeThreads / 32,
                       wst, lst, slot, red, kTcMaxGrid, out, fml, [] { __syncthreads(); });
 }
@@ -1382,10 +1383,10 @@ bool encode_pool_map(CUtensorMap *map, const void *pool, uint64_t rows, uint64_t
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int G, typename T, typename OT, bool PAIR>
+template <int G, typename T, typename OT, bool PAIR, bool MASS>
 int launch_tc(const TcArgs &args, const TcMaps &mp, int ncta,
               cudaStream_t stream) {
-    auto kern = paged_decode_tc_kernel<G, T, OT, PAIR>;
+    auto kern = paged_decode_tc_kernel<G, T, OT, PAIR, MASS>;
     constexpr int GV = PAIR ? 2 * G : G;  // query heads per segment
     static int configured[64];
     int dev = 0;
@@ -1417,43 +1418,45 @@ int launch_tc(const TcArgs &args, const TcMaps &mp, int ncta,
         mc.gridDim = dim3(args.kv_heads * GV, args.batch);
         mc.blockDim = dim3(kMergeThreads);
         mc.dynamicSmemBytes = 0;
-        if (cudaLaunchKernelEx(&mc, pkv_tc_merge_kernel<OT>, args, GV, ncta) != cudaSuccess)
+        if (cudaLaunchKernelEx(&mc, pkv_tc_merge_kernel<OT, MASS>, args, GV, ncta) != cudaSuccess)
             return 0;
     }
     return cudaGetLastError() == cudaSuccess;
 }
 
-template <typename T, typename OT>
+template <typename T, typename OT, bool MASS>
 int dispatch_tc_group(const TcArgs &args, int group, bool pair, const TcMaps &mp, int ncta,
                       cudaStream_t s) {
     if (pair) {
         switch (group) {
-            case 1: return launch_tc<1, T, OT, true>(args, mp, ncta, s);
-            case 2: return launch_tc<2, T, OT, true>(args, mp, ncta, s);
-            case 4: return launch_tc<4, T, OT, true>(args, mp, ncta, s);
-            case 8: return launch_tc<8, T, OT, true>(args, mp, ncta, s);
+            case 1: return launch_tc<1, T, OT, true, MASS>(args, mp, ncta, s);
+            case 2: return launch_tc<2, T, OT, true, MASS>(args, mp, ncta, s);
+            case 4: return launch_tc<4, T, OT, true, MASS>(args, mp, ncta, s);
+            case 8: return launch_tc<8, T, OT, true, MASS>(args, mp, ncta, s);
             default: return 0;
         }
     }
     switch (group) {
-        case 1: return launch_tc<1, T, OT, false>(args, mp, ncta, s);
-        case 2: return launch_tc<2, T, OT, false>(args, mp, ncta, s);
-        case 4: return launch_tc<4, T, OT, false>(args, mp, ncta, s);
-        case 8: return launch_tc<8, T, OT, false>(args, mp, ncta, s);
-        case 16: return launch_tc<16, T, OT, false>(args, mp, ncta, s);
+        case 1: return launch_tc<1, T, OT, false, MASS>(args, mp, ncta, s);
+        case 2: return launch_tc<2, T, OT, false, MASS>(args, mp, ncta, s);
+        case 4: return launch_tc<4, T, OT, false, MASS>(args, mp, ncta, s);
+        case 8: return launch_tc<8, T, OT, false, MASS>(args, mp, ncta, s);
+        case 16: return launch_tc<16, T, OT, false, MASS>(args, mp, ncta, s);
         default: return 0;
     }
 }
 
+template <bool MASS>
 int dispatch_tc(const TcArgs &args, int group, bool pair, bool bf16, PkvDType out,
                 const TcMaps &mp, int ncta, cudaStream_t s) {
     if (!bf16)
         return out == PKV_DTYPE_F32
-                   ? dispatch_tc_group<__half, float>(args, group, pair, mp, ncta, s)
-                   : dispatch_tc_group<__half, __half>(args, group, pair, mp, ncta, s);
+                   ? dispatch_tc_group<__half, float, MASS>(args, group, pair, mp, ncta, s)
+                   : dispatch_tc_group<__half, __half, MASS>(args, group, pair, mp, ncta, s);
     return out == PKV_DTYPE_F32
-               ? dispatch_tc_group<__nv_bfloat16, float>(args, group, pair, mp, ncta, s)
-               : dispatch_tc_group<__nv_bfloat16, __nv_bfloat16>(args, group, pair, mp, ncta, s);
+               ? dispatch_tc_group<__nv_bfloat16, float, MASS>(args, group, pair, mp, ncta, s)
+               : dispatch_tc_group<__nv_bfloat16, __nv_bfloat16, MASS>(args, group, pair, mp, ncta,
+                                                                        s);
 }
 
 // The tensor-core kernel takes head_dim 128 (GQA groups up to 16), and
@@ -1722,7 +1725,9 @@ int paged_decode_impl(const char *what, const PkvPagedLayer *layer, const PkvBat
                 sl.new_k += b0 * (size_t)t.row_vecs;
                 sl.new_v += b0 * (size_t)t.row_vecs;
             }
-            ok = pkv::dispatch_tc(sl, (int)group, pair, bf16, output_dtype, mp, ncta, s);
+            ok = mass != nullptr
+                     ? pkv::dispatch_tc<true>(sl, (int)group, pair, bf16, output_dtype, mp, ncta, s)
+                     : pkv::dispatch_tc<false>(sl, (int)group, pair, bf16, output_dtype, mp, ncta, s);
             if (ok && mass != nullptr) {
                 const pkv::MassShape shape = {n,
                                               q_heads,

@@ -24,15 +24,6 @@ constexpr int kTcMaxUnits = kTcMaxGrid * (1 + kMaxRounds);  // work units of one
 constexpr size_t kTicketsAt = 256;
 constexpr size_t kZeroBytes = kTicketsAt + (kTcMaxUnits * 4 + 255) / 256 * 256;
 
-// a / b for a >= 0, b > 0.  A 64-bit division costs a GPU thread several
-// hundred cycles, and a handful of them precede every CTA's first load and its
-// last ticket; tile counts times the grid stay below 2^32 for all but absurd
-// batches, and then a 32-bit division gives the same quotient.
-__host__ __device__ inline int64_t quotient(int64_t a, int64_t b) {
-    if ((((uint64_t)a | (uint64_t)b) >> 32) == 0) return (int64_t)((uint32_t)a / (uint32_t)b);
-    return a / b;
-}
-
 // Work units of one launch; every CTA (and the merge kernel) derives the same
 // schedule from T, the grid and the smallest unit.
 struct Sched {
@@ -50,7 +41,7 @@ __host__ __device__ inline void make_sched(Sched &s, int64_t T, int grid, int mi
     int64_t dyn = 0;
     // an eighth of a CTA's share first, halving down to min_unit: the
     // dynamic tiles stay under a quarter of T, every unit >= min_unit
-    int64_t sz = quotient(T, (int64_t)s.n * 8);
+    int64_t sz = T / ((int64_t)s.n * 8);
     if (min_unit > 0 && sz >= min_unit) {
         while (s.rounds < kMaxRounds) {
             const int64_t cur = sz > min_unit ? sz : min_unit;
@@ -67,7 +58,7 @@ __host__ __device__ inline int sched_units(const Sched &s) { return s.n * (1 + s
 
 // First tile of unit u (T for u == sched_units).
 __device__ __forceinline__ int64_t unit_start(const Sched &s, int u) {
-    if (u < s.n) return quotient(s.S * u, s.n);
+    if (u < s.n) return s.S * u / s.n;
     int64_t off = s.S;
     int k = u - s.n;
     for (int r = 0; r < s.rounds; ++r) {
@@ -80,12 +71,12 @@ __device__ __forceinline__ int64_t unit_start(const Sched &s, int u) {
 
 // The unit that holds tile t.
 __device__ __forceinline__ int unit_of_tile(const Sched &s, int64_t t) {
-    if (t < s.S) return (int)quotient((t + 1) * s.n - 1, s.S);
+    if (t < s.S) return (int)(((t + 1) * s.n - 1) / s.S);
     int64_t off = t - s.S;
     int u = s.n;
     for (int r = 0; r < s.rounds; ++r) {
         const int64_t span = (int64_t)s.n * s.size[r];
-        if (off < span) return u + (int)quotient(off, s.size[r]);
+        if (off < span) return u + (int)(off / s.size[r]);
         off -= span;
         u += s.n;
     }
@@ -154,7 +145,7 @@ __device__ __forceinline__ Piece piece_at(int64_t t, int64_t end, const int *pre
     P.b = lo;
     P.nt = (prefix[lo + 1] - prefix[lo]) / a.kv_heads;
     const int64_t within = t - prefix[lo];
-    P.g = (int)quotient(within, P.nt);
+    P.g = (int)(within / P.nt);
     P.k0 = (int)(within - (int64_t)P.g * P.nt);
     P.seg = prefix[lo] + (int64_t)P.g * P.nt;
     P.k1 = (int)min((int64_t)P.nt, (int64_t)P.k0 + (end - t));
