@@ -334,7 +334,9 @@ int pkv_q8_evict(const PkvQ8Layer *layer, const PkvBatch *batch, float *mass, si
  * bounds seq_lens (a longer sequence gets no output and records fault code 2
  * or 3).  The pages'
  * 8-bit numbers are widened to 16-bit rows in the workspace first (exact) and
- * the scales applied to scores and weights.  The byte count is
+ * the scales applied to scores and weights.  A weight times its V scale is kept
+ * as two 16-bit halves: F16 rows 2^-22 of it, down to 2^-36 of the row's largest,
+ * BF16 rows 2^-16.  The byte count is
  * for the whole batch; a smaller workspace that holds at least one sequence
  * (the count for batch 1) also works and runs the batch in parts. */
 size_t pkv_q8_prefill_workspace_bytes(size_t batch, size_t kv_heads, size_t head_dim,

@@ -36,6 +36,7 @@
 #include <math.h>
 #include <stdio.h>
 
+#include <type_traits>
 #include <utility>
 
 #include "pkv_device.cuh"
@@ -352,7 +353,11 @@ __device__ __forceinline__ void add_mask_chunk(uint32_t (&v)[32], const uint16_t
 // is vs 2^(c s - m) = 2^(c s + e - m): the scales sit in the multiplier and the
 // addend of the exponent and cost nothing per score.  m is the running maximum
 // of c s + e, and the softmax sum is the blocks' sums times 1 / vs, so scores,
-// weights and sums are those of the exact values kq ks and vq vs.
+// weights and sums are those of the exact values kq ks and vq vs.  fp16 weights
+// are raised by 2^11 and the running maximum follows within 2^4, so that they
+// fill fp16's range up to 2^15: beside a dominant token with V near zero the
+// others together carry a row's output, and relative to 1 those below 2^-25
+// (17 nats) would be lost.
 // HD = head_dim (64 or 128).
 template <typename T, typename OT, bool GEN, bool Q8, int HD>
 __global__ void __launch_bounds__(kPfThreads, 1)
@@ -646,11 +651,14 @@ paged_prefill_tc_kernel(const PfArgs a, const __grid_constant__ CUtensorMap qmap
                         mc[c] = max3(mc[c], __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
                     mc[c] = fmaxf(mc[c], __uint_as_float(v[c][31]));
                 }
+                constexpr bool RAISED = Q8 && std::is_same<T, __half>::value;
+                constexpr float kRaise = RAISED ? 11.f : 0.f;
+                constexpr float kThreshold = RAISED ? 4.f : kRescaleThreshold;
                 float mx = max3(mc[0], mc[1], fmaxf(mc[2], mc[3]));
                 if constexpr (!GEN && !Q8) mx *= a.scale_log2;  // scale > 0 commutes with max
                 float alpha = 1.f;
                 bool rescale = false;
-                if (mx > m_run + kRescaleThreshold) {  // first tile: m_run = -inf
+                if (mx > m_run + kThreshold) {  // first tile: m_run = -inf
                     alpha = ex2_approx(m_run - mx);
                     m_run = mx;
                     rescale = jt > 0;
@@ -695,7 +703,7 @@ paged_prefill_tc_kernel(const PfArgs a, const __grid_constant__ CUtensorMap qmap
                 // P is 0); one whose max is +inf is dead (P = 0, output 0)
                 // a row that has seen only masked keys so far keeps m = -inf:
                 // use 0 (its P is 0) rather than produce NaN from -inf + inf
-                float nm = m_run == -INFINITY ? 0.f : -m_run;
+                float nm = m_run == -INFINITY ? 0.f : kRaise - m_run;
                 if constexpr (GEN) {
                     dead = dead || m_run == INFINITY;
                     if (dead) {

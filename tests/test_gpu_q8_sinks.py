@@ -143,3 +143,32 @@ def test_decode_of_scores_that_overflow(lib, cuda):
     assert P.device_fault(0) == 0
     # 256 equal weights of one value: 64 roundings of the sum, the digits' half step
     assert np.all(np.abs(got.double().cpu().numpy() - 0.5) <= 0.5 * (64 + 1) * 2.0 ** -24 + 2.0 ** -22)
+
+
+@pytest.mark.parametrize("q_heads,kv_heads,hd,bs,dtype", [
+    (4, 1, 128, 16, "f16"), (3, 1, 128, 32, "bf16"), (4, 2, 64, 16, "f16"), (2, 2, 64, 64, "bf16"),
+])
+@pytest.mark.parametrize("L,at", [(300, 0), (700, 300), (20000, 0), (20000, 19000)])
+@pytest.mark.parametrize("gap", [14, 17])
+def test_prefill_beside_a_dominant_token(lib, cuda, q_heads, kv_heads, hd, bs, dtype, L, at, gap):
+    """A weight is kept as two 16-bit halves: fp16 2^-22 of it and down to 2^-36
+    of the row's largest weight times V scale (half of fp16's least step,
+    weights up to 2^15 above the running maximum), bf16 2^-16.  The first
+    multiplies a whole number up to 127 and is divided by a sum of 1 / max(vs)
+    at least, so L keys are off by L 2^-36 vmax.  The sum over the keys in 32
+    bits takes an addition a half and 16 keys, each off by 2^-23 at most."""
+    import torch
+    n = 5
+    case, q, scale = _case(L, at, gap, q_heads, kv_heads, hd, bs, dtype, cuda, rows=n)
+    got = torch.full((n, q_heads, hd), float("nan"), device=cuda)
+    P.q8_prefill(case.layer(), case.batch(), case.d_q, torch.tensor([0, n], dtype=torch.int32,
+                                                                    device=cuda), got, scale, n, L,
+                 P.q8_prefill_workspace(case.layer(), 1, L))
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 0
+    want, mag, worst, vmax = _want(case, q, scale, L - n + 1 + np.arange(n))
+    halves = 2.0 ** -16 if dtype == "bf16" else 2.0 ** -22
+    tol = (_relative(worst + 16) + halves + L / 8 * 2.0 ** -23) * mag
+    tol += (L * 2.0 ** -36 if dtype == "f16" else 0) * vmax
+    diff = np.abs(got.double().cpu().numpy() - want)
+    assert np.all(diff <= tol), (float((diff / want).max()), float((tol / want).min()))
