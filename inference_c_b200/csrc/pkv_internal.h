@@ -78,8 +78,9 @@ void pkv_internal_comm_set_probe(PkvComm *comm, int (*probe)(void *arg, PkvStrea
 
 /* 8-bit pages widened to whole numbers in 16-bit rows (exact), for the prefill:
  * per sequence, KV head and 16 keys the K scale, log2 of the V scale and its
- * inverse ([batch][kv_heads][stride]; scales of 0 stand as 1, their rows are
- * zeros).  Device pointers, 16-byte aligned rows, stride a multiple of 8. */
+ * inverse ([batch][kv_heads][stride]; scales of 0 stand as 1 in K and 2^-31 in V,
+ * their rows are zeros; V scales are within 2^-31 .. 2^32 for BF16).  Device
+ * pointers, 16-byte aligned rows, stride a multiple of 8. */
 typedef struct {
     const float *k, *v_log2, *v_inverse;
     size_t stride;

@@ -17,8 +17,11 @@
 // 128-row query tile and head pair, so widening them inside the attention
 // kernel would repeat each conversion that many times, while the expansion is
 // one pass of 3 bytes a value.  The rows it writes are the whole numbers q, exact
-// in either 16-bit type; the scales go beside them and enter the exponent.
+// in either 16-bit type (bf16 V rows of very small or large scales: times a power
+// of two); the scales go beside them and enter the exponent.
 #include <math.h>
+
+#include <type_traits>
 
 #include "pkv_q8.cuh"
 #include "pkv_trace.h"
@@ -197,13 +200,24 @@ q8_rows_kernel(const Q8RowArgs a) {
         if constexpr (!WRITE) {
             float s = on ? __ldg(sp) : 1.f;
             if (a.pad_rows > 0) {
+                // A block of zeros, or none.  Its weights meet zeros of V and only
+                // enter the softmax sum, in FP32, but they also enter the maximum
+                // that the others are relative to: 2^-31 is below every scale of
+                // fp16 rows, whose weights would else run out of fp16's exponents
+                // (V near 1e-3 beside one block of zeros).
+                float t = s != 0.f ? s : kv == 0 ? 1.f : 4.65661287e-10f;
+                s = 1.f;
+                if (kv == 1 && std::is_same<T, __nv_bfloat16>::value) {
+                    // bf16 rows have scales from 2^-126 to 2^121, and a weight times a
+                    // scale 2^-100 of another's would leave FP32 and with it the
+                    // softmax sum: beyond 2^-31 .. 2^31 a power of two goes into the
+                    // rows, whose whole numbers bf16 holds exactly with it.
+                    const int e = (int)(__float_as_uint(t) >> 23 & 255u) - 127;
+                    const int j = e < -31 ? e + 31 : e > 31 ? e - 31 : 0;
+                    s = __uint_as_float((uint32_t)(127 + j) << 23);
+                    t *= __uint_as_float((uint32_t)(127 - j) << 23);
+                }
                 if (unit_live && head < a.kv_heads && (lane == 0 || (HD == 64 && lane == 8))) {
-                    // A block of zeros, or none.  Its weights meet zeros of V and only
-                    // enter the softmax sum, in FP32, but they also enter the maximum
-                    // that the others are relative to: 2^-31 is below every scale of
-                    // fp16 rows, whose weights would else run out of fp16's exponents
-                    // (V near 1e-3 beside one block of zeros).
-                    const float t = s != 0.f ? s : kv == 0 ? 1.f : 4.65661287e-10f;
                     const int64_t at = ((int64_t)b * a.kv_heads + head) * (a.pad_rows / 16) +
                                        (page * a.block_size) / 16 + part;
                     if (kv == 0) a.wide_k[at] = t;
@@ -212,7 +226,6 @@ q8_rows_kernel(const Q8RowArgs a) {
                         a.wide_inverse[at] = __fdiv_rn(1.f, t);
                     }
                 }
-                s = 1.f;
             }
             if (!on) continue;
             uint2 q[8];
