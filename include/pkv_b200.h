@@ -258,8 +258,7 @@ int pkv_q8_gather(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t 
  * whole group), query in layer->dtype (16-byte aligned), output F32 or
  * layer->dtype.  K and V are used exactly (q * s); the query is kept to 2^-22
  * of its head's largest element, a softmax weight times its V scale to 2^-31 of
- * the largest weight times the largest V scale (taken as 2^-94 at least) of its
- * 256 tokens.  max_seq_len
+ * the largest weight times the largest V scale of its 256 tokens.  max_seq_len
  * bounds seq_lens: a longer sequence is cut there and fault code 2 recorded.
  * block_count * lanes * block_size must be below 2^31.  The workspace starts
  * zeroed once (pkv_decode_workspace_init), and again after a fault code 4.  It

@@ -81,9 +81,6 @@ constexpr int kRing = 4;             // unit ids in flight between the roles
 constexpr int kScaleSlots = 16;      // tiles whose scales are in shared memory
 constexpr uint32_t kTileBytes = 16384;
 constexpr float kDigitMax = 2130706432.f;  // 127 * 2^24: four signed digits hold +-this
-// 2^-94, the least V scale that weights are cut against: kDigitMax over it and
-// it over kDigitMax are normal FP32 numbers.
-constexpr float kLeastTop = 5.04870979e-29f;
 constexpr float kLowest = -3.40282347e38f;  // FP32's lowest finite number
 
 template <int GV>
@@ -673,8 +670,11 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                     tc_fence_before();
 #pragma unroll
                     for (int h = 0; h < GV; ++h)
-                        acc[h] = fmaf(fmaf((float)two(o[h], o[GV + h]), 65536.f,
-                                           (float)two(o[2 * GV + h], o[3 * GV + h])),
+                        // (1 / kDigitMax here and not in f_prev, which would leave
+                        // FP32 with V scales below 2^-95)
+                        acc[h] = fmaf(fmaf((float)two(o[h], o[GV + h]), 65536.f / kDigitMax,
+                                           (float)two(o[2 * GV + h], o[3 * GV + h]) *
+                                               (1.f / kDigitMax)),
                                       f_prev[h], acc[h] * alpha_prev[h]);
                 };
                 int64_t mine = -1;  // this group's previous pair of the piece
@@ -700,18 +700,18 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                         const float4 v2 = *reinterpret_cast<const float4 *>(sl1 + e * 16 + 8);
                         const float4 v3 = *reinterpret_cast<const float4 *>(sl1 + e * 16 + 12);
                         top[e] = fmaxf(
-                            kLeastTop,
+                            kQ8MinScale,
                             fmaxf(fmaxf(fmaxf(fmaxf(v0.x, v0.y), fmaxf(v0.z, v0.w)),
                                         fmaxf(fmaxf(v1.x, v1.y), fmaxf(v1.z, v1.w))),
                                   fmaxf(fmaxf(fmaxf(v2.x, v2.y), fmaxf(v2.z, v2.w)),
                                         fmaxf(fmaxf(v3.x, v3.y), fmaxf(v3.z, v3.w)))));
-                        // weight digits: p * vs / top * kDigitMax
-                        const float f = __fdividef(kDigitMax, top[e]);
+                        // weight digits: p * (vs / top) * kDigitMax
+                        const float inv = __fdividef(1.f, top[e]);
                         const int at = e * 16 + (row >> page_shift);
                         ks[0][e] = sl0[at];
                         ks[1][e] = sl1[at];
-                        pf[0][e] = sl0[at + 8] * f;
-                        pf[1][e] = sl1[at + 8] * f;
+                        pf[0][e] = sl0[at + 8] * inv * kDigitMax;
+                        pf[1][e] = sl1[at + 8] * inv * kDigitMax;
                     }
                     tmem_wait_ld();
                     tc_fence_before();
@@ -748,7 +748,7 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                         const float p0 = ex2_fast(x[0][h] - m_pair);
                         const float p1 = ex2_fast(x[1][h] - m_pair);
                         l_part[h] = fmaf(l_part[h], alpha[h], (p0 + p1) * step);
-                        f_cur[h] = top[e] * (1.f / kDigitMax) * step;
+                        f_cur[h] = top[e] * step;
                         const uint32_t d0 = digits4(__float2int_rn(p0 * pf[0][e]));
                         const uint32_t d1 = digits4(__float2int_rn(p1 * pf[1][e]));
 #pragma unroll

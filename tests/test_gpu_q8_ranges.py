@@ -17,7 +17,7 @@ pytestmark = pytest.mark.gpu
 @pytest.mark.parametrize("amps", [
     (1.0, 1e-36), (1e-36, 1.0), (1e-30, 1e-34), (1e-36, 1e-36), (1e30, 1.0), (1e30, 1e-30),
 ])
-@pytest.mark.parametrize("prefill", [True])
+@pytest.mark.parametrize("prefill", [True, False])
 def test_scales_far_apart(lib, cuda, hd, kv, amps, prefill):
     """The errors stay in proportion to the largest value (bounds of the prefill
     and decode tests, vmax the case's own)."""
