@@ -474,8 +474,14 @@ int pkv_pool_create(TensorPagedKVCache *cache, int device, PkvDType dtype,
 /* The same pool of 8-bit pages: int8 K and V pages with their scales, zeroed,
  * and with `mass` non-zero the attention mass of every layer; dtype is that of
  * rows and queries (F16 or BF16), and the cache's block size 16, 32, 64 or 128.
- * Steps, tables and lengths work as with 16-bit pages; pkv_pool_layer refuses
- * such a pool, pkv_pool_q8_layer any other. */
+ * Steps, tables and lengths work as with 16-bit pages; a step that is rolled
+ * back leaves the rows below its sequences' lengths as they were, bytes and
+ * scales (an append may have rounded the last page's earlier rows to a larger
+ * scale: they are kept aside while a step is open, in max_batch pages a layer).
+ * It does not take back mass that its decodes added, nor an eviction in place:
+ * evict in a step of its own and commit it.  A sequence that is shortened later
+ * keeps its pages' scales.  pkv_pool_layer refuses such a pool,
+ * pkv_pool_q8_layer any other. */
 int pkv_pool_create_q8(TensorPagedKVCache *cache, int device, PkvDType dtype, size_t layer_count,
                        size_t kv_heads, size_t head_dim, size_t max_batch,
                        size_t max_pages_per_seq, int mass, PkvPool **pool, char *error,
@@ -503,7 +509,8 @@ int pkv_step_batch(PkvPool *pool, PkvBatch *out);
 /* Device row offsets of the open step's new tokens ([batch+1], int32). */
 const int32_t *pkv_step_row_offsets(PkvPool *pool);
 /* Closes the step: commit sets every length to past + new; otherwise the
- * reservations are rolled back.  Always releases the decode locks. */
+ * reservations are rolled back (8-bit pools: and the open pages restored, on the
+ * step's stream).  Always releases the decode locks. */
 int pkv_step_end(PkvPool *pool, int commit, char *error,
                  size_t error_capacity);
 

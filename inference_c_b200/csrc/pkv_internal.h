@@ -86,6 +86,31 @@ typedef struct {
     size_t stride;
 } PkvRowScales;
 
+/* One layer of an 8-bit pool; scales: [block_count][kv_heads] of K, then of V. */
+typedef struct {
+    void *key_pool, *value_pool;
+    float *scales;
+} PkvQ8Pages;
+
+/* The open page of each sequence of a step (the page its first new row goes to,
+ * where it holds earlier rows) as it is before the step: those rows' bytes and
+ * the page's scales. */
+typedef struct {
+    const PkvQ8Pages *layers; /* device, [layer_count] */
+    unsigned char *saved;     /* device, [layer_count][max_batch][slot_bytes] */
+    size_t slot_bytes, layer_count, max_batch;
+    size_t kv_heads, lanes, block_size, block_count;
+    const uint32_t *tables;   /* the step's, from its first sequence on */
+    size_t table_stride;
+    const int32_t *lens, *offsets;
+} PkvQ8Undo;
+
+size_t pkv_internal_q8_undo_slot(size_t kv_heads, size_t lanes, size_t block_size);
+/* Saves the open pages of sequences [first, first + count) of a step, or with
+ * `restore` puts them back. */
+int pkv_internal_q8_undo(const PkvQ8Undo *undo, size_t first, size_t count, int restore,
+                         PkvStream stream);
+
 /* pkv_paged_prefill with the general options the dense SDPA needs: an
  * additive FP16 mask [query row of the chunk][key] with a row stride in
  * elements (NULL: none), dense mode (a chunk may be longer than its

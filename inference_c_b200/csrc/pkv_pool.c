@@ -46,6 +46,9 @@ struct PkvPool {
     int q8, has_mass;       /* 8-bit pages; with the attention mass */
     float **scales;         /* 8-bit pages, per layer: K scales, V scales, mass */
     size_t mass_offset;     /* floats before the mass */
+    PkvQ8Undo undo;         /* open pages of the open step, to roll it back */
+    PkvStream step_stream;
+    int step_saved;         /* some sequence of the open step has an open page */
     size_t layer_count, kv_heads, head_dim, block_size, block_count;
     size_t max_batch, max_pages;
     void **kpools;
@@ -85,6 +88,8 @@ static void pool_free_device(PkvPool *p) {
         for (size_t l = 0; l < p->layer_count; ++l) cudaFree(p->vpools[l]);
     if (p->scales)
         for (size_t l = 0; l < p->layer_count; ++l) cudaFree(p->scales[l]);
+    cudaFree((void *)p->undo.layers);
+    cudaFree(p->undo.saved);
     cudaFree(p->d_tables);
     for (int s = 0; s < kStageSlots; ++s) {
         cudaFreeHost(p->h_stage[s]);
@@ -194,6 +199,32 @@ static int pool_create(TensorPagedKVCache *cache, int device, PkvDType dtype,
         if (st == cudaSuccess) st = cudaMemset(p->vpools[l], 0, pool_bytes);
         if (q8 && st == cudaSuccess) st = cudaMalloc((void **)&p->scales[l], extra_bytes);
         if (q8 && st == cudaSuccess) st = cudaMemset(p->scales[l], 0, extra_bytes);
+    }
+    if (q8 && st == cudaSuccess) {
+        PkvQ8Undo *u = &p->undo;
+        u->layer_count = layer_count;
+        u->max_batch = max_batch;
+        u->kv_heads = kv_heads;
+        u->lanes = row_bytes / 128;
+        u->block_size = p->block_size;
+        u->block_count = p->block_count;
+        u->slot_bytes = pkv_internal_q8_undo_slot(kv_heads, u->lanes, p->block_size);
+        PkvQ8Pages *pages = (PkvQ8Pages *)malloc(layer_count * sizeof(PkvQ8Pages));
+        void *layers = NULL;
+        if (pages == NULL) st = cudaErrorMemoryAllocation;
+        for (size_t l = 0; pages != NULL && l < layer_count; ++l) {
+            pages[l].key_pool = p->kpools[l];
+            pages[l].value_pool = p->vpools[l];
+            pages[l].scales = p->scales[l];
+        }
+        if (st == cudaSuccess) st = cudaMalloc(&layers, layer_count * sizeof(PkvQ8Pages));
+        u->layers = (const PkvQ8Pages *)layers;
+        if (st == cudaSuccess)
+            st = cudaMemcpy(layers, pages, layer_count * sizeof(PkvQ8Pages),
+                            cudaMemcpyHostToDevice);
+        if (st == cudaSuccess)
+            st = cudaMalloc((void **)&u->saved, layer_count * max_batch * u->slot_bytes);
+        free(pages);
     }
     const size_t table_bytes = max_batch * max_pages_per_seq * sizeof(uint32_t);
     if (st == cudaSuccess) st = cudaMalloc((void **)&p->d_tables, table_bytes);
@@ -432,6 +463,17 @@ static int step_begin_impl(PkvPool *pool, const TensorPagedKVSequence *sequences
         st = cudaErrorLaunchFailure;
     else
         p->stage_ticket[slot] = ticket;
+    p->step_saved = 0;
+    for (size_t b = 0; p->q8 && b < batch; ++b)
+        if (new_tokens[b] > 0 && (p->step_target[b] - new_tokens[b]) % p->block_size != 0)
+            p->step_saved = 1;
+    if (st == cudaSuccess && p->step_saved) {
+        p->undo.tables = p->d_tables;
+        p->undo.table_stride = p->max_pages;
+        p->undo.lens = (const int32_t *)p->d_stage[slot];
+        p->undo.offsets = p->undo.lens + p->max_batch;
+        if (!pkv_internal_q8_undo(&p->undo, 0, batch, 0, stream)) st = cudaErrorLaunchFailure;
+    }
     if (have_prev) cudaSetDevice(prev);
     if (st != cudaSuccess) {
         for (size_t b = 0; b < batch; ++b) p->rows[b].seq = 0;
@@ -441,6 +483,7 @@ static int step_begin_impl(PkvPool *pool, const TensorPagedKVSequence *sequences
     }
     p->open = 1;
     p->step_batch = batch;
+    p->step_stream = stream;
     return 1;
 }
 
@@ -468,27 +511,50 @@ const int32_t *pkv_step_row_offsets(PkvPool *pool) {
     return (const int32_t *)pool->d_stage[pool->slot] + pool->max_batch;
 }
 
+/* The open pages of sequences [first, first + count) of the open step as they
+ * were when it began (8-bit pools). */
+static int restore_pages(PkvPool *p, size_t first, size_t count) {
+    if (!p->step_saved) return 1;
+    int prev = 0;
+    const int have_prev = cudaGetDevice(&prev) == cudaSuccess;
+    cudaSetDevice(p->device);
+    const int ok = pkv_internal_q8_undo(&p->undo, first, count, 1, p->step_stream);
+    if (have_prev) cudaSetDevice(prev);
+    return ok;
+}
+
 static int step_end_impl(PkvPool *pool, int commit, char *error, size_t cap) {
     PkvPool *p = pool;
     if (p == NULL || !p->open) {
         pkv_internal_set_error(error, cap, "pkv_step_end: no open step");
         return 0;
     }
-    int ok = 1;
+    int ok = 1, restored = 1;
+    /* before their locks go: the pages of a sequence given back may get new rows
+     * on the stream at once */
+    if (!commit) restored = restore_pages(p, 0, p->step_batch);
     for (size_t b = 0; b < p->step_batch; ++b) {
         const TensorPagedKVSequence s = p->step_seq[b];
         if (commit && tensor_paged_kv_sequence_set_length(p->cache, s, p->step_target[b]))
             ;
         else {
-            if (commit) ok = 0;
+            if (commit) {
+                ok = 0;
+                restored = restore_pages(p, b, 1) && restored;
+            }
             (void)tensor_paged_kv_sequence_set_length(p->cache, s, p->step_current[b]);
         }
         tensor_paged_kv_sequence_end_decode(p->cache, s);
     }
     p->open = 0;
     p->slot = (p->slot + 1) % kStageSlots;
-    if (!ok) pkv_internal_set_error(error, cap, "pkv_step_end: commit failed; rolled back");
-    return commit ? ok : 1;
+    if (!restored)
+        pkv_internal_set_error(error, cap, "pkv_step_end: rolled back, but the open pages could "
+                                           "not be restored: %s",
+                               cudaGetErrorString(cudaPeekAtLastError()));
+    else if (!ok)
+        pkv_internal_set_error(error, cap, "pkv_step_end: commit failed; rolled back");
+    return restored && (commit ? ok : 1);
 }
 
 int pkv_step_end(PkvPool *pool, int commit, char *error, size_t cap) {

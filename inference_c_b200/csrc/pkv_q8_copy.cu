@@ -423,6 +423,44 @@ int q8_rows(const PkvQ8Layer *layer, const PkvBatch *batch, const int32_t *offse
     return 1;
 }
 
+// A rolled-back step must leave the committed rows as they were, and an append
+// that raises the open page's scale rounds that page's earlier rows again: so
+// they are kept aside while a step is open, one page a sequence and layer (CTA:
+// one of those), 2 bytes a value and row of K and V read and written in all.
+template <bool RESTORE>
+__global__ void __launch_bounds__(256) q8_undo_kernel(const PkvQ8Undo a, int b0) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int b = b0 + blockIdx.x, tid = threadIdx.x;
+    const int bs = (int)a.block_size, kvh = (int)a.kv_heads;
+    const int n = __ldg(a.offsets + b + 1) - __ldg(a.offsets + b);
+    const int first = __ldg(a.lens + b) - n;
+    const int rows = first % bs;  // held
+    if (n <= 0 || first <= 0 || rows == 0) return;
+    const uint32_t pid = __ldg(a.tables + (int64_t)b * a.table_stride + first / bs);
+    if (pid >= a.block_count) return;
+    const PkvQ8Pages layer = a.layers[blockIdx.y];
+    const int64_t half = (int64_t)a.lanes * bs * 8;  // uint4 of a page
+    uint4 *saved = reinterpret_cast<uint4 *>(
+        a.saved + ((int64_t)blockIdx.y * a.max_batch + b) * a.slot_bytes);
+    const int per = rows * 8;  // uint4 of a lane's held rows
+    for (int kv = 0; kv < 2; ++kv) {
+        uint4 *page = static_cast<uint4 *>(kv == 0 ? layer.key_pool : layer.value_pool) +
+                      (int64_t)pid * half;
+        for (int i = tid; i < (int)a.lanes * per; i += 256) {
+            const int at = i / per * bs * 8 + i % per;
+            if (RESTORE) page[at] = saved[kv * half + at];
+            else saved[kv * half + at] = page[at];
+        }
+        float *s = layer.scales + ((int64_t)kv * (int64_t)a.block_count + pid) * kvh;
+        float *kept = reinterpret_cast<float *>(saved + 2 * half) + kv * kvh;
+        for (int h = tid; h < kvh; h += 256) {
+            if (RESTORE) s[h] = kept[h];
+            else kept[h] = s[h];
+        }
+    }
+}
+
 // Scratch of the prefill: 16-bit rows of every sequence, padded to whole pages
 // of 128, and their identity table.
 struct PrefillSpace {
@@ -564,6 +602,27 @@ int pkv_q8_prefill(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_head
             return 0;
     }
     return 1;
+}
+
+size_t pkv_internal_q8_undo_slot(size_t kv_heads, size_t lanes, size_t block_size) {
+    return 2 * lanes * block_size * 128 + (2 * kv_heads * sizeof(float) + 15) / 16 * 16;
+}
+
+int pkv_internal_q8_undo(const PkvQ8Undo *undo, size_t first, size_t count, int restore,
+                         PkvStream stream) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)count, (unsigned)undo->layer_count);
+    cfg.blockDim = dim3(256);
+    cfg.stream = (cudaStream_t)stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t st =
+        restore ? cudaLaunchKernelEx(&cfg, pkv::q8_undo_kernel<true>, *undo, (int)first)
+                : cudaLaunchKernelEx(&cfg, pkv::q8_undo_kernel<false>, *undo, (int)first);
+    return st == cudaSuccess && cudaGetLastError() == cudaSuccess;
 }
 
 int pkv_internal_take_q8_copy_fault(uint32_t *code) {
