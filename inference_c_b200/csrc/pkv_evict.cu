@@ -437,6 +437,24 @@ cudaError_t launch_move(const EvictArgs &a, size_t batch, bool in_place, cudaStr
 }
 
 constexpr int32_t kCachedMax = 49152;  // keys of a select CTA: 198 KiB with the gaps
+constexpr size_t cached_bytes(int32_t keys) { return ((size_t)keys + keys / 32 + 1) * 4; }
+
+// The most shared memory any call takes, once a device: a limit set to each
+// call's own size could be lowered by another thread before its launch.
+cudaError_t allow_cached_keys() {
+    static int configured[64];
+    int dev = 0;
+    cudaError_t st = cudaGetDevice(&dev);
+    if (st != cudaSuccess || (dev >= 0 && dev < 64 && configured[dev])) return st;
+    const int bytes = (int)cached_bytes(kCachedMax);
+    st = cudaFuncSetAttribute(evict_select_kernel<1, 0>,
+                              cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (st == cudaSuccess)
+        st = cudaFuncSetAttribute(evict_select_kernel<8, 0>,
+                                  cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (st == cudaSuccess && dev >= 0 && dev < 64) configured[dev] = 1;
+    return st;
+}
 
 int evict(EvictArgs &a, const PkvBatch *batch, size_t head_dim, bool q8, float *mass, size_t keep,
           size_t recent, const uint32_t *dst_tables, size_t dst_stride, int32_t *kept,
@@ -500,7 +518,7 @@ int evict(EvictArgs &a, const PkvBatch *batch, size_t head_dim, bool q8, float *
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(cs * (unsigned)a.kv_heads, (unsigned)batch->batch);
     cfg.blockDim = dim3(kSelThreads);
-    cfg.dynamicSmemBytes = a.cached > 0 ? ((size_t)a.cached + a.cached / 32 + 1) * 4 : 0;
+    cfg.dynamicSmemBytes = a.cached > 0 ? cached_bytes(a.cached) : 0;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
@@ -511,9 +529,7 @@ int evict(EvictArgs &a, const PkvBatch *batch, size_t head_dim, bool q8, float *
                            : held == 16 ? evict_select_kernel<8, 16>
                                         : evict_select_kernel<8, 0>);
     cudaError_t st = cudaSuccess;
-    if (cfg.dynamicSmemBytes > 0)
-        st = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  (int)cfg.dynamicSmemBytes);
+    if (a.cached > 0) st = allow_cached_keys();
     if (st == cudaSuccess) st = cudaLaunchKernelEx(&cfg, kern, a);
     if (st == cudaSuccess) {
         if (q8)

@@ -532,3 +532,52 @@ def test_mass_and_output_of_lengths_past_the_bound(lib, cuda, q8, lens, bound):
     assert np.all(np.abs(after - want) <= (want - before) * 2.0 ** -10 + np.abs(want) * 2.0 ** -22)
     same = want == before
     assert np.array_equal(after[same].view(np.uint32), before[same].view(np.uint32))
+
+
+def test_evict_from_two_threads(lib, cuda):
+    """Calls of different bounds, whose select kernels take different amounts of
+    shared memory, from two threads on streams of their own."""
+    import ctypes
+    import threading
+
+    import torch
+    kv, n = 4, 40  # more lists than SMs: one CTA a list
+    cases = [_evict_case(False, np.full(n, 40), kv, 64, 16, "f16", 90 + i, cuda, 20)
+             for i in range(2)]
+    want, errors = [], []
+    for case, pages in cases:
+        kept = torch.empty(n, kv, 20, dtype=torch.int32, device=cuda)
+        mass = torch.rand(pages, kv, 16, device=cuda)
+        dst = torch.tensor([p for p in range(pages) if p not in set(case.tables[:, :3].ravel())]
+                           [:2 * n], dtype=torch.int32, device=cuda).view(n, 2)
+        want.append((kept, mass, dst))
+    torch.cuda.synchronize()
+
+    def run(i, bound):
+        (case, _), (kept, mass, dst) = cases[i], want[i]
+        stream, err = torch.cuda.Stream(), ctypes.create_string_buffer(256)
+        layer, batch = case.layer(), case.batch()
+        # the arguments once, so that the threads spend their time in the calls
+        args = (ctypes.byref(layer), ctypes.byref(batch), mass.data_ptr(), 20, 4, dst.data_ptr(),
+                2, kept.data_ptr(), bound, stream.cuda_stream, err, 256)
+        for k in range(3000):
+            if not lib.pkv_kv_evict(*args):
+                errors.append(err.value.decode())
+            if k % 200 == 0:
+                stream.synchronize()
+        stream.synchronize()
+    threads = [threading.Thread(target=run, args=a)
+               for a in ((0, 17000), (1, 49000), (0, 20000), (1, 48000))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    assert P.device_fault(0) == 0
+    for (case, _), (kept, mass, _) in zip(cases, want):
+        m, got = mass.cpu().numpy(), kept.cpu().numpy()
+        t = np.arange(40)
+        for b in range(0, n, 13):
+            for g in range(kv):
+                w = m[case.tables[b][t // 16].astype(np.int64), g, t % 16]
+                assert np.array_equal(got[b, g], keep_list(w, 40, 20, 4))
