@@ -307,7 +307,8 @@ int pkv_q8_decode_mass(const PkvQ8Layer *layer, const PkvBatch *batch, size_t q_
 /* Eviction by accumulated attention weight.  For each sequence b (length L =
  * seq_lens[b]) and KV head g by itself, min(L, keep) positions stay: all when
  * L <= keep, else the newest `recent` and, of the others, those with the
- * largest mass, ties to the lower position (NaN counts as lowest).  Their
+ * largest mass, ties to the lower position (NaN counts as lowest, and so does a
+ * position whose page id is out of range, which records fault code 1).  Their
  * ascending list goes to kept[b][g][0 ..] ([batch][kv_heads][keep], -1 behind
  * it), and row i of the result -- K and V columns of the head, and its mass --
  * is row kept[i] of the sequence.  Since every head keeps as many, the result

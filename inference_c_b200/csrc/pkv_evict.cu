@@ -136,22 +136,24 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
     uint32_t reg[RUN > 0 ? RUN : 1];
     if constexpr (RUN > 0) {  // all loads in flight; four tokens share a page
         float4 m[RUN / 4];
+        bool good[RUN / 4];
 #pragma unroll
         for (int i = 0; i < RUN / 4; ++i) {
             uint32_t pid = 0;
             m[i] = make_float4(0.f, 0.f, 0.f, 0.f);
             const int32_t t = r0 + 4 * i;
-            if (t < r1 && page_at(a, trow, a.table_stride, t, pid))
+            good[i] = t < r1 && page_at(a, trow, a.table_stride, t, pid);
+            if (good[i])
                 m[i] = __ldg(reinterpret_cast<const float4 *>(
                     a.mass + ((int64_t)pid * a.kv_heads + g) * a.block_size +
                     (t & (a.block_size - 1))));
         }
 #pragma unroll
         for (int i = 0; i < RUN / 4; ++i) {
-            reg[4 * i] = mass_key(m[i].x);
-            reg[4 * i + 1] = mass_key(m[i].y);
-            reg[4 * i + 2] = mass_key(m[i].z);
-            reg[4 * i + 3] = mass_key(m[i].w);
+            reg[4 * i] = good[i] ? mass_key(m[i].x) : 0u;
+            reg[4 * i + 1] = good[i] ? mass_key(m[i].y) : 0u;
+            reg[4 * i + 2] = good[i] ? mass_key(m[i].z) : 0u;
+            reg[4 * i + 3] = good[i] ? mass_key(m[i].w) : 0u;
         }
     }
     if (RUN == 0 && held) {

@@ -581,3 +581,31 @@ def test_evict_from_two_threads(lib, cuda):
             for g in range(kv):
                 w = m[case.tables[b][t // 16].astype(np.int64), g, t % 16]
                 assert np.array_equal(got[b, g], keep_list(w, 40, 20, 4))
+
+
+@pytest.mark.parametrize("max_len", [3000, 5000, 100000, 200000, 1 << 20])
+def test_positions_of_bad_source_pages_rank_last(lib, cuda, max_len):
+    """However a list is shared (as in the test of ties), positions that cannot
+    be read come after all others, masses of zero and below included."""
+    import torch
+    L, keep = 3000, 777
+    case, pages = _evict_case(False, np.array([L]), 2, 64, 16, "f16", 73, cuda, keep)
+    rng = np.random.default_rng(9)
+    mass = rng.choice(np.array([0.0, -2.0, 0.5], np.float32), (pages, 2, 16), p=[.6, .2, .2])
+    tables = case.d_tables.clone()
+    bad = np.arange(0, L // 16 - 4, 3)  # none among the newest positions
+    tables[0, torch.from_numpy(bad).to(cuda)] = 1 << 30
+    used = set(case.tables[0][:-(-L // 16)].tolist())
+    dst = torch.tensor([[p for p in range(pages) if p not in used][:-(-keep // 16)]],
+                       dtype=torch.int32, device=cuda)
+    kept = torch.empty(1, 2, keep, dtype=torch.int32, device=cuda)
+    P.kv_evict(case.layer(), P.make_batch(tables, case.d_lens), torch.from_numpy(mass).to(cuda),
+               keep, 20, kept, max_len, dst_tables=dst)
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 1 and P.device_fault(0) == 0
+    t = np.arange(L)
+    got = kept.cpu().numpy()[0]
+    for g in range(2):
+        w = mass[case.tables[0][t // 16].astype(np.int64), g, t % 16].copy()
+        w[np.isin(t // 16, bad)] = np.nan
+        assert np.array_equal(got[g], keep_list(w, L, keep, 20))
