@@ -546,9 +546,11 @@ def _check_mass(mass, layer) -> int:
     """Address of a mass tensor of this layer (an address passes through)."""
     if isinstance(mass, int):
         return mass
+    import torch
     if mass.shape != (layer.block_count, layer.kv_heads, layer.block_size) or \
-            not mass.is_contiguous() or mass.element_size() != 4:
-        raise ValueError("mass is a contiguous float32 [block_count, kv_heads, block_size] tensor")
+            not mass.is_contiguous() or mass.dtype != torch.float32 or not mass.is_cuda:
+        raise ValueError("mass is a contiguous float32 [block_count, kv_heads, block_size] CUDA "
+                         "tensor")
     return mass.data_ptr()
 
 
@@ -586,13 +588,16 @@ def kv_evict(layer, batch: PkvBatch, mass, keep: int, recent: int, kept, max_seq
     positions of every sequence and KV head stay, listed in kept (int32
     [batch, kv_heads, keep]); dst_tables [batch, stride]: pages of the result
     (None: in place)."""
+    import torch
     if kept.shape != (batch.batch, layer.kv_heads, keep) or not kept.is_contiguous() or \
-            kept.element_size() != 4:
-        raise ValueError("kept is a contiguous int32 [batch, kv_heads, keep] tensor")
-    if dst_tables is not None and (dst_tables.shape[0] != batch.batch or
+            kept.dtype != torch.int32 or not kept.is_cuda:
+        raise ValueError("kept is a contiguous int32 [batch, kv_heads, keep] CUDA tensor")
+    if dst_tables is not None and (dst_tables.dim() != 2 or
+                                   dst_tables.shape[0] != batch.batch or
                                    not dst_tables.is_contiguous() or
-                                   dst_tables.element_size() != 4):
-        raise ValueError("dst_tables is a contiguous int32 [batch, stride] tensor")
+                                   dst_tables.dtype not in (torch.int32, torch.uint32) or
+                                   not dst_tables.is_cuda):
+        raise ValueError("dst_tables is a contiguous int32 [batch, stride] CUDA tensor")
     name = "pkv_q8_evict" if isinstance(layer, PkvQ8Layer) else "pkv_kv_evict"
     _call(name, ctypes.byref(layer), ctypes.byref(batch), _check_mass(mass, layer), keep, recent,
           _ptr(dst_tables), 0 if dst_tables is None else dst_tables.shape[1], kept.data_ptr(),

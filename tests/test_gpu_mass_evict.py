@@ -609,3 +609,23 @@ def test_positions_of_bad_source_pages_rank_last(lib, cuda, max_len):
         w = mass[case.tables[0][t // 16].astype(np.int64), g, t % 16].copy()
         w[np.isin(t // 16, bad)] = np.nan
         assert np.array_equal(got[g], keep_list(w, L, keep, 20))
+
+
+def test_tensors_of_other_four_byte_types_are_refused(lib, cuda):
+    import torch
+    case = Q8Case([40], 4, 2, 128, 16, "f16", seed=3, device=cuda)
+    pages = case.k.q.shape[0]
+    mass = torch.zeros(pages, 2, 16, device=cuda)
+    kept = torch.zeros(1, 2, 8, dtype=torch.int32, device=cuda)
+    dst = torch.zeros(1, 1, dtype=torch.int32, device=cuda)
+    with pytest.raises(ValueError, match="mass"):
+        P.kv_evict(case.layer(), case.batch(), mass.int(), 8, 2, kept, 40)
+    with pytest.raises(ValueError, match="kept"):
+        P.kv_evict(case.layer(), case.batch(), mass, 8, 2, kept.float(), 40)
+    for bad in (dst.float(), dst.cpu(), dst.view(-1)):
+        with pytest.raises(ValueError, match="dst_tables"):
+            P.kv_evict(case.layer(), case.batch(), mass, 8, 2, kept, 40, dst_tables=bad)
+    for d in (dst + pages - 1, (dst + pages - 1).view(torch.uint32)):
+        P.kv_evict(case.layer(), case.batch(), mass, 8, 2, kept, 40, dst_tables=d)
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 0

@@ -166,3 +166,22 @@ def test_q8_pool_shapes_are_checked(lib):
         with pytest.raises(P.PkvError, match="8|pages"):
             P.PagedPool.q8(cache, 0, dtype, 1, kv, hd, 1, 4)
         cache.free()
+
+
+def test_python_calls_check_their_tensors(lib):
+    """Types, shapes and devices of mass, kept and dst_tables: a ValueError
+    before the library is called (which would refuse these addresses too)."""
+    import torch
+    L, B = _layer(key_pool=None), _batch()
+    mass = torch.zeros(4, 2, 16)
+    for bad in (mass, mass.to(torch.int32), mass.half(), mass[:, :1],
+                mass.transpose(0, 1).contiguous().transpose(0, 1)):
+        with pytest.raises(ValueError, match="mass is a contiguous float32"):
+            P.mass_clear(L, B, bad)
+        with pytest.raises(ValueError, match="mass is a contiguous float32"):
+            P.q8_decode_mass(L, B, torch.zeros(2, 4, 128).half(), torch.zeros(2, 4, 128), 1.0, 64,
+                             bad, mass)
+    kept = torch.zeros(2, 2, 8, dtype=torch.int32)
+    for bad in (kept, kept.float(), kept.long(), kept[:, :, :7]):
+        with pytest.raises(ValueError, match="kept is a contiguous int32"):
+            P.kv_evict(L, B, 256, 8, 2, bad, 64)
