@@ -114,7 +114,8 @@ struct Q8Args {
     void *out;
     const float *kscales, *vscales;
     uint32_t *claim;         // [2]
-    // Partials: [slot][2 groups][GV] of (m, l) and of 128 columns; slots 2 u and
+    // Partials: [slot][pairs 0, 2, .. and 1, 3, .. of the piece][GV] of (m, l) and
+    // of 128 columns; slots 2 u and
     // 2 u + 1 are unit u's first and last piece, whole_slot + i segment i whole.
     float *part_ml, *part_o;
     int32_t whole_slot;
@@ -678,6 +679,10 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                                       f_prev[h], acc[h] * alpha_prev[h]);
                 };
                 int64_t mine = -1;  // this group's previous pair of the piece
+                // The group with the piece's first pair fills its first partial:
+                // which of the two that is depends on the units this CTA claimed
+                // before, and with it the order of the merge's sums would.
+                const int part = grp ^ (int)(pc & 1);
                 for (int k = 0; k < n; k += 2, ++pc) {
                     const int n2 = min(2, n - k);
                     const uint32_t j0 = j;
@@ -788,7 +793,7 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                     const float ls = warp_sum(l_part[h]);
                     if (lane == 0) my_l[q4 * 16 + h] = ls;
                 }
-                const int64_t at = ((int64_t)slot * 2 + grp) * GV;
+                const int64_t at = ((int64_t)slot * 2 + part) * GV;
                 if (mine >= 0) {
                     fold((uint32_t)mine);
 #pragma unroll

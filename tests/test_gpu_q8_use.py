@@ -320,3 +320,49 @@ def test_rows_outside_their_buffer_are_reported(lib, cuda):
         assert P.device_fault(0) == 3
     keep = case.d_kq.clone()
     assert not torch.equal(before, torch.zeros_like(before)) and keep.shape == before.shape
+
+
+def test_refused_rows_leave_their_sequence_and_not_the_other(lib, cuda):
+    """Of a call whose offsets leave the rows' buffer for one sequence, that
+    sequence's pages stay bit for bit and the other's rows are written."""
+    import torch
+    for offs, good in (([0, 2, 9], 0), ([-1, 1, 3], 1)):
+        case = Q8Case([40, 40], 2, 2, 128, 16, "f16", seed=100, device=cuda)
+        bits = [W.normal_bits(101, (3, 256), "f16", stream=s) for s in (1, 2)]
+        P.q8_append(case.layer(), case.batch(), *(to_device_bits(b, "f16", cuda) for b in bits),
+                    torch.tensor(offs, dtype=torch.int32, device=cuda))
+        torch.cuda.synchronize()
+        assert P.device_fault(0) == 3 and P.device_fault(0) == 0
+        a, z = offs[good], offs[good + 1]
+        for pool, b in zip((case.k, case.v), bits):
+            x = widen(b, "f16").reshape(3, 2, 128)
+            pool.write(case.tables[good], 40 - (z - a), x[a:z])
+        case.same_pages()  # every page, the refused sequence's among them
+
+
+@pytest.mark.parametrize("qh,kv,hd", [(32, 8, 128), (16, 16, 64)])
+def test_the_same_call_gives_the_same_bits(lib, cuda, qh, kv, hd):
+    """Work units are claimed by whichever CTA is free: no sum depends on it."""
+    import torch
+    lens = [3000 + 311 * i for i in range(24)]  # more than 64 tiles a CTA
+    bs, per = 16, [-(-n // 16) for n in lens]
+    g = torch.Generator(device="cuda").manual_seed(13)
+    pages, lanes = sum(per), lanes_of(kv, hd)
+    pools = [torch.randint(-127, 128, (pages, lanes, bs, 128), generator=g, device=cuda,
+                           dtype=torch.int8) for _ in range(2)]
+    scales = [torch.rand(pages, kv, generator=g, device=cuda) * 0.02 + 0.005 for _ in range(2)]
+    layer = P.make_q8_layer(*pools, *scales, kv, hd, torch.bfloat16)
+    tables = torch.zeros(24, max(per), dtype=torch.int32, device=cuda)
+    perm = torch.randperm(pages, generator=g, device=cuda).int()
+    for b, n in enumerate(per):
+        tables[b, :n] = perm[sum(per[:b]):sum(per[:b]) + n]
+    d_lens = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    batch = P.make_batch(tables, d_lens)
+    q = torch.randn(24, qh, hd, generator=g, device=cuda).bfloat16()
+    ws = P.q8_decode_workspace(24, qh, kv, hd, max(lens))
+    outs = [torch.empty(24, qh, hd, device=cuda) for _ in range(12)]
+    for o in outs:
+        P.q8_decode(layer, batch, q, o, hd ** -0.5, max(lens), ws)
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 0
+    assert all(torch.equal(o, outs[0]) for o in outs)
