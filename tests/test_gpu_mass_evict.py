@@ -629,3 +629,94 @@ def test_tensors_of_other_four_byte_types_are_refused(lib, cuda):
         P.kv_evict(case.layer(), case.batch(), mass, 8, 2, kept, 40, dst_tables=d)
     torch.cuda.synchronize()
     assert P.device_fault(0) == 0
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("lens,q_heads,kv_heads,hd,bs", [
+    # segments cut over CTAs, merged in the 16-bit decode kernel itself
+    ([300 + 97 * i for i in range(24)], 32, 8, 128, 16),
+    ([1 + 143 * i for i in range(20)], 128, 8, 128, 32),
+    ([40 + 211 * i for i in range(16)], 24, 12, 64, 16),
+    # above 64 tiles a CTA: units of the dynamic tail as well
+    ([3000 + 311 * i for i in range(24)], 32, 8, 128, 64),
+    ([2900 + 401 * i for i in range(20)], 24, 24, 64, 128),
+    # more sequences than a launch holds: the scratch serves the next launch
+    ([(7 * i) % 300 for i in range(1100)], 4, 2, 128, 16),
+    # few segments: the merge kernel
+    ([9000, 0, 17], 8, 2, 128, 16),
+])
+def test_mass_of_every_way_to_merge(lib, cuda, q8, lens, q_heads, kv_heads, hd, bs):
+    """Weights and outputs against 64 bits on the GPU."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(11)
+    per = [-(-n // bs) for n in lens]
+    pages = sum(per) + 2
+    tables = torch.zeros(len(lens), max(per), dtype=torch.int32, device=cuda)
+    perm = torch.randperm(pages, generator=g, device=cuda).int()
+    at = 0
+    for b, n in enumerate(per):
+        tables[b, :n] = perm[at:at + n]
+        at += n
+    half = torch.float16
+    if q8:
+        lanes = P.q8_lanes(kv_heads, hd)
+        pools = [torch.randint(-127, 128, (pages, lanes, bs, 128), generator=g, device=cuda,
+                               dtype=torch.int8) for _ in range(2)]
+        scales = [torch.rand(pages, kv_heads, generator=g, device=cuda) * 0.02 + 0.005
+                  for _ in range(2)]
+        layer = P.make_q8_layer(*pools, *scales, kv_heads, hd, half)
+
+        def rows(i, idx):  # [pages, bs, kv_heads, hd]
+            x = pools[i][idx].transpose(1, 2).reshape(len(idx), bs, -1)[..., :kv_heads * hd]
+            return x.reshape(len(idx), bs, kv_heads, hd).double() * scales[i][idx].double()[:, None, :, None]
+    else:
+        pools = [torch.randn(pages * bs, kv_heads * hd, generator=g, device=cuda, dtype=half)
+                 for _ in range(2)]
+        layer = P.make_layer(*pools, bs, kv_heads, hd)
+
+        def rows(i, idx):
+            return pools[i].view(pages, bs, kv_heads, hd)[idx].double()
+    q = torch.randn(len(lens), q_heads, hd, generator=g, device=cuda, dtype=half)
+    before = torch.rand(pages, kv_heads, bs, generator=g, device=cuda) * 0.05
+    mass, out = before.clone(), torch.full((len(lens), q_heads, hd), float("nan"), device=cuda)
+    d_lens = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    batch = P.make_batch(tables, d_lens)
+    ws = P.decode_mass_workspace(len(lens), q_heads, kv_heads, hd, max(lens))
+    call = P.q8_decode_mass if q8 else P.paged_decode_mass
+    call(layer, batch, q, out, hd ** -0.5, max(lens), mass, ws)
+    plain = torch.empty_like(out)
+    if q8:
+        P.q8_decode(layer, batch, q, plain, hd ** -0.5, max(lens), ws)
+    else:
+        P.paged_decode(layer, batch, q, plain, hd ** -0.5, max(lens), ws)
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 0
+    assert torch.equal(plain, out)
+    want, slack = before.double(), torch.zeros_like(before).double()
+    group = q_heads // kv_heads
+    for b, n in enumerate(lens):
+        if n == 0:
+            assert not out[b].any()
+            continue
+        idx = tables[b, :per[b]].long()
+        k, v = (rows(i, idx).reshape(-1, kv_heads, hd)[:n] for i in range(2))
+        qd = q[b].double().view(kv_heads, group, hd)
+        s = torch.einsum("ghd,tgd->ght", qd, k) * hd ** -0.5
+        worst = float(torch.einsum("ghd,tgd->ght", qd.abs(), k.abs()).max()) * hd ** -0.5
+        w = torch.softmax(s, -1)
+        o = torch.einsum("ght,tgd->ghd", w, v).reshape(q_heads, hd)
+        vmax = float(v.abs().max())
+        # the 16-bit kernel keeps a weight as two fp16 halves
+        tol = attend_tol(worst, hd, vmax, o.cpu().numpy(), 0) + (0 if q8 else 2.0 ** -21 * vmax)
+        assert np.all(np.abs((out[b].double() - o).cpu().numpy()) <= tol), b
+        # as in _check_mass
+        delta = (hd + 4) * 2.0 ** -24 * worst * 1.5 + 2.0 ** -21
+        pad = torch.zeros(kv_heads, per[b] * bs, dtype=torch.float64, device=cuda)
+        pad[:, :n] = w.sum(dim=1)
+        add = pad.view(kv_heads, per[b], bs).transpose(0, 1)
+        want[idx] += add
+        slack[idx] += add * (2 * delta + (group + 4) * 2.0 ** -24)
+    slack += want.abs() * 2.0 ** -23 + 2.0 ** -100
+    assert bool(((mass.double() - want).abs() <= slack).all())
+    untouched = want == before.double()
+    assert torch.equal(mass[untouched], before[untouched])
