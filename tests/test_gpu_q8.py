@@ -339,3 +339,31 @@ def test_prefill_longer_than_bound_is_reported(lib, cuda):
         want, _, _ = attend64(q[1:2], case.k.read64(case.tables[1], 20),
                               case.v.read64(case.tables[1], 20), case.scale)
         assert np.abs(out[1].double().cpu().numpy() - want[0]).max() < 1e-4
+
+
+def test_prefill_of_more_sequences_than_a_launch(lib, cuda):
+    """1,100 sequences, some of no rows: each reads its own pages' scales."""
+    import torch
+    r = np.random.RandomState(5)
+    lengths = r.randint(0, 70, 1100)
+    rows = np.minimum(lengths, r.randint(0, 4, 1100))
+    case = Q8Case(lengths, 2, 1, 64, 16, "bf16", seed=61, device=cuda)
+    offs = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+    n = int(offs[-1])
+    qbits = W.normal_bits(63, (n, 2, 64), "bf16", stream=9)
+    got = torch.full((n, 2, 64), float("nan"), device=cuda)
+    ws = P.q8_prefill_workspace(case.layer(), 1100, 70)
+    P.q8_prefill(case.layer(), case.batch(), to_device_bits(qbits, "bf16", cuda),
+                 torch.from_numpy(offs).to(cuda), got, case.scale, 3, 70, ws)
+    torch.cuda.synchronize()
+    assert P.device_fault(0) == 0
+    q, got = widen(qbits, "bf16").astype(np.float64), got.double().cpu().numpy()
+    for b in range(1100):
+        L, m = int(lengths[b]), int(rows[b])
+        if m == 0:
+            continue
+        k, v = case.k.read64(case.tables[b], L), case.v.read64(case.tables[b], L)
+        want, _, worst = attend64(q[offs[b]:offs[b + 1]], k, v, case.scale, L - m + 1 + np.arange(m))
+        vmax = float(np.abs(v).max())
+        tol = attend_tol(worst, 64, vmax, want, 0) + 2.0 ** -16 * vmax  # as test_prefill
+        assert np.all(np.abs(got[offs[b]:offs[b + 1]] - want) <= tol), b
