@@ -174,6 +174,11 @@ __device__ __forceinline__ uint32_t sw_byte(uint32_t row, uint32_t col) {
     return (row >> 3) * 1024u + (row & 7u) * 128u + (((col >> 4) ^ (row & 7u)) << 4) + (col & 15u);
 }
 
+// The lowest byte of v to shared memory.
+__device__ __forceinline__ void store_byte(uint32_t at, uint32_t v) {
+    asm volatile("st.shared.b8 [%0], %1;\n" ::"r"(at), "r"(v) : "memory");
+}
+
 __device__ __forceinline__ void store_out(const Q8Args &a, int64_t at, float v) {
     if (a.out_f32) static_cast<float *>(a.out)[at] = v;
     else if (a.bf16) static_cast<__nv_bfloat16 *>(a.out)[at] = __float2bfloat16_rn(v);
@@ -627,13 +632,12 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                 const int n = desc[qb_i].x;
                 if (aborted || n == 0) break;
                 const int len = desc[qb_i].y, slot = desc[qb_i].z, tile0 = desc[qb_i].w;
-                float m_run[GV], l_part[GV], acc[GV], alpha_prev[GV], f_prev[GV], qs[GV];
+                float m_run[GV], l_part[GV], acc[GV], alpha_prev[GV], f_prev[GV];
 #pragma unroll
                 for (int h = 0; h < GV; ++h) {
                     m_run[h] = -INFINITY;
                     l_part[h] = 0.f;
                     acc[h] = 0.f;
-                    qs[h] = qscale[qb_i * 16 + h];
                 }
                 // COLS columns of TMEM at `col`, this thread's row
                 auto load_cols = [&](uint32_t col, auto &v) {
@@ -664,19 +668,32 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                 auto fold = [&](uint32_t pair) {
                     const uint32_t buf = pair % NB;
                     await(&o_full[buf], (pair / NB) & 1);
-                    float o[NP];
                     tc_fence_after();
-                    load_cols(C::O_COL + buf * NP, o);
-                    tmem_wait_ld();
-                    tc_fence_before();
+                    // (1 / kDigitMax here and not in f_prev, which would leave FP32
+                    // with V scales below 2^-95)
+                    auto add = [&](const float (&o)[2 * GV], float unit) {
 #pragma unroll
-                    for (int h = 0; h < GV; ++h)
-                        // (1 / kDigitMax here and not in f_prev, which would leave
-                        // FP32 with V scales below 2^-95)
-                        acc[h] = fmaf(fmaf((float)two(o[h], o[GV + h]), 65536.f / kDigitMax,
-                                           (float)two(o[2 * GV + h], o[3 * GV + h]) *
-                                               (1.f / kDigitMax)),
-                                      f_prev[h], acc[h] * alpha_prev[h]);
+                        for (int h = 0; h < GV; ++h)
+                            acc[h] = fmaf((float)two(o[h], o[GV + h]) * unit, f_prev[h], acc[h]);
+                    };
+#pragma unroll
+                    for (int h = 0; h < GV; ++h) acc[h] *= alpha_prev[h];
+                    if constexpr (GV == 16) {  // two digits at a time: registers
+                        float o[2 * GV];
+                        load_cols(C::O_COL + buf * NP, o);
+                        tmem_wait_ld();
+                        add(o, 65536.f / kDigitMax);
+                        load_cols(C::O_COL + buf * NP + 2 * GV, o);
+                        tmem_wait_ld();
+                        add(o, 1.f / kDigitMax);
+                    } else {
+                        float o[2][2 * GV];
+                        load_cols(C::O_COL + buf * NP, reinterpret_cast<float (&)[NP]>(o));
+                        tmem_wait_ld();
+                        add(o[0], 65536.f / kDigitMax);
+                        add(o[1], 1.f / kDigitMax);
+                    }
+                    tc_fence_before();
                 };
                 int64_t mine = -1;  // this group's previous pair of the piece
                 // The group with the piece's first pair fills its first partial:
@@ -690,10 +707,13 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                     if ((int)(pc & 1) != grp) continue;
                     const uint32_t buf = pc % NB;
                     await(&s_full[buf], (pc / NB) & 1);
-                    float s[2][NQ];
+                    // Both tiles' sums at once, or with 16 heads one tile at a time
+                    // (registers); past an odd end: not used
+                    constexpr int AT_ONCE = GV == 16 ? 1 : 2;
+                    float s[AT_ONCE][NQ];
                     tc_fence_after();
-                    load_cols(2 * buf * NQ, s[0]);
-                    load_cols((2 * buf + 1) * NQ, s[1]);  // past an odd end: not used
+#pragma unroll
+                    for (int i = 0; i < AT_ONCE; ++i) load_cols((2 * buf + i) * NQ, s[i]);
                     // scales: a token's own, and the largest V scale of the pair
                     float ks[2][PAIR ? 2 : 1], pf[2][PAIR ? 2 : 1], top[PAIR ? 2 : 1];
                     const float *sl0 = scales + (j0 % kScaleSlots) * 32;
@@ -718,19 +738,27 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                         pf[0][e] = sl0[at + 8] * inv * kDigitMax;
                         pf[1][e] = sl1[at + 8] * inv * kDigitMax;
                     }
-                    tmem_wait_ld();
-                    tc_fence_before();
                     const int left = len - k * kTcTile;
-                    const bool live0 = row < left, live1 = row + kTcTile < left && n2 > 1;
+                    const bool live[2] = {row < left, row + kTcTile < left && n2 > 1};
                     // two buffers: a warp writes a pair's maxima only after all
                     // read those of the group's pair before the last
                     float *myred = red + grp * 128 + ((pc >> 1) & 1) * 64;  // [slot][warp]
                     float x[2][GV];
 #pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        if (AT_ONCE == 1 && i == 1) load_cols((2 * buf + 1) * NQ, s[0]);
+                        if (AT_ONCE == 1 || i == 0) tmem_wait_ld();
+#pragma unroll
+                        for (int h = 0; h < GV; ++h) {
+                            const int e = PAIR && h >= GV / 2 ? 1 : 0;
+                            x[i][h] = live[i] ? number(s[i % AT_ONCE], h) *
+                                                    (qscale[qb_i * 16 + h] * ks[i][e])
+                                              : -INFINITY;
+                        }
+                    }
+                    tc_fence_before();
+#pragma unroll
                     for (int h = 0; h < GV; ++h) {
-                        const int e = PAIR && h >= GV / 2 ? 1 : 0;
-                        x[0][h] = live0 ? number(s[0], h) * (qs[h] * ks[0][e]) : -INFINITY;
-                        x[1][h] = live1 ? number(s[1], h) * (qs[h] * ks[1][e]) : -INFINITY;
                         const float wm = redux_max(fmaxf(x[0][h], x[1][h]));
                         if (lane == 0) myred[h * 4 + q4] = wm;
                     }
@@ -738,7 +766,11 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                         if (mine >= 0) fold((uint32_t)mine);
                     group_sync();
                     float alpha[GV], f_cur[GV];
-                    unsigned char *pb = sm + C::P_OFF + 2 * buf * C::PT;
+                    // this token's column of the swizzled B tiles: row r's byte is at
+                    // ((r & 7) << 4 ^ column) + 128 r, one operation a store (with 16
+                    // heads the generic form took 448 us of what is now 416, 64
+                    // sequences of 512-32k)
+                    const uint32_t pcol = smem_u32(sm + C::P_OFF + 2 * buf * C::PT) + (uint32_t)row;
 #pragma unroll
                     for (int h = 0; h < GV; ++h) {
                         const int e = PAIR && h >= GV / 2 ? 1 : 0;
@@ -746,10 +778,12 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                         // the pair's maximum (finite, should every score be -inf)
                         const float m_pair =
                             fmaxf(kLowest, fmaxf(fmaxf(r.x, r.y), fmaxf(r.z, r.w)));
-                        const float m_new = fmaxf(m_run[h], m_pair);
-                        const float step = ex2_fast(m_pair - m_new);
-                        alpha[h] = ex2_fast(m_run[h] - m_new);
-                        m_run[h] = m_new;
+                        // steps to the new running maximum: one of them is 1
+                        const float up = m_run[h] - m_pair;
+                        const float less = ex2_fast(-fabsf(up));
+                        const float step = up >= 0.f ? less : 1.f;
+                        alpha[h] = up >= 0.f ? 1.f : less;
+                        m_run[h] = fmaxf(m_run[h], m_pair);
                         const float p0 = ex2_fast(x[0][h] - m_pair);
                         const float p1 = ex2_fast(x[1][h] - m_pair);
                         l_part[h] = fmaf(l_part[h], alpha[h], (p0 + p1) * step);
@@ -758,9 +792,10 @@ q8_decode_tc_kernel(const Q8Args a, const __grid_constant__ CUtensorMap kmap,
                         const uint32_t d1 = digits4(__float2int_rn(p1 * pf[1][e]));
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const uint32_t at = sw_byte(i * GV + h, row);
-                            pb[at] = (unsigned char)(d0 >> (24 - 8 * i));
-                            pb[C::PT + at] = (unsigned char)(d1 >> (24 - 8 * i));
+                            const uint32_t r = (uint32_t)(i * GV + h);
+                            const uint32_t at = (pcol ^ (r & 7u) << 4) + r * 128u;
+                            store_byte(at, d0 >> (24 - 8 * i));
+                            store_byte(at + C::PT, d1 >> (24 - 8 * i));
                         }
                     }
                     fence_proxy_async_smem();
@@ -998,9 +1033,9 @@ int launch(const Q8Args &a, const CUtensorMap &k, const CUtensorMap &v, int ncta
     cfg.numAttrs = 1;
     if (cudaLaunchKernelEx(&cfg, kern, a, k, v) != cudaSuccess) return 0;
     // One head a CTA where that makes two CTAs an SM or fewer (one sequence of
-    // 131072, 64 heads: 57 us against 67), else the start of more CTAs costs
-    // more than their parallelism gives (32 sequences, 256 segments: 45 us
-    // against 41 with all heads in one).
+    // 131072, 64 heads: 56 us against 67), else the start of more CTAs costs
+    // more than their parallelism gives (32 sequences, 256 segments: 42 us
+    // against 38 with all heads in one).
     const bool all_heads = (int64_t)a.kv_heads * GV * a.batch > 2 * ncta;
     cfg.gridDim = dim3(all_heads ? a.kv_heads : a.kv_heads * GV, a.batch);
     cfg.blockDim = dim3(kMergeThreads);
