@@ -374,7 +374,8 @@ paged_prefill_tc_kernel(const PfArgs a, const __grid_constant__ CUtensorMap qmap
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *bars = reinterpret_cast<uint64_t *>(sm + kBarOff);
     uint64_t *kfull = bars, *kempty = bars + 2, *vfull = bars + 4, *vempty = bars + 6;
-    uint64_t *s_full = bars + 8, *p_full = bars + 10, *pv_done = bars + 12;  // [head A, head B]
+    // one of each for each S/P buffer
+    uint64_t *s_full = bars + 8, *p_full = bars + 10, *pv_done = bars + 12;
     uint64_t *q_full = bars + 14, *q_empty = bars + 15;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sm + kMiscOff);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(sm + kMiscOff + 4);
@@ -415,6 +416,17 @@ paged_prefill_tc_kernel(const PfArgs a, const __grid_constant__ CUtensorMap qmap
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const int64_t total_items = prefix[a.batch];
+    // S/P buffer of head w's tile t, and the parity of its barriers for it.  A
+    // parity tells a phase from the one before it only: a barrier must not complete
+    // two phases before its waiter looks, nor may a waiter look two phases ahead.
+    // Unpaired, the S of a tile is issued while the one before it may be unread (at
+    // the end of an item the softmax still stores it when the next two are done), P
+    // of a tile may be written before the V of the one before it lands, and after
+    // the last P the PV before the last may still run; each buffer's own barriers
+    // move on only when the buffer was used, and S of a tile is done only after the
+    // PV that used its buffer.
+    auto sp_buf = [&](int w, uint32_t t) -> uint32_t { return paired ? (uint32_t)w : (t & 1u); };
+    auto sp_par = [&](uint32_t t) -> uint32_t { return (paired ? t : t >> 1) & 1u; };
     const bool serp = a.dense_layout != 0;
     uint32_t *fault = &g_prefill_fault;
 
@@ -506,9 +518,7 @@ paged_prefill_tc_kernel(const PfArgs a, const __grid_constant__ CUtensorMap qmap
             bool ok = true;
             // Paired: head w owns S/P buffer w and O buffer w.  Unpaired: the
             // one head alternates S/P buffers by tile and accumulates in O 0.
-            auto sbuf = [&](int w, uint32_t t) -> uint32_t {
-                return tmem + (paired ? (uint32_t)w : (t & 1u)) * 256u;
-            };
+            auto sbuf = [&](int w, uint32_t t) -> uint32_t { return tmem + sp_buf(w, t) * 256u; };
             // S of head w for global tile t.  Its S/P buffer was last read by
             // a PV MMA this thread issued earlier; tcgen05.mma operations of
             // one thread execute in issue order, so the new S overwrites the
@@ -524,7 +534,7 @@ paged_prefill_tc_kernel(const PfArgs a, const __grid_constant__ CUtensorMap qmap
                 const uint64_t kd = kdesc + (uint64_t)((t % kStages) * (32768u >> 4));
                 s_mmas(sbuf(w, t), qd, kd, kIdescS,
                        std::make_integer_sequence<uint32_t, HD / 16>{});
-                mma_commit(&s_full[w]);
+                mma_commit(&s_full[sp_buf(w, t)]);
                 return true;
             };
             // PV of head w for global tile t (jt: its index within the item),
@@ -532,14 +542,14 @@ paged_prefill_tc_kernel(const PfArgs a, const __grid_constant__ CUtensorMap qmap
             auto issue_pv = [&](int w, uint32_t t, int jt, bool last_reader) -> bool {
                 const int st = (int)(t % kStages);
                 if (!mbar_wait(&vfull[st], (t / kStages) & 1, abort_flag, fault) ||
-                    !mbar_wait(&p_full[w], t & 1, abort_flag, fault))
+                    !mbar_wait(&p_full[sp_buf(w, t)], sp_par(t), abort_flag, fault))
                     return false;
                 tc_fence_after();
                 const uint64_t vd = vdesc + (uint64_t)((uint32_t)st * (32768u >> 4));
                 const uint32_t ocol = tmem + (paired ? (uint32_t)w * 256u : 0u) + 128u;
                 pv_mmas(ocol, sbuf(w, t), vd, kIdescPV, jt > 0 ? 1u : 0u,
                         std::make_integer_sequence<uint32_t, 8>{});
-                mma_commit(&pv_done[w]);
+                mma_commit(&pv_done[sp_buf(w, t)]);
                 if (last_reader) mma_commit(&vempty[st]);
                 return true;
             };
@@ -599,8 +609,9 @@ paged_prefill_tc_kernel(const PfArgs a, const __grid_constant__ CUtensorMap qmap
             for (int jt = 0; jt < I.ntiles; ++jt, ++jj) {
                 const int k0 = jt * kPfTile;
                 const bool masked = k0 + kPfTile > limit;
-                const uint32_t scol = tmem + (paired ? (uint32_t)w : (jj & 1u)) * 256u + lane_off;
-                if (!wait(&s_full[w], jj & 1)) { ok = false; break; }
+                const uint32_t buf = sp_buf(w, jj);
+                const uint32_t scol = tmem + buf * 256u + lane_off;
+                if (!wait(&s_full[buf], sp_par(jj))) { ok = false; break; }
                 tc_fence_after();
                 // the row's 128 scores in registers with one TMEM round trip
                 uint32_t v[4][32];
@@ -682,7 +693,7 @@ paged_prefill_tc_kernel(const PfArgs a, const __grid_constant__ CUtensorMap qmap
                 }
                 // rescaling O needs this head's previous PV to be done
                 if (__any_sync(0xffffffffu, rescale)) {
-                    if (!wait(&pv_done[w], (jj - 1) & 1)) { ok = false; break; }
+                    if (!wait(&pv_done[sp_buf(w, jj - 1)], sp_par(jj - 1))) { ok = false; break; }
                     tc_fence_after();
 #pragma unroll
                     for (int c = 0; c < HD / 32; ++c) {
@@ -761,10 +772,10 @@ paged_prefill_tc_kernel(const PfArgs a, const __grid_constant__ CUtensorMap qmap
                 l += lsum2.x + lsum2.y;
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(&p_full[w]);
+                mbar_arrive(&p_full[buf]);
             }
             // ---- O / l for this head's rows ----
-            if (!ok || !wait(&pv_done[w], (jj - 1) & 1)) {
+            if (!ok || !wait(&pv_done[sp_buf(w, jj - 1)], sp_par(jj - 1))) {
                 ok = false;
                 break;
             }
