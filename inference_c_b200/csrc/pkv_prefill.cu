@@ -425,8 +425,9 @@ paged_prefill_tc_kernel(const PfArgs a, const __grid_constant__ CUtensorMap qmap
     // the last P the PV before the last may still run; each buffer's own barriers
     // move on only when the buffer was used, and S of a tile is done only after the
     // PV that used its buffer.
-    auto sp_buf = [&](int w, uint32_t t) -> uint32_t { return paired ? (uint32_t)w : (t & 1u); };
-    auto sp_par = [&](uint32_t t) -> uint32_t { return (paired ? t : t >> 1) & 1u; };
+    const uint32_t alternate = paired ? 0u : 1u;
+    auto sp_buf = [&](int w, uint32_t t) -> uint32_t { return (uint32_t)w | (t & alternate); };
+    auto sp_par = [&](uint32_t t) -> uint32_t { return t >> alternate & 1u; };
     const bool serp = a.dense_layout != 0;
     uint32_t *fault = &g_prefill_fault;
 
